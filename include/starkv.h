@@ -32,7 +32,9 @@ enum {
   STARKV_BF16 = 2,
   STARKV_F32 = 3,
   STARKV_I8 = 4,
-  STARKV_U8 = 5
+  STARKV_U8 = 5,
+  STARKV_E4M3 = 6,            /* OCP 8-bit float, 4 exponent and 3 mantissa bits (largest 448, no infinity) */
+  STARKV_E8M0 = 7             /* block scale 2^(byte - 127); 255 is NaN */
 };
 
 /* status codes */
@@ -479,6 +481,110 @@ typedef struct {
 } starkv_skinny_gemm_desc;
 
 int starkv_skinny_gemm(const starkv_skinny_gemm_desc* d, void* stream);
+
+/* ---------------------------------------------------------------------
+ * Projections in 8-bit floating point (e4m3) with a scale for each block of
+ * 128 columns.  No counterpart in the reference, whose projections are fp16
+ * nn.Linear; they take half the bytes of a decode step's weight stream and
+ * run prompts at the matrix cores' 8-bit rate.
+ *
+ * Block formats.  A row of k values holds ceil(k / 128) blocks (the last may
+ * be shorter); value = scale * e4m3.  Activation rows have one scale for
+ * each block of the row, weights [n][k] one for each block of 128 rows x 128
+ * columns.  Scales are STARKV_E8M0 (powers of two, one byte) or STARKV_F32,
+ * scale (r, b) at scale + r * scale_stride_r + b * scale_stride_b elements,
+ * r the row of an activation and row / 128 of a weight.
+ *
+ * starkv_fp8_quantize: x (dtype F16 or BF16, row r at x + r * x_stride
+ * elements) to e4m3 rows at q + r * q_stride bytes and their scales.  With
+ * a = max |x| of a block:
+ *   E8M0: s = 2^e, e the least integer >= -126 with a <= 448 2^e;
+ *         q = e4m3(x / s), the quotient exact
+ *   F32:  a' = max(a, 2^-100), s = a' / 448, q = e4m3(x * (448 / a')), the
+ *         two divisions and the product rounded to fp32
+ * (round to nearest even); a = 0 gives s = 1.  A block that holds a NaN or an
+ * infinity gets the scale NaN and the values NaN, so that every product with
+ * it is NaN.  Bytes from k up to the next multiple of 16 of a row are
+ * written as zero; q is 16-byte aligned and q_stride a multiple of 16 of at
+ * least that (STARKV_ERR_ALIGN, STARKV_ERR_SHAPE).  x may lie at any 2-byte
+ * alignment and stride >= k (aligned 16-byte pieces that hold at least one
+ * byte of a row are read whole).
+ * ------------------------------------------------------------------- */
+typedef struct {
+  int rows, k, dtype;
+  const void* x; int64_t x_stride;
+  void* q; int64_t q_stride;
+  void* scale; int scale_dtype; int64_t scale_stride_r, scale_stride_b;
+} starkv_fp8_quantize_desc;
+
+int starkv_fp8_quantize(const starkv_fp8_quantize_desc* d, void* stream);
+
+/* starkv_fp8_gemm: nn.Linear by an e4m3 weight,
+ *   y[i][j] = r_i * sum_b sx[i][b] sw[j / 128][b] sum_{k in b} qx[i][k] qw[j][k]
+ * accumulated in fp32 and rounded once to out_dtype (the act dtypes or F32):
+ *   out[i][j] = y[i][j] (+ residual[i][j])                        j < n
+ *   silu_mul: out[i][j] = y[i][j] / (1 + exp(-y[i][j])) * y[i][n/2 + j]   j < n/2
+ *             (LlamaMLP over the gate rows followed by the up rows of one
+ *             merged weight; n a multiple of 256, no residual)
+ * x of dtype STARKV_E4M3 comes with x_scale (of scale_dtype); x of F16 or
+ * BF16 is quantised on the way exactly as starkv_fp8_quantize does with
+ * scale_dtype, and then rms = 1 takes it as the raw input of an RMSNorm whose
+ * weight the caller folded into w: r_i = rsqrt(sum_k x[i][k]^2 / k + rms_eps)
+ * (r_i = 1 otherwise).  e4m3 rows (x and w) are 16-byte aligned with strides
+ * that are multiples of 16 (STARKV_ERR_ALIGN); they are read in whole 16-byte
+ * pieces that hold at least one byte of a row, and what lies behind column k
+ * never reaches a result.  residual (row stride residual_stride elements, of
+ * out_dtype) may be out itself.  Any m >= 0, n >= 1, k >= 1.  Up to
+ * STARKV_FP8_FEW_ROWS rows run as one weight stream that needs no workspace.
+ * Results do not depend on the order of atomics; the same call gives the
+ * same bits.
+ */
+#define STARKV_FP8_FEW_ROWS 16
+typedef struct {
+  int m, n, k, dtype, out_dtype;
+  const void* x; int64_t x_stride;                       /* elements of dtype */
+  const void* x_scale; int64_t x_scale_stride_r, x_scale_stride_b;   /* STARKV_E4M3 x only */
+  const void* w; int64_t w_stride;                       /* bytes */
+  const void* w_scale; int64_t w_scale_stride_r, w_scale_stride_b;
+  int scale_dtype;                                       /* of w_scale and x_scale */
+  const void* residual; int64_t residual_stride;         /* optional */
+  int silu_mul;
+  int rms; float rms_eps;
+  void* out; int64_t out_stride;
+} starkv_fp8_gemm_desc;
+
+size_t starkv_fp8_gemm_workspace_bytes(const starkv_fp8_gemm_desc* d);   /* 0: none needed, or invalid */
+int starkv_fp8_gemm(const starkv_fp8_gemm_desc* d, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------
+ * starkv_token_logprobs: for each of `rows` rows of `vocab` logits (dtype
+ * F16, BF16 or F32, row r at logits + r * stride elements, any alignment of
+ * whole elements),
+ *   logprob[r] = x[t] - lse,  lse = max x + ln sum exp(x - max x),  t = tokens[r]
+ *   entropy[r] = -sum_v p_v ln p_v,  p = exp(x - lse)  (0 where p is 0)
+ *   top_id[r][i], top_logprob[r][i], i < top: the top greatest logits in
+ *   descending order, equal ones by ascending index (a NaN before all)
+ * in fp32, in one pass over the logits.  What the reference's perplexity run
+ * takes from cross_entropy over shifted labels (eval.py:54-103).  tokens may
+ * be NULL (logprob is then not written), as may entropy; a token outside
+ * [0, vocab) has the log probability NaN.  Logits of -inf are barred tokens;
+ * a row without a finite logit, or with a NaN or +inf, gives NaN.
+ * 0 <= top <= STARKV_MAX_TOP and <= vocab; 1 <= vocab <= 2^24 (STARKV_ERR_LIMIT).
+ * Workspace: only for few long rows (0 otherwise), which are split.
+ */
+#define STARKV_MAX_TOP 64
+typedef struct {
+  int rows, vocab, dtype, top;
+  const void* logits; int64_t stride;
+  const int64_t* tokens;                     /* [rows], optional */
+  float* logprob;                            /* [rows] */
+  float* entropy;                            /* [rows], optional */
+  float* top_logprob;                        /* [rows][top] */
+  int64_t* top_id;                           /* [rows][top] */
+} starkv_logprobs_desc;
+
+size_t starkv_token_logprobs_workspace_bytes(const starkv_logprobs_desc* d);
+int starkv_token_logprobs(const starkv_logprobs_desc* d, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1486,3 +1486,153 @@ int starkv_prefill_attention_timed(const starkv_prefill_desc* d, void* workspace
 }
 
 }  // extern "C"
+
+extern "C" {
+
+static int scale_size(int dt) { return dt == STARKV_E8M0 ? 1 : dt == STARKV_F32 ? 4 : 0; }
+// e4m3 rows: 16-byte aligned pieces
+static bool rows_e4m3(const void* p, int64_t stride) { return al(p, 16) && stride % 16 == 0; }
+static bool act16(int dt) { return dt == STARKV_F16 || dt == STARKV_BF16; }
+
+int starkv_fp8_quantize(const starkv_fp8_quantize_desc* d, void* stream) {
+  if (!d) return STARKV_ERR_NULL;
+  if (d->rows < 0 || d->k < 1) return STARKV_ERR_SHAPE;
+  if (!act16(d->dtype) || !scale_size(d->scale_dtype)) return STARKV_ERR_DTYPE;
+  if (d->rows == 0) return STARKV_OK;
+  if (!d->x || !d->q || !d->scale) return STARKV_ERR_NULL;
+  if ((d->rows > 1 && (d->x_stride < d->k || d->q_stride < round_up(d->k, 16))) || d->scale_stride_r < 0 ||
+      d->scale_stride_b < 0)
+    return STARKV_ERR_SHAPE;
+  if (!al(d->x, 2) || !rows_e4m3(d->q, d->q_stride) || !al(d->scale, scale_size(d->scale_dtype))) return STARKV_ERR_ALIGN;
+  Fp8QuantArgs a = {};
+  a.x = d->x; a.xs = d->x_stride; a.q = (uint8_t*)d->q; a.qs = d->q_stride;
+  a.s = d->scale; a.ssr = d->scale_stride_r; a.ssb = d->scale_stride_b;
+  a.rows = d->rows; a.k = d->k; a.kb = (int)ceil_div(d->k, FP8_BLOCK);
+  a.vec = al(d->x, 16) && d->x_stride % 8 == 0;
+  if (ceil_div((int64_t)a.rows * a.kb, 32) > INT32_MAX / 256) return STARKV_ERR_LIMIT;
+  return launch_fp8_quant(a, d->dtype, d->scale_dtype, (hipStream_t)stream);
+}
+
+// workspace of a product of many rows: quantised activations, their scales
+// (block-major), row factors, partial sums
+struct Fp8Space { Fp8Plan plan; size_t off_s, off_r, off_p, total; };
+
+static int plan_fp8(const starkv_fp8_gemm_desc* d, Fp8Space& s) {
+  if (!d) return STARKV_ERR_NULL;
+  if (d->m < 0 || d->n < 1 || d->k < 1) return STARKV_ERR_SHAPE;
+  const bool q = d->dtype != STARKV_E4M3;
+  if ((q && !act16(d->dtype)) || !scale_size(d->scale_dtype)) return STARKV_ERR_DTYPE;
+  if (!act16(d->out_dtype) && d->out_dtype != STARKV_F32) return STARKV_ERR_DTYPE;
+  if (d->silu_mul && (d->n % 256 || d->residual)) return STARKV_ERR_SHAPE;
+  if (d->rms && (!q || !(d->rms_eps >= 0.f))) return STARKV_ERR_SHAPE;
+  if (d->k > (1 << 30) || d->n > (1 << 30) || d->m > (1 << 30)) return STARKV_ERR_LIMIT;
+  s = Fp8Space{};
+  if (d->m <= STARKV_FP8_FEW_ROWS) return STARKV_OK;
+  const int64_t kb = ceil_div(d->k, FP8_BLOCK);
+  s.plan = plan_fp8_gemm(d->m, d->n, (int)kb, d->out_dtype == STARKV_F32, device_cus());
+  const int64_t wgs = ceil_div(d->m, s.plan.bm) * ceil_div(d->n, s.plan.bn) * s.plan.splits;
+  const int64_t join = ceil_div((int64_t)d->m * ceil_div(d->n, 4), 256);
+  if (wgs > (INT32_MAX >> 9) - 8 || join > (INT32_MAX >> 8) || (int64_t)d->m * kb > INT32_MAX) return STARKV_ERR_LIMIT;
+  if (q) {
+    s.off_s = a256((size_t)d->m * round_up(d->k, 16));
+    s.off_r = s.off_s + a256((size_t)d->m * kb * scale_size(d->scale_dtype));
+    s.off_p = s.off_r + a256((size_t)d->m * 4);
+  }
+  s.total = s.off_p + s.plan.part_bytes;
+  return STARKV_OK;
+}
+
+size_t starkv_fp8_gemm_workspace_bytes(const starkv_fp8_gemm_desc* d) {
+  Fp8Space s;
+  return plan_fp8(d, s) ? 0 : s.total;
+}
+
+int starkv_fp8_gemm(const starkv_fp8_gemm_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
+  Fp8Space sp;
+  int st = plan_fp8(d, sp);
+  if (st) return st;
+  if (d->m == 0) return STARKV_OK;
+  const bool q = d->dtype != STARKV_E4M3;
+  const int n_out = d->silu_mul ? d->n / 2 : d->n, os = esize(d->out_dtype), ss = scale_size(d->scale_dtype);
+  if (!d->x || !d->w || !d->w_scale || !d->out || (!q && !d->x_scale)) return STARKV_ERR_NULL;
+  if ((d->m > 1 && (d->x_stride < d->k || d->out_stride < n_out || (d->residual && d->residual_stride < n_out))) ||
+      (d->n > 1 && d->w_stride < d->k) || d->w_scale_stride_r < 0 || d->w_scale_stride_b < 0 ||
+      (!q && (d->x_scale_stride_r < 0 || d->x_scale_stride_b < 0)))
+    return STARKV_ERR_SHAPE;
+  if (!rows_e4m3(d->w, d->w_stride) || (q ? !al(d->x, 2) : !rows_e4m3(d->x, d->x_stride)) || !al(d->out, os) ||
+      !al(d->residual, os) || !al(d->w_scale, ss) || (!q && !al(d->x_scale, ss)))
+    return STARKV_ERR_ALIGN;
+  if (sp.total) {
+    if (!workspace || workspace_bytes < sp.total) return STARKV_ERR_WORKSPACE;
+    if (!al(workspace, 256)) return STARKV_ERR_ALIGN;
+  }
+  Fp8GemmArgs a = {};
+  a.x = d->x; a.xs = d->x_stride; a.sx = d->x_scale; a.sxr = d->x_scale_stride_r; a.sxb = d->x_scale_stride_b;
+  a.w = (const uint8_t*)d->w; a.ws = d->w_stride; a.sw = d->w_scale; a.swr = d->w_scale_stride_r; a.swb = d->w_scale_stride_b;
+  a.rms = d->rms != 0; a.rms_eps = d->rms_eps;
+  a.res = d->residual; a.rs = d->residual_stride; a.out = d->out; a.os = d->out_stride;
+  a.m = d->m; a.n = d->n; a.k = d->k; a.kb = (int)ceil_div(d->k, FP8_BLOCK); a.half = d->n / 2;
+  a.vec_x = q && al(d->x, 16) && d->x_stride % 8 == 0;
+  a.vec_out = al(d->out, 4 * os) && d->out_stride % 4 == 0 &&
+              (!d->residual || (al(d->residual, 4 * os) && d->residual_stride % 4 == 0));
+  hipStream_t s = (hipStream_t)stream;
+  if (d->m <= STARKV_FP8_FEW_ROWS) return launch_fp8_few(a, d->dtype, d->out_dtype, d->scale_dtype, d->silu_mul != 0, s);
+  if (q) {
+    char* ws = (char*)workspace;
+    Fp8QuantArgs qa = {};
+    qa.x = d->x; qa.xs = d->x_stride; qa.q = (uint8_t*)ws; qa.qs = round_up(d->k, 16);
+    qa.s = ws + sp.off_s; qa.ssr = 1; qa.ssb = d->m;
+    if (d->rms) { qa.rscale = (float*)(ws + sp.off_r); qa.rms_eps = d->rms_eps; }
+    qa.rows = d->m; qa.k = d->k; qa.kb = a.kb; qa.vec = a.vec_x;
+    if ((st = launch_fp8_quant(qa, d->dtype, d->scale_dtype, s))) return st;
+    a.x = qa.q; a.xs = qa.qs; a.sx = qa.s; a.sxr = 1; a.sxb = d->m; a.rscale = qa.rscale;
+  }
+  if (sp.plan.splits > 1) a.part = (float*)((char*)workspace + sp.off_p);
+  return launch_fp8_gemm(a, sp.plan, d->out_dtype, d->scale_dtype, d->silu_mul != 0, s);
+}
+
+static int plan_lp(const starkv_logprobs_desc* d, LogprobArgs& a, size_t& bytes) {
+  if (!d) return STARKV_ERR_NULL;
+  if (d->rows < 0 || d->vocab < 1 || d->top < 0 || d->top > d->vocab) return STARKV_ERR_SHAPE;
+  if (d->top > STARKV_MAX_TOP || d->vocab > (1 << 24)) return STARKV_ERR_LIMIT;
+  if (!act16(d->dtype) && d->dtype != STARKV_F32) return STARKV_ERR_DTYPE;
+  a = LogprobArgs{};
+  a.rows = d->rows; a.vocab = d->vocab; a.top = d->top;
+  a.pieces = d->rows ? plan_logprobs(d->rows, d->vocab, esize(d->dtype), device_cus()) : 1;
+  a.piece_len = (int)round_up(ceil_div(d->vocab, a.pieces), 1024);
+  a.pieces = (int)ceil_div(d->vocab, a.piece_len);
+  if ((int64_t)d->rows * a.pieces > INT32_MAX / 1024) return STARKV_ERR_LIMIT;
+  const size_t stat = a256((size_t)d->rows * a.pieces * 16);
+  bytes = a.pieces > 1 ? stat + (size_t)d->rows * a.pieces * d->top * 8 : 0;
+  return STARKV_OK;
+}
+
+size_t starkv_token_logprobs_workspace_bytes(const starkv_logprobs_desc* d) {
+  LogprobArgs a;
+  size_t bytes = 0;
+  return plan_lp(d, a, bytes) ? 0 : bytes;
+}
+
+int starkv_token_logprobs(const starkv_logprobs_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
+  LogprobArgs a;
+  size_t bytes = 0;
+  const int st = plan_lp(d, a, bytes);
+  if (st) return st;
+  if (d->rows == 0) return STARKV_OK;
+  if (!d->logits || (d->tokens && !d->logprob) || (d->top && (!d->top_logprob || !d->top_id))) return STARKV_ERR_NULL;
+  if (d->rows > 1 && d->stride < d->vocab) return STARKV_ERR_SHAPE;
+  if (!al(d->logits, esize(d->dtype)) || !al(d->tokens, 8) || !al(d->logprob, 4) || !al(d->entropy, 4) ||
+      !al(d->top_logprob, 4) || !al(d->top_id, 8))
+    return STARKV_ERR_ALIGN;
+  if (bytes) {
+    if (!workspace || workspace_bytes < bytes) return STARKV_ERR_WORKSPACE;
+    if (!al(workspace, 256)) return STARKV_ERR_ALIGN;
+    a.pstat = (float*)workspace;
+    a.ptop = (uint64_t*)((char*)workspace + a256((size_t)d->rows * a.pieces * 16));
+  }
+  a.x = d->logits; a.xs = d->stride; a.tok = d->tokens;
+  a.lp = d->logprob; a.ent = d->entropy; a.tlp = d->top_logprob; a.tid = d->top_id;
+  return launch_logprobs(a, d->dtype, (hipStream_t)stream);
+}
+
+}  // extern "C"

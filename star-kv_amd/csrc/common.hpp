@@ -14,6 +14,7 @@ typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef int intx8 __attribute__((ext_vector_type(8)));
 
 constexpr int HEAD_DIM = 128;
 constexpr int TILE = 32;            // positions per K-logit tile (the MFMA N dimension)
@@ -285,6 +286,45 @@ struct GemmArgs {                                  // skinny_gemm.hip
   int nst, pps;                                    // LDS ring stages per wave, 64-k pairs per stage (launcher)
 };
 
+// ---------------------------------------------------------------------------
+// e4m3 projections (fp8_quant.hip, fp8_few.hip, fp8_gemm.hip) and token log
+// probabilities (logprobs.hip).
+// ---------------------------------------------------------------------------
+constexpr int FP8_BLOCK = 128;                     // columns (and weight rows) that share a scale
+constexpr float FP8_MAX = 448.0f;                  // largest e4m3 value
+constexpr float FP8_AMAX_FLOOR = 0x1p-100f;        // least block maximum of fp32 scales: 448 / it is finite
+struct Fp8QuantArgs {
+  const void* x; int64_t xs;                       // [rows][k] act dtype, row stride (elements)
+  uint8_t* q; int64_t qs;                          // e4m3 rows (bytes)
+  void* s; int64_t ssr, ssb;                       // scale of (row, block), elements
+  float* rscale; float rms_eps;                    // optional: rsqrt(mean x^2 + eps) per row
+  int rows, k, kb;                                 // kb = blocks per row
+  int vec;                                         // rows allow 16-byte loads
+};
+struct Fp8GemmArgs {
+  const void* x; int64_t xs;                       // activations: act dtype (elements) or e4m3 (bytes)
+  const void* sx; int64_t sxr, sxb;                // scales of e4m3 activations
+  const uint8_t* w; int64_t ws;
+  const void* sw; int64_t swr, swb;
+  const float* rscale;                             // optional per-row factor (tile kernel)
+  int rms; float rms_eps;                          // few-rows kernel: the row factor from x itself
+  const void* res; int64_t rs;                     // optional, of the output's type
+  void* out; int64_t os;
+  int m, n, k, kb, half;                           // half = n / 2 (SiLU-multiply)
+  int vec_x, vec_out;                              // 16-byte loads of act rows; 4-column loads / stores of out and res
+  float* part;                                     // split K: [splits][m][n] partial sums
+  int splits, kb_per;                              // k blocks per split
+  int tiles_m, tiles_n;
+};
+struct LogprobArgs {
+  const void* x; int64_t xs;
+  const int64_t* tok;
+  float* lp; float* ent; float* tlp; int64_t* tid;
+  int rows, vocab, top;
+  int pieces, piece_len;                           // workgroups per row, elements per piece (a multiple of 1024)
+  float* pstat; uint64_t* ptop;                    // pieces > 1: [rows][pieces][4] statistics, [rows][pieces][top] keys
+};
+
 // A decode step's cache writes and query rotation in one launch (quant.hip)
 struct StepAppendArgs {
   KAppendArgs k;
@@ -425,6 +465,13 @@ int launch_rope_apply(const RopeApplyArgs& a, int dtype, hipStream_t st);
 int launch_rms_norm(const NormArgs& a, int dtype, hipStream_t st);
 int launch_silu_mul(const SiluMulArgs& a, int dtype, hipStream_t st);
 int launch_skinny_gemm(const GemmArgs& a, int dtype, int epi, hipStream_t st);
+int launch_fp8_quant(const Fp8QuantArgs& a, int dtype, int scale_dtype, hipStream_t st);
+int launch_fp8_few(const Fp8GemmArgs& a, int dtype, int out_dtype, int scale_dtype, bool silu, hipStream_t st);
+struct Fp8Plan { int bm, bn, splits, kb_per; size_t part_bytes; };
+Fp8Plan plan_fp8_gemm(int m, int n, int kb, bool exact, int cus);   // exact: fp32 output
+int launch_fp8_gemm(const Fp8GemmArgs& a, const Fp8Plan& p, int out_dtype, int scale_dtype, bool silu, hipStream_t st);
+int plan_logprobs(int rows, int vocab, int esize, int cus);          // workgroups per row
+int launch_logprobs(const LogprobArgs& a, int dtype, hipStream_t st);
 int launch_k_logits(const KArgs& a, int dtype, int fmt, bool out_f32, int out_dtype, bool fast, int B, hipStream_t st);
 int launch_k_logits_ws(const KArgs& a, int dtype, bool out_f32, int out_dtype, int B, hipStream_t st);
 int launch_k_logits_gqa(const KArgs& a, int dtype, bool out_f32, int out_dtype, int B, hipStream_t st);

@@ -11,7 +11,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libstarkv.so")
 
-F16, BF16, F32, I8, U8 = 1, 2, 3, 4, 5
+F16, BF16, F32, I8, U8, E4M3, E8M0 = 1, 2, 3, 4, 5, 6, 7
 FMT_DENSE, FMT_INT4_REF, FMT_INT8_SYM, FMT_INT4_G64 = 0, 1, 2, 3
 
 c_i64p = ctypes.POINTER(ctypes.c_int64)
@@ -186,6 +186,42 @@ class SkinnyGemmDesc(ctypes.Structure):
     ]
 
 
+class Fp8QuantizeDesc(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int), ("k", ctypes.c_int), ("dtype", ctypes.c_int),
+        ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64),
+        ("q", ctypes.c_void_p), ("q_stride", ctypes.c_int64),
+        ("scale", ctypes.c_void_p), ("scale_dtype", ctypes.c_int),
+        ("scale_stride_r", ctypes.c_int64), ("scale_stride_b", ctypes.c_int64),
+    ]
+
+
+class Fp8GemmDesc(ctypes.Structure):
+    _fields_ = [
+        ("m", ctypes.c_int), ("n", ctypes.c_int), ("k", ctypes.c_int), ("dtype", ctypes.c_int),
+        ("out_dtype", ctypes.c_int),
+        ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64),
+        ("x_scale", ctypes.c_void_p), ("x_scale_stride_r", ctypes.c_int64), ("x_scale_stride_b", ctypes.c_int64),
+        ("w", ctypes.c_void_p), ("w_stride", ctypes.c_int64),
+        ("w_scale", ctypes.c_void_p), ("w_scale_stride_r", ctypes.c_int64), ("w_scale_stride_b", ctypes.c_int64),
+        ("scale_dtype", ctypes.c_int),
+        ("residual", ctypes.c_void_p), ("residual_stride", ctypes.c_int64),
+        ("silu_mul", ctypes.c_int),
+        ("rms", ctypes.c_int), ("rms_eps", ctypes.c_float),
+        ("out", ctypes.c_void_p), ("out_stride", ctypes.c_int64),
+    ]
+
+
+class LogprobsDesc(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int), ("vocab", ctypes.c_int), ("dtype", ctypes.c_int), ("top", ctypes.c_int),
+        ("logits", ctypes.c_void_p), ("stride", ctypes.c_int64),
+        ("tokens", ctypes.c_void_p),
+        ("logprob", ctypes.c_void_p), ("entropy", ctypes.c_void_p),
+        ("top_logprob", ctypes.c_void_p), ("top_id", ctypes.c_void_p),
+    ]
+
+
 EXPORTS = (
     "starkv_abi_version", "starkv_status_string",
     "starkv_rope_table_bytes", "starkv_rope_build", "starkv_rope_apply",
@@ -196,6 +232,8 @@ EXPORTS = (
     "starkv_k_append", "starkv_v_append", "starkv_decode_append",
     "starkv_prefill_workspace_bytes", "starkv_prefill_attention", "starkv_prefill_attention_timed",
     "starkv_rms_norm", "starkv_silu_mul", "starkv_skinny_gemm",
+    "starkv_fp8_quantize", "starkv_fp8_gemm_workspace_bytes", "starkv_fp8_gemm",
+    "starkv_token_logprobs_workspace_bytes", "starkv_token_logprobs",
 )
 
 ABI_VERSION = 5          # STARKV_ABI_VERSION of include/starkv.h that these structs mirror
@@ -257,6 +295,13 @@ def lib() -> ctypes.CDLL:
     L.starkv_silu_mul.argtypes = [ctypes.POINTER(SiluMulDesc), ctypes.c_void_p]
     L.starkv_skinny_gemm.restype = ctypes.c_int
     L.starkv_skinny_gemm.argtypes = [ctypes.POINTER(SkinnyGemmDesc), ctypes.c_void_p]
+    L.starkv_fp8_quantize.restype = ctypes.c_int
+    L.starkv_fp8_quantize.argtypes = [ctypes.POINTER(Fp8QuantizeDesc), ctypes.c_void_p]
+    for name, desc in (("fp8_gemm", Fp8GemmDesc), ("token_logprobs", LogprobsDesc)):
+        wsf, f = getattr(L, f"starkv_{name}_workspace_bytes"), getattr(L, f"starkv_{name}")
+        wsf.restype, f.restype = ctypes.c_size_t, ctypes.c_int
+        wsf.argtypes = [ctypes.POINTER(desc)]
+        f.argtypes = [ctypes.POINTER(desc), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
     _lib = L
     return L
 

@@ -39,6 +39,11 @@ def _stream(device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+# the current stream's handle without torch's Stream object (2 us a call, half a launch)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _require_cuda(*ts):
     for t in ts:
         if t is not None and not t.is_cuda:
@@ -57,7 +62,7 @@ POISON = False
 
 def _poison(t: torch.Tensor) -> torch.Tensor:
     if POISON and t.is_cuda and not torch.cuda.is_current_stream_capturing():
-        t.view(torch.uint8).fill_(0xFF)
+        (t if t.dim() else t.view(1)).view(torch.uint8).fill_(0xFF)
     return t
 
 
@@ -85,6 +90,29 @@ def _workspace(device, nbytes: int) -> torch.Tensor:
         _WS[key] = ws
     _poison(ws[:max(nbytes, 1)])
     return ws
+
+
+def _launch(name: str, desc, device, workspace: Optional[bool] = None) -> None:
+    """Call the entry point ``name`` on ``device``'s current stream.  Entry
+    points with a workspace (``workspace`` not None; False where the call is
+    known to need none) get one of their own: torch's caching allocator orders
+    its reuse by stream and keeps it with a graph under capture."""
+    index = device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _launch(name, desc, torch.device("cuda", torch.cuda.current_device()), workspace)
+    L, ref = _lib.lib(), ctypes.byref(desc)
+    stream = _raw_stream(index)
+    if workspace is None:
+        st = getattr(L, name)(ref, stream)
+    elif not workspace:
+        st = getattr(L, name)(ref, None, 0, stream)
+    else:
+        nb = getattr(L, name + "_workspace_bytes")(ref)
+        ws = _poison(torch.empty(nb, dtype=torch.uint8, device=device)) if nb else None
+        st = getattr(L, name)(ref, ws.data_ptr() if nb else None, nb, stream)
+    if st:
+        check(st, name)
 
 
 class KLatentSpec:

@@ -1525,7 +1525,7 @@ static int plan_fp8(const starkv_fp8_gemm_desc* d, Fp8Space& s) {
   if (!act16(d->out_dtype) && d->out_dtype != STARKV_F32) return STARKV_ERR_DTYPE;
   if (d->silu_mul && (d->n % 256 || d->residual)) return STARKV_ERR_SHAPE;
   if (d->rms && (!q || !(d->rms_eps >= 0.f))) return STARKV_ERR_SHAPE;
-  if (d->k > (1 << 30) || d->n > (1 << 30) || d->m > (1 << 30)) return STARKV_ERR_LIMIT;
+  if (d->k > (1 << 24) || d->n > (1 << 30) || d->m > (1 << 30)) return STARKV_ERR_LIMIT;
   s = Fp8Space{};
   if (d->m <= STARKV_FP8_FEW_ROWS) return STARKV_OK;
   const int64_t kb = ceil_div(d->k, FP8_BLOCK);
@@ -1565,6 +1565,13 @@ int starkv_fp8_gemm(const starkv_fp8_gemm_desc* d, void* workspace, size_t works
   if (sp.total) {
     if (!workspace || workspace_bytes < sp.total) return STARKV_ERR_WORKSPACE;
     if (!al(workspace, 256)) return STARKV_ERR_ALIGN;
+  }
+  // many rows: a tile's rows (256, the up rows half a weight further) and their scales at 32-bit offsets
+  if (d->m > STARKV_FP8_FEW_ROWS) {
+    const int64_t lim = ((int64_t)1 << 32) - 1, wr = 256 + (d->silu_mul ? d->n / 2 : 0);
+    if ((q ? round_up(d->k, 16) : d->x_stride) > (lim - d->k) / 256 || d->w_stride > (lim - d->k) / wr ||
+        (!q && d->x_scale_stride_r > lim / 1024))
+      return STARKV_ERR_LIMIT;
   }
   Fp8GemmArgs a = {};
   a.x = d->x; a.xs = d->x_stride; a.sx = d->x_scale; a.sxr = d->x_scale_stride_r; a.sxb = d->x_scale_stride_b;

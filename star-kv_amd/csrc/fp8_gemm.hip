@@ -30,7 +30,45 @@ namespace starkv {
 namespace {
 typedef __attribute__((address_space(3))) void lds_void;
 __device__ inline int swz(int r) { return (r & 7) ^ ((r >> 3) & 1); }
+
+// 1 KB to LDS byte address `lds` (16 bytes a lane) from base + the lane's
+// offset.  In inline assembly, so that the compiler, which then does not see
+// it write LDS, adds no wait of its own before reads of the other stage: one
+// loop body serves both stages.  Volatile statements keep their order, so the
+// loads stay between the barriers; nothing else in these kernels uses m0.  A
+// wait state separates the scalar write of m0 from the load that takes it.
+__device__ inline void dma_1k(const uint8_t* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "m0");
+}
+
+// Workgroup -> tile (tm, tn) and 1 + its split of k; 0: none.  Workgroup i
+// runs on XCD i % 8; each XCD takes a contiguous run of tiles, which go down
+// eight row tiles before the next column, so that its L2 serves most reads.
+__device__ inline int tile_of(const Fp8GemmArgs& a, int wg, int& tm, int& tn) {
+  constexpr int GROUP = 8;
+  const int tiles = a.tiles_m * a.tiles_n, total = tiles * a.splits;
+  const int per = (total + 7) >> 3;
+  const int idx = (wg & 7) * per + (wg >> 3);
+  if (idx >= total) return 0;
+  const int split = idx / tiles, tl = idx - split * tiles;
+  const int grp = tl / (GROUP * a.tiles_n), rem = tl - grp * GROUP * a.tiles_n;
+  const int gm = min(GROUP, a.tiles_m - grp * GROUP);
+  tm = grp * GROUP + rem % gm;
+  tn = rem / gm;
+  return split + 1;
+}
 }  // namespace
+
+// Zero the bytes past column k of a stage that holds the row's last, short
+// block (nv < 128 columns): they are any value, also NaN.
+template <int ROWS, int THREADS> __device__ inline void zero_tail(uint8_t* st, int nv) {
+  const int p0 = nv >> 4, np = 8 - p0;             // pieces from the first short one on
+  for (int i = threadIdx.x; i < ROWS * np; i += THREADS) {
+    const int r = i / np, p = p0 + i - r * np;
+    uint4* q = (uint4*)(st + r * 128 + ((p ^ swz(r & 15)) << 4));
+    *q = keep_bytes(*q, nv - 16 * p);
+  }
+}
 
 // WM x WN waves; SILU: the tile's columns are BN / 2 gate columns and the same up columns
 template <int BM, int BN, int WM, int WN, typename S, typename O, bool SILU, bool SPLIT>
@@ -41,26 +79,17 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN >= 32768 ? 2 : 1) void fp8_ge
   static_assert(LOADS * 8 * NW == BM + BN && BM % 8 == 0, "whole loads");
   static_assert(!SILU || NF % 2 == 0, "gate and up halves");
   constexpr bool EXACT = __is_same(O, float);      // 16-bit instructions (see half_of)
-  __shared__ __attribute__((aligned(16))) uint8_t st0[(BM + BN) * 128];
-  __shared__ __attribute__((aligned(16))) uint8_t st1[(BM + BN) * 128];
+  constexpr int STAGE = (BM + BN) * 128;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % WM, wn = wave / WM;
   const int c = lane & 15, g = lane >> 4;
 
-  // workgroup -> tile: workgroup i runs on XCD i % 8; each XCD takes a
-  // contiguous run of tiles, which go down eight row tiles before the next column
-  const int tiles = a.tiles_m * a.tiles_n;
-  const int total = tiles * a.splits;
-  const int per = (total + 7) >> 3;
-  const int idx = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= per || idx >= total) return;
-  const int split = idx / tiles, tl = idx - split * tiles;
-  constexpr int GROUP = 8;
-  const int grp = tl / (GROUP * a.tiles_n), rem = tl - grp * GROUP * a.tiles_n;
-  const int gm = min(GROUP, a.tiles_m - grp * GROUP);
-  const int tm = grp * GROUP + rem % gm, tn = rem / gm;
+  int tm, tn;
+  const int split = tile_of(a, blockIdx.x, tm, tn) - 1;
+  if (split < 0) return;
   const int m0 = tm * BM, n0 = tn * (SILU ? BN / 2 : BN);
   const int kb0 = split * a.kb_per, kb1 = min(a.kb, kb0 + a.kb_per);
 
@@ -74,32 +103,35 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN >= 32768 ? 2 : 1) void fp8_ge
     return n0 + j;
   };
 
-  // this lane's source of each of the wave's loads: 8 rows x 8 pieces
+  // this lane's source of each of the wave's loads (8 rows x 8 pieces), from the tile's first row
   const int rs = lane >> 3, q8 = lane & 7;
-  const uint8_t* src[LOADS];
-  int piece[LOADS];
+  const uint8_t* const xbase = (const uint8_t*)a.x + (int64_t)m0 * a.xs;
+  const uint8_t* const wbase = a.w + (int64_t)n0 * a.ws;
+  uint32_t off[LOADS];
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) {
     const int row = (wave * LOADS + i) * 8 + rs;
-    piece[i] = q8 ^ swz(row & 15);
-    src[i] = row < BM ? (const uint8_t*)a.x + (int64_t)min(m0 + row, a.m - 1) * a.xs
-                      : a.w + (int64_t)min(wrow_of(row - BM), a.n - 1) * a.ws;
+    const int64_t r = row < BM ? min(m0 + row, a.m - 1) - m0 : min(wrow_of(row - BM), a.n - 1) - n0;
+    off[i] = (uint32_t)(r * (row < BM ? a.xs : a.ws));
   }
   const int last = (a.k - 1) >> 4;
-  auto issue = [&](uint8_t* st, int kb) __attribute__((always_inline)) {
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)lds;
+  auto issue = [&](int stage, int kb) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i)
-      __builtin_amdgcn_global_load_lds((const void*)(src[i] + (int64_t)min(kb * 8 + piece[i], last) * 16),
-                                       (lds_void*)(st + (wave * LOADS + i) * 1024), 16, 0, 0);
+    for (int i = 0; i < LOADS; ++i) {
+      const int row = (wave * LOADS + i) * 8;      // uniform; the lane's piece of its row is q8 ^ swz(row + rs)
+      const int p = min(kb * 8 + (q8 ^ rs ^ ((row >> 3) & 1)), last);
+      dma_1k(row < BM ? xbase : wbase, off[i] + (uint32_t)p * 16, lds0 + stage + row * 128);
+    }
   };
 
   // scales: activation row m0 + wm TM + 16 i + c, weight block of the wave's (gate / up) rows
   typedef typename S::T ST;
   constexpr int NS = SILU ? 2 : 1;
-  const ST* sxp[MF];
+  const ST* const sxp = (const ST*)a.sx + (int64_t)m0 * a.sxr;
+  uint32_t sxo[MF];
 #pragma unroll
-  for (int i = 0; i < MF; ++i)
-    sxp[i] = (const ST*)a.sx + (int64_t)min(m0 + wm * TM + 16 * i + c, a.m - 1) * a.sxr;
+  for (int i = 0; i < MF; ++i) sxo[i] = (uint32_t)((min(m0 + wm * TM + 16 * i + c, a.m - 1) - m0) * a.sxr);
   const ST* swp[NS];
 #pragma unroll
   for (int t = 0; t < NS; ++t)
@@ -115,39 +147,42 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN >= 32768 ? 2 : 1) void fp8_ge
   struct Sc { ST x[MF], w[NS]; };
   auto scales = [&](Sc& sc, int kb) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < MF; ++i) sc.x[i] = sxp[i][(int64_t)kb * a.sxb];
+    for (int i = 0; i < MF; ++i) sc.x[i] = (sxp + (int64_t)kb * a.sxb)[sxo[i]];
 #pragma unroll
     for (int t = 0; t < NS; ++t) sc.w[t] = swp[t][(int64_t)kb * a.swb];
   };
-  // block kb from stage `cur` with the scales `sc`, the next one's loads into
-  // `nxt` and `sn` issued first; LAST: none follows, and it may end before 128 columns
-  auto step = [&](auto last_c, const uint8_t* cur, uint8_t* nxt, int kb, const Sc& sc, Sc& sn) __attribute__((always_inline)) {
-    constexpr bool LAST = decltype(last_c)::value;
-    // this wave's loads of block kb (issued a block ago) landed, and its reads of the other stage are done ...
+  // The blocks in the order last, first, second ..: the row's last one may be
+  // short, and what lies behind it is zeroed before the loop starts.
+  const int n = kb1 - kb0;
+  auto block = [&](int t) { return t == 0 || t >= n ? kb1 - 1 : kb0 + t - 1; };
+  Sc sc, sn;
+  issue(0, block(0));
+  scales(sc, block(0));
+  if (kb1 == a.kb && (a.k & (FP8_BLOCK - 1))) {
+    __builtin_amdgcn_s_waitcnt(0x0070);
+    __syncthreads();
+    zero_tail<BM + BN, 64 * NW>(lds, a.k & (FP8_BLOCK - 1));
+  }
+  int at = 0;
+  for (int t = 0; t < n; ++t, at ^= STAGE) {
+    // this wave's loads of block t (issued a block ago) landed, and its reads of the other stage are done ...
     __builtin_amdgcn_s_waitcnt(0x0070);
     asm volatile("s_barrier" ::: "memory");        // ... and everyone's
-    if constexpr (!LAST) {
-      issue(nxt, kb + 1);
-      scales(sn, kb + 1);
-    }
-    const int nv = a.k - kb * FP8_BLOCK - 16 * g;
+    issue(at ^ STAGE, block(t + 1));               // (after the last block: one of them again, for nobody)
+    scales(sn, block(t + 1));
+    const uint8_t* const cur = lds + at;
     auto frag = [&](int row16) __attribute__((always_inline)) {
       const uint8_t* p = cur + row16 * 128;
-      uint4 lo = *(const uint4*)(p + rd0), hi = *(const uint4*)(p + (rd0 ^ 64));
-      if constexpr (LAST) {                        // bytes past column k: any value in either operand
-        lo = keep_bytes(lo, nv);
-        hi = keep_bytes(hi, nv - 64);
-      }
-      return frag8(lo, hi);
+      return frag8(*(const uint4*)(p + rd0), *(const uint4*)(p + (rd0 ^ 64)));
     };
-    intx8 wf[NF];
+    intx8 xf[MF];
 #pragma unroll
-    for (int j = 0; j < NF; ++j) wf[j] = frag(BM + wn * TN + 16 * j);
+    for (int i = 0; i < MF; ++i) xf[i] = frag(wm * TM + 16 * i);
     if constexpr (EXACT) {
-      intx8 xf[MF];
+      intx8 wf[NF];
       floatx4 p[NF][MF];
 #pragma unroll
-      for (int i = 0; i < MF; ++i) xf[i] = frag(wm * TM + 16 * i);
+      for (int j = 0; j < NF; ++j) wf[j] = frag(BM + wn * TN + 16 * j);
 #pragma unroll
       for (int j = 0; j < NF; ++j)
 #pragma unroll
@@ -172,41 +207,27 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN >= 32768 ? 2 : 1) void fp8_ge
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[j][i][e] = fmaf(p[j][i][e], s, acc[j][i][e]);
         }
-      return;
-    }
+    } else {
 #pragma unroll
-    for (int i = 0; i < MF; ++i) {
-      const intx8 xf = frag(wm * TM + 16 * i);
-      if constexpr (S::pow2) {
+      for (int j = 0; j < NF; ++j) {
+        const intx8 wf = frag(BM + wn * TN + 16 * j);
+        const ST sw = sc.w[SILU ? j / (NF / 2) : 0];
 #pragma unroll
-        for (int j = 0; j < NF; ++j) acc[j][i] = mfma8(wf[j], xf, acc[j][i], sc.w[SILU ? j / (NF / 2) : 0], sc.x[i]);
-      } else {
+        for (int i = 0; i < MF; ++i) {
+          if constexpr (S::pow2) {
+            acc[j][i] = mfma8(wf, xf[i], acc[j][i], sw, sc.x[i]);
+          } else {
+            const float s = sc.x[i] * sw;
+            const floatx4 p = mfma8(wf, xf[i], floatx4{0.f, 0.f, 0.f, 0.f}, E8_ONE, E8_ONE);
 #pragma unroll
-        for (int j = 0; j < NF; ++j) {
-          const float s = sc.x[i] * sc.w[SILU ? j / (NF / 2) : 0];
-          const floatx4 p = mfma8(wf[j], xf, floatx4{0.f, 0.f, 0.f, 0.f}, E8_ONE, E8_ONE);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[j][i][e] = fmaf(p[e], s, acc[j][i][e]);
+            for (int e = 0; e < 4; ++e) acc[j][i][e] = fmaf(p[e], s, acc[j][i][e]);
+          }
         }
       }
     }
-  };
-  const std::false_type more{};
-  const std::true_type end{};
-  Sc s0, s1;
-  issue(st0, kb0);
-  scales(s0, kb0);
-  int kb = kb0;
-  for (; kb + 2 < kb1; kb += 2) {
-    step(more, st0, st1, kb, s0, s1);
-    step(more, st1, st0, kb + 1, s1, s0);
+    sc = sn;
   }
-  if (kb + 1 < kb1) {
-    step(more, st0, st1, kb, s0, s1);
-    step(end, st1, st0, kb + 1, s1, s0);
-  } else {
-    step(end, st0, st1, kb, s0, s1);
-  }
+  __builtin_amdgcn_s_waitcnt(0x0070);              // the last loads, before the workgroup gives up its LDS
 
   // lane (c, g): columns 16 j + 4 g .. + 3 of row 16 i + c of the wave's tile
 #pragma unroll
@@ -240,6 +261,182 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN >= 32768 ? 2 : 1) void fp8_ge
         store4<O>((O*)a.out + (int64_t)row * a.os + col, v, nv, a.vec_out != 0);
       }
     }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Power-of-two scales, 256 x 256 tiles: four waves of 128 x 128 (one per SIMD,
+// 256 accumulators each), 32 x 32 x 64 instructions.  The matrix cores need
+// 2048 cycles for a block; the operands of four 128 x 128 wave tiles take
+// 128 KB of LDS reads and 64 KB of writes per block, 1536 cycles at 128
+// bytes, where eight waves of 64 x 128 would take all of the 2048.
+//
+// A block is two halves of 64 columns, each with operand registers of its own:
+//   * half 0's products run while half 1's operands are read;
+//   * then every wave has read this stage and (its loads have landed and) the
+//     next stage is whole: the one barrier of the block;
+//   * half 1's products run while the next block's half 0 is read, and the
+//     block after that is loaded into the stage just freed.
+// So neither the barrier nor an LDS read is waited for with the matrix cores idle.
+// ---------------------------------------------------------------------------
+constexpr int WT = 256;                            // tile rows and columns
+constexpr int WSTAGE = 2 * WT * 128;               // bytes of a stage
+
+__device__ inline floatx16 mfma8_32(intx8 a, intx8 b, floatx16 c, int scale_a, int scale_b) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, scale_a, 0, scale_b);
+}
+
+template <typename O, bool SILU>
+__global__ __launch_bounds__(256, 1) void fp8_gemm_wide_kernel(const Fp8GemmArgs a) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * WSTAGE];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave & 1, wn = wave >> 1;
+  const int c = lane & 31, g = lane >> 5;
+  int tm, tn;
+  if (!tile_of(a, blockIdx.x, tm, tn)) return;
+  const int m0 = tm * WT, n0 = tn * (SILU ? WT / 2 : WT);
+
+  // Loads: 512 rows of 128 bytes, X then W; this wave takes rows 128 wave .. (X: waves 0, 1), eight rows and
+  // their eight pieces at a time.  Offsets from the tile's first row fit 32 bits.
+  const int rs = lane >> 3, q8 = lane & 7;
+  const bool isx = wave < 2;
+  // W rows of the tile: with SILU, wave column wn owns 64 gate rows and the same 64 up rows
+  auto wrow = [&](int j) {
+    if constexpr (SILU) return ((j & 64) ? a.half : 0) + n0 + (j >> 7) * 64 + (j & 63);
+    return n0 + j;
+  };
+  uint32_t off[16];
+  const int last = (a.k - 1) >> 4;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int r = (wave & 1) * 128 + 8 * i + rs;
+    const int64_t row = isx ? min(m0 + r, a.m - 1) - m0 : min(wrow(r), a.n - 1) - n0;
+    off[i] = (uint32_t)(row * (isx ? a.xs : a.ws));
+  }
+  const uint8_t* base = isx ? (const uint8_t*)a.x + (int64_t)m0 * a.xs : a.w + (int64_t)n0 * a.ws;
+  const int piece0 = q8 ^ rs;                      // piece of row r at slot q8: q8 ^ swz(r), swz(8 i + rs) = rs ^ (i & 1)
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)lds + wave * 16 * 1024;
+  auto issue1 = [&](int stage, int kb, int i) __attribute__((always_inline)) {
+    // pieces past the row's last one (the last block only) read that one again
+    const int p = min(kb * 8 + (piece0 ^ (i & 1)), last);
+    dma_1k(base, off[i] + (uint32_t)p * 16, lds0 + stage + i * 1024);
+  };
+
+  const uint8_t* const sxp = (const uint8_t*)a.sx + (int64_t)m0 * a.sxr;
+  uint32_t sxo[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sxo[i] = (uint32_t)((min(m0 + wm * 128 + 32 * i + c, a.m - 1) - m0) * a.sxr);
+  const uint8_t* swb[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+    swb[t] = (const uint8_t*)a.sw + (int64_t)(min(wrow(wn * 128 + 64 * t), a.n - 1) >> 7) * a.swr;
+  struct Sc { uint8_t x[4], w[2]; };
+  auto scales = [&](Sc& sc, int kb) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sc.x[i] = (sxp + (int64_t)kb * a.sxb)[sxo[i]];
+#pragma unroll
+    for (int t = 0; t < (SILU ? 2 : 1); ++t) sc.w[t] = swb[t][(int64_t)kb * a.swb];
+  };
+
+  // operand reads: lane (c, g) takes pieces 4 h + 2 g and + 1 of row c
+  const int f = (c & 7) ^ ((c >> 3) & 1);
+  int rd[2][2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) rd[h][t] = c * 128 + (((4 * h + 2 * g + t) ^ f) << 4);
+  struct Half { intx8 x[4], w[4]; };
+  auto read1 = [&](Half& o, const uint8_t* st, int h, int i) __attribute__((always_inline)) {
+    const uint8_t* px = st + (wm * 128 + 32 * i) * 128;
+    const uint8_t* pw = st + (WT + wn * 128 + 32 * i) * 128;
+    o.x[i] = frag8(*(const uint4*)(px + rd[h][0]), *(const uint4*)(px + rd[h][1]));
+    o.w[i] = frag8(*(const uint4*)(pw + rd[h][0]), *(const uint4*)(pw + rd[h][1]));
+  };
+
+  floatx16 acc[4][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[j][i] = floatx16{};
+  Half h0, h1;
+  auto products = [&](const Half& o, const Sc& sc) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[j][i] = mfma8_32(o.w[j], o.x[i], acc[j][i], sc.w[SILU ? j >> 1 : 0], sc.x[i]);
+  };
+  // the blocks in the order last, first, second .., as above; after them the
+  // loads repeat one and the reads take what is there, for nobody
+  const int end = a.kb - 1;
+  auto block = [&](int t) { return t == 0 || t > end ? end : t - 1; };
+  Sc sc, sn;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) issue1(0, end, i);
+  scales(sc, end);
+  __builtin_amdgcn_s_waitcnt(0x0070);
+  asm volatile("s_barrier" ::: "memory");
+  if (a.k & (FP8_BLOCK - 1)) {
+    zero_tail<2 * WT, 256>(lds, a.k & (FP8_BLOCK - 1));
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) issue1(WSTAGE, block(1), i);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) read1(h0, lds, 0, i);
+  int cur = 0;
+  for (int t = 0; t <= end; ++t, cur ^= WSTAGE) {  // block(t) in stage `cur`, its half 0 in h0, its scales in sc
+    scales(sn, block(t + 1));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) read1(h1, lds + cur, 1, i);
+    products(h0, sc);
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);         // 1 MFMA
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);         // 1 LDS read
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    // half 1 read; this wave's part of the next stage landed
+    __builtin_amdgcn_s_waitcnt(0x0070);
+    asm volatile("s_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int d = 0; d < 4; ++d) issue1(cur, block(t + 2), 4 * i + d);
+      read1(h0, lds + (cur ^ WSTAGE), 0, i);
+    }
+    products(h1, sc);
+    sc = sn;
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  __builtin_amdgcn_s_waitcnt(0x0070);              // the last loads, before the workgroup gives up its LDS
+
+  // lane (c, g): columns 32 j + 8 q + 4 g .. + 3 of row 32 i + c of the wave's tile
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = m0 + wm * 128 + 32 * i + c;
+    if (row >= a.m) continue;
+    const float r = a.rscale ? a.rscale[row] : 1.f;
+#pragma unroll
+    for (int j = 0; j < (SILU ? 2 : 4); ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int col = n0 + wn * (SILU ? 64 : 128) + 32 * j + 8 * q + 4 * g;
+        const int nv = (SILU ? a.half : a.n) - col;
+        if (nv <= 0) continue;
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[e] = SILU ? silu_mul_f32(r * acc[j][i][4 * q + e], r * acc[(j + 2) & 3][i][4 * q + e]) : r * acc[j][i][4 * q + e];
+        if (!SILU && a.res) {
+          float t[4];
+          load4<O>((const O*)a.res + (int64_t)row * a.rs + col, t, nv, a.vec_out != 0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] += t[e];
+        }
+        store4<O>((O*)a.out + (int64_t)row * a.os + col, v, nv, a.vec_out != 0);
+      }
   }
 }
 
@@ -307,9 +504,19 @@ static int launch_tile(Fp8GemmArgs a, hipStream_t st) {
   }
   return (int)hipGetLastError();
 }
+template <typename O, bool SILU> static int launch_wide(Fp8GemmArgs a, hipStream_t st) {
+  a.tiles_m = (int)ceil_div(a.m, WT);
+  a.tiles_n = (int)ceil_div(a.n, WT);
+  const dim3 grid((unsigned)(8 * ceil_div((int64_t)a.tiles_m * a.tiles_n, 8)));
+  hipLaunchKernelGGL((fp8_gemm_wide_kernel<O, SILU>), grid, dim3(256), 0, st, a);
+  return (int)hipGetLastError();
+}
 template <typename S, typename O, bool SILU> static int launch_shape(const Fp8GemmArgs& a, const Fp8Plan& p, hipStream_t st) {
   if constexpr (!__is_same(O, float))
-    if (p.bm == 256) return launch_tile<256, 256, 4, 2, S, O, SILU>(a, st);
+    if (p.bm == 256) {
+      if constexpr (S::pow2) return launch_wide<O, SILU>(a, st);
+      else return launch_tile<256, 256, 4, 2, S, O, SILU>(a, st);
+    }
   if (p.bm == 128) return launch_tile<128, 128, 2, 2, S, O, SILU>(a, st);
   return launch_tile<64, 128, 1, 4, S, O, SILU>(a, st);
 }

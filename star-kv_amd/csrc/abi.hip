@@ -1580,8 +1580,11 @@ int starkv_fp8_gemm(const starkv_fp8_gemm_desc* d, void* workspace, size_t works
   a.res = d->residual; a.rs = d->residual_stride; a.out = d->out; a.os = d->out_stride;
   a.m = d->m; a.n = d->n; a.k = d->k; a.kb = (int)ceil_div(d->k, FP8_BLOCK); a.half = d->n / 2;
   a.vec_x = q && al(d->x, 16) && d->x_stride % 8 == 0;
-  a.vec_out = al(d->out, 4 * os) && d->out_stride % 4 == 0 &&
-              (!d->residual || (al(d->residual, 4 * os) && d->residual_stride % 4 == 0));
+  auto vec = [&](int n) {
+    return al(d->out, n * os) && d->out_stride % n == 0 &&
+           (!d->residual || (al(d->residual, n * os) && d->residual_stride % n == 0));
+  };
+  a.vec_out = os == 2 && vec(8) ? 2 : vec(4);
   hipStream_t s = (hipStream_t)stream;
   if (d->m <= STARKV_FP8_FEW_ROWS) return launch_fp8_few(a, d->dtype, d->out_dtype, d->scale_dtype, d->silu_mul != 0, s);
   if (q) {

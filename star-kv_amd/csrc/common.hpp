@@ -311,7 +311,8 @@ struct Fp8GemmArgs {
   const void* res; int64_t rs;                     // optional, of the output's type
   void* out; int64_t os;
   int m, n, k, kb, half;                           // half = n / 2 (SiLU-multiply)
-  int vec_x, vec_out;                              // 16-byte loads of act rows; 4-column loads / stores of out and res
+  int vec_x;                                       // 16-byte loads of act rows
+  int vec_out;                                     // out and res allow loads / stores of 4 (1) or 8 (2) columns
   float* part;                                     // split K: [splits][m][n] partial sums
   int splits, kb_per;                              // k blocks per split
   int tiles_m, tiles_n;
@@ -467,7 +468,7 @@ int launch_silu_mul(const SiluMulArgs& a, int dtype, hipStream_t st);
 int launch_skinny_gemm(const GemmArgs& a, int dtype, int epi, hipStream_t st);
 int launch_fp8_quant(const Fp8QuantArgs& a, int dtype, int scale_dtype, hipStream_t st);
 int launch_fp8_few(const Fp8GemmArgs& a, int dtype, int out_dtype, int scale_dtype, bool silu, hipStream_t st);
-struct Fp8Plan { int bm, bn, splits, kb_per; size_t part_bytes; };
+struct Fp8Plan { int bm, bn, splits, kb_per, cus; size_t part_bytes; };
 Fp8Plan plan_fp8_gemm(int m, int n, int kb, bool exact, int cus);   // exact: fp32 output
 int launch_fp8_gemm(const Fp8GemmArgs& a, const Fp8Plan& p, int out_dtype, int scale_dtype, bool silu, hipStream_t st);
 int plan_logprobs(int rows, int vocab, int esize, int cus);          // workgroups per row

@@ -44,18 +44,49 @@ __device__ inline void dma_1k(const uint8_t* base, uint32_t off, uint32_t lds) {
 // Workgroup -> tile (tm, tn) and 1 + its split of k; 0: none.  Workgroup i
 // runs on XCD i % 8; each XCD takes a contiguous run of tiles, which go down
 // eight row tiles before the next column, so that its L2 serves most reads.
-__device__ inline int tile_of(const Fp8GemmArgs& a, int wg, int& tm, int& tn) {
+__device__ inline void tile_at(const Fp8GemmArgs& a, int tl, int& tm, int& tn) {
   constexpr int GROUP = 8;
-  const int tiles = a.tiles_m * a.tiles_n, total = tiles * a.splits;
-  const int per = (total + 7) >> 3;
-  const int idx = (wg & 7) * per + (wg >> 3);
-  if (idx >= total) return 0;
-  const int split = idx / tiles, tl = idx - split * tiles;
   const int grp = tl / (GROUP * a.tiles_n), rem = tl - grp * GROUP * a.tiles_n;
   const int gm = min(GROUP, a.tiles_m - grp * GROUP);
   tm = grp * GROUP + rem % gm;
   tn = rem / gm;
+}
+__device__ inline int tile_of(const Fp8GemmArgs& a, int wg, int& tm, int& tn) {
+  const int tiles = a.tiles_m * a.tiles_n, total = tiles * a.splits;
+  const int per = (total + 7) >> 3;
+  const int idx = (wg & 7) * per + (wg >> 3);
+  if (idx >= total) return 0;
+  const int split = idx / tiles;
+  tile_at(a, idx - split * tiles, tm, tn);
   return split + 1;
+}
+
+// eight consecutive results (16-bit, and the residual added) from column col on, nv of them inside the row
+template <typename O> __device__ inline void store8(const Fp8GemmArgs& a, int row, int col, int nv, float (&v)[8]) {
+  O* o = (O*)a.out + (int64_t)row * a.os + col;
+  const O* rp = (const O*)a.res + (int64_t)row * a.rs + col;
+  if (a.vec_out >= 2 && nv >= 8) {
+    if (a.res) {
+      const uint4 t = *(const uint4*)rp;
+      O r[8];
+      __builtin_memcpy(r, &t, 16);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += (float)r[e];
+    }
+    O t[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t[e] = (O)v[e];
+    uint4 u;
+    __builtin_memcpy(&u, t, 16);
+    *(uint4*)o = u;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < nv) {
+        if (a.res) v[e] += (float)rp[e];
+        o[e] = (O)v[e];
+      }
+  }
 }
 }  // namespace
 
@@ -277,10 +308,15 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN >= 32768 ? 2 : 1) void fp8_ge
 //     next stage is whole: the one barrier of the block;
 //   * half 1's products run while the next block's half 0 is read, and the
 //     block after that is loaded into the stage just freed.
-// So neither the barrier nor an LDS read is waited for with the matrix cores idle.
+// So neither the barrier nor an LDS read is waited for with the matrix cores
+// idle.  A workgroup takes tile after tile: the next tile's first blocks load
+// while this one's results are stored, by way of LDS so that whole 128-byte
+// lines leave (straight from the accumulators' layout, 16 bytes a row, the
+// stores of a tile took as long as 1600 columns of products).
 // ---------------------------------------------------------------------------
 constexpr int WT = 256;                            // tile rows and columns
 constexpr int WSTAGE = 2 * WT * 128;               // bytes of a stage
+constexpr int WOUT = 32 * 64 * 4;                  // bytes a wave stages of its results: 32 rows x 64 columns, fp32
 
 __device__ inline floatx16 mfma8_32(intx8 a, intx8 b, floatx16 c, int scale_a, int scale_b) {
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, scale_a, 0, scale_b);
@@ -288,55 +324,71 @@ __device__ inline floatx16 mfma8_32(intx8 a, intx8 b, floatx16 c, int scale_a, i
 
 template <typename O, bool SILU>
 __global__ __launch_bounds__(256, 1) void fp8_gemm_wide_kernel(const Fp8GemmArgs a) {
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * WSTAGE];
+  static_assert(sizeof(O) == 2, "16-bit outputs");
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * WSTAGE + 4 * WOUT];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave & 1, wn = wave >> 1;
   const int c = lane & 31, g = lane >> 5;
-  int tm, tn;
-  if (!tile_of(a, blockIdx.x, tm, tn)) return;
-  const int m0 = tm * WT, n0 = tn * (SILU ? WT / 2 : WT);
+  const int end = a.kb - 1;
 
   // Loads: 512 rows of 128 bytes, X then W; this wave takes rows 128 wave .. (X: waves 0, 1), eight rows and
   // their eight pieces at a time.  Offsets from the tile's first row fit 32 bits.
   const int rs = lane >> 3, q8 = lane & 7;
   const bool isx = wave < 2;
+  const int last = (a.k - 1) >> 4;
+  const int piece0 = q8 ^ rs;                      // piece of row r at slot q8: q8 ^ swz(r), swz(8 i + rs) = rs ^ (i & 1)
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)lds + wave * 16 * 1024;
+
+  // the tile in hand
+  int m0, n0;
+  const uint8_t* base;
+  uint32_t off[16];                                // of the wave's loads' lane: row and piece
+  const uint8_t *sxp, *swp[2];
+  uint32_t sxo[4];
   // W rows of the tile: with SILU, wave column wn owns 64 gate rows and the same 64 up rows
   auto wrow = [&](int j) {
     if constexpr (SILU) return ((j & 64) ? a.half : 0) + n0 + (j >> 7) * 64 + (j & 63);
     return n0 + j;
   };
-  uint32_t off[16];
-  const int last = (a.k - 1) >> 4;
+  auto take = [&](int idx) __attribute__((always_inline)) {
+    int tm, tn;
+    tile_at(a, idx, tm, tn);
+    m0 = tm * WT;
+    n0 = tn * (SILU ? WT / 2 : WT);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int r = (wave & 1) * 128 + 8 * i + rs;
-    const int64_t row = isx ? min(m0 + r, a.m - 1) - m0 : min(wrow(r), a.n - 1) - n0;
-    off[i] = (uint32_t)(row * (isx ? a.xs : a.ws));
-  }
-  const uint8_t* base = isx ? (const uint8_t*)a.x + (int64_t)m0 * a.xs : a.w + (int64_t)n0 * a.ws;
-  const int piece0 = q8 ^ rs;                      // piece of row r at slot q8: q8 ^ swz(r), swz(8 i + rs) = rs ^ (i & 1)
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)lds + wave * 16 * 1024;
-  auto issue1 = [&](int stage, int kb, int i) __attribute__((always_inline)) {
-    // pieces past the row's last one (the last block only) read that one again
-    const int p = min(kb * 8 + (piece0 ^ (i & 1)), last);
-    dma_1k(base, off[i] + (uint32_t)p * 16, lds0 + stage + i * 1024);
+    for (int i = 0; i < 16; ++i) {
+      const int r = (wave & 1) * 128 + 8 * i + rs;
+      const int64_t row = isx ? min(m0 + r, a.m - 1) - m0 : min(wrow(r), a.n - 1) - n0;
+      off[i] = (uint32_t)(row * (isx ? a.xs : a.ws));
+    }
+    base = isx ? (const uint8_t*)a.x + (int64_t)m0 * a.xs : a.w + (int64_t)n0 * a.ws;
+    sxp = (const uint8_t*)a.sx + (int64_t)m0 * a.sxr;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sxo[i] = (uint32_t)((min(m0 + wm * 128 + 32 * i + c, a.m - 1) - m0) * a.sxr);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      swp[t] = (const uint8_t*)a.sw + (int64_t)(min(wrow(wn * 128 + 64 * t), a.n - 1) >> 7) * a.swr;
   };
-
-  const uint8_t* const sxp = (const uint8_t*)a.sx + (int64_t)m0 * a.sxr;
-  uint32_t sxo[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) sxo[i] = (uint32_t)((min(m0 + wm * 128 + 32 * i + c, a.m - 1) - m0) * a.sxr);
-  const uint8_t* swb[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-    swb[t] = (const uint8_t*)a.sw + (int64_t)(min(wrow(wn * 128 + 64 * t), a.n - 1) >> 7) * a.swr;
   struct Sc { uint8_t x[4], w[2]; };
   auto scales = [&](Sc& sc, int kb) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) sc.x[i] = (sxp + (int64_t)kb * a.sxb)[sxo[i]];
 #pragma unroll
-    for (int t = 0; t < (SILU ? 2 : 1); ++t) sc.w[t] = swb[t][(int64_t)kb * a.swb];
+    for (int t = 0; t < (SILU ? 2 : 1); ++t) sc.w[t] = swp[t][(int64_t)kb * a.swb];
+  };
+  // The blocks in the order last, first, second .. (the last may be short:
+  // what lies behind it is zeroed before the loop starts).  A full block's
+  // pieces need no check against the row's end.
+  auto block = [&](int t) { return t == 0 ? end : t > end ? 0 : t - 1; };
+  auto issue_last = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      dma_1k(base, off[i] + (uint32_t)min(end * 8 + (piece0 ^ (i & 1)), last) * 16, lds0 + i * 1024);
+  };
+  const uint32_t po[2] = {(uint32_t)min(piece0, last) * 16, (uint32_t)min(piece0 ^ 1, last) * 16};
+  auto issue1 = [&](int stage, int kb, int i) __attribute__((always_inline)) {
+    dma_1k(base + (int64_t)kb * FP8_BLOCK, off[i] + po[i & 1], lds0 + stage + i * 1024);
   };
 
   // operand reads: lane (c, g) takes pieces 4 h + 2 g and + 1 of row c
@@ -346,97 +398,139 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_wide_kernel(const Fp8GemmArgs
   for (int h = 0; h < 2; ++h)
 #pragma unroll
     for (int t = 0; t < 2; ++t) rd[h][t] = c * 128 + (((4 * h + 2 * g + t) ^ f) << 4);
-  struct Half { intx8 x[4], w[4]; };
-  auto read1 = [&](Half& o, const uint8_t* st, int h, int i) __attribute__((always_inline)) {
-    const uint8_t* px = st + (wm * 128 + 32 * i) * 128;
-    const uint8_t* pw = st + (WT + wn * 128 + 32 * i) * 128;
-    o.x[i] = frag8(*(const uint4*)(px + rd[h][0]), *(const uint4*)(px + rd[h][1]));
-    o.w[i] = frag8(*(const uint4*)(pw + rd[h][0]), *(const uint4*)(pw + rd[h][1]));
+  struct Half { uint4 x[4][2], w[4][2]; };
+  // the q-th of the half's 16 reads: activations and weights of row group 0, then 1 ..
+  auto read1 = [&](Half& o, const uint8_t* st, int h, int q) __attribute__((always_inline)) {
+    const int i = q >> 2, t = q & 1;
+    if (q & 2) o.w[i][t] = *(const uint4*)(st + (WT + wn * 128 + 32 * i) * 128 + rd[h][t]);
+    else o.x[i][t] = *(const uint4*)(st + (wm * 128 + 32 * i) * 128 + rd[h][t]);
   };
 
-  floatx16 acc[4][4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[j][i] = floatx16{};
-  Half h0, h1;
-  auto products = [&](const Half& o, const Sc& sc) __attribute__((always_inline)) {
+  // tiles of this XCD (workgroup i runs on XCD i % 8), one after the other
+  const int total = a.tiles_m * a.tiles_n, per = (total + 7) >> 3;
+  const int first = (blockIdx.x & 7) * per, stop = min(total, first + per), stride = gridDim.x >> 3;
+  int idx = first + (blockIdx.x >> 3);
+  if (idx >= stop) return;
+  take(idx);
+  Sc sc, sn;
+  issue_last();
+  scales(sc, end);
+  while (true) {
+    floatx16 acc[4][4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[j][i] = mfma8_32(o.w[j], o.x[i], acc[j][i], sc.w[SILU ? j >> 1 : 0], sc.x[i]);
-  };
-  // the blocks in the order last, first, second .., as above; after them the
-  // loads repeat one and the reads take what is there, for nobody
-  const int end = a.kb - 1;
-  auto block = [&](int t) { return t == 0 || t > end ? end : t - 1; };
-  Sc sc, sn;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) issue1(0, end, i);
-  scales(sc, end);
-  __builtin_amdgcn_s_waitcnt(0x0070);
-  asm volatile("s_barrier" ::: "memory");
-  if (a.k & (FP8_BLOCK - 1)) {
-    zero_tail<2 * WT, 256>(lds, a.k & (FP8_BLOCK - 1));
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 0; i < 16; ++i) issue1(WSTAGE, block(1), i);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) read1(h0, lds, 0, i);
-  int cur = 0;
-  for (int t = 0; t <= end; ++t, cur ^= WSTAGE) {  // block(t) in stage `cur`, its half 0 in h0, its scales in sc
-    scales(sn, block(t + 1));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) read1(h1, lds + cur, 1, i);
-    products(h0, sc);
-#pragma unroll
-    for (int q = 0; q < 16; ++q) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);         // 1 MFMA
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);         // 1 LDS read
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    // half 1 read; this wave's part of the next stage landed
+      for (int i = 0; i < 4; ++i) acc[j][i] = floatx16{};
     __builtin_amdgcn_s_waitcnt(0x0070);
     asm volatile("s_barrier" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-#pragma unroll
-      for (int d = 0; d < 4; ++d) issue1(cur, block(t + 2), 4 * i + d);
-      read1(h0, lds + (cur ^ WSTAGE), 0, i);
+    if (a.k & (FP8_BLOCK - 1)) {
+      zero_tail<2 * WT, 256>(lds, a.k & (FP8_BLOCK - 1));
+      __syncthreads();
     }
-    products(h1, sc);
-    sc = sn;
-    __builtin_amdgcn_sched_barrier(0);
-  }
-  __builtin_amdgcn_s_waitcnt(0x0070);              // the last loads, before the workgroup gives up its LDS
-
-  // lane (c, g): columns 32 j + 8 q + 4 g .. + 3 of row 32 i + c of the wave's tile
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = m0 + wm * 128 + 32 * i + c;
-    if (row >= a.m) continue;
-    const float r = a.rscale ? a.rscale[row] : 1.f;
+    for (int i = 0; i < 16; ++i) issue1(WSTAGE, block(1), i);
+    Half h0, h1;
 #pragma unroll
-    for (int j = 0; j < (SILU ? 2 : 4); ++j)
+    for (int q = 0; q < 16; ++q) read1(h0, lds, 0, q);
+    int cur = 0;
+    auto product = [&](const Half& o, int q) __attribute__((always_inline)) {
+      // row groups in the order in which the reads bring them
+      constexpr int ORDER[16] = {0, 1, 4, 5, 2, 6, 8, 9, 10, 3, 7, 11, 12, 13, 14, 15};
+      const int j = ORDER[q] >> 2, i = ORDER[q] & 3;
+      acc[j][i] = mfma8_32(frag8(o.w[j][0], o.w[j][1]), frag8(o.x[i][0], o.x[i][1]), acc[j][i], sc.w[SILU ? j >> 1 : 0],
+                           sc.x[i]);
+    };
+    for (int t = 0; t <= end; ++t, cur ^= WSTAGE) {    // block(t) in stage `cur`, its half 0 in h0, its scales in sc
+      scales(sn, block(t + 1));
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int col = n0 + wn * (SILU ? 64 : 128) + 32 * j + 8 * q + 4 * g;
-        const int nv = (SILU ? a.half : a.n) - col;
-        if (nv <= 0) continue;
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          v[e] = SILU ? silu_mul_f32(r * acc[j][i][4 * q + e], r * acc[(j + 2) & 3][i][4 * q + e]) : r * acc[j][i][4 * q + e];
-        if (!SILU && a.res) {
-          float t[4];
-          load4<O>((const O*)a.res + (int64_t)row * a.rs + col, t, nv, a.vec_out != 0);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] += t[e];
-        }
-        store4<O>((O*)a.out + (int64_t)row * a.os + col, v, nv, a.vec_out != 0);
+      for (int q = 0; q < 16; ++q) {
+        product(h0, q);
+        read1(h1, lds + cur, 1, q);
+        __builtin_amdgcn_sched_barrier(0);
       }
+      // half 1 read; this wave's part of the next stage landed
+      __builtin_amdgcn_s_waitcnt(0x0070);
+      asm volatile("s_barrier" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      const int kn = block(t + 2);
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        product(h1, q);
+        issue1(cur, kn, q);
+        read1(h0, lds + (cur ^ WSTAGE), 0, q);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      sc = sn;
+    }
+    // after the last blocks the loads repeated one and the reads took what was there, for nobody
+    __builtin_amdgcn_s_waitcnt(0x0070);
+    asm volatile("s_barrier" ::: "memory");
+    const int om = m0 + wm * 128, on = n0 + wn * (SILU ? 64 : 128);
+    idx += stride;
+    const bool more = idx < stop;
+    if (more) {
+      take(idx);
+      issue_last();
+      scales(sc, end);
+    }
+
+    // Results: lane (c, g) holds columns 32 j + 8 q + 4 g .. + 3 of row 32 i + c of acc[j][i].  Two accumulators
+    // (SILU: gate and up) go through the wave's own part of LDS at a time, 32 rows of 256 bytes, 16-byte piece p of
+    // row r at p ^ (r & 15).  One copy of the code that finishes and stores them serves all: a tile's stores are run
+    // once, and unrolled they came from memory instruction by instruction (48 KB of code: 25 us a tile).
+    uint8_t* const ob = lds + 2 * WSTAGE + wave * WOUT;
+    const int ncol = SILU ? a.half : a.n;
+#pragma unroll 1
+    for (int ch = 0; ch < 8; ++ch) {
+      auto put = [&](auto chc) __attribute__((always_inline)) {
+        constexpr int C = decltype(chc)::value, I = C >> 1, J = C & 1;
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const floatx16& v = acc[SILU ? J + 2 * jj : 2 * J + jj][I];
+            *(floatx4*)(ob + c * 256 + (((8 * jj + 2 * q + g) ^ (c & 15)) << 4)) =
+                floatx4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+          }
+      };
+      switch (ch) {
+        case 0: put(std::integral_constant<int, 0>{}); break;
+        case 1: put(std::integral_constant<int, 1>{}); break;
+        case 2: put(std::integral_constant<int, 2>{}); break;
+        case 3: put(std::integral_constant<int, 3>{}); break;
+        case 4: put(std::integral_constant<int, 4>{}); break;
+        case 5: put(std::integral_constant<int, 5>{}); break;
+        case 6: put(std::integral_constant<int, 6>{}); break;
+        default: put(std::integral_constant<int, 7>{}); break;
+      }
+      // eight columns a lane: 8 lanes to a row of 64 columns, or 4 to a row of 32 gate and 32 up columns
+      constexpr int LPR = SILU ? 4 : 8, RPI = 64 / LPR;
+      const int rc = lane & (LPR - 1);
+      const int col = on + (ch & 1) * (SILU ? 32 : 64) + 8 * rc;
+#pragma unroll 1
+      for (int lr = lane / LPR; lr < 32; lr += RPI) {
+        const int row = om + 32 * (ch >> 1) + lr;
+        const uint8_t* p = ob + lr * 256;
+        const int sw = lr & 15;
+        const floatx4 u0 = *(const floatx4*)(p + (((2 * rc) ^ sw) << 4)), u1 = *(const floatx4*)(p + (((2 * rc + 1) ^ sw) << 4));
+        if (row >= a.m || col >= ncol) continue;
+        const float r = a.rscale ? a.rscale[row] : 1.f;
+        float v[8];
+        if constexpr (SILU) {
+          const floatx4 w0 = *(const floatx4*)(p + (((2 * rc + 8) ^ sw) << 4)), w1 = *(const floatx4*)(p + (((2 * rc + 9) ^ sw) << 4));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[e] = silu_mul_f32(r * u0[e], r * w0[e]);
+            v[4 + e] = silu_mul_f32(r * u1[e], r * w1[e]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { v[e] = r * u0[e]; v[4 + e] = r * u1[e]; }
+        }
+        store8<O>(a, row, col, ncol - col, v);
+      }
+    }
+    if (!more) break;
   }
 }
 
@@ -477,6 +571,7 @@ template <typename O, bool SILU> __global__ __launch_bounds__(256) void fp8_join
 
 Fp8Plan plan_fp8_gemm(int m, int n, int kb, bool exact, int cus) {
   Fp8Plan p = {};
+  p.cus = cus;
   const bool big = !exact && (int64_t)ceil_div(m, 256) * ceil_div(n, 256) >= cus;
   p.bm = big ? 256 : m <= 64 ? 64 : 128;
   p.bn = big ? 256 : 128;
@@ -504,17 +599,18 @@ static int launch_tile(Fp8GemmArgs a, hipStream_t st) {
   }
   return (int)hipGetLastError();
 }
-template <typename O, bool SILU> static int launch_wide(Fp8GemmArgs a, hipStream_t st) {
+template <typename O, bool SILU> static int launch_wide(Fp8GemmArgs a, int cus, hipStream_t st) {
   a.tiles_m = (int)ceil_div(a.m, WT);
   a.tiles_n = (int)ceil_div(a.n, WT);
-  const dim3 grid((unsigned)(8 * ceil_div((int64_t)a.tiles_m * a.tiles_n, 8)));
+  const int64_t per = ceil_div((int64_t)a.tiles_m * a.tiles_n, 8);        // tiles of an XCD
+  const dim3 grid((unsigned)(8 * std::min<int64_t>(per, std::max(1, cus / 8))));
   hipLaunchKernelGGL((fp8_gemm_wide_kernel<O, SILU>), grid, dim3(256), 0, st, a);
   return (int)hipGetLastError();
 }
 template <typename S, typename O, bool SILU> static int launch_shape(const Fp8GemmArgs& a, const Fp8Plan& p, hipStream_t st) {
   if constexpr (!__is_same(O, float))
     if (p.bm == 256) {
-      if constexpr (S::pow2) return launch_wide<O, SILU>(a, st);
+      if constexpr (S::pow2) return launch_wide<O, SILU>(a, p.cus, st);
       else return launch_tile<256, 256, 4, 2, S, O, SILU>(a, st);
     }
   if (p.bm == 128) return launch_tile<128, 128, 2, 2, S, O, SILU>(a, st);

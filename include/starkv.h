@@ -534,12 +534,11 @@ int starkv_fp8_quantize(const starkv_fp8_quantize_desc* d, void* stream);
  * that are multiples of 16 (STARKV_ERR_ALIGN); they are read in whole 16-byte
  * pieces that hold at least one byte of a row, and what lies behind column k
  * never reaches a result.  residual (row stride residual_stride elements, of
- * out_dtype) may be out itself.  Any m >= 0, n >= 1, k >= 1.  Up to
- * STARKV_FP8_FEW_ROWS rows run as one weight stream that needs no workspace.
+ * out_dtype) may be out itself.  Any m >= 0, n >= 1, k >= 1.
+ * Workspace: the quantised activations (0 for e4m3 ones).
  * Results do not depend on the order of atomics; the same call gives the
  * same bits.
  */
-#define STARKV_FP8_FEW_ROWS 16
 typedef struct {
   int m, n, k, dtype, out_dtype;
   const void* x; int64_t x_stride;                       /* elements of dtype */

@@ -1513,9 +1513,9 @@ int starkv_fp8_quantize(const starkv_fp8_quantize_desc* d, void* stream) {
   return launch_fp8_quant(a, d->dtype, d->scale_dtype, (hipStream_t)stream);
 }
 
-// workspace of a product of many rows: quantised activations, their scales
-// (block-major), row factors, partial sums
-struct Fp8Space { Fp8Plan plan; size_t off_s, off_r, off_p, total; };
+// workspace of a product: quantised activations, their scales (block-major),
+// row factors
+struct Fp8Space { Fp8Plan plan; size_t off_s, off_r, total; };
 
 static int plan_fp8(const starkv_fp8_gemm_desc* d, Fp8Space& s) {
   if (!d) return STARKV_ERR_NULL;
@@ -1527,18 +1527,17 @@ static int plan_fp8(const starkv_fp8_gemm_desc* d, Fp8Space& s) {
   if (d->rms && (!q || !(d->rms_eps >= 0.f))) return STARKV_ERR_SHAPE;
   if (d->k > (1 << 24) || d->n > (1 << 30) || d->m > (1 << 30)) return STARKV_ERR_LIMIT;
   s = Fp8Space{};
-  if (d->m <= STARKV_FP8_FEW_ROWS) return STARKV_OK;
   const int64_t kb = ceil_div(d->k, FP8_BLOCK);
-  s.plan = plan_fp8_gemm(d->m, d->n, (int)kb, d->out_dtype == STARKV_F32, device_cus());
-  const int64_t wgs = ceil_div(d->m, s.plan.bm) * ceil_div(d->n, s.plan.bn) * s.plan.splits;
-  const int64_t join = ceil_div((int64_t)d->m * ceil_div(d->n, 4), 256);
-  if (wgs > (INT32_MAX >> 9) - 8 || join > (INT32_MAX >> 8) || (int64_t)d->m * kb > INT32_MAX) return STARKV_ERR_LIMIT;
-  if (q) {
+  if (q && d->m > 0) {
     s.off_s = a256((size_t)d->m * round_up(d->k, 16));
     s.off_r = s.off_s + a256((size_t)d->m * kb * scale_size(d->scale_dtype));
-    s.off_p = s.off_r + a256((size_t)d->m * 4);
+    s.total = s.off_r + a256((size_t)d->m * 4);
   }
-  s.total = s.off_p + s.plan.part_bytes;
+  s.plan = plan_fp8_gemm(d->m, d->n, (int)kb, d->silu_mul != 0, d->out_dtype == STARKV_F32,
+                         d->scale_dtype == STARKV_E8M0, device_cus());
+  // grids of at most 2^22 workgroups (2^31 threads), rows' blocks below 2^31
+  if ((ceil_div(d->m, s.plan.bm) + 1) * (ceil_div(d->n, s.plan.bn) + 8) > (1 << 22) || (int64_t)d->m * kb > INT32_MAX / 8)
+    return STARKV_ERR_LIMIT;
   return STARKV_OK;
 }
 
@@ -1566,8 +1565,8 @@ int starkv_fp8_gemm(const starkv_fp8_gemm_desc* d, void* workspace, size_t works
     if (!workspace || workspace_bytes < sp.total) return STARKV_ERR_WORKSPACE;
     if (!al(workspace, 256)) return STARKV_ERR_ALIGN;
   }
-  // many rows: a tile's rows (256, the up rows half a weight further) and their scales at 32-bit offsets
-  if (d->m > STARKV_FP8_FEW_ROWS) {
+  // tiles in LDS: a tile's rows (256, the up rows half a weight further) and their scales at 32-bit offsets
+  if (!sp.plan.few) {
     const int64_t lim = ((int64_t)1 << 32) - 1, wr = 256 + (d->silu_mul ? d->n / 2 : 0);
     if ((q ? round_up(d->k, 16) : d->x_stride) > (lim - d->k) / 256 || d->w_stride > (lim - d->k) / wr ||
         (!q && d->x_scale_stride_r > lim / 1024))
@@ -1576,28 +1575,25 @@ int starkv_fp8_gemm(const starkv_fp8_gemm_desc* d, void* workspace, size_t works
   Fp8GemmArgs a = {};
   a.x = d->x; a.xs = d->x_stride; a.sx = d->x_scale; a.sxr = d->x_scale_stride_r; a.sxb = d->x_scale_stride_b;
   a.w = (const uint8_t*)d->w; a.ws = d->w_stride; a.sw = d->w_scale; a.swr = d->w_scale_stride_r; a.swb = d->w_scale_stride_b;
-  a.rms = d->rms != 0; a.rms_eps = d->rms_eps;
   a.res = d->residual; a.rs = d->residual_stride; a.out = d->out; a.os = d->out_stride;
   a.m = d->m; a.n = d->n; a.k = d->k; a.kb = (int)ceil_div(d->k, FP8_BLOCK); a.half = d->n / 2;
-  a.vec_x = q && al(d->x, 16) && d->x_stride % 8 == 0;
   auto vec = [&](int n) {
     return al(d->out, n * os) && d->out_stride % n == 0 &&
            (!d->residual || (al(d->residual, n * os) && d->residual_stride % n == 0));
   };
   a.vec_out = os == 2 && vec(8) ? 2 : vec(4);
   hipStream_t s = (hipStream_t)stream;
-  if (d->m <= STARKV_FP8_FEW_ROWS) return launch_fp8_few(a, d->dtype, d->out_dtype, d->scale_dtype, d->silu_mul != 0, s);
   if (q) {
     char* ws = (char*)workspace;
     Fp8QuantArgs qa = {};
     qa.x = d->x; qa.xs = d->x_stride; qa.q = (uint8_t*)ws; qa.qs = round_up(d->k, 16);
     qa.s = ws + sp.off_s; qa.ssr = 1; qa.ssb = d->m;
     if (d->rms) { qa.rscale = (float*)(ws + sp.off_r); qa.rms_eps = d->rms_eps; }
-    qa.rows = d->m; qa.k = d->k; qa.kb = a.kb; qa.vec = a.vec_x;
+    qa.rows = d->m; qa.k = d->k; qa.kb = a.kb; qa.vec = al(d->x, 16) && d->x_stride % 8 == 0;
     if ((st = launch_fp8_quant(qa, d->dtype, d->scale_dtype, s))) return st;
     a.x = qa.q; a.xs = qa.qs; a.sx = qa.s; a.sxr = 1; a.sxb = d->m; a.rscale = qa.rscale;
   }
-  if (sp.plan.splits > 1) a.part = (float*)((char*)workspace + sp.off_p);
+  if (sp.plan.few) return launch_fp8_few(a, sp.plan, d->out_dtype, d->scale_dtype, d->silu_mul != 0, s);
   return launch_fp8_gemm(a, sp.plan, d->out_dtype, d->scale_dtype, d->silu_mul != 0, s);
 }
 

@@ -302,19 +302,15 @@ struct Fp8QuantArgs {
   int vec;                                         // rows allow 16-byte loads
 };
 struct Fp8GemmArgs {
-  const void* x; int64_t xs;                       // activations: act dtype (elements) or e4m3 (bytes)
-  const void* sx; int64_t sxr, sxb;                // scales of e4m3 activations
+  const void* x; int64_t xs;                       // e4m3 activations (bytes)
+  const void* sx; int64_t sxr, sxb;                // and their scales
   const uint8_t* w; int64_t ws;
   const void* sw; int64_t swr, swb;
-  const float* rscale;                             // optional per-row factor (tile kernel)
-  int rms; float rms_eps;                          // few-rows kernel: the row factor from x itself
+  const float* rscale;                             // optional per-row factor
   const void* res; int64_t rs;                     // optional, of the output's type
   void* out; int64_t os;
   int m, n, k, kb, half;                           // half = n / 2 (SiLU-multiply)
-  int vec_x;                                       // 16-byte loads of act rows
   int vec_out;                                     // out and res allow loads / stores of 4 (1) or 8 (2) columns
-  float* part;                                     // split K: [splits][m][n] partial sums
-  int splits, kb_per;                              // k blocks per split
   int tiles_m, tiles_n;
 };
 struct LogprobArgs {
@@ -467,9 +463,9 @@ int launch_rms_norm(const NormArgs& a, int dtype, hipStream_t st);
 int launch_silu_mul(const SiluMulArgs& a, int dtype, hipStream_t st);
 int launch_skinny_gemm(const GemmArgs& a, int dtype, int epi, hipStream_t st);
 int launch_fp8_quant(const Fp8QuantArgs& a, int dtype, int scale_dtype, hipStream_t st);
-int launch_fp8_few(const Fp8GemmArgs& a, int dtype, int out_dtype, int scale_dtype, bool silu, hipStream_t st);
-struct Fp8Plan { int bm, bn, splits, kb_per, cus; size_t part_bytes; };
-Fp8Plan plan_fp8_gemm(int m, int n, int kb, bool exact, int cus);   // exact: fp32 output
+struct Fp8Plan { bool few; int bm, bn, ks, cus; };   // the stream kernel; tile rows and columns, k groups of waves
+int launch_fp8_few(const Fp8GemmArgs& a, const Fp8Plan& p, int out_dtype, int scale_dtype, bool silu, hipStream_t st);
+Fp8Plan plan_fp8_gemm(int m, int n, int kb, bool silu, bool exact, bool pow2, int cus);   // exact: fp32 output
 int launch_fp8_gemm(const Fp8GemmArgs& a, const Fp8Plan& p, int out_dtype, int scale_dtype, bool silu, hipStream_t st);
 int plan_logprobs(int rows, int vocab, int esize, int cus);          // workgroups per row
 int launch_logprobs(const LogprobArgs& a, int dtype, hipStream_t st);

@@ -113,27 +113,56 @@ __device__ inline uint32_t amax16(const uint32_t (&w)[8]) {
   return m;
 }
 
-// 16 values scaled and rounded to e4m3
-template <typename T> __device__ inline uint4 quant16(const uint32_t (&w)[8], float inv) {
+// Two 16-bit values of a dword divided by the power of two `scale` and rounded to e4m3, into the low or high half of v
+typedef short short2v __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+template <typename T, bool HI> __device__ inline uint32_t cvt2_pow2(uint32_t v, uint32_t w, float scale);
+template <> __device__ inline uint32_t cvt2_pow2<_Float16, false>(uint32_t v, uint32_t w, float scale) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(__builtin_bit_cast(short2v, v), __builtin_bit_cast(kh2, w), scale, false));
+}
+template <> __device__ inline uint32_t cvt2_pow2<_Float16, true>(uint32_t v, uint32_t w, float scale) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(__builtin_bit_cast(short2v, v), __builtin_bit_cast(kh2, w), scale, true));
+}
+template <> __device__ inline uint32_t cvt2_pow2<__bf16, false>(uint32_t v, uint32_t w, float scale) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(__builtin_bit_cast(short2v, v), __builtin_bit_cast(bf16x2, w), scale, false));
+}
+template <> __device__ inline uint32_t cvt2_pow2<__bf16, true>(uint32_t v, uint32_t w, float scale) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(__builtin_bit_cast(short2v, v), __builtin_bit_cast(bf16x2, w), scale, true));
+}
+
+// 16 values to e4m3 by block_scale()'s result: one instruction for two values where the scale is a power of two,
+// else the product with the reciprocal, rounded to fp32, first
+template <typename T, typename S> __device__ inline uint4 quant16(const uint32_t (&w)[8], float inv, float scale) {
   uint32_t o[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float a, b, c, d;
-    unpack2<T>(w[2 * i], a, b);
-    unpack2<T>(w[2 * i + 1], c, d);
-    o[i] = pack_e4m3(a * inv, b * inv, c * inv, d * inv);
+    if constexpr (S::pow2) {
+      o[i] = cvt2_pow2<T, true>(cvt2_pow2<T, false>(0u, w[2 * i], scale), w[2 * i + 1], scale);
+    } else {
+      float a, b, c, d;
+      unpack2<T>(w[2 * i], a, b);
+      unpack2<T>(w[2 * i + 1], c, d);
+      o[i] = pack_e4m3(a * inv, b * inv, c * inv, d * inv);
+    }
   }
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-// sum of squares of 16 values
-template <typename T> __device__ inline float sumsq16(const uint32_t (&w)[8], float ss) {
+// sum of squares of 16 values, added in fp32
+template <typename T> __device__ inline float sumsq16(const uint32_t (&w)[8], float ss);
+template <> __device__ inline float sumsq16<_Float16>(const uint32_t (&w)[8], float ss) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    float a, b;
-    unpack2<T>(w[i], a, b);
-    ss = fmaf(a, a, ss);
-    ss = fmaf(b, b, ss);
+    const kh2 h = __builtin_bit_cast(kh2, w[i]);
+    ss = __builtin_amdgcn_fdot2(h, h, ss, false);
+  }
+  return ss;
+}
+template <> __device__ inline float sumsq16<__bf16>(const uint32_t (&w)[8], float ss) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const bf16x2 h = __builtin_bit_cast(bf16x2, w[i]);
+    ss = __builtin_amdgcn_fdot2_f32_bf16(h, h, ss, false);
   }
   return ss;
 }

@@ -1,13 +1,13 @@
 // e4m3 projection of many rows: out[m][n] = X W^T over blocks of 128 columns,
 // each with its own scales (the definition is in starkv.h).
 //
-// A workgroup computes a BM x BN tile of the output, k block by k block: the
-// block's BM + BN rows of 128 bytes go to LDS by direct loads (16 bytes a
-// lane), one stage ahead of the matrix instructions.  One 16 x 16 x 128
-// instruction is one block's partial sum:
+// A workgroup computes a tile of the output, k block by k block: the block's
+// rows of 128 bytes go to LDS by direct loads (16 bytes a lane), NST stages
+// ahead of the matrix instructions.  Instructions are 32 x 32 x 64, so a block
+// is two halves:
 //   * power-of-two scales ride in the instruction itself (its operands carry
 //     an exponent byte each), so the accumulators take the sums directly;
-//   * fp32 scales multiply each partial sum, acc += p * (sx sw).
+//   * with fp32 scales both halves' sums p are formed first, acc += p (sx sw).
 // The weight rows are the instruction's A operand and the activations its B
 // operand: a lane then holds four consecutive columns of one output row, and
 // one activation scale.
@@ -17,9 +17,12 @@
 // read touches at the same piece fall on distinct banks, taken 8 or 16 lanes
 // at a time.
 //
-// Two stages, each an array of its own, the loop unrolled over them (the
-// compiler then sees that reading one cannot alias the loads in flight into
-// the other), and one barrier per block.
+// The loop overlaps its three resources: half 0's products run while half 1's
+// operands are read; then, behind the block's one barrier, half 1's products
+// run while the next block's half 0 is read and another block is loaded into
+// the stage just consumed.  (One after the other - load, read, multiply -
+// each 128 x 128 block took 1850 cycles, the sum of the three, where the
+// products take 512.)
 #include <algorithm>
 #include <type_traits>
 
@@ -41,9 +44,25 @@ __device__ inline void dma_1k(const uint8_t* base, uint32_t off, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "m0");
 }
 
-// Workgroup -> tile (tm, tn) and 1 + its split of k; 0: none.  Workgroup i
-// runs on XCD i % 8; each XCD takes a contiguous run of tiles, which go down
-// eight row tiles before the next column, so that its L2 serves most reads.
+// one dword a lane from its own address to LDS byte address `lds` + 4 * lane
+__device__ inline void dma_dword(const void* src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds) : "m0");
+}
+// Wait until at most n stages of LOADS loads each are on their way (n is uniform, at most NST - 2), and for this
+// wave's LDS reads.
+template <int NST, int LOADS> __device__ inline void wait_stages(int n) {
+  constexpr auto code = [](int v) constexpr { return 0x0070 | (v & 15) | ((v >> 4) << 14); };
+  static_assert(NST <= 7, "cases");
+  if (NST > 6 && n == 5) __builtin_amdgcn_s_waitcnt(code(NST > 6 ? 5 * LOADS : 0));
+  else if (NST > 5 && n == 4) __builtin_amdgcn_s_waitcnt(code(NST > 5 ? 4 * LOADS : 0));
+  else if (NST > 4 && n == 3) __builtin_amdgcn_s_waitcnt(code(NST > 4 ? 3 * LOADS : 0));
+  else if (NST > 3 && n == 2) __builtin_amdgcn_s_waitcnt(code(NST > 3 ? 2 * LOADS : 0));
+  else if (NST > 2 && n == 1) __builtin_amdgcn_s_waitcnt(code(NST > 2 ? LOADS : 0));
+  else __builtin_amdgcn_s_waitcnt(code(0));
+}
+
+// Tile number -> (tm, tn): down eight row tiles before the next column, so that an XCD's L2 serves most reads of a
+// contiguous run of tiles.
 __device__ inline void tile_at(const Fp8GemmArgs& a, int tl, int& tm, int& tn) {
   constexpr int GROUP = 8;
   const int grp = tl / (GROUP * a.tiles_n), rem = tl - grp * GROUP * a.tiles_n;
@@ -51,16 +70,6 @@ __device__ inline void tile_at(const Fp8GemmArgs& a, int tl, int& tm, int& tn) {
   tm = grp * GROUP + rem % gm;
   tn = rem / gm;
 }
-__device__ inline int tile_of(const Fp8GemmArgs& a, int wg, int& tm, int& tn) {
-  const int tiles = a.tiles_m * a.tiles_n, total = tiles * a.splits;
-  const int per = (total + 7) >> 3;
-  const int idx = (wg & 7) * per + (wg >> 3);
-  if (idx >= total) return 0;
-  const int split = idx / tiles;
-  tile_at(a, idx - split * tiles, tm, tn);
-  return split + 1;
-}
-
 // eight consecutive results (16-bit, and the residual added) from column col on, nv of them inside the row
 template <typename O> __device__ inline void store8(const Fp8GemmArgs& a, int row, int col, int nv, float (&v)[8]) {
   O* o = (O*)a.out + (int64_t)row * a.os + col;
@@ -92,37 +101,52 @@ template <typename O> __device__ inline void store8(const Fp8GemmArgs& a, int ro
 
 // Zero the bytes past column k of a stage that holds the row's last, short
 // block (nv < 128 columns): they are any value, also NaN.
-template <int ROWS, int THREADS> __device__ inline void zero_tail(uint8_t* st, int nv) {
+template <int ROWS, int THREADS> __device__ inline void zero_tail(uint8_t* st, int nv, int tid) {
   const int p0 = nv >> 4, np = 8 - p0;             // pieces from the first short one on
-  for (int i = threadIdx.x; i < ROWS * np; i += THREADS) {
+  for (int i = tid; i < ROWS * np; i += THREADS) {
     const int r = i / np, p = p0 + i - r * np;
     uint4* q = (uint4*)(st + r * 128 + ((p ^ swz(r & 15)) << 4));
     *q = keep_bytes(*q, nv - 16 * p);
   }
 }
 
-// WM x WN waves; SILU: the tile's columns are BN / 2 gate columns and the same up columns
-template <int BM, int BN, int WM, int WN, typename S, typename O, bool SILU, bool SPLIT>
-__global__ __launch_bounds__(64 * WM * WN, BM * BN >= 32768 ? 2 : 1) void fp8_gemm_kernel(const Fp8GemmArgs a) {
-  constexpr int NW = WM * WN, TM = BM / WM, TN = BN / WN;    // wave tile
-  constexpr int MF = TM / 16, NF = TN / 16;
-  constexpr int LOADS = (BM + BN) / 8 / NW;                  // 1 KB loads per wave and stage
-  static_assert(LOADS * 8 * NW == BM + BN && BM % 8 == 0, "whole loads");
-  static_assert(!SILU || NF % 2 == 0, "gate and up halves");
+__device__ inline floatx16 mfma8_32(intx8 a, intx8 b, floatx16 c, int scale_a, int scale_b) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, scale_a, 0, scale_b);
+}
+
+// WM x WN waves of 32 I x 32 J, NST stages; KS such groups of waves take every KS-th block, each with stages of its
+// own, and meet in LDS at the end; SILU: a wave's columns are half gate columns and half the same up columns
+template <int WM, int WN, int I, int J, int KS, int NST, typename S, typename O, bool SILU>
+__global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN * KS + 3) / 4 * (KS * NST * (WM * I + WN * J) * 4096 <= 78000 ? 2 : 1))
+void fp8_gemm_kernel(const Fp8GemmArgs a) {
+  constexpr int NW = WM * WN, TM = 32 * I, TN = 32 * J, BM = WM * TM, BN = WN * TN;
+  constexpr int LOADS = (BM + BN) / 8 / NW, LW = LOADS + 1;  // 1 KB loads (and one of scales) per wave and stage
+  static_assert(LOADS * 8 * NW == BM + BN, "whole loads");
+  static_assert(!SILU || J % 2 == 0, "gate and up halves");
+  static_assert(NST >= 2 && (NST - 2) * LW < 64, "vmcnt");
   constexpr bool EXACT = __is_same(O, float);      // 16-bit instructions (see half_of)
-  constexpr int STAGE = (BM + BN) * 128;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * STAGE];
+  constexpr bool PART = EXACT || !S::pow2;         // a block's sums are scaled afterwards
+  // a stage: rows, then a dword with the scale of each activation row and of two weight blocks
+  constexpr int SLOTS = (BM + 2 + 63) / 64 * 64, ROWS = (BM + BN) * 128, STAGE = ROWS + SLOTS * 4;
+  constexpr int SLW = SLOTS / 64;                  // loads that fill the scales' slots
+  static_assert(SLW <= NW, "one load of scales per wave");
+  __shared__ __attribute__((aligned(16))) uint8_t lds_all[KS * NST * STAGE];
+  static_assert((KS - 1) * NW * I * J * 4096 <= KS * NST * STAGE, "the groups' sums fit");
 
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kg = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / NW;     // group of waves
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) - kg * NW;
   const int wm = wave % WM, wn = wave / WM;
-  const int c = lane & 15, g = lane >> 4;
+  const int c = lane & 31, g = lane >> 5;
+  uint8_t* const lds = lds_all + kg * NST * STAGE;
 
+  // workgroup i runs on XCD i % 8; each XCD takes a contiguous run of tiles
+  const int total = a.tiles_m * a.tiles_n, per = (total + 7) >> 3;
+  const int idx = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (idx >= total) return;
   int tm, tn;
-  const int split = tile_of(a, blockIdx.x, tm, tn) - 1;
-  if (split < 0) return;
+  tile_at(a, idx, tm, tn);
   const int m0 = tm * BM, n0 = tn * (SILU ? BN / 2 : BN);
-  const int kb0 = split * a.kb_per, kb1 = min(a.kb, kb0 + a.kb_per);
 
   // weight row of tile row j (wave-contiguous: wave wn owns rows wn TN ..; with SILU
   // its first half are gate rows, its second half the up rows of the same columns)
@@ -145,144 +169,195 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN >= 32768 ? 2 : 1) void fp8_ge
     const int64_t r = row < BM ? min(m0 + row, a.m - 1) - m0 : min(wrow_of(row - BM), a.n - 1) - n0;
     off[i] = (uint32_t)(r * (row < BM ? a.xs : a.ws));
   }
+  // Scales go the same way, a dword a lane: this wave's load takes slots 64 (wave % SLW) .., which hold the scale
+  // of activation row slot, then of the tile's two weight blocks (the gate and the up rows', or 128 rows each).
+  // (Power-of-two scales are bytes: the aligned dword that holds it is loaded, and the byte taken from it at the end.)
+  typedef typename S::T ST;
+  const int slot0 = (wave % SLW) * 64, slot = slot0 + lane;
+  const bool xslot = slot < BM;
+  auto wblock = [&](int u) { return min(SILU ? n0 + u * a.half : n0 + u * FP8_BLOCK, a.n - 1) >> 7; };
+  const ST* const sptr = xslot ? (const ST*)a.sx + (int64_t)min(m0 + slot, a.m - 1) * a.sxr
+                               : (const ST*)a.sw + (int64_t)wblock(slot == BM + 1) * a.swr;
+  const int64_t sstep = xslot ? a.sxb : a.swb;
   const int last = (a.k - 1) >> 4;
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)lds;
-  auto issue = [&](int stage, int kb) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)lds_all + kg * NST * STAGE;
+  // load number i < LW of a stage for block kb
+  auto issue1 = [&](int stage, int kb, int i) __attribute__((always_inline)) {
+    if (i < LOADS) {
       const int row = (wave * LOADS + i) * 8;      // uniform; the lane's piece of its row is q8 ^ swz(row + rs)
       const int p = min(kb * 8 + (q8 ^ rs ^ ((row >> 3) & 1)), last);
       dma_1k(row < BM ? xbase : wbase, off[i] + (uint32_t)p * 16, lds0 + stage + row * 128);
+    } else {
+      dma_dword((const void*)((uintptr_t)(sptr + kb * sstep) & ~(uintptr_t)3), lds0 + stage + ROWS + slot0 * 4);
+    }
+  };
+  // the scale in slot `s` of a stage, p its address: as the instruction takes it (its byte in a register) or in fp32
+  auto scale_of = [&](const uint8_t* st, int s, const ST* p) __attribute__((always_inline)) {
+    const uint32_t v = *(const uint32_t*)(st + ROWS + s * 4);
+    if constexpr (S::pow2) return (int)(v >> (8 * ((uint32_t)(uintptr_t)p & 3)) & 0xffu);
+    else return __uint_as_float(v);
+  };
+  typedef std::conditional_t<S::pow2, int, float> SR;
+  struct Sc { SR x[I], w[SILU ? 2 : 1]; };
+  const ST* sxp[I];
+#pragma unroll
+  for (int i = 0; i < I; ++i) sxp[i] = (const ST*)a.sx + (int64_t)min(m0 + wm * TM + 32 * i + c, a.m - 1) * a.sxr;
+  auto scales = [&](Sc& sc, const uint8_t* st, int kb) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < I; ++i) sc.x[i] = scale_of(st, wm * TM + 32 * i + c, sxp[i] + kb * a.sxb);
+#pragma unroll
+    for (int u = 0; u < (SILU ? 2 : 1); ++u) {
+      const int v = SILU ? u : wn * TN / FP8_BLOCK;
+      sc.w[u] = scale_of(st, BM + v, (const ST*)a.sw + (int64_t)wblock(v) * a.swr + kb * a.swb);
     }
   };
 
-  // scales: activation row m0 + wm TM + 16 i + c, weight block of the wave's (gate / up) rows
-  typedef typename S::T ST;
-  constexpr int NS = SILU ? 2 : 1;
-  const ST* const sxp = (const ST*)a.sx + (int64_t)m0 * a.sxr;
-  uint32_t sxo[MF];
+  // operand reads: lane (c, g) takes pieces 4 h + 2 g and + 1 of row c
+  const int f = (c & 7) ^ ((c >> 3) & 1);
+  int rd[2][2];
 #pragma unroll
-  for (int i = 0; i < MF; ++i) sxo[i] = (uint32_t)((min(m0 + wm * TM + 16 * i + c, a.m - 1) - m0) * a.sxr);
-  const ST* swp[NS];
+  for (int h = 0; h < 2; ++h)
 #pragma unroll
-  for (int t = 0; t < NS; ++t)
-    swp[t] = (const ST*)a.sw + (int64_t)(min(wrow_of(wn * TN + t * (TN / 2)), a.n - 1) >> 7) * a.swr;
-
-  floatx4 acc[NF][MF];
+    for (int t = 0; t < 2; ++t) rd[h][t] = c * 128 + (((4 * h + 2 * g + t) ^ f) << 4);
+  struct Half { intx8 x[I], w[J]; };
+  auto read = [&](Half& o, const uint8_t* st, int h) __attribute__((always_inline)) {
+    auto get = [&](int row) { return frag8(*(const uint4*)(st + row * 128 + rd[h][0]), *(const uint4*)(st + row * 128 + rd[h][1])); };
 #pragma unroll
-  for (int j = 0; j < NF; ++j)
+    for (int i = 0; i < I; ++i) o.x[i] = get(wm * TM + 32 * i);
 #pragma unroll
-    for (int i = 0; i < MF; ++i) acc[j][i] = floatx4{0.f, 0.f, 0.f, 0.f};
-
-  const int rd0 = c * 128 + ((g ^ swz(c)) << 4);            // piece g of row c; piece g + 4 lies 64 bytes off (xor)
-  struct Sc { ST x[MF], w[NS]; };
-  auto scales = [&](Sc& sc, int kb) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < MF; ++i) sc.x[i] = (sxp + (int64_t)kb * a.sxb)[sxo[i]];
-#pragma unroll
-    for (int t = 0; t < NS; ++t) sc.w[t] = swp[t][(int64_t)kb * a.swb];
+    for (int j = 0; j < J; ++j) o.w[j] = get(BM + wn * TN + 32 * j);
   };
+
+  floatx16 acc[J][I], part[PART ? J : 1][PART ? I : 1];
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+#pragma unroll
+    for (int i = 0; i < I; ++i) acc[j][i] = floatx16{};
+  auto products = [&](const Half& o, const Sc& sc, auto h) __attribute__((always_inline)) {
+    constexpr bool FIRST = decltype(h)::value == 0;
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int i = 0; i < I; ++i) {
+        if constexpr (EXACT) {
+          floatx16 p = FIRST ? floatx16{} : part[j][i];
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            p = __builtin_amdgcn_mfma_f32_32x32x16_f16(half_of(o.w[j], q), half_of(o.x[i], q), p, 0, 0, 0);
+          part[j][i] = p;
+        } else if constexpr (PART) {
+          part[j][i] = mfma8_32(o.w[j], o.x[i], FIRST ? floatx16{} : part[j][i], E8_ONE, E8_ONE);
+        } else {
+          acc[j][i] = mfma8_32(o.w[j], o.x[i], acc[j][i], sc.w[SILU ? j / (J / 2) : 0], sc.x[i]);
+        }
+      }
+  };
+  auto rescale = [&](const Sc& sc) __attribute__((always_inline)) {
+    if constexpr (PART) {
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+          const float s = scale_f32((ST)sc.x[i]) * scale_f32((ST)sc.w[SILU ? j / (J / 2) : 0]);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[j][i][e] = fmaf(part[j][i][e], s, acc[j][i][e]);
+        }
+    }
+  };
+
   // The blocks in the order last, first, second ..: the row's last one may be
-  // short, and what lies behind it is zeroed before the loop starts.
-  const int n = kb1 - kb0;
-  auto block = [&](int t) { return t == 0 || t >= n ? kb1 - 1 : kb0 + t - 1; };
-  Sc sc, sn;
-  issue(0, block(0));
-  scales(sc, block(0));
-  if (kb1 == a.kb && (a.k & (FP8_BLOCK - 1))) {
-    __builtin_amdgcn_s_waitcnt(0x0070);
-    __syncthreads();
-    zero_tail<BM + BN, 64 * NW>(lds, a.k & (FP8_BLOCK - 1));
+  // short, and what lies behind it is zeroed before the loop starts.  Group kg
+  // takes the blocks kg, kg + KS .. of that order, n of them.
+  const int n = (a.kb - kg + KS - 1) / KS, most = (a.kb + KS - 1) / KS;
+  auto block = [&](int t) { return t == 0 && kg == 0 ? a.kb - 1 : kg + KS * t - 1; };
+#pragma unroll 1
+  for (int t = 0; t < min(n, NST); ++t)
+#pragma unroll
+    for (int i = 0; i < LW; ++i) issue1(t * STAGE, block(t), i);
+  wait_stages<NST + 1, LW>(max(0, min(n, NST) - 1));
+  asm volatile("s_barrier" ::: "memory");
+  if (a.k & (FP8_BLOCK - 1)) {
+    if (kg == 0) zero_tail<BM + BN, 64 * NW>(lds, a.k & (FP8_BLOCK - 1), wave * 64 + lane);
+    __builtin_amdgcn_s_waitcnt(0xC07F);            // LDS writes done; the loads in flight are not waited for
+    asm volatile("s_barrier" ::: "memory");
   }
-  int at = 0;
-  for (int t = 0; t < n; ++t, at ^= STAGE) {
-    // this wave's loads of block t (issued a block ago) landed, and its reads of the other stage are done ...
-    __builtin_amdgcn_s_waitcnt(0x0070);
-    asm volatile("s_barrier" ::: "memory");        // ... and everyone's
-    issue(at ^ STAGE, block(t + 1));               // (after the last block: one of them again, for nobody)
-    scales(sn, block(t + 1));
-    const uint8_t* const cur = lds + at;
-    auto frag = [&](int row16) __attribute__((always_inline)) {
-      const uint8_t* p = cur + row16 * 128;
-      return frag8(*(const uint4*)(p + rd0), *(const uint4*)(p + (rd0 ^ 64)));
-    };
-    intx8 xf[MF];
+  const std::integral_constant<int, 0> first{};
+  const std::integral_constant<int, 1> second{};
+  Half h0, h1;
+  Sc sc, sn;
+  read(h0, lds, 0);
+  scales(sc, lds, block(0));
+  int cur = 0;
+  for (int t = 0; t < n; ++t) {                    // block(t) in stage `cur`, its half 0 in h0, its scales in sc
+    read(h1, lds + cur, 1);
+    products(h0, sc, first);
+    __builtin_amdgcn_sched_barrier(0);
+    // half 1 read; this wave's part of the next stage landed (those of up to NST - 2 more may be on their way)
+    wait_stages<NST, LW>(max(0, min(n - 2 - t, NST - 2)));
+    asm volatile("s_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    const int nxt = cur == (NST - 1) * STAGE ? 0 : cur + STAGE;
+    // (behind the last block: reads of what is there, for nobody)
+    read(h0, lds + nxt, 0);
+    scales(sn, lds + nxt, block(t + 1));
+    if (t + NST < n) {
 #pragma unroll
-    for (int i = 0; i < MF; ++i) xf[i] = frag(wm * TM + 16 * i);
-    if constexpr (EXACT) {
-      intx8 wf[NF];
-      floatx4 p[NF][MF];
+      for (int i = 0; i < LW; ++i) issue1(cur, block(t + NST), i);
+    }
+    products(h1, sc, second);
+    rescale(sc);
+    sc = sn;
+    cur = nxt;
+  }
+  if constexpr (KS > 1) {
+    if (n < most) asm volatile("s_barrier" ::: "memory");      // as many as the other groups' loops
+    // the groups' sums, in group order
+    __syncthreads();
+    floatx4* const red = (floatx4*)lds_all;        // [group - 1][wave][j][i][q][lane]
+    if (kg > 0) {
 #pragma unroll
-      for (int j = 0; j < NF; ++j) wf[j] = frag(BM + wn * TN + 16 * j);
+      for (int j = 0; j < J; ++j)
 #pragma unroll
-      for (int j = 0; j < NF; ++j)
+        for (int i = 0; i < I; ++i)
 #pragma unroll
-        for (int i = 0; i < MF; ++i) p[j][i] = floatx4{0.f, 0.f, 0.f, 0.f};
+          for (int q = 0; q < 4; ++q)
+            red[(((((kg - 1) * NW + wave) * J + j) * I + i) * 4 + q) * 64 + lane] =
+                floatx4{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
+    }
+    __syncthreads();
+    if (kg > 0) return;
+#pragma unroll
+    for (int v = 0; v < KS - 1; ++v)
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const floatx4 t = red[((((v * NW + wave) * J + j) * I + i) * 4 + q) * 64 + lane];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[j][i][4 * q + e] += t[e];
+          }
+  }
+
+  // lane (c, g): columns 32 j + 8 q + 4 g .. + 3 of row 32 i + c of the wave's tile
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+    const int row = m0 + wm * TM + 32 * i + c;
+    if (row >= a.m) continue;
+    const float r = a.rscale ? a.rscale[row] : 1.f;
+#pragma unroll
+    for (int j = 0; j < (SILU ? J / 2 : J); ++j)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        half8 wh[NF], xh[MF];
-#pragma unroll
-        for (int j = 0; j < NF; ++j) wh[j] = half_of(wf[j], q);
-#pragma unroll
-        for (int i = 0; i < MF; ++i) xh[i] = half_of(xf[i], q);
-#pragma unroll
-        for (int j = 0; j < NF; ++j)
-#pragma unroll
-          for (int i = 0; i < MF; ++i) p[j][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[j], xh[i], p[j][i], 0, 0, 0);
-      }
-#pragma unroll
-      for (int i = 0; i < MF; ++i)
-#pragma unroll
-        for (int j = 0; j < NF; ++j) {
-          const float s = scale_f32(sc.x[i]) * scale_f32(sc.w[SILU ? j / (NF / 2) : 0]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[j][i][e] = fmaf(p[j][i][e], s, acc[j][i][e]);
-        }
-    } else {
-#pragma unroll
-      for (int j = 0; j < NF; ++j) {
-        const intx8 wf = frag(BM + wn * TN + 16 * j);
-        const ST sw = sc.w[SILU ? j / (NF / 2) : 0];
-#pragma unroll
-        for (int i = 0; i < MF; ++i) {
-          if constexpr (S::pow2) {
-            acc[j][i] = mfma8(wf, xf[i], acc[j][i], sw, sc.x[i]);
-          } else {
-            const float s = sc.x[i] * sw;
-            const floatx4 p = mfma8(wf, xf[i], floatx4{0.f, 0.f, 0.f, 0.f}, E8_ONE, E8_ONE);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[j][i][e] = fmaf(p[e], s, acc[j][i][e]);
-          }
-        }
-      }
-    }
-    sc = sn;
-  }
-  __builtin_amdgcn_s_waitcnt(0x0070);              // the last loads, before the workgroup gives up its LDS
-
-  // lane (c, g): columns 16 j + 4 g .. + 3 of row 16 i + c of the wave's tile
-#pragma unroll
-  for (int i = 0; i < MF; ++i) {
-    const int row = m0 + wm * TM + 16 * i + c;
-    if (row >= a.m) continue;
-    const float r = !SPLIT && a.rscale ? a.rscale[row] : 1.f;
-#pragma unroll
-    for (int j = 0; j < (SILU && !SPLIT ? NF / 2 : NF); ++j) {
-      float v[4];
-      if constexpr (SPLIT) {
-        const int col = wrow_of(wn * TN + 16 * j) + 4 * g, nv = a.n - col;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[j][i][e];
-        // the row pitch of the partial sums is a whole number of 4 columns
-        const int np = (a.n + 3) & ~3;
-        if (nv > 0) *(float4*)(a.part + ((int64_t)split * a.m + row) * np + col) = make_float4(v[0], v[1], v[2], v[3]);
-      } else {
-        const int col = (SILU ? n0 + wn * (TN / 2) + 16 * j : n0 + wn * TN + 16 * j) + 4 * g;
+        const int col = n0 + wn * (SILU ? TN / 2 : TN) + 32 * j + 8 * q + 4 * g;
         const int nv = (SILU ? a.half : a.n) - col;
         if (nv <= 0) continue;
+        float v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          v[e] = SILU ? silu_mul_f32(r * acc[j][i][e], r * acc[SILU ? j + NF / 2 : j][i][e]) : r * acc[j][i][e];
+          v[e] = SILU ? silu_mul_f32(r * acc[j][i][4 * q + e], r * acc[SILU ? j + J / 2 : j][i][4 * q + e])
+                      : r * acc[j][i][4 * q + e];
         if (!SILU && a.res) {
           float t[4];
           load4<O>((const O*)a.res + (int64_t)row * a.rs + col, t, nv, a.vec_out != 0);
@@ -291,7 +366,6 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN >= 32768 ? 2 : 1) void fp8_ge
         }
         store4<O>((O*)a.out + (int64_t)row * a.os + col, v, nv, a.vec_out != 0);
       }
-    }
   }
 }
 
@@ -317,10 +391,6 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN >= 32768 ? 2 : 1) void fp8_ge
 constexpr int WT = 256;                            // tile rows and columns
 constexpr int WSTAGE = 2 * WT * 128;               // bytes of a stage
 constexpr int WOUT = 32 * 64 * 4;                  // bytes a wave stages of its results: 32 rows x 64 columns, fp32
-
-__device__ inline floatx16 mfma8_32(intx8 a, intx8 b, floatx16 c, int scale_a, int scale_b) {
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, scale_a, 0, scale_b);
-}
 
 template <typename O, bool SILU>
 __global__ __launch_bounds__(256, 1) void fp8_gemm_wide_kernel(const Fp8GemmArgs a) {
@@ -424,7 +494,7 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_wide_kernel(const Fp8GemmArgs
     __builtin_amdgcn_s_waitcnt(0x0070);
     asm volatile("s_barrier" ::: "memory");
     if (a.k & (FP8_BLOCK - 1)) {
-      zero_tail<2 * WT, 256>(lds, a.k & (FP8_BLOCK - 1));
+      zero_tail<2 * WT, 256>(lds, a.k & (FP8_BLOCK - 1), threadIdx.x);
       __syncthreads();
     }
 #pragma unroll
@@ -534,69 +604,51 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_wide_kernel(const Fp8GemmArgs
   }
 }
 
-// out = epilogue of the splits' partial sums, added in split order
-template <typename O, bool SILU> __global__ __launch_bounds__(256) void fp8_join_kernel(const Fp8GemmArgs a) {
-  const int np = (a.n + 3) & ~3, cols = SILU ? a.half : a.n;
-  const int c4 = (cols + 3) >> 2;
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (id >= (int64_t)a.m * c4) return;
-  const int64_t row = id / c4;
-  const int col = (int)(id - row * c4) * 4;
-  float4 s = make_float4(0.f, 0.f, 0.f, 0.f), u = s;
-  for (int z = 0; z < a.splits; ++z) {
-    const float* p = a.part + ((int64_t)z * a.m + row) * np + col;
-    const float4 t = *(const float4*)p;
-    s.x += t.x; s.y += t.y; s.z += t.z; s.w += t.w;
-    if constexpr (SILU) {
-      const float4 t2 = *(const float4*)(p + a.half);
-      u.x += t2.x; u.y += t2.y; u.z += t2.z; u.w += t2.w;
-    }
-  }
-  const float r = a.rscale ? a.rscale[row] : 1.f;
-  float v[4] = {r * s.x, r * s.y, r * s.z, r * s.w};
-  if constexpr (SILU) {
-    const float w[4] = {r * u.x, r * u.y, r * u.z, r * u.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = silu_mul_f32(v[e], w[e]);
-  }
-  const int nv = cols - col;
-  if (!SILU && a.res) {
-    float t[4];
-    load4<O>((const O*)a.res + row * a.rs + col, t, nv, a.vec_out != 0);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] += t[e];
-  }
-  store4<O>((O*)a.out + row * a.os + col, v, nv, a.vec_out != 0);
-}
-
-Fp8Plan plan_fp8_gemm(int m, int n, int kb, bool exact, int cus) {
+// Which kernel and tile, by modelled time: rounds of resident workgroups times
+// the k blocks times what a block takes with one and with two workgroups on a
+// CU (microseconds, measured at n 4096 and 7376, k 1640 to 11008, 8 to 8192
+// rows: the model picks the fastest of them within 10 %).  Small tiles fill
+// the chip with few rows; large ones read less per product.
+//   few rows  16 weight rows a workgroup, no LDS (m <= 16; to 32 rows while a
+//             second group of rows costs less than the tiles' fixed 4 us:
+//             n 4096, k 4096: 9.2 against 9.7 us; k 11008: 18.2 against 17.4)
+//   64 x 32   4 k groups of waves, one workgroup a CU; 2 k groups, two
+//   64 x 64   2 k groups      64 x 128, 128 x 128   one
+//   256 x 256 power-of-two scales and 16-bit outputs
+Fp8Plan plan_fp8_gemm(int m, int n, int kb, bool silu, bool exact, bool pow2, int cus) {
   Fp8Plan p = {};
   p.cus = cus;
-  const bool big = !exact && (int64_t)ceil_div(m, 256) * ceil_div(n, 256) >= cus;
-  p.bm = big ? 256 : m <= 64 ? 64 : 128;
-  p.bn = big ? 256 : 128;
-  const int64_t tiles = ceil_div(m, p.bm) * ceil_div(n, p.bn);
-  int splits = 1;
-  while (splits < 16 && tiles * splits * 2 <= 2 * cus && kb / (splits * 2) >= 4) splits *= 2;
-  p.kb_per = (int)ceil_div(kb, splits);
-  p.splits = (int)ceil_div(kb, p.kb_per);
-  p.part_bytes = p.splits > 1 ? (size_t)p.splits * m * (size_t)round_up(n, 4) * 4 : 0;
+  if (m <= 16 || (m <= 32 && (int64_t)n * kb <= 131072)) {
+    p.few = true;
+    p.bm = m <= 16 ? 16 : 32;
+    p.bn = silu ? 32 : 16;
+    return p;
+  }
+  struct Shape { int bm, bn; float one, two, fixed; };
+  static const Shape shapes[] = {{64, 32, 0.20f, 0.30f, 0.f}, {64, 64, 0.37f, 0.45f, 0.f}, {64, 128, 0.52f, 0.80f, 0.f},
+                                 {128, 128, 0.75f, 1.25f, 0.f}, {256, 256, 1.45f, 2.90f, 12.f}};
+  float best = 0.f;
+  for (const Shape& h : shapes) {
+    if ((h.bn == 32 && silu) || (h.bm == 256 && (exact || !pow2))) continue;
+    const int64_t tiles = ceil_div(m, h.bm) * ceil_div(n, h.bn), pairs = tiles / (2 * cus), rest = tiles - pairs * 2 * cus;
+    const float rest_t = rest == 0 ? 0.f : rest <= cus ? h.one : h.two;
+    const float t = kb * (pairs * h.two + rest_t) + h.fixed * (float)ceil_div(tiles, cus);
+    if (p.bm == 0 || t < best) {
+      best = t;
+      p.bm = h.bm;
+      p.bn = h.bn;
+      p.ks = h.bm == 64 && h.bn == 32 && tiles <= cus ? 4 : 2;
+    }
+  }
   return p;
 }
 
-template <int BM, int BN, int WM, int WN, typename S, typename O, bool SILU>
+template <int WM, int WN, int I, int J, int KS, int NST, typename S, typename O, bool SILU>
 static int launch_tile(Fp8GemmArgs a, hipStream_t st) {
-  a.tiles_m = (int)ceil_div(a.m, BM);
-  a.tiles_n = (int)ceil_div(a.n, BN);
-  const int64_t total = (int64_t)a.tiles_m * a.tiles_n * a.splits;
-  const dim3 grid((unsigned)(8 * ceil_div(total, 8))), block(64 * WM * WN);
-  if (a.splits > 1) {
-    hipLaunchKernelGGL((fp8_gemm_kernel<BM, BN, WM, WN, S, O, SILU, true>), grid, block, 0, st, a);
-    const int64_t ids = (int64_t)a.m * ceil_div(SILU ? a.half : a.n, 4);
-    hipLaunchKernelGGL((fp8_join_kernel<O, SILU>), dim3((unsigned)ceil_div(ids, 256)), dim3(256), 0, st, a);
-  } else {
-    hipLaunchKernelGGL((fp8_gemm_kernel<BM, BN, WM, WN, S, O, SILU, false>), grid, block, 0, st, a);
-  }
+  a.tiles_m = (int)ceil_div(a.m, 32 * WM * I);
+  a.tiles_n = (int)ceil_div(a.n, 32 * WN * J);
+  const dim3 grid((unsigned)(8 * ceil_div((int64_t)a.tiles_m * a.tiles_n, 8))), block(64 * WM * WN * KS);
+  hipLaunchKernelGGL((fp8_gemm_kernel<WM, WN, I, J, KS, NST, S, O, SILU>), grid, block, 0, st, a);
   return (int)hipGetLastError();
 }
 template <typename O, bool SILU> static int launch_wide(Fp8GemmArgs a, int cus, hipStream_t st) {
@@ -608,13 +660,13 @@ template <typename O, bool SILU> static int launch_wide(Fp8GemmArgs a, int cus, 
   return (int)hipGetLastError();
 }
 template <typename S, typename O, bool SILU> static int launch_shape(const Fp8GemmArgs& a, const Fp8Plan& p, hipStream_t st) {
-  if constexpr (!__is_same(O, float))
-    if (p.bm == 256) {
-      if constexpr (S::pow2) return launch_wide<O, SILU>(a, p.cus, st);
-      else return launch_tile<256, 256, 4, 2, S, O, SILU>(a, st);
-    }
-  if (p.bm == 128) return launch_tile<128, 128, 2, 2, S, O, SILU>(a, st);
-  return launch_tile<64, 128, 1, 4, S, O, SILU>(a, st);
+  if constexpr (!__is_same(O, float) && S::pow2)
+    if (p.bm == 256) return launch_wide<O, SILU>(a, p.cus, st);
+  if (p.bm == 128) return launch_tile<2, 2, 2, 2, 1, 2, S, O, SILU>(a, st);
+  if (p.bn == 128) return launch_tile<2, 2, 1, 2, 1, 3, S, O, SILU>(a, st);
+  if constexpr (!SILU)
+    if (p.bn == 32) return p.ks == 4 ? launch_tile<2, 1, 1, 1, 4, 3, S, O, SILU>(a, st) : launch_tile<2, 1, 1, 1, 2, 3, S, O, SILU>(a, st);
+  return launch_tile<2, 1, 1, 2, 2, 2, S, O, SILU>(a, st);
 }
 template <typename S, typename O> static int launch_silu(const Fp8GemmArgs& a, const Fp8Plan& p, bool silu, hipStream_t st) {
   return silu ? launch_shape<S, O, true>(a, p, st) : launch_shape<S, O, false>(a, p, st);
@@ -624,10 +676,7 @@ template <typename S> static int launch_out(const Fp8GemmArgs& a, const Fp8Plan&
   if (od == STARKV_BF16) return launch_silu<S, __bf16>(a, p, silu, st);
   return launch_silu<S, float>(a, p, silu, st);
 }
-int launch_fp8_gemm(const Fp8GemmArgs& a0, const Fp8Plan& p, int out_dtype, int scale_dtype, bool silu, hipStream_t st) {
-  Fp8GemmArgs a = a0;
-  a.splits = p.splits;
-  a.kb_per = p.kb_per;
+int launch_fp8_gemm(const Fp8GemmArgs& a, const Fp8Plan& p, int out_dtype, int scale_dtype, bool silu, hipStream_t st) {
   return scale_dtype == STARKV_E8M0 ? launch_out<ScaleE8>(a, p, out_dtype, silu, st)
                                     : launch_out<ScaleF32>(a, p, out_dtype, silu, st);
 }

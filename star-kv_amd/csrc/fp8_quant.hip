@@ -31,7 +31,7 @@ __device__ inline void quant_block(const Fp8QuantArgs& a, int64_t row, int kb, i
   for (int o = 1; o < 8; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
   float inv;
   const typename S::T s = block_scale<S>(mag_bits<T>(m), inv);
-  uint4 q = quant16<T>(w, inv);
+  uint4 q = quant16<T, S>(w, inv, scale_f32(s));
   if (c0 + 16 > a.k) q = keep_bytes(q, a.k - c0);   // the row's padding is zero, also where the scale is NaN
   if (c0 < a.k) *(uint4*)(a.q + row * a.qs + c0) = q;
   if (sub == 0) ((typename S::T*)a.s)[row * a.ssr + kb * a.ssb] = s;

@@ -23,7 +23,6 @@ __all__ = ["fp8_quantize", "fp8_quantize_weight", "fp8_matmul", "fp8_linear"]
 
 BLOCK = 128
 E4M3_MAX = 448.0
-FEW_ROWS = 16                        # STARKV_FP8_FEW_ROWS
 _ACT = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 _OUT = {**_ACT, torch.float32: _lib.F32}
 _SCALE = {torch.float8_e8m0fnu: _lib.E8M0, torch.float32: _lib.F32}
@@ -184,7 +183,7 @@ def _product(name, x, x_scale, weight, weight_scale, residual, silu_mul, rms_eps
     d = Fp8GemmDesc(m, n, k, xd, od, xr.data_ptr(), xs, xp, xsr, xsb, wr.data_ptr(), ws, weight_scale.data_ptr(),
                     weight_scale.stride(0), weight_scale.stride(1), sd, rp, rs, 1 if silu_mul else 0,
                     0 if rms_eps is None else 1, rms_eps or 0.0, orr.data_ptr(), os_)
-    _launch("starkv_fp8_gemm", d, dev, workspace=m > FEW_ROWS)
+    _launch("starkv_fp8_gemm", d, dev, workspace=True)
     return out
 
 
@@ -209,8 +208,7 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor
                residual: Optional[torch.Tensor] = None, silu_mul: bool = False, rms_eps: Optional[float] = None,
                out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``fp8_matmul`` of fp16 / bf16 activations x [..., k], quantised on the
-    way as ``fp8_quantize(x, weight_scale.dtype)`` would (at most 16 rows: in
-    the one launch that streams the weight).  ``rms_eps``: x is the raw input
+    way as ``fp8_quantize(x, weight_scale.dtype)`` would.  ``rms_eps``: x is the raw input
     of an RMSNorm whose weight is folded into ``weight``
     (``fp8_quantize_weight(w, norm_weight=...)``); each row of the product is
     scaled by rsqrt(mean(x^2) + rms_eps).  The result has x's type unless

@@ -26,12 +26,11 @@ def test_struct_layouts_match_the_c_compiler(tmp_path):
                    for c, py in _STRUCTS.items())
     src = tmp_path / "layout.c"
     src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "starkv.h"\nint main(void) {' + body
-                   + 'printf("codes e4m3 %d\\ncodes e8m0 %d\\ncodes few %d\\ncodes top %d\\n", STARKV_E4M3, STARKV_E8M0, '
-                     'STARKV_FP8_FEW_ROWS, STARKV_MAX_TOP); return 0; }')
+                   + 'printf("codes e4m3 %d\\ncodes e8m0 %d\\ncodes top %d\\n", STARKV_E4M3, STARKV_E8M0, STARKV_MAX_TOP); return 0; }')
     exe = tmp_path / "layout"
     subprocess.run(["gcc", "-std=c99", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
-    from starkv import fp8, logprobs
-    codes = {"e4m3": L.E4M3, "e8m0": L.E8M0, "few": fp8.FEW_ROWS, "top": logprobs.MAX_TOP}
+    from starkv import logprobs
+    codes = {"e4m3": L.E4M3, "e8m0": L.E8M0, "top": logprobs.MAX_TOP}
     for line in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines():
         c, f, v = line.split()
         got = codes[f] if c == "codes" else ctypes.sizeof(_STRUCTS[c]) if f == "sizeof" else getattr(_STRUCTS[c], f).offset
@@ -75,7 +74,7 @@ def _gemm(**kw):
     (dict(rms=1, rms_eps=-1.0), SHAPE), (dict(rms=1, rms_eps=float("nan")), SHAPE),
     (dict(rms=1, dtype=L.E4M3, x_stride=1008, x_scale=FAKE), SHAPE), (dict(w_scale_stride_r=-1), SHAPE),
     (dict(dtype=L.E4M3, x_scale=FAKE, x_stride=1000), ALIGN), (dict(scale_dtype=L.F32, w_scale=FAKE + 2), ALIGN),
-    (dict(m=100), WORKSPACE), (dict(m=1 << 30, n=1 << 30), LIMIT), (dict(m=0, x=None), OK),
+    (dict(m=100), WORKSPACE), (dict(), WORKSPACE), (dict(m=1 << 30, n=1 << 30, dtype=L.E4M3, x_stride=1008, x_scale=FAKE), LIMIT), (dict(m=0, x=None), OK),
 ])
 def test_gemm_refuses(kw, code):
     assert L.lib().starkv_fp8_gemm(ctypes.byref(_gemm(**kw)), None, 0, None) == code
@@ -83,9 +82,9 @@ def test_gemm_refuses(kw, code):
 
 def test_gemm_workspace():
     size = lambda **kw: L.lib().starkv_fp8_gemm_workspace_bytes(ctypes.byref(_gemm(**kw)))
-    assert size() == 0 and size(m=16) == 0 and size(m=0) == 0 and size(k=0) == 0
+    assert size(m=0) == 0 and size(k=0) == 0 and size(dtype=L.E4M3) == 0 and size(dtype=L.E4M3, m=16) == 0
     # quantised rows, their scales, and partial sums where k is split
-    assert size(m=17) >= 17 * 1008 + 17 * 8
+    assert size(m=17) >= 17 * 1008 + 17 * 8 and size(m=3) >= 3 * 1008 + 3 * 8
     assert size(m=8192, n=22016) >= 8192 * 1008
     assert L.lib().starkv_fp8_gemm(ctypes.byref(_gemm(m=17)), FAKE, size(m=17) - 1, None) == WORKSPACE
     assert L.lib().starkv_fp8_gemm(ctypes.byref(_gemm(m=17)), FAKE + 64, size(m=17), None) == ALIGN

@@ -5,21 +5,26 @@
 //   logprob(t) = x_t - m - ln Z,   entropy = ln Z - S / Z
 //
 // (both terms of the entropy are >= 0: nothing cancels).  Every thread keeps
-// its own m, Z and S over 16-byte pieces of the row; a larger maximum rescales
-// them, which soon gets rare.  exp2 underflows to 0 at -inf, where S takes a
-// clamped difference instead of 0 * inf.
+// its own m, Z and S over 16-byte pieces of the row, in units of log 2: with
+// c = log2 e and M = fl(m c), y = fma(x, c, -M) and 2^y replace x - m and
+// e^(x - m), S sums 2^y y.  The rounding of M is the same for all terms and is
+// taken back once (ln Z - (m c - M) ln 2).  y stops at -150, where 2^y is 0,
+// so that -inf adds 0 and not 0 * inf.  A larger maximum rescales the sums,
+// which soon gets rare.  That leaves nine and a half issue slots an element,
+// four of them the exponential: 16-bit logits are bound by those nearly as
+// much as by HBM.  Rows whose maximum is beyond +-1e30 (where x c may
+// overflow) are summed again with x - m formed first.
 //
 // Top alternatives: keys are (logit, lowest index first) as one 64-bit number
-// in a total order.  Each thread knows its greatest key from the pass.  With
-// NW waves, the ceil(top / NW)-th greatest thread key of every wave is taken,
-// and the least of those is a bound that at least `top` elements reach; only
-// threads at or above it read their pieces again and gather the elements
-// there, a few dozen as a rule.  The gathered keys are then ranked.  Where
-// more elements than the buffer holds reach the bound (rows built so), the
-// row is searched `top` times instead.
+// in a total order.  Each thread knows the piece of its greatest key from the
+// pass.  With NW waves, the ceil(top / NW)-th greatest thread key of every
+// wave is taken, and the least of those is a bound that at least `top`
+// elements reach; only threads at or above it read their pieces again and
+// gather the elements there, a few dozen as a rule.  The gathered keys are then
+// ranked.  Where more elements than the buffer holds reach the bound (rows
+// built so), the row is searched `top` times instead.
 //
-// Bound by HBM on many rows (16-bit logits: nearly as much by the exponential
-// of every element).
+// Few rows are split over workgroups, and a second launch joins the pieces.
 #include <algorithm>
 
 #include "common.hpp"
@@ -28,9 +33,11 @@ namespace starkv {
 
 namespace {
 
-constexpr float LOWEST = -3.402823466e38f;
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr float FAR = -1000.f;                     // e^FAR is 0 in fp32
+constexpr int LP_NT = 256;                         // threads per workgroup
+constexpr int LP_MAX_PIECES = 16;                  // of a row
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float START = -1e30f, HUGE_X = 1e30f;    // maxima in between take the fast sums
+constexpr float FAR = -150.f;                      // 2^FAR is 0 in fp32
 
 // logits ordered as unsigned integers: -0 = +0, a NaN above everything
 __device__ inline uint32_t order32(float f) {
@@ -44,26 +51,50 @@ __device__ inline float unorder32(uint32_t k) {
 }
 __device__ inline uint64_t make_key(float f, uint32_t idx) { return ((uint64_t)order32(f) << 32) | (uint32_t)~idx; }
 
+// Sums over some elements: z = sum 2^y, s = sum 2^y y with y = x log2 e - fl(m log2 e)
 struct Stat { float m, z, s; };
-__device__ inline float exp_diff(float d) { return __builtin_amdgcn_exp2f(d * LOG2E); }
-// both over the larger maximum (empty sides: m = LOWEST, z = s = 0)
-__device__ inline Stat merge(const Stat& a, const Stat& b) {
-  const float m = fmaxf(a.m, b.m);
-  const float da = fmaxf(a.m - m, FAR), db = fmaxf(b.m - m, FAR);
-  const float fa = exp_diff(da), fb = exp_diff(db);
-  return {m, a.z * fa + b.z * fb, fa * (a.s + a.z * da) + fb * (b.s + b.z * db)};
+// (rounded, wherever it is used: a product fused into a difference would leave what the rounding took)
+__device__ inline float log2_of(float m) {
+#pragma clang fp contract(off)
+  return m * LOG2E;
 }
-__device__ inline uint64_t shfl_xor64(uint64_t v, int o) {
-  const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)v, o, 64), hi = (uint32_t)__shfl_xor((int)(uint32_t)(v >> 32), o, 64);
-  return ((uint64_t)hi << 32) | lo;
+// the sums z, s of maximum `from` over the maximum `to` >= from instead
+__device__ inline void rebase(Stat& a, float to) {
+  const float d = fmaxf(log2_of(a.m) - log2_of(to), FAR), f = __builtin_amdgcn_exp2f(d);
+  a.s = f * fmaf(a.z, d, a.s);
+  a.z *= f;
+  a.m = to;
+}
+
+// wave reductions by lane shifts inside rows of 16 and broadcasts between them; lane 63 ends with the result
+template <int CTRL, int ROWS, typename F> __device__ inline uint32_t dpp_step(uint32_t v, uint32_t id, F f) {
+  return f(v, (uint32_t)__builtin_amdgcn_update_dpp((int)id, (int)v, CTRL, ROWS, 0xf, false));
+}
+template <typename F> __device__ inline uint32_t wave_reduce(uint32_t v, uint32_t id, F f) {
+  v = dpp_step<0x111, 0xf>(v, id, f);
+  v = dpp_step<0x112, 0xf>(v, id, f);
+  v = dpp_step<0x114, 0xf>(v, id, f);
+  v = dpp_step<0x118, 0xf>(v, id, f);
+  v = dpp_step<0x142, 0xa>(v, id, f);
+  v = dpp_step<0x143, 0xc>(v, id, f);
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ inline uint32_t wave_max32(uint32_t v) {
+  return wave_reduce(v, 0u, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+}
+__device__ inline float wave_maxf(float v) {
+  return __uint_as_float(wave_reduce(__float_as_uint(v), 0xff800000u, [](uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }));
+}
+__device__ inline float wave_sumf(float v) {
+  return __uint_as_float(wave_reduce(__float_as_uint(v), 0u, [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
 }
 __device__ inline uint64_t wave_max64(uint64_t v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    const uint64_t t = shfl_xor64(v, o);
-    v = t > v ? t : v;
-  }
-  return v;
+  const uint32_t hi = (uint32_t)(v >> 32), top = wave_max32(hi);
+  return ((uint64_t)top << 32) | wave_max32(hi == top ? (uint32_t)v : 0u);
 }
 
 template <typename T> struct Piece;                // 16 bytes of logits
@@ -95,14 +126,29 @@ template <> struct Piece<__bf16> {
 
 }  // namespace
 
-// NT threads per workgroup; TOP: alternatives are asked for
-template <typename T, int NT, bool TOP>
-__global__ __launch_bounds__(NT) void logprobs_kernel(const LogprobArgs a) {
-  constexpr int N = Piece<T>::N, NW = NT / 64;
+// the results of a row with the sums st: its token's log probability, its entropy
+template <typename T> __device__ inline float finish_row(const LogprobArgs& a, int64_t row, const Stat& st, bool nan, bool write) {
+  const float none = __uint_as_float(0x7fc00000u);
+  const float eps = fmaf(st.m, LOG2E, -log2_of(st.m));       // what fl(m log2 e) is short of m log2 e
+  const float lnz = nan ? none : logf(st.z) - (fabsf(st.m) < HUGE_X ? eps * LN2 : 0.f);
+  if (write) {
+    if (a.tok) {
+      const int64_t t = a.tok[row];
+      a.lp[row] = t >= 0 && t < a.vocab ? ((float)((const T*)a.x)[row * a.xs + t] - st.m) - lnz : none;
+    }
+    if (a.ent) a.ent[row] = nan ? none : logf(st.z) - LN2 * (st.s / st.z);
+  }
+  return lnz;
+}
+
+// TOP: alternatives are asked for
+template <typename T, bool TOP> __global__ __launch_bounds__(LP_NT) void logprobs_kernel(const LogprobArgs a) {
+  constexpr int NT = LP_NT, N = Piece<T>::N, NW = NT / 64;
   constexpr int CAP = TOP ? NT * N + 64 : 1;       // one piece of every thread fits
   __shared__ uint64_t buf[CAP];
   __shared__ uint64_t wkey[NW];
   __shared__ Stat wstat[NW];
+  __shared__ int wnan[NW];
   __shared__ int count;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x / a.pieces;
@@ -116,71 +162,79 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LogprobArgs a) {
   const int head = min(hi - lo, mis ? N - mis : 0);
   const int body = (hi - lo - head) / N, tail0 = lo + head + body * N;
   const T* xb = x + lo + head;
+  // f(value, index) of this thread's single elements and of its pieces' p
   auto each_head = [&](auto f) {
     if (tid < head) f((float)x[lo + tid], lo + tid);
   };
   auto each_tail = [&](auto f) {
     if (tid < N && tail0 + tid < hi) f((float)x[tail0 + tid], tail0 + tid);
   };
+  auto of_piece = [&](int p, auto f) {
+    float v[N];
+    Piece<T>::get(*(const uint4*)(xb + (int64_t)p * N), v);
+#pragma unroll
+    for (int e = 0; e < N; ++e) f(v[e], lo + head + p * N + e);
+  };
+  auto each = [&](auto f) {
+    each_head(f);
+#pragma unroll 1
+    for (int p = tid; p < body; p += NT) of_piece(p, f);
+    each_tail(f);
+  };
 
-  Stat st = {LOWEST, 0.f, 0.f};
-  uint64_t best = 0;                               // this thread's greatest key
-  auto raise = [&](float cm) {
-    const float d = fmaxf(st.m - cm, FAR), f = exp_diff(d);
-    st.s = f * (st.s + st.z * d);
-    st.z *= f;
-    st.m = cm;
+  constexpr int AT_NONE = -1, AT_HEAD = -2, AT_TAIL = -3;
+  Stat st = {START, 0.f, 0.f};
+  float ml = log2_of(START);
+  bool nan = false;
+  int at = AT_NONE;                                // where this thread's greatest key is; of equal ones the first met
+  auto raise = [&](float cm, int where) {
+    if (nan) return;
+    at = where;
+    nan = cm != cm;
+    if (!nan) {
+      rebase(st, cm);
+      ml = log2_of(cm);
+    }
   };
   auto add = [&](float v) {
-    const float d = v - st.m, e = exp_diff(d);
+    const float y = fmaxf(fmaf(v, LOG2E, -ml), FAR), e = __builtin_amdgcn_exp2f(y);
     st.z += e;
-    st.s = fmaf(e, fmaxf(d, FAR), st.s);
+    st.s = fmaf(e, y, st.s);
   };
-  auto single = [&](float v, int i) {
-    if (v > st.m) raise(v);
+  each_head([&](float v, int) {
+    if (!(v <= st.m)) raise(v, AT_HEAD);
     add(v);
-    if constexpr (TOP) {
+  });
+#pragma unroll 2
+  for (int p = tid; p < body; p += NT) {
+    float v[N];
+    Piece<T>::get(*(const uint4*)(xb + (int64_t)p * N), v);
+    float cm = v[0];                               // a NaN stays in it
+#pragma unroll
+    for (int e = 1; e < N; ++e) cm = __builtin_elementwise_maximum(cm, v[e]);
+    if (!(cm <= st.m)) raise(cm, p);
+#pragma unroll
+    for (int e = 0; e < N; ++e) add(v[e]);
+  }
+  each_tail([&](float v, int) {
+    if (!(v <= st.m)) raise(v, AT_TAIL);
+    add(v);
+  });
+
+  uint64_t best = 0;                               // this thread's greatest key
+  if constexpr (TOP) {
+    auto better = [&](float v, int i) {
       const uint64_t k = make_key(v, i);
       best = k > best ? k : best;
-    }
-  };
-  // in the order of their indices: of equal logits the first one met is the greatest key
-  each_head(single);
-  for (int p = tid; p < body; p += NT) {
-    float f[N];
-    Piece<T>::get(*(const uint4*)(xb + (int64_t)p * N), f);
-    float cm = f[0];
-#pragma unroll
-    for (int e = 1; e < N; ++e) cm = fmaxf(cm, f[e]);
-    if (cm > st.m) raise(cm);
-    if constexpr (TOP) {
-      // fmaxf passes over a NaN; the sum below does not
-      bool nan = false;
-#pragma unroll
-      for (int e = 0; e < N; ++e) nan |= f[e] != f[e];
-      if (nan || order32(cm) > (uint32_t)(best >> 32)) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const uint64_t k = make_key(f[e], lo + head + p * N + e);
-          best = k > best ? k : best;
-        }
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < N; ++e) add(f[e]);
-  }
-  each_tail(single);
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    const Stat t = {__shfl_xor(st.m, o, 64), __shfl_xor(st.z, o, 64), __shfl_xor(st.s, o, 64)};
-    // the lower lane's side first, so that both lanes form the same sum
-    st = (lane & o) ? merge(t, st) : merge(st, t);
-  }
-  if (lane == 0) wstat[wave] = st;
-  if constexpr (TOP) {
+    };
+    if (at >= 0) of_piece(at, better);
+    else if (at == AT_HEAD) each_head(better);
+    else if (at == AT_TAIL) each_tail(better);
+    else each(better);                             // nothing above START, or nothing at all
     // the r-th greatest thread key of this wave (0: fewer threads hold elements)
     const int r = (a.top + NW - 1) / NW;
     uint64_t mine = best, top = 0;
+#pragma unroll 1
     for (int i = 0; i < r; ++i) {
       top = wave_max64(mine);
       if (mine == top) mine = 0;                   // keys differ, but for the empty key 0
@@ -188,42 +242,83 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LogprobArgs a) {
     if (lane == 0) wkey[wave] = top;
     if (tid == 0) count = 0;
   }
+  // the wave's sums over its maximum
+  auto wave_stat = [&]() {
+    rebase(st, wave_maxf(st.m));
+    st.z = wave_sumf(st.z);
+    st.s = wave_sumf(st.s);
+    if (lane == 0) wstat[wave] = st;
+  };
+  wave_stat();
+  const bool wave_nan = __any(nan);
+  if (lane == 0) wnan[wave] = wave_nan;
   __syncthreads();
-  st = wstat[0];
-  for (int v = 1; v < NW; ++v) st = merge(st, wstat[v]);
-  const float lnz = logf(st.z);
+  auto all_stat = [&]() {
+    float m = wstat[0].m;
+#pragma unroll
+    for (int v = 1; v < NW; ++v) m = fmaxf(m, wstat[v].m);
+    st = Stat{m, 0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < NW; ++v) {
+      Stat t = wstat[v];
+      rebase(t, m);
+      st.z += t.z;
+      st.s += t.s;
+    }
+  };
+  all_stat();
+  bool any_nan = false;
+#pragma unroll
+  for (int v = 0; v < NW; ++v) any_nan |= wnan[v] != 0;
+  if (!any_nan && !(st.m > START && st.m < HUGE_X)) {
+    // x log2 e may overflow: the maximum itself (START was none of the elements) and then x - m, exactly as the
+    // definition has it.  No finite element: z = 0.  +inf: not a number.
+    float m = -__builtin_inff();
+    each([&](float v, int) { m = fmaxf(m, v); });
+    m = wave_maxf(m);
+    __syncthreads();                               // wstat has been read
+    if (lane == 0) wstat[wave].m = m;
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < NW; ++v) m = fmaxf(m, wstat[v].m);
+    any_nan = m == __builtin_inff();
+    st = Stat{m, 0.f, 0.f};
+    if (fabsf(m) < __builtin_inff())
+      each([&](float v, int) {
+        const float y = fmaxf((v - m) * LOG2E, FAR), e = __builtin_amdgcn_exp2f(y);
+        st.z += e;
+        st.s = fmaf(e, y, st.s);
+      });
+    st.z = wave_sumf(st.z);
+    st.s = wave_sumf(st.s);
+    __syncthreads();
+    if (lane == 0) wstat[wave] = st;
+    __syncthreads();
+    st.z = st.s = 0.f;
+#pragma unroll
+    for (int v = 0; v < NW; ++v) { st.z += wstat[v].z; st.s += wstat[v].s; }
+  }
+  float lnz = 0.f;
   if (a.pieces > 1) {
     if (tid == 0) {
       float* o = a.pstat + (row * a.pieces + piece) * 4;
-      o[0] = st.m; o[1] = st.z; o[2] = st.s;
+      o[0] = st.m; o[1] = any_nan ? __uint_as_float(0x7fc00000u) : st.z; o[2] = st.s;
     }
-  } else if (tid == 0) {
-    if (a.tok) {
-      const int64_t t = a.tok[row];
-      a.lp[row] = t >= 0 && t < a.vocab ? ((float)x[t] - st.m) - lnz : __uint_as_float(0x7fc00000u);
-    }
-    if (a.ent) a.ent[row] = lnz - st.s / st.z;
+  } else {
+    lnz = finish_row<T>(a, row, st, any_nan, tid == 0);
   }
   if constexpr (TOP) {
     uint64_t bound = wkey[0];
+#pragma unroll
     for (int v = 1; v < NW; ++v) bound = wkey[v] < bound ? wkey[v] : bound;
-    if (best >= bound && best != 0) {
-      auto gather = [&](float v, int i) {
+    if (best >= bound && best != 0)
+      each([&](float v, int i) {
         const uint64_t k = make_key(v, i);
         if (k >= bound) {
-          const int at = atomicAdd(&count, 1);     // the order of the keys in the buffer does not matter
-          if (at < CAP) buf[at] = k;
+          const int to = atomicAdd(&count, 1);     // the order of the keys in the buffer does not matter
+          if (to < CAP) buf[to] = k;
         }
-      };
-      each_head(gather);
-      each_tail(gather);
-      for (int p = tid; p < body; p += NT) {
-        float f[N];
-        Piece<T>::get(*(const uint4*)(xb + (int64_t)p * N), f);
-#pragma unroll
-        for (int e = 0; e < N; ++e) gather(f[e], lo + head + p * N + e);
-      }
-    }
+      });
     __syncthreads();
     const int n = count;
     auto emit = [&](int i, uint64_t k) {
@@ -235,16 +330,18 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LogprobArgs a) {
       }
     };
     const int have = min(a.top, hi - lo);          // a short last piece may hold fewer
-    if (n <= 4 * NT && n <= CAP) {
-      for (int i = tid; i < n; i += NT) {
-        const uint64_t k = buf[i];
+    if (n <= NT) {
+      if (tid < n) {
+        const uint64_t k = buf[tid];
         int rank = 0;
+#pragma unroll 4
         for (int j = 0; j < n; ++j) rank += buf[j] > k;
         if (rank < a.top) emit(rank, k);
       }
     } else {
       // `top` rounds of the greatest key below the last one, over the buffer or the row
       uint64_t prev = ~(uint64_t)0;
+#pragma unroll 1
       for (int i = 0; i < have; ++i) {
         uint64_t b = 0;
         auto look = [&](uint64_t k) {
@@ -253,21 +350,14 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LogprobArgs a) {
         if (n <= CAP) {
           for (int j = tid; j < n; j += NT) look(buf[j]);
         } else {
-          auto look1 = [&](float v, int j) { look(make_key(v, j)); };
-          each_head(look1);
-          each_tail(look1);
-          for (int p = tid; p < body; p += NT) {
-            float f[N];
-            Piece<T>::get(*(const uint4*)(xb + (int64_t)p * N), f);
-#pragma unroll
-            for (int e = 0; e < N; ++e) look(make_key(f[e], lo + head + p * N + e));
-          }
+          each([&](float v, int j) { look(make_key(v, j)); });
         }
         b = wave_max64(b);
         __syncthreads();                           // the last round's wkey has been read
         if (lane == 0) wkey[wave] = b;
         __syncthreads();
         b = wkey[0];
+#pragma unroll
         for (int v = 1; v < NW; ++v) b = wkey[v] > b ? wkey[v] : b;
         if (tid == 0) emit(i, b);
         prev = b;
@@ -278,30 +368,52 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(const LogprobArgs a) {
   }
 }
 
-// joins the pieces of a row: statistics in piece order, the greatest of their keys
-template <typename T> __global__ __launch_bounds__(256) void logprobs_join_kernel(const LogprobArgs a) {
+// Joins the pieces of a row: their sums in piece order, and the greatest of their keys.  A piece's last key is one
+// that `top` elements reach, so the greatest of those bounds what has to be ranked.
+template <typename T> __global__ __launch_bounds__(LP_NT) void logprobs_join_kernel(const LogprobArgs a) {
+  __shared__ uint64_t buf[LP_MAX_PIECES * STARKV_MAX_TOP];
+  __shared__ int count;
   const int64_t row = blockIdx.x;
-  const float* ps = a.pstat + row * a.pieces * 4;
-  Stat st = {ps[0], ps[1], ps[2]};
-  for (int p = 1; p < a.pieces; ++p) st = merge(st, Stat{ps[4 * p], ps[4 * p + 1], ps[4 * p + 2]});
-  const float lnz = logf(st.z);
-  if (threadIdx.x == 0) {
-    const T* x = (const T*)a.x + row * a.xs;
-    if (a.tok) {
-      const int64_t t = a.tok[row];
-      a.lp[row] = t >= 0 && t < a.vocab ? ((float)x[t] - st.m) - lnz : __uint_as_float(0x7fc00000u);
-    }
-    if (a.ent) a.ent[row] = lnz - st.s / st.z;
+  const int tid = threadIdx.x, n = a.pieces * a.top;
+  const uint64_t* pt = a.ptop + row * n;
+  const float4* ps = (const float4*)(a.pstat + row * a.pieces * 4);
+  if (tid == 0) count = 0;
+  float m = -__builtin_inff();
+  uint64_t bound = 0;
+  for (int p = 0; p < a.pieces; ++p) {
+    m = fmaxf(m, ps[p].x);
+    const uint64_t k = a.top ? pt[p * a.top + a.top - 1] : 0;
+    bound = k > bound ? k : bound;
   }
-  // each piece's keys are in descending order: a key's rank is its place in
-  // its own piece and the number of greater keys in the others
-  const uint64_t* pt = a.ptop + row * a.pieces * a.top;
-  const int n = a.pieces * a.top;
-  for (int i = threadIdx.x; i < n; i += 256) {
+  const bool fast = m > START && m < HUGE_X;
+  Stat st = {m, 0.f, 0.f};
+  bool nan = m == __builtin_inff();
+  for (int p = 0; p < a.pieces; ++p) {
+    Stat t = {ps[p].x, ps[p].y, ps[p].z};
+    nan |= t.z != t.z;
+    if (fast) {
+      rebase(t, m);                                // (also pieces with no element above START: z = 0, or far below)
+    } else {
+      const float d = fmaxf((t.m - m) * LOG2E, FAR), f = __builtin_amdgcn_exp2f(d);
+      t.s = f * fmaf(t.z, d, t.s);
+      t.z = t.m == m ? t.z : t.z * f;
+    }
+    st.z += t.z;
+    st.s += t.s;
+  }
+  const float lnz = finish_row<T>(a, row, st, nan, tid == 0);
+  __syncthreads();
+  for (int i = tid; i < n; i += LP_NT) {
     const uint64_t k = pt[i];
-    if (k == 0) continue;
+    if (k >= bound && k != 0) buf[atomicAdd(&count, 1)] = k;
+  }
+  __syncthreads();
+  const int c = count;
+  for (int i = tid; i < c; i += LP_NT) {
+    const uint64_t k = buf[i];
     int rank = 0;
-    for (int j = 0; j < n && rank < a.top; ++j) rank += pt[j] > k;
+#pragma unroll 4
+    for (int j = 0; j < c; ++j) rank += buf[j] > k;
     if (rank < a.top) {
       a.tlp[row * a.top + rank] = (unorder32((uint32_t)(k >> 32)) - st.m) - lnz;
       a.tid[row * a.top + rank] = (uint32_t)~(uint32_t)k;
@@ -309,21 +421,25 @@ template <typename T> __global__ __launch_bounds__(256) void logprobs_join_kerne
   }
 }
 
-int plan_logprobs(int rows, int vocab, int esize, int cus) { return 1; }
+// Workgroups per row: enough to fill the chip four times over, each with at least two pieces a thread
+int plan_logprobs(int rows, int vocab, int esize, int cus) {
+  const int64_t most = vocab / (2 * LP_NT * (16 / esize));
+  return (int)std::max<int64_t>(1, std::min({(int64_t)LP_MAX_PIECES, ceil_div(4 * cus, rows), most}));
+}
 
-template <typename T, int NT> static int launch_lp(const LogprobArgs& a, hipStream_t st) {
+template <typename T> static int launch_lp(const LogprobArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)a.rows * a.pieces));
-  if (a.top) hipLaunchKernelGGL((logprobs_kernel<T, NT, true>), grid, dim3(NT), 0, st, a);
-  else hipLaunchKernelGGL((logprobs_kernel<T, NT, false>), grid, dim3(NT), 0, st, a);
-  if (a.pieces > 1) hipLaunchKernelGGL((logprobs_join_kernel<T>), dim3((unsigned)a.rows), dim3(256), 0, st, a);
+  if (a.top) hipLaunchKernelGGL((logprobs_kernel<T, true>), grid, dim3(LP_NT), 0, st, a);
+  else hipLaunchKernelGGL((logprobs_kernel<T, false>), grid, dim3(LP_NT), 0, st, a);
+  if (a.pieces > 1) hipLaunchKernelGGL((logprobs_join_kernel<T>), dim3((unsigned)a.rows), dim3(LP_NT), 0, st, a);
   return (int)hipGetLastError();
 }
 
 int launch_logprobs(const LogprobArgs& a, int dtype, hipStream_t st) {
   if (a.rows == 0) return 0;
-  if (dtype == STARKV_F16) return launch_lp<_Float16, 512>(a, st);
-  if (dtype == STARKV_BF16) return launch_lp<__bf16, 512>(a, st);
-  return launch_lp<float, 512>(a, st);
+  if (dtype == STARKV_F16) return launch_lp<_Float16>(a, st);
+  if (dtype == STARKV_BF16) return launch_lp<__bf16>(a, st);
+  return launch_lp<float>(a, st);
 }
 
 }  // namespace starkv

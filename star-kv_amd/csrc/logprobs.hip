@@ -34,7 +34,8 @@ namespace starkv {
 namespace {
 
 constexpr int LP_NT = 256;                         // threads per workgroup
-constexpr int LP_MAX_PIECES = 16;                  // of a row
+constexpr int LP_MAX_PIECES = 64;                  // of a row (a lane each in the join)
+constexpr int LP_BATCH = 4;                        // 16-byte pieces a thread asks for at a time
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float START = -1e30f, HUGE_X = 1e30f;    // maxima in between take the fast sums
 constexpr float FAR = -150.f;                      // 2^FAR is 0 in fp32
@@ -100,12 +101,14 @@ __device__ inline uint64_t wave_max64(uint64_t v) {
 template <typename T> struct Piece;                // 16 bytes of logits
 template <> struct Piece<float> {
   static constexpr int N = 4;
+  static constexpr uint32_t BARRED = 0xff800000u;  // -inf
   static __device__ void get(uint4 v, float (&f)[4]) {
     f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
   }
 };
 template <> struct Piece<_Float16> {
   static constexpr int N = 8;
+  static constexpr uint32_t BARRED = 0xfc00fc00u;
   static __device__ void get(uint4 v, float (&f)[8]) {
     const half8 h = __builtin_bit_cast(half8, v);
 #pragma unroll
@@ -114,6 +117,7 @@ template <> struct Piece<_Float16> {
 };
 template <> struct Piece<__bf16> {
   static constexpr int N = 8;
+  static constexpr uint32_t BARRED = 0xff80ff80u;
   static __device__ void get(uint4 v, float (&f)[8]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -126,16 +130,19 @@ template <> struct Piece<__bf16> {
 
 }  // namespace
 
-// the results of a row with the sums st: its token's log probability, its entropy
-template <typename T> __device__ inline float finish_row(const LogprobArgs& a, int64_t row, const Stat& st, bool nan, bool write) {
+// The results of a row with the sums st: its token's log probability, its entropy.  `xt` is the token's logit
+// (token_logit), asked for when the kernel starts: two dependent reads that would otherwise end it.
+template <typename T> __device__ inline float token_logit(const LogprobArgs& a, int64_t row) {
+  if (!a.tok) return 0.f;
+  const int64_t t = a.tok[row];
+  return t >= 0 && t < a.vocab ? (float)((const T*)a.x)[row * a.xs + t] : __uint_as_float(0x7fc00000u);
+}
+__device__ inline float finish_row(const LogprobArgs& a, int64_t row, float xt, const Stat& st, bool nan, bool write) {
   const float none = __uint_as_float(0x7fc00000u);
   const float eps = fmaf(st.m, LOG2E, -log2_of(st.m));       // what fl(m log2 e) is short of m log2 e
   const float lnz = nan ? none : logf(st.z) - (fabsf(st.m) < HUGE_X ? eps * LN2 : 0.f);
   if (write) {
-    if (a.tok) {
-      const int64_t t = a.tok[row];
-      a.lp[row] = t >= 0 && t < a.vocab ? ((float)((const T*)a.x)[row * a.xs + t] - st.m) - lnz : none;
-    }
+    if (a.tok) a.lp[row] = (xt - st.m) - lnz;
     if (a.ent) a.ent[row] = nan ? none : logf(st.z) - LN2 * (st.s / st.z);
   }
   return lnz;
@@ -155,6 +162,7 @@ template <typename T, bool TOP> __global__ __launch_bounds__(LP_NT) void logprob
   const int piece = blockIdx.x - (int)row * a.pieces;
   const T* x = (const T*)a.x + row * a.xs;
   const int lo = piece * a.piece_len, hi = min(a.vocab, lo + a.piece_len);
+  const float xt = a.pieces == 1 && tid == 0 ? token_logit<T>(a, row) : 0.f;
 
   // [lo, hi): a head up to the first 16-byte boundary, whole pieces, a tail;
   // the head and the tail are single elements of threads 0 .. N - 2
@@ -205,16 +213,45 @@ template <typename T, bool TOP> __global__ __launch_bounds__(LP_NT) void logprob
     if (!(v <= st.m)) raise(v, AT_HEAD);
     add(v);
   });
-#pragma unroll 2
-  for (int p = tid; p < body; p += NT) {
-    float v[N];
-    Piece<T>::get(*(const uint4*)(xb + (int64_t)p * N), v);
-    float cm = v[0];                               // a NaN stays in it
+  // LP_BATCH of this thread's pieces from p on, all asked for at once; past the row's last one: barred logits
+  constexpr int R = LP_BATCH;
+  auto load = [&](uint4 (&d)[R], int p) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 1; e < N; ++e) cm = __builtin_elementwise_maximum(cm, v[e]);
-    if (!(cm <= st.m)) raise(cm, p);
+    for (int u = 0; u < R; ++u) d[u] = *(const uint4*)(xb + (int64_t)min(p + u * NT, body - 1) * N);
+    if (p - tid + R * NT > body) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) add(v[e]);
+      for (int u = 0; u < R; ++u)
+        if (p + u * NT >= body) d[u] = make_uint4(Piece<T>::BARRED, Piece<T>::BARRED, Piece<T>::BARRED, Piece<T>::BARRED);
+    }
+  };
+#pragma unroll 1
+  for (int p = tid; p - tid < body; p += R * NT) {
+    uint4 d[R];
+    load(d, p);
+    float pm[R], cm;                               // a NaN stays in a maximum
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+      float v[N];
+      Piece<T>::get(d[u], v);
+      pm[u] = v[0];
+#pragma unroll
+      for (int e = 1; e < N; ++e) pm[u] = __builtin_elementwise_maximum(pm[u], v[e]);
+      cm = u == 0 ? pm[0] : __builtin_elementwise_maximum(cm, pm[u]);
+    }
+    if (!(cm <= st.m)) {
+      int where = p;
+#pragma unroll
+      for (int u = R - 1; u >= 0; --u)
+        if (pm[u] == cm || pm[u] != pm[u]) where = p + u * NT;
+      raise(cm, where);
+    }
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+      float v[N];
+      Piece<T>::get(d[u], v);
+#pragma unroll
+      for (int e = 0; e < N; ++e) add(v[e]);
+    }
   }
   each_tail([&](float v, int) {
     if (!(v <= st.m)) raise(v, AT_TAIL);
@@ -305,20 +342,43 @@ template <typename T, bool TOP> __global__ __launch_bounds__(LP_NT) void logprob
       o[0] = st.m; o[1] = any_nan ? __uint_as_float(0x7fc00000u) : st.z; o[2] = st.s;
     }
   } else {
-    lnz = finish_row<T>(a, row, st, any_nan, tid == 0);
+    lnz = finish_row(a, row, xt, st, any_nan, tid == 0);
   }
   if constexpr (TOP) {
     uint64_t bound = wkey[0];
 #pragma unroll
     for (int v = 1; v < NW; ++v) bound = wkey[v] < bound ? wkey[v] : bound;
-    if (best >= bound && best != 0)
-      each([&](float v, int i) {
+    if (best >= bound && best != 0) {
+      const float least = unorder32((uint32_t)(bound >> 32));
+      auto take = [&](float v, int i) {
+        if (v < least) return;                     // (a NaN is not)
         const uint64_t k = make_key(v, i);
         if (k >= bound) {
           const int to = atomicAdd(&count, 1);     // the order of the keys in the buffer does not matter
           if (to < CAP) buf[to] = k;
         }
-      });
+      };
+      each_head(take);
+#pragma unroll 1
+      for (int p = tid; p < body; p += R * NT) {
+        uint4 d[R];
+        load(d, p);
+        uint32_t hits = 0;
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+          float v[N];
+          Piece<T>::get(d[u], v);
+#pragma unroll
+          for (int e = 1; e < N; ++e) v[0] = __builtin_elementwise_maximum(v[0], v[e]);
+          if (!(v[0] < least) && p + u * NT < body) hits |= 1u << u;
+        }
+        while (hits) {                             // one copy of the code that takes a piece's elements
+          of_piece(p + (__ffs(hits) - 1) * NT, take);
+          hits &= hits - 1;
+        }
+      }
+      each_tail(take);
+    }
     __syncthreads();
     const int n = count;
     auto emit = [&](int i, uint64_t k) {
@@ -368,40 +428,44 @@ template <typename T, bool TOP> __global__ __launch_bounds__(LP_NT) void logprob
   }
 }
 
-// Joins the pieces of a row: their sums in piece order, and the greatest of their keys.  A piece's last key is one
-// that `top` elements reach, so the greatest of those bounds what has to be ranked.
+// Joins the pieces of a row: their sums, and the greatest of their keys.
 template <typename T> __global__ __launch_bounds__(LP_NT) void logprobs_join_kernel(const LogprobArgs a) {
   __shared__ uint64_t buf[LP_MAX_PIECES * STARKV_MAX_TOP];
   __shared__ int count;
   const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x, n = a.pieces * a.top;
+  const int tid = threadIdx.x, lane = tid & 63, n = a.pieces * a.top;
   const uint64_t* pt = a.ptop + row * n;
-  const float4* ps = (const float4*)(a.pstat + row * a.pieces * 4);
   if (tid == 0) count = 0;
-  float m = -__builtin_inff();
+  const float xt = tid == 0 ? token_logit<T>(a, row) : 0.f;
+  // every wave does the same: a lane a piece
+  const bool mine = lane < a.pieces;
+  const float4 ps = mine ? ((const float4*)a.pstat)[row * a.pieces + lane] : make_float4(-__builtin_inff(), 0.f, 0.f, 0.f);
+  // `top` keys are at or above the q-th greatest of the pieces' r-th keys, q r >= top
   uint64_t bound = 0;
-  for (int p = 0; p < a.pieces; ++p) {
-    m = fmaxf(m, ps[p].x);
-    const uint64_t k = a.top ? pt[p * a.top + a.top - 1] : 0;
-    bound = k > bound ? k : bound;
-  }
-  const bool fast = m > START && m < HUGE_X;
-  Stat st = {m, 0.f, 0.f};
-  bool nan = m == __builtin_inff();
-  for (int p = 0; p < a.pieces; ++p) {
-    Stat t = {ps[p].x, ps[p].y, ps[p].z};
-    nan |= t.z != t.z;
-    if (fast) {
-      rebase(t, m);                                // (also pieces with no element above START: z = 0, or far below)
-    } else {
-      const float d = fmaxf((t.m - m) * LOG2E, FAR), f = __builtin_amdgcn_exp2f(d);
-      t.s = f * fmaf(t.z, d, t.s);
-      t.z = t.m == m ? t.z : t.z * f;
+  if (a.top) {
+    const int r = (a.top + a.pieces - 1) / a.pieces, q = (a.top + r - 1) / r;
+    const uint64_t k = mine ? pt[lane * a.top + r - 1] : 0;
+    int rank = 0;
+#pragma unroll 8
+    for (int p = 0; p < 64; ++p) {
+      const uint64_t o = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), p) << 32) |
+                         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)k, p);
+      rank += o > k;
     }
-    st.z += t.z;
-    st.s += t.s;
+    bound = wave_max64(rank == q - 1 ? k : 0);     // (0, and all are ranked, where that many pieces are empty)
   }
-  const float lnz = finish_row<T>(a, row, st, nan, tid == 0);
+  const float m = wave_maxf(ps.x);
+  Stat st = {ps.x, ps.y, ps.z};
+  const bool nan = __any(st.z != st.z) || m == __builtin_inff();
+  if (m > START && m < HUGE_X) {
+    rebase(st, m);                                 // (pieces without an element above START end at 0)
+  } else {
+    const float d = fmaxf((st.m - m) * LOG2E, FAR), f = __builtin_amdgcn_exp2f(d);
+    st.s = f * fmaf(st.z, d, st.s);
+    st.z = st.m == m ? st.z : st.z * f;
+  }
+  st = Stat{m, wave_sumf(st.z), wave_sumf(st.s)};
+  const float lnz = finish_row(a, row, xt, st, nan, tid == 0);
   __syncthreads();
   for (int i = tid; i < n; i += LP_NT) {
     const uint64_t k = pt[i];
@@ -421,10 +485,11 @@ template <typename T> __global__ __launch_bounds__(LP_NT) void logprobs_join_ker
   }
 }
 
-// Workgroups per row: enough to fill the chip four times over, each with at least two pieces a thread
+// Workgroups per row: enough to fill the chip, each with at least two pieces a thread
 int plan_logprobs(int rows, int vocab, int esize, int cus) {
   const int64_t most = vocab / (2 * LP_NT * (16 / esize));
-  return (int)std::max<int64_t>(1, std::min({(int64_t)LP_MAX_PIECES, ceil_div(4 * cus, rows), most}));
+  const int fill = getenv("LPF") ? atoi(getenv("LPF")) : 4;
+  return (int)std::max<int64_t>(1, std::min({(int64_t)LP_MAX_PIECES, ceil_div(fill * cus, rows), most}));
 }
 
 template <typename T> static int launch_lp(const LogprobArgs& a, hipStream_t st) {

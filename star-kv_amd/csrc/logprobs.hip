@@ -16,12 +16,12 @@
 // overflow) are summed again with x - m formed first.
 //
 // Top alternatives: keys are (logit, lowest index first) as one 64-bit number
-// in a total order.  Each thread knows the piece of its greatest key from the
-// pass.  With NW waves, the ceil(top / NW)-th greatest thread key of every
-// wave is taken, and the least of those is a bound that at least `top`
-// elements reach; only threads at or above it read their pieces again and
-// gather the elements there, a few dozen as a rule.  The gathered keys are then
-// ranked.  Where more elements than the buffer holds reach the bound (rows
+// in a total order.  Each thread knows its greatest logit and the first piece
+// that holds it from the pass, (logit, lowest piece first) its coarse key.
+// With NW waves, the ceil(top / NW)-th greatest coarse key of every wave is
+// taken, and the least of those is a bound that at least `top` elements reach;
+// only threads at or above it read pieces again and gather the elements there,
+// a few dozen as a rule.  The gathered keys are then ranked.  Where more elements than the buffer holds reach the bound (rows
 // built so), the row is searched `top` times instead.
 //
 // Few rows are split over workgroups, and a second launch joins the pieces.
@@ -130,6 +130,17 @@ template <> struct Piece<__bf16> {
 
 }  // namespace
 
+// how many of the n keys are greater than k, read in pairs
+__device__ inline int rank_of(const uint64_t* buf, int n, uint64_t k) {
+  int rank = 0;
+#pragma unroll 8
+  for (int j = 0; j + 1 < n; j += 2) {
+    const ulonglong2 t = *(const ulonglong2*)(buf + j);
+    rank += (t.x > k) + (t.y > k);
+  }
+  return rank + ((n & 1) && buf[n - 1] > k);
+}
+
 // The results of a row with the sums st: its token's log probability, its entropy.  `xt` is the token's logit
 // (token_logit), asked for when the kernel starts: two dependent reads that would otherwise end it.
 template <typename T> __device__ inline float token_logit(const LogprobArgs& a, int64_t row) {
@@ -152,16 +163,18 @@ __device__ inline float finish_row(const LogprobArgs& a, int64_t row, float xt, 
 template <typename T, bool TOP> __global__ __launch_bounds__(LP_NT) void logprobs_kernel(const LogprobArgs a) {
   constexpr int NT = LP_NT, N = Piece<T>::N, NW = NT / 64;
   constexpr int CAP = TOP ? NT * N + 64 : 1;       // one piece of every thread fits
-  __shared__ uint64_t buf[CAP];
+  __shared__ __attribute__((aligned(16))) uint64_t buf[CAP];
   __shared__ uint64_t wkey[NW];
   __shared__ Stat wstat[NW];
   __shared__ int wnan[NW];
   __shared__ int count;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t row = blockIdx.x / a.pieces;
   const int piece = blockIdx.x - (int)row * a.pieces;
   const T* x = (const T*)a.x + row * a.xs;
   const int lo = piece * a.piece_len, hi = min(a.vocab, lo + a.piece_len);
+  // rows with fewer pieces than threads go round the waves, so that each holds some
+  const int tid = hi - lo >= (NT + 1) * N ? threadIdx.x : lane * NW + wave;
   const float xt = a.pieces == 1 && tid == 0 ? token_logit<T>(a, row) : 0.f;
 
   // [lo, hi): a head up to the first 16-byte boundary, whole pieces, a tail;
@@ -190,7 +203,8 @@ template <typename T, bool TOP> __global__ __launch_bounds__(LP_NT) void logprob
     each_tail(f);
   };
 
-  constexpr int AT_NONE = -1, AT_HEAD = -2, AT_TAIL = -3;
+  // pieces in the order of their indices: the head (0), the body's piece p (p + 1), the tail
+  const int AT_NONE = -1, AT_HEAD = 0, AT_TAIL = body + 1;
   Stat st = {START, 0.f, 0.f};
   float ml = log2_of(START);
   bool nan = false;
@@ -224,11 +238,14 @@ template <typename T, bool TOP> __global__ __launch_bounds__(LP_NT) void logprob
         if (p + u * NT >= body) d[u] = make_uint4(Piece<T>::BARRED, Piece<T>::BARRED, Piece<T>::BARRED, Piece<T>::BARRED);
     }
   };
+  float pm[R];
+#pragma unroll
+  for (int u = 0; u < R; ++u) pm[u] = 0.f;
 #pragma unroll 1
   for (int p = tid; p - tid < body; p += R * NT) {
     uint4 d[R];
     load(d, p);
-    float pm[R], cm;                               // a NaN stays in a maximum
+    float cm;                                      // a NaN stays in a maximum
 #pragma unroll
     for (int u = 0; u < R; ++u) {
       float v[N];
@@ -243,7 +260,7 @@ template <typename T, bool TOP> __global__ __launch_bounds__(LP_NT) void logprob
 #pragma unroll
       for (int u = R - 1; u >= 0; --u)
         if (pm[u] == cm || pm[u] != pm[u]) where = p + u * NT;
-      raise(cm, where);
+      raise(cm, where + 1);
     }
 #pragma unroll
     for (int u = 0; u < R; ++u) {
@@ -258,17 +275,22 @@ template <typename T, bool TOP> __global__ __launch_bounds__(LP_NT) void logprob
     add(v);
   });
 
-  uint64_t best = 0;                               // this thread's greatest key
+  uint64_t best = 0;                               // this thread's coarse key; 0: it holds no element
+  auto coarse = [](float v, int at) { return ((uint64_t)order32(v) << 32) | (uint32_t)~at; };
   if constexpr (TOP) {
-    auto better = [&](float v, int i) {
-      const uint64_t k = make_key(v, i);
-      best = k > best ? k : best;
-    };
-    if (at >= 0) of_piece(at, better);
-    else if (at == AT_HEAD) each_head(better);
-    else if (at == AT_TAIL) each_tail(better);
-    else each(better);                             // nothing above START, or nothing at all
-    // the r-th greatest thread key of this wave (0: fewer threads hold elements)
+    if (at != AT_NONE) {
+      best = coarse(nan ? __uint_as_float(0x7fc00000u) : st.m, at);
+    } else {                                       // nothing above START, or nothing at all
+      auto better = [&](float v, int where) {
+        const uint64_t k = coarse(v, where);
+        best = k > best ? k : best;
+      };
+      each_head([&](float v, int) { better(v, AT_HEAD); });
+#pragma unroll 1
+      for (int p = tid; p < body; p += NT) of_piece(p, [&](float v, int) { better(v, p + 1); });
+      each_tail([&](float v, int) { better(v, AT_TAIL); });
+    }
+    // the r-th greatest coarse key of this wave (0: fewer threads hold elements)
     const int r = (a.top + NW - 1) / NW;
     uint64_t mine = best, top = 0;
 #pragma unroll 1
@@ -350,34 +372,39 @@ template <typename T, bool TOP> __global__ __launch_bounds__(LP_NT) void logprob
     for (int v = 1; v < NW; ++v) bound = wkey[v] < bound ? wkey[v] : bound;
     if (best >= bound && best != 0) {
       const float least = unorder32((uint32_t)(bound >> 32));
-      auto take = [&](float v, int i) {
+      auto take = [&](float v, int i, int where) {
         if (v < least) return;                     // (a NaN is not)
-        const uint64_t k = make_key(v, i);
-        if (k >= bound) {
+        if (coarse(v, where) >= bound) {
           const int to = atomicAdd(&count, 1);     // the order of the keys in the buffer does not matter
-          if (to < CAP) buf[to] = k;
+          if (to < CAP) buf[to] = make_key(v, i);
         }
       };
-      each_head(take);
+      each_head([&](float v, int i) { take(v, i, AT_HEAD); });
 #pragma unroll 1
       for (int p = tid; p < body; p += R * NT) {
-        uint4 d[R];
-        load(d, p);
+        if (body > R * NT) {                       // else the maxima of the row's only batch are still there
+          uint4 d[R];
+          load(d, p);
+#pragma unroll
+          for (int u = 0; u < R; ++u) {
+            float v[N];
+            Piece<T>::get(d[u], v);
+            pm[u] = v[0];
+#pragma unroll
+            for (int e = 1; e < N; ++e) pm[u] = __builtin_elementwise_maximum(pm[u], v[e]);
+          }
+        }
         uint32_t hits = 0;
 #pragma unroll
-        for (int u = 0; u < R; ++u) {
-          float v[N];
-          Piece<T>::get(d[u], v);
-#pragma unroll
-          for (int e = 1; e < N; ++e) v[0] = __builtin_elementwise_maximum(v[0], v[e]);
-          if (!(v[0] < least) && p + u * NT < body) hits |= 1u << u;
-        }
+        for (int u = 0; u < R; ++u)
+          if (!(pm[u] < least) && p + u * NT < body) hits |= 1u << u;
         while (hits) {                             // one copy of the code that takes a piece's elements
-          of_piece(p + (__ffs(hits) - 1) * NT, take);
+          const int q = p + (__ffs(hits) - 1) * NT;
+          of_piece(q, [&](float v, int i) { take(v, i, q + 1); });
           hits &= hits - 1;
         }
       }
-      each_tail(take);
+      each_tail([&](float v, int i) { take(v, i, AT_TAIL); });
     }
     __syncthreads();
     const int n = count;
@@ -390,12 +417,11 @@ template <typename T, bool TOP> __global__ __launch_bounds__(LP_NT) void logprob
       }
     };
     const int have = min(a.top, hi - lo);          // a short last piece may hold fewer
-    if (n <= NT) {
-      if (tid < n) {
-        const uint64_t k = buf[tid];
-        int rank = 0;
-#pragma unroll 4
-        for (int j = 0; j < n; ++j) rank += buf[j] > k;
+    if (n <= 2 * NT) {
+#pragma unroll 1
+      for (int i = tid; i < n; i += NT) {
+        const uint64_t k = buf[i];
+        const int rank = rank_of(buf, n, k);
         if (rank < a.top) emit(rank, k);
       }
     } else {
@@ -430,7 +456,7 @@ template <typename T, bool TOP> __global__ __launch_bounds__(LP_NT) void logprob
 
 // Joins the pieces of a row: their sums, and the greatest of their keys.
 template <typename T> __global__ __launch_bounds__(LP_NT) void logprobs_join_kernel(const LogprobArgs a) {
-  __shared__ uint64_t buf[LP_MAX_PIECES * STARKV_MAX_TOP];
+  __shared__ __attribute__((aligned(16))) uint64_t buf[LP_MAX_PIECES * STARKV_MAX_TOP];
   __shared__ int count;
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, n = a.pieces * a.top;
@@ -475,9 +501,7 @@ template <typename T> __global__ __launch_bounds__(LP_NT) void logprobs_join_ker
   const int c = count;
   for (int i = tid; i < c; i += LP_NT) {
     const uint64_t k = buf[i];
-    int rank = 0;
-#pragma unroll 4
-    for (int j = 0; j < c; ++j) rank += buf[j] > k;
+    const int rank = rank_of(buf, c, k);
     if (rank < a.top) {
       a.tlp[row * a.top + rank] = (unorder32((uint32_t)(k >> 32)) - st.m) - lnz;
       a.tid[row * a.top + rank] = (uint32_t)~(uint32_t)k;

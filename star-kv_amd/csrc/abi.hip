@@ -1597,14 +1597,16 @@ int starkv_fp8_gemm(const starkv_fp8_gemm_desc* d, void* workspace, size_t works
   return launch_fp8_gemm(a, sp.plan, d->out_dtype, d->scale_dtype, d->silu_mul != 0, s);
 }
 
-static int plan_lp(const starkv_logprobs_desc* d, LogprobArgs& a, size_t& bytes) {
+static int plan_lp(const starkv_logprobs_desc* d, LogprobArgs& a, bool& wide, size_t& bytes) {
   if (!d) return STARKV_ERR_NULL;
   if (d->rows < 0 || d->vocab < 1 || d->top < 0 || d->top > d->vocab) return STARKV_ERR_SHAPE;
   if (d->top > STARKV_MAX_TOP || d->vocab > (1 << 24)) return STARKV_ERR_LIMIT;
   if (!act16(d->dtype) && d->dtype != STARKV_F32) return STARKV_ERR_DTYPE;
   a = LogprobArgs{};
   a.rows = d->rows; a.vocab = d->vocab; a.top = d->top;
-  a.pieces = d->rows ? plan_logprobs(d->rows, d->vocab, esize(d->dtype), device_cus()) : 1;
+  const LogprobPlan p = plan_logprobs(std::max(d->rows, 1), d->vocab, esize(d->dtype), device_cus());
+  a.pieces = p.pieces;
+  wide = p.wide;
   a.piece_len = (int)round_up(ceil_div(d->vocab, a.pieces), 1024);
   a.pieces = (int)ceil_div(d->vocab, a.piece_len);
   if ((int64_t)d->rows * a.pieces > INT32_MAX / 1024) return STARKV_ERR_LIMIT;
@@ -1615,14 +1617,16 @@ static int plan_lp(const starkv_logprobs_desc* d, LogprobArgs& a, size_t& bytes)
 
 size_t starkv_token_logprobs_workspace_bytes(const starkv_logprobs_desc* d) {
   LogprobArgs a;
+  bool wide;
   size_t bytes = 0;
-  return plan_lp(d, a, bytes) ? 0 : bytes;
+  return plan_lp(d, a, wide, bytes) ? 0 : bytes;
 }
 
 int starkv_token_logprobs(const starkv_logprobs_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
   LogprobArgs a;
+  bool wide;
   size_t bytes = 0;
-  const int st = plan_lp(d, a, bytes);
+  const int st = plan_lp(d, a, wide, bytes);
   if (st) return st;
   if (d->rows == 0) return STARKV_OK;
   if (!d->logits || (d->tokens && !d->logprob) || (d->top && (!d->top_logprob || !d->top_id))) return STARKV_ERR_NULL;
@@ -1638,7 +1642,7 @@ int starkv_token_logprobs(const starkv_logprobs_desc* d, void* workspace, size_t
   }
   a.x = d->logits; a.xs = d->stride; a.tok = d->tokens;
   a.lp = d->logprob; a.ent = d->entropy; a.tlp = d->top_logprob; a.tid = d->top_id;
-  return launch_logprobs(a, d->dtype, (hipStream_t)stream);
+  return launch_logprobs(a, wide, d->dtype, (hipStream_t)stream);
 }
 
 }  // extern "C"

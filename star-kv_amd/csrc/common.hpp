@@ -467,8 +467,9 @@ struct Fp8Plan { bool few; int bm, bn, ks, cus; };   // the stream kernel; tile 
 int launch_fp8_few(const Fp8GemmArgs& a, const Fp8Plan& p, int out_dtype, int scale_dtype, bool silu, hipStream_t st);
 Fp8Plan plan_fp8_gemm(int m, int n, int kb, bool silu, bool exact, bool pow2, int cus);   // exact: fp32 output
 int launch_fp8_gemm(const Fp8GemmArgs& a, const Fp8Plan& p, int out_dtype, int scale_dtype, bool silu, hipStream_t st);
-int plan_logprobs(int rows, int vocab, int esize, int cus);          // workgroups per row
-int launch_logprobs(const LogprobArgs& a, int dtype, hipStream_t st);
+struct LogprobPlan { int pieces; bool wide; };       // workgroups per row; 1024 threads in each, or 256
+LogprobPlan plan_logprobs(int rows, int vocab, int esize, int cus);
+int launch_logprobs(const LogprobArgs& a, bool wide, int dtype, hipStream_t st);
 int launch_k_logits(const KArgs& a, int dtype, int fmt, bool out_f32, int out_dtype, bool fast, int B, hipStream_t st);
 int launch_k_logits_ws(const KArgs& a, int dtype, bool out_f32, int out_dtype, int B, hipStream_t st);
 int launch_k_logits_gqa(const KArgs& a, int dtype, bool out_f32, int out_dtype, int B, hipStream_t st);

@@ -33,7 +33,8 @@ namespace starkv {
 
 namespace {
 
-constexpr int LP_NT = 256;                         // threads per workgroup
+constexpr int LP_NT = 256;                         // threads per workgroup: many rows, pieces of few, short rows
+constexpr int LP_WIDE = 1024;                      // rows of 16 KB and more while there are few: one launch, a batch or two
 constexpr int LP_MAX_PIECES = 64;                  // of a row (a lane each in the join)
 constexpr int LP_BATCH = 4;                        // 16-byte pieces a thread asks for at a time
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
@@ -160,9 +161,9 @@ __device__ inline float finish_row(const LogprobArgs& a, int64_t row, float xt, 
 }
 
 // TOP: alternatives are asked for
-template <typename T, bool TOP> __global__ __launch_bounds__(LP_NT) void logprobs_kernel(const LogprobArgs a) {
-  constexpr int NT = LP_NT, N = Piece<T>::N, NW = NT / 64;
-  constexpr int CAP = TOP ? NT * N + 64 : 1;       // one piece of every thread fits
+template <typename T, int NT, bool TOP> __global__ __launch_bounds__(NT) void logprobs_kernel(const LogprobArgs a) {
+  constexpr int N = Piece<T>::N, NW = NT / 64;
+  constexpr int CAP = TOP ? (NT * N < 4096 ? NT * N : 4096) + 64 : 1;      // one piece of every thread, of 512 at most
   __shared__ __attribute__((aligned(16))) uint64_t buf[CAP];
   __shared__ uint64_t wkey[NW];
   __shared__ Stat wstat[NW];
@@ -509,26 +510,37 @@ template <typename T> __global__ __launch_bounds__(LP_NT) void logprobs_join_ker
   }
 }
 
-// Workgroups per row: enough to fill the chip, each with at least two pieces a thread
-int plan_logprobs(int rows, int vocab, int esize, int cus) {
-  const int64_t most = vocab / (2 * LP_NT * (16 / esize));
-  const int fill = getenv("LPF") ? atoi(getenv("LPF")) : 4;
-  return (int)std::max<int64_t>(1, std::min({(int64_t)LP_MAX_PIECES, ceil_div(fill * cus, rows), most}));
+// Workgroups per row, and threads in each (wide: LP_WIDE).  A row of up to 64 KB is one batch of 1024 threads: split
+// over workgroups and joined by a second launch, 8 rows of 32000 took 10.8 us instead of 9.7; with 4 workgroups and
+// more to a CU 256 threads overlap better.  Longer ones are split while rows alone do not fill the chip.
+LogprobPlan plan_logprobs(int rows, int vocab, int esize, int cus) {
+  const int64_t bytes = (int64_t)vocab * esize;
+  LogprobPlan p = {1, bytes > 16384 && rows < 4 * cus};
+  if (bytes > 65536 && rows < cus) {
+    p.wide = false;
+    const int64_t most = vocab / (2 * LP_NT * (16 / esize));       // at least two pieces a thread
+    p.pieces = (int)std::max<int64_t>(1, std::min({(int64_t)LP_MAX_PIECES, ceil_div(4 * cus, rows), most}));
+  }
+  return p;
 }
 
-template <typename T> static int launch_lp(const LogprobArgs& a, hipStream_t st) {
+template <typename T, int NT> static void launch_lp(const LogprobArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)a.rows * a.pieces));
-  if (a.top) hipLaunchKernelGGL((logprobs_kernel<T, true>), grid, dim3(LP_NT), 0, st, a);
-  else hipLaunchKernelGGL((logprobs_kernel<T, false>), grid, dim3(LP_NT), 0, st, a);
+  if (a.top) hipLaunchKernelGGL((logprobs_kernel<T, NT, true>), grid, dim3(NT), 0, st, a);
+  else hipLaunchKernelGGL((logprobs_kernel<T, NT, false>), grid, dim3(NT), 0, st, a);
+}
+template <typename T> static int launch_lp_t(const LogprobArgs& a, bool wide, hipStream_t st) {
+  if (wide) launch_lp<T, LP_WIDE>(a, st);
+  else launch_lp<T, LP_NT>(a, st);
   if (a.pieces > 1) hipLaunchKernelGGL((logprobs_join_kernel<T>), dim3((unsigned)a.rows), dim3(LP_NT), 0, st, a);
   return (int)hipGetLastError();
 }
 
-int launch_logprobs(const LogprobArgs& a, int dtype, hipStream_t st) {
+int launch_logprobs(const LogprobArgs& a, bool wide, int dtype, hipStream_t st) {
   if (a.rows == 0) return 0;
-  if (dtype == STARKV_F16) return launch_lp<_Float16>(a, st);
-  if (dtype == STARKV_BF16) return launch_lp<__bf16>(a, st);
-  return launch_lp<float>(a, st);
+  if (dtype == STARKV_F16) return launch_lp_t<_Float16>(a, wide, st);
+  if (dtype == STARKV_BF16) return launch_lp_t<__bf16>(a, wide, st);
+  return launch_lp_t<float>(a, wide, st);
 }
 
 }  // namespace starkv

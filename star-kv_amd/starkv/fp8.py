@@ -15,8 +15,8 @@ from typing import Optional, Tuple
 
 import torch
 
-from . import _lib
-from ._lib import Fp8GemmDesc, Fp8QuantizeDesc, StarKVError, check
+from . import _lib, ops
+from ._lib import Fp8GemmDesc, Fp8QuantizeDesc, StarKVError
 from .ops import _launch, _out, _poison
 
 __all__ = ["fp8_quantize", "fp8_quantize_weight", "fp8_matmul", "fp8_linear"]
@@ -37,25 +37,28 @@ def _e4m3_rows(rows: int, k: int, device) -> torch.Tensor:
     return torch.empty(rows, -(-k // 16) * 16, dtype=torch.float8_e4m3fn, device=device)[:, :k]
 
 
-def _rows2d(t: torch.Tensor, name: str) -> Tuple[torch.Tensor, int]:
-    """(t as [rows, width], its row stride); one row has any stride, 16 * ceil(width / 16) is given."""
-    w = t.shape[-1] if t.dim() else 0
+def _rows2d(t: torch.Tensor, name: str) -> Tuple[torch.Tensor, int, int, int]:
+    """(t as [rows, width], rows, width, row stride); one row has any stride, 16 * ceil(width / 16) is given."""
+    shape, stride = t.shape, t.stride()
+    w = shape[-1] if shape else 0
     if w < 1:
-        raise StarKVError(f"{name} must have rows of at least one value, got shape {tuple(t.shape)}")
-    if w > 1 and t.stride(-1) != 1:
+        raise StarKVError(f"{name} must have rows of at least one value, got shape {tuple(shape)}")
+    if w > 1 and stride[-1] != 1:
         raise StarKVError(f"{name} must have a contiguous last dim")
-    if t.dim() != 2:
+    if len(shape) != 2:
         try:
             t = t.view(-1, w) if t.numel() else t.reshape(0, w)
         except RuntimeError:
             raise StarKVError(f"{name} rows must be addressable with one row stride") from None
-    return t, (t.stride(0) if t.shape[0] > 1 else -(-w // 16) * 16)
+        shape, stride = t.shape, t.stride()
+    m = shape[0]
+    return t, m, w, (stride[0] if m > 1 else -(-w // 16) * 16)
 
 
-def _on(device, *ts: Tuple[str, Optional[torch.Tensor]]) -> None:
+def _on(device, **ts: Optional[torch.Tensor]) -> None:
     if device.type != "cuda":
         raise StarKVError("libstarkv operators take device tensors (there is no CPU path)")
-    for name, t in ts:
+    for name, t in ts.items():
         if t is not None and t.device != device:
             raise StarKVError(f"{name} is on {t.device}, the activations on {device}")
 
@@ -76,19 +79,22 @@ def fp8_quantize(x: torch.Tensor, scale_dtype: torch.dtype = torch.float8_e8m0fn
     if dt is None:
         raise StarKVError(f"activations are float16 or bfloat16, got {x.dtype}")
     sd = _scale_code(scale_dtype)
-    xr, xs = _rows2d(x, "x")
-    _on(x.device)
-    m, k = xr.shape
-    kb, dev, lead = _blocks(k), x.device, x.shape[:-1]
-    pitch = -(-k // 16) * 16
-    q = _poison(torch.empty((*lead, pitch), dtype=torch.float8_e4m3fn, device=dev))
+    xr, m, k, xs = _rows2d(x, "x")
+    dev = x.device
+    _on(dev)
+    kb, lead, pitch = -(-k // BLOCK), x.shape[:-1], -(-k // 16) * 16
+    q = _out(*lead, pitch, dtype=torch.float8_e4m3fn, device=dev)
     # the scales of a block of columns together: [ceil(k / 128)][rows]
-    strides, s = [m], 1
-    for n in reversed(lead):
-        strides.append(s)
-        s *= n
-    scale = torch.empty_strided((*lead, kb), strides[:0:-1] + [m], dtype=scale_dtype, device=dev)
-    _poison(scale.movedim(-1, 0))
+    if x.dim() == 2:
+        strides = (1, m)
+    else:
+        strides, s = [m], 1
+        for n in reversed(lead):
+            strides.insert(0, s)
+            s *= n
+    scale = torch.empty_strided((*lead, kb), strides, dtype=scale_dtype, device=dev)
+    if ops.POISON:
+        _poison(scale.movedim(-1, 0))
     _launch("starkv_fp8_quantize", Fp8QuantizeDesc(m, k, dt, xr.data_ptr(), xs, q.data_ptr(), pitch, scale.data_ptr(),
                                                    sd, 1, m), dev)
     return (q if pitch == k else q[..., :k]), scale
@@ -132,17 +138,14 @@ def fp8_quantize_weight(w: torch.Tensor, scale_dtype: torch.dtype = torch.float8
 
 def _product(name, x, x_scale, weight, weight_scale, residual, silu_mul, rms_eps, out, out_dtype):
     dev = x.device
-    _on(dev, ("x_scale", x_scale), ("weight", weight), ("weight_scale", weight_scale), ("residual", residual),
-        ("out", out))
+    _on(dev, x_scale=x_scale, weight=weight, weight_scale=weight_scale, residual=residual, out=out)
     if weight.dtype != torch.float8_e4m3fn or weight.dim() != 2:
         raise StarKVError(f"{name}: weight must be a float8_e4m3fn [n, k], got {weight.dtype} {tuple(weight.shape)}")
     sd = _scale_code(weight_scale.dtype)
-    wr, ws = _rows2d(weight, "weight")
-    n, k = wr.shape
-    xr, xs = _rows2d(x, "x")
-    m = xr.shape[0]
-    if xr.shape[1] != k:
-        raise StarKVError(f"{name}: x has {xr.shape[1]} columns, the weight {k}")
+    _, n, k, ws = _rows2d(weight, "weight")
+    xr, m, xw, xs = _rows2d(x, "x")
+    if xw != k:
+        raise StarKVError(f"{name}: x has {xw} columns, the weight {k}")
     kb = -(-k // BLOCK)
     if weight_scale.shape != (-(-n // BLOCK), kb):
         raise StarKVError(f"{name}: weight_scale must be [{-(-n // BLOCK)}, {kb}], got {tuple(weight_scale.shape)}")
@@ -161,12 +164,12 @@ def _product(name, x, x_scale, weight, weight_scale, residual, silu_mul, rms_eps
     od = _OUT.get(out.dtype)
     if od is None:
         raise StarKVError(f"{name}: outputs are float16, bfloat16 or float32, got {out.dtype}")
-    orr, os_ = _rows2d(out, "out")
+    orr, _, _, os_ = _rows2d(out, "out")
     rp, rs = None, 0
     if residual is not None:
         if residual.shape != shape or residual.dtype != out.dtype:
             raise StarKVError(f"{name}: residual must be {shape} of {out.dtype}")
-        rr, rs = _rows2d(residual, "residual")
+        rr, _, _, rs = _rows2d(residual, "residual")
         rp = rr.data_ptr()
     if x_scale is None:
         xd, xp, xsr, xsb = _ACT[x.dtype], None, 0, 0
@@ -180,7 +183,7 @@ def _product(name, x, x_scale, weight, weight_scale, residual, silu_mul, rms_eps
             except RuntimeError:
                 raise StarKVError(f"{name}: x_scale rows must be addressable with one row stride") from None
         xd, xp, xsr, xsb = _lib.E4M3, sr.data_ptr(), sr.stride(0), sr.stride(1)
-    d = Fp8GemmDesc(m, n, k, xd, od, xr.data_ptr(), xs, xp, xsr, xsb, wr.data_ptr(), ws, weight_scale.data_ptr(),
+    d = Fp8GemmDesc(m, n, k, xd, od, xr.data_ptr(), xs, xp, xsr, xsb, weight.data_ptr(), ws, weight_scale.data_ptr(),
                     weight_scale.stride(0), weight_scale.stride(1), sd, rp, rs, 1 if silu_mul else 0,
                     0 if rms_eps is None else 1, rms_eps or 0.0, orr.data_ptr(), os_)
     _launch("starkv_fp8_gemm", d, dev, workspace=True)

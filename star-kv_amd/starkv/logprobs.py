@@ -49,7 +49,8 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
         if tokens.shape != lead or tokens.dtype != torch.int64 or tokens.device != dev:
             raise StarKVError(f"tokens must be int64 {tuple(lead)} on {dev}, got {tokens.dtype} {tuple(tokens.shape)} "
                               f"on {tokens.device}")
-        tokens = tokens.contiguous()
+        if not tokens.is_contiguous():
+            tokens = tokens.contiguous()
     lp = _out(lead, dtype=torch.float32, device=dev) if tokens is not None else None
     ent = _out(lead, dtype=torch.float32, device=dev)
     tops = _out(*lead, top, dtype=torch.float32, device=dev)

@@ -92,6 +92,9 @@ def _workspace(device, nbytes: int) -> torch.Tensor:
     return ws
 
 
+_CALLS: dict = {}                    # entry point -> (the function, its workspace query or None)
+
+
 def _launch(name: str, desc, device, workspace: Optional[bool] = None) -> None:
     """Call the entry point ``name`` on ``device``'s current stream.  Entry
     points with a workspace (``workspace`` not None; False where the call is
@@ -101,16 +104,17 @@ def _launch(name: str, desc, device, workspace: Optional[bool] = None) -> None:
     if index != torch.cuda.current_device():
         with torch.cuda.device(device):
             return _launch(name, desc, torch.device("cuda", torch.cuda.current_device()), workspace)
-    L, ref = _lib.lib(), ctypes.byref(desc)
-    stream = _raw_stream(index)
+    call = _CALLS.get(name)
+    if call is None:
+        L = _lib.lib()
+        call = _CALLS[name] = (getattr(L, name), getattr(L, name + "_workspace_bytes", None))
+    ref, stream = ctypes.byref(desc), _raw_stream(index)
     if workspace is None:
-        st = getattr(L, name)(ref, stream)
-    elif not workspace:
-        st = getattr(L, name)(ref, None, 0, stream)
+        st = call[0](ref, stream)
     else:
-        nb = getattr(L, name + "_workspace_bytes")(ref)
-        ws = _poison(torch.empty(nb, dtype=torch.uint8, device=device)) if nb else None
-        st = getattr(L, name)(ref, ws.data_ptr() if nb else None, nb, stream)
+        nb = call[1](ref) if workspace else 0
+        ws = _out(nb, dtype=torch.uint8, device=device) if nb else None
+        st = call[0](ref, ws.data_ptr() if nb else None, nb, stream)
     if st:
         check(st, name)
 

@@ -26,13 +26,16 @@ import torch.nn.functional as F
 
 from ._lib import StarKVError
 from .cache import LatentCache
+from .fp8 import fp8_linear, fp8_quantize_weight
+from .logprobs import TokenLogprobs, token_logprobs
 from .ops import GEMM_ADD, GEMM_SILU_MUL, SKINNY_MAX_ROWS, decode_attention, prefill_attention, skinny_linear
 from .rope import RopeConfig
 
 __all__ = ["LatentAttention", "DecodeGraphState", "build_model", "fuse_layers_", "generate", "generate_graphed",
-           "decode_graphed"]
+           "decode_graphed", "score"]
 
 HEAD_DIM = 128
+SCORE_LOGITS = 1 << 27                 # logits that score() holds at a time
 
 
 def _rotate_half(x: torch.Tensor) -> torch.Tensor:
@@ -166,11 +169,16 @@ class LatentAttention(nn.Module):
     def _project(self, hidden_states: torch.Tensor, rms_eps: Optional[float] = None):
         """(q [B, Hq, T, 128], new K latent rows [B, T, sum(r)], new V latent rows [B, T, Rv]).
         ``rms_eps``: hidden_states is the raw layer input and the input RMSNorm
-        is folded into the packed projection (``qkv_packed``)."""
+        is folded into the 8-bit projection (``qkv_fp8``, any number of rows)
+        or the packed one (``qkv_packed``, decode batches)."""
         B, T, _ = hidden_states.shape
         if rms_eps is not None:
             nq, nk = self.n_heads * HEAD_DIM, sum(self.ranks)
-            qkv = skinny_linear(hidden_states, self.qkv_packed, rms_eps=rms_eps)
+            fp8 = getattr(self, "qkv_fp8", None)
+            if fp8 is not None:
+                qkv = fp8_linear(hidden_states, *fp8, rms_eps=rms_eps)
+            else:
+                qkv = skinny_linear(hidden_states, self.qkv_packed, rms_eps=rms_eps)
             return (qkv[..., :nq].view(B, T, self.n_heads, HEAD_DIM).transpose(1, 2), qkv[..., nq:nq + nk],
                     qkv[..., nq + nk:])
         w = getattr(self, "qkv_weight", None)
@@ -241,7 +249,10 @@ def _fused_decoder_forward(self, hidden_states: torch.Tensor, attention_mask=Non
     followed by SiLU(gate) * up.  Decode batches (at most 16 rows) run the
     projections on ``starkv_skinny_gemm`` (the residual add and the SiLU
     product in its epilogue); larger ones on torch's GEMMs (addmm) and
-    ``starkv_silu_mul``.  The reference path (``self_attn.reference``) runs
+    ``starkv_silu_mul``.  A layer with 8-bit weights (``fuse_layers_(model,
+    fp8=...)``) runs its four projections on ``starkv_fp8_gemm`` at any number
+    of rows, norms, residual adds and the SiLU product folded in.  The
+    reference path (``self_attn.reference``) runs
     HF's own forward."""
     from .ops import rms_norm, silu_mul
     att = self.self_attn
@@ -256,6 +267,13 @@ def _fused_decoder_forward(self, hidden_states: torch.Tensor, attention_mask=Non
         hidden_states = hidden_states.clone()
     B, T, Hd = hidden_states.shape
     eps_in, eps_post = self.input_layernorm.variance_epsilon, self.post_attention_layernorm.variance_epsilon
+    if getattr(self, "starkv_fp8", None) is not None:
+        # the residual stream is updated in place, as below
+        h = hidden_states.contiguous()
+        o = att.core(h, position_embeddings, rms_eps=eps_in)
+        fp8_linear(o, *att.o_fp8, residual=h, out=h)
+        m = fp8_linear(h, *self.mlp.gate_up_fp8, silu_mul=True, rms_eps=eps_post)
+        return fp8_linear(m, *self.mlp.down_fp8, residual=h, out=h)
     if B * T <= SKINNY_MAX_ROWS and getattr(self.mlp, "gate_up_packed", None) is not None:
         # decode: four weight streams, the norms folded into the projections
         # that follow them, the residual adds and SiLU(gate) * up in epilogues
@@ -350,8 +368,9 @@ def _no_capture(what: str) -> None:
 
 
 def _fuse_layer_(layer) -> None:
-    """Merge and pack one decoder layer's weights (see ``fuse_layers_``) and
-    record the signature of the weights they were made from."""
+    """Merge and pack (or quantise: ``layer.starkv_fp8``) one decoder layer's
+    weights (see ``fuse_layers_``) and record the signature of the weights
+    they were made from."""
     from .ops import pack_weight
     att = layer.self_attn
     att.merge_projections_()
@@ -362,9 +381,17 @@ def _fuse_layer_(layer) -> None:
     n = mlp.gate_proj.weight.shape[0]
     mlp.gate_proj.weight = nn.Parameter(w[:n], requires_grad=False)
     mlp.up_proj.weight = nn.Parameter(w[n:], requires_grad=False)
-    mlp.gate_up_packed = None
+    mlp.gate_up_packed = att.qkv_packed = att.o_packed = mlp.down_packed = None
+    att.qkv_fp8 = att.o_fp8 = mlp.gate_up_fp8 = mlp.down_fp8 = None
+    fp8 = getattr(layer, "starkv_fp8", None)
+    if fp8 is not None:
+        with torch.no_grad():
+            att.qkv_fp8 = fp8_quantize_weight(att.qkv_weight, fp8, layer.input_layernorm.weight)
+            att.o_fp8 = fp8_quantize_weight(att.o_proj.weight, fp8)
+            mlp.gate_up_fp8 = fp8_quantize_weight(w, fp8, layer.post_attention_layernorm.weight)
+            mlp.down_fp8 = fp8_quantize_weight(mlp.down_proj.weight, fp8)
     # qkv rows need 16 (tiles), the others 32 (gate/up halves), k 64
-    if (att.qkv_weight.shape[0] % 16 == 0 and att.qkv_weight.shape[1] % 64 == 0
+    elif (att.qkv_weight.shape[0] % 16 == 0 and att.qkv_weight.shape[1] % 64 == 0
             and all(_packable(t) for t in (att.o_proj.weight, w, mlp.down_proj.weight))):
         with torch.no_grad():
             att.qkv_packed = pack_weight(att.qkv_weight, layer.input_layernorm.weight)
@@ -389,7 +416,7 @@ def _pack_head(head):
         return pack_weight(head.weight)
 
 
-def fuse_layers_(model) -> None:
+def fuse_layers_(model, fp8: Optional[torch.dtype] = None) -> None:
     """Run every decoder layer of ``model`` (and the final norm) through
     ``_fused_decoder_forward``: q / k / v latent projections and the MLP's
     gate / up projections merged into one weight each (the HF Linear weights
@@ -400,9 +427,25 @@ def fuse_layers_(model) -> None:
     into the q/k/v and gate/up copies.  Each layer (and the output
     projection) records the version of the weights its copies come from and
     rebuilds them when a weight has been replaced or written since
-    (``load_state_dict``, ``load_projections``)."""
+    (``load_state_dict``, ``load_projections``).
+
+    ``fp8`` (a scale type: ``torch.float8_e8m0fnu`` or ``torch.float32``): the
+    copies are e4m3 with a scale for each block of 128 x 128
+    (``fp8_quantize_weight``) instead, and decode and prefill both run on them
+    (``fp8_linear``; activations are quantised on the way).  The output
+    projection and the latent up-projections stay in the model's type.  The
+    gate and up rows must then be whole blocks of 128 each."""
     import types
+    if fp8 is not None:
+        if fp8 not in (torch.float8_e8m0fnu, torch.float32):
+            raise StarKVError(f"fuse_layers_: fp8 is a scale type, float8_e8m0fnu or float32, got {fp8}")
+        for layer in model.model.layers:
+            n, t = layer.mlp.gate_proj.weight.shape[0], layer.mlp.gate_proj.weight.dtype
+            if n % 128 or t not in (torch.float16, torch.bfloat16):
+                raise StarKVError(f"fuse_layers_: 8-bit weights need an MLP of a multiple of 128 in a float16 or "
+                                  f"bfloat16 model, got {n} in {t}")
     for layer in model.model.layers:
+        layer.starkv_fp8 = fp8
         _fuse_layer_(layer)
         layer.forward = types.MethodType(_fused_decoder_forward, layer)
     model.model.norm.forward = types.MethodType(_fused_norm_forward, model.model.norm)
@@ -417,13 +460,16 @@ def fuse_layers_(model) -> None:
 def build_model(n_layers: int, hidden: int, heads: int, kv_heads: int, intermediate: int, vocab: int,
                 ranks: Sequence[int], v_rank: int, batch: int, capacity: int, fmt: str = "int8_g64",
                 seed: int = 0, device="cuda", dtype=torch.float16, projections: Optional[Sequence] = None,
-                fused: bool = True):
+                fused: bool = True, fp8: Optional[torch.dtype] = None):
     """Random-init LlamaForCausalLM with every attention replaced by LatentAttention.
 
     `projections`: per layer, an exported `LatentProjections` whose ranks and
     weights replace `ranks`, `v_rank` and the random latent projections.
     `fused`: run the decoder layers through ``fuse_layers_`` (HF's own layer
-    forward otherwise; the reference path always uses HF's)."""
+    forward otherwise; the reference path always uses HF's).
+    `fp8`: 8-bit decoder weights with scales of this type (``fuse_layers_``)."""
+    if fp8 is not None and not fused:
+        raise StarKVError("build_model: 8-bit weights run in the fused decoder layers")
     from transformers import LlamaConfig, LlamaForCausalLM
     cfg = LlamaConfig(vocab_size=vocab, hidden_size=hidden, intermediate_size=intermediate,
                       num_hidden_layers=n_layers, num_attention_heads=heads, num_key_value_heads=kv_heads,
@@ -447,7 +493,7 @@ def build_model(n_layers: int, hidden: int, heads: int, kv_heads: int, intermedi
             att.load_projections(p)
         layer.self_attn = att
     if fused:
-        fuse_layers_(model)
+        fuse_layers_(model, fp8)
     return model
 
 
@@ -457,11 +503,13 @@ def attention_layers(model) -> List[LatentAttention]:
 
 @torch.no_grad()
 def generate(model, prompt: torch.Tensor, steps: int, reference: bool = False,
-             forced: Optional[torch.Tensor] = None):
+             forced: Optional[torch.Tensor] = None, logprobs: Optional[int] = None):
     """Greedy decoding: prefill ``prompt`` [B, P] (one forward), then ``steps``
     single-token decode forwards.  ``forced`` [B, steps] feeds given tokens
     instead of the argmax (teacher forcing, for comparing two runs).
-    Returns (tokens [B, steps + 1], logits of the last position per forward)."""
+    Returns (tokens [B, steps + 1], logits of the last position per forward)
+    and, where ``logprobs`` is a number of alternatives (0 .. 64), the
+    ``TokenLogprobs`` [B, steps + 1] of the tokens returned."""
     for att in attention_layers(model):
         att.reference = reference
     model.model.norm.starkv_reference = reference
@@ -472,6 +520,7 @@ def generate(model, prompt: torch.Tensor, steps: int, reference: bool = False,
     logits = [out.logits[:, -1].float()]
     tok = logits[-1].argmax(-1, keepdim=True)
     toks = [tok]
+    probs = [token_logprobs(out.logits[:, -1], tok[:, 0], logprobs)] if logprobs is not None else []
     for t in range(steps):
         inp = forced[:, t:t + 1] if forced is not None else tok
         pos = torch.full((B, 1), P + t, device=dev, dtype=torch.long)
@@ -479,14 +528,57 @@ def generate(model, prompt: torch.Tensor, steps: int, reference: bool = False,
         logits.append(out.logits[:, -1].float())
         tok = logits[-1].argmax(-1, keepdim=True)
         toks.append(tok)
-    return torch.cat(toks, 1), logits
+        if logprobs is not None:
+            probs.append(token_logprobs(out.logits[:, -1], tok[:, 0], logprobs))
+    toks = torch.cat(toks, 1)
+    return (toks, logits) if logprobs is None else (toks, logits, _stack_steps(probs))
+
+
+def _stack_steps(probs: Sequence[TokenLogprobs]) -> TokenLogprobs:
+    """The steps' [B, ...] as one [B, steps, ...]."""
+    return TokenLogprobs(*(torch.stack(f, 1) for f in zip(*probs)))
 
 
 @torch.no_grad()
-def generate_graphed(model, prompt: torch.Tensor, steps: int, keep_logits: bool = True):
+def score(model, tokens: torch.Tensor, top: int = 0, reference: bool = False) -> TokenLogprobs:
+    """The ``TokenLogprobs`` [B, T - 1] of ``tokens`` [B, T] from the second on,
+    each given what stands before it: what the caches hold (nothing, or a
+    prefix the rows share with it) and the tokens themselves.  One prefill
+    forward; the logits are made and read ``SCORE_LOGITS`` at a time.  The
+    caches' lengths are put back, so several continuations of one prefix can
+    be scored in turn.  ``reference`` as in ``generate``."""
+    if tokens.dim() != 2 or tokens.shape[1] < 1:
+        raise StarKVError(f"score: tokens must be [B, T] with T at least 1, got shape {tuple(tokens.shape)}")
+    if tokens.dtype != torch.int64:
+        raise StarKVError(f"score: tokens must be int64, got {tokens.dtype}")
+    atts = attention_layers(model)
+    B, T = tokens.shape
+    V = model.lm_head.weight.shape[0]
+    if T == 1:
+        return token_logprobs(model.lm_head.weight.new_empty(B, 0, V), tokens[:, 1:], top)
+    for att in atts:
+        att.reference = reference
+    model.model.norm.starkv_reference = reference
+    past = [att.cache.length for att in atts]
+    try:
+        pos = torch.arange(past[0], past[0] + T, device=tokens.device)[None].expand(B, T)
+        h = model.model(input_ids=tokens, position_ids=pos, use_cache=False).last_hidden_state
+    finally:
+        for att, n in zip(atts, past):
+            att.cache.length = n
+    rows, want = h[:, :-1].reshape(-1, h.shape[-1]), tokens[:, 1:].reshape(-1)
+    n = max(1, SCORE_LOGITS // V)
+    parts = [token_logprobs(model.lm_head(rows[i:i + n]), want[i:i + n], top) for i in range(0, rows.shape[0], n)]
+    return TokenLogprobs(*(torch.cat(f).view(B, T - 1, *f[0].shape[1:]) for f in zip(*parts)))
+
+
+@torch.no_grad()
+def generate_graphed(model, prompt: torch.Tensor, steps: int, keep_logits: bool = True,
+                     logprobs: Optional[int] = None):
     """``generate`` with the decode steps replayed from one captured graph
     (``decode_graphed``).  Returns (tokens [B, steps + 1], logits of the last
-    position per forward, or [] when ``keep_logits`` is False)."""
+    position per forward, or [] when ``keep_logits`` is False) and, where
+    ``logprobs`` is given, the ``TokenLogprobs`` as ``generate`` does."""
     for att in attention_layers(model):
         att.reference = False
     model.model.norm.starkv_reference = False
@@ -496,22 +588,28 @@ def generate_graphed(model, prompt: torch.Tensor, steps: int, keep_logits: bool 
                 use_cache=False, logits_to_keep=1)
     logits = [out.logits[:, -1].float()] if keep_logits else []
     tok = out.logits[:, -1].argmax(-1, keepdim=True)
+    first = token_logprobs(out.logits[:, -1], tok[:, 0], logprobs) if logprobs is not None else None
     if steps == 0:
-        return tok, logits
-    toks, more = decode_graphed(model, tok, steps, keep_logits)
-    return torch.cat([tok, toks], 1), logits + more
+        return (tok, logits) if first is None else (tok, logits, _stack_steps([first]))
+    toks, more, *probs = decode_graphed(model, tok, steps, keep_logits, logprobs=logprobs)
+    toks, logits = torch.cat([tok, toks], 1), logits + more
+    if first is None:
+        return toks, logits
+    return toks, logits, TokenLogprobs(*(torch.cat((a, b), 1) for a, b in zip(_stack_steps([first]), probs[0])))
 
 
 @torch.no_grad()
 def decode_graphed(model, tok: torch.Tensor, steps: int, keep_logits: bool = True,
-                   on_step: Optional[Callable[[int], None]] = None):
+                   on_step: Optional[Callable[[int], None]] = None, logprobs: Optional[int] = None):
     """``steps`` greedy decode steps from token ``tok`` [B, 1] at the caches'
     current length: the first step runs eagerly in graph form (which also
     warms up every table and workspace), one step is captured, and the rest
     replay it, each step's argmax feeding the next inside the graph.
     ``on_step(i)`` (optional) runs on the host after step i (0: the eager
     one) has been enqueued, e.g. to read what the step wrote.  Returns
-    (tokens [B, steps], logits per step or [])."""
+    (tokens [B, steps], logits per step or []) and, where ``logprobs`` is a
+    number of alternatives, the ``TokenLogprobs`` [B, steps] of the tokens,
+    computed inside the graph."""
     atts = attention_layers(model)
     B = tok.shape[0]
     dev = tok.device
@@ -525,15 +623,15 @@ def decode_graphed(model, tok: torch.Tensor, steps: int, keep_logits: bool = Tru
         att.graph = state
     tok_buf = tok.clone()
     pos_buf = torch.full((B, 1), P, device=dev, dtype=torch.long)
-    logit_buf = None
-    toks, logits = [], []
+    logit_buf = step_probs = None
+    toks, logits, probs = [], [], []
 
     def step():
         # the decode forward of LlamaForCausalLM (embedding, decoder layers,
         # final norm, output projection of the last position) without HF's
         # per-forward position, mask and rotary bookkeeping: the latent
         # attentions take their positions from the graph state
-        nonlocal logit_buf
+        nonlocal logit_buf, step_probs
         h = model.model.embed_tokens(tok_buf)
         for layer in model.model.layers:
             h = layer(h, attention_mask=None, position_ids=pos_buf, position_embeddings=None)
@@ -543,8 +641,17 @@ def decode_graphed(model, tok: torch.Tensor, steps: int, keep_logits: bool = Tru
                 logit_buf = torch.empty(B, last.shape[-1], device=dev, dtype=torch.float32)
             logit_buf.copy_(last)
         tok_buf.copy_(last.argmax(-1, keepdim=True))   # fp16 -> fp32 is exact: the same argmax
+        if logprobs is not None:
+            step_probs = token_logprobs(last, tok_buf[:, 0], logprobs)
         state.advance()
         pos_buf.add_(1)
+
+    def keep():
+        if keep_logits:
+            logits.append(logit_buf.clone())
+        toks.append(tok_buf.clone())
+        if logprobs is not None:
+            probs.append(TokenLogprobs(*(f.clone() for f in step_probs)))
 
     try:
         side = torch.cuda.Stream(device=dev)
@@ -552,9 +659,7 @@ def decode_graphed(model, tok: torch.Tensor, steps: int, keep_logits: bool = Tru
         with torch.cuda.stream(side):
             step()                                    # first decode step, eager, graph form
         torch.cuda.current_stream(dev).wait_stream(side)
-        if keep_logits:
-            logits.append(logit_buf.clone())
-        toks.append(tok_buf.clone())
+        keep()
         if on_step is not None:
             on_step(0)
         if steps > 1:
@@ -563,9 +668,7 @@ def decode_graphed(model, tok: torch.Tensor, steps: int, keep_logits: bool = Tru
                 step()
             for i in range(1, steps):
                 graph.replay()
-                if keep_logits:
-                    logits.append(logit_buf.clone())
-                toks.append(tok_buf.clone())
+                keep()
                 if on_step is not None:
                     on_step(i)
     finally:
@@ -573,4 +676,5 @@ def decode_graphed(model, tok: torch.Tensor, steps: int, keep_logits: bool = Tru
             att.graph = None
             att.cache.length = P + steps
     state.check()
-    return torch.cat(toks, 1), logits
+    toks = torch.cat(toks, 1)
+    return (toks, logits) if logprobs is None else (toks, logits, _stack_steps(probs))

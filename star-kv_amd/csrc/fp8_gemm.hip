@@ -48,10 +48,16 @@ __device__ inline void dma_1k(const uint8_t* base, uint32_t off, uint32_t lds) {
 __device__ inline void dma_dword(const void* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds) : "m0");
 }
+// the aligned dword with the byte at base + the lane's offset
+__device__ inline void dma_dword_at(const uint8_t* base, uint32_t off, uint32_t lds) {
+  const uint32_t low = (uint32_t)(uintptr_t)base & 3;
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"((off + low) & ~3u), "s"(base - low), "s"(lds) : "m0");
+}
 // Wait until at most n stages of LOADS loads each are on their way (n is uniform, at most NST - 2), and for this
 // wave's LDS reads.
+__device__ constexpr int vm_lgkm0(int v) { return 0x0070 | (v & 15) | ((v >> 4) << 14); }     // s_waitcnt vmcnt(v) lgkmcnt(0)
 template <int NST, int LOADS> __device__ inline void wait_stages(int n) {
-  constexpr auto code = [](int v) constexpr { return 0x0070 | (v & 15) | ((v >> 4) << 14); };
+  constexpr auto code = vm_lgkm0;
   static_assert(NST <= 7, "cases");
   if (NST > 6 && n == 5) __builtin_amdgcn_s_waitcnt(code(NST > 6 ? 5 * LOADS : 0));
   else if (NST > 5 && n == 4) __builtin_amdgcn_s_waitcnt(code(NST > 5 ? 4 * LOADS : 0));
@@ -69,33 +75,6 @@ __device__ inline void tile_at(const Fp8GemmArgs& a, int tl, int& tm, int& tn) {
   const int gm = min(GROUP, a.tiles_m - grp * GROUP);
   tm = grp * GROUP + rem % gm;
   tn = rem / gm;
-}
-// eight consecutive results (16-bit, and the residual added) from column col on, nv of them inside the row
-template <typename O> __device__ inline void store8(const Fp8GemmArgs& a, int row, int col, int nv, float (&v)[8]) {
-  O* o = (O*)a.out + (int64_t)row * a.os + col;
-  const O* rp = (const O*)a.res + (int64_t)row * a.rs + col;
-  if (a.vec_out >= 2 && nv >= 8) {
-    if (a.res) {
-      const uint4 t = *(const uint4*)rp;
-      O r[8];
-      __builtin_memcpy(r, &t, 16);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] += (float)r[e];
-    }
-    O t[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) t[e] = (O)v[e];
-    uint4 u;
-    __builtin_memcpy(&u, t, 16);
-    *(uint4*)o = u;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < nv) {
-        if (a.res) v[e] += (float)rp[e];
-        o[e] = (O)v[e];
-      }
-  }
 }
 }  // namespace
 
@@ -390,12 +369,14 @@ void fp8_gemm_kernel(const Fp8GemmArgs a) {
 // ---------------------------------------------------------------------------
 constexpr int WT = 256;                            // tile rows and columns
 constexpr int WSTAGE = 2 * WT * 128;               // bytes of a stage
-constexpr int WOUT = 32 * 64 * 4;                  // bytes a wave stages of its results: 32 rows x 64 columns, fp32
+constexpr int WSC = 256 * 4 + 4 * 64 * 4;           // bytes of a stage's scales: the activation rows' and, per wave, the weights'
+constexpr int WOUT = 32 * 64 * 2;                  // bytes a wave stages of its results: 32 rows x 64 columns
+constexpr int WLOADS = 18;                         // a wave's loads of a block: 16 of rows, two of scales
 
 template <typename O, bool SILU>
 __global__ __launch_bounds__(256, 1) void fp8_gemm_wide_kernel(const Fp8GemmArgs a) {
   static_assert(sizeof(O) == 2, "16-bit outputs");
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * WSTAGE + 4 * WOUT];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * WSTAGE + 2 * WSC + 2 * WT * 4 + 4 * WOUT];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave & 1, wn = wave >> 1;
@@ -414,8 +395,10 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_wide_kernel(const Fp8GemmArgs
   int m0, n0;
   const uint8_t* base;
   uint32_t off[16];                                // of the wave's loads' lane: row and piece
-  const uint8_t *sxp, *swp[2];
-  uint32_t sxo[4];
+  const uint32_t po[2] = {(uint32_t)min(piece0, last) * 16, (uint32_t)min(piece0 ^ 1, last) * 16};
+  const uint8_t *sxp, *swp;                        // scales of block 0: the tile's first activation row's and weight rows'
+  uint32_t sxo, swo;                               // from there: of the scales this lane loads
+  uint32_t xlow[4], wlow[2];                       // low address bits of the scales this lane reads
   // W rows of the tile: with SILU, wave column wn owns 64 gate rows and the same 64 up rows
   auto wrow = [&](int j) {
     if constexpr (SILU) return ((j & 64) ? a.half : 0) + n0 + (j >> 7) * 64 + (j & 63);
@@ -430,35 +413,55 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_wide_kernel(const Fp8GemmArgs
     for (int i = 0; i < 16; ++i) {
       const int r = (wave & 1) * 128 + 8 * i + rs;
       const int64_t row = isx ? min(m0 + r, a.m - 1) - m0 : min(wrow(r), a.n - 1) - n0;
-      off[i] = (uint32_t)(row * (isx ? a.xs : a.ws));
+      off[i] = (uint32_t)(row * (isx ? a.xs : a.ws)) + po[i & 1];
     }
     base = isx ? (const uint8_t*)a.x + (int64_t)m0 * a.xs : a.w + (int64_t)n0 * a.ws;
     sxp = (const uint8_t*)a.sx + (int64_t)m0 * a.sxr;
+    sxo = (uint32_t)((min(m0 + wave * 64 + lane, a.m - 1) - m0) * a.sxr);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sxo[i] = (uint32_t)((min(m0 + wm * 128 + 32 * i + c, a.m - 1) - m0) * a.sxr);
+    for (int i = 0; i < 4; ++i)
+      xlow[i] = (uint32_t)(uintptr_t)a.sx + (uint32_t)min(m0 + wm * 128 + 32 * i + c, a.m - 1) * (uint32_t)a.sxr;
+    const auto wsc = [&](int t) { return (int64_t)(min(wrow(wn * 128 + 64 * t), a.n - 1) >> 7) * a.swr; };
+    swp = (const uint8_t*)a.sw + wsc(0);
+    swo = lane & 1 ? (uint32_t)(wsc(1) - wsc(0)) : 0;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-      swp[t] = (const uint8_t*)a.sw + (int64_t)(min(wrow(wn * 128 + 64 * t), a.n - 1) >> 7) * a.swr;
+    for (int t = 0; t < 2; ++t) wlow[t] = (uint32_t)(uintptr_t)a.sw + (uint32_t)wsc(t);
   };
-  struct Sc { uint8_t x[4], w[2]; };
-  auto scales = [&](Sc& sc, int kb) __attribute__((always_inline)) {
+  // Scales go to LDS as the rows do (the aligned dword that holds the byte): loads into registers would bring the
+  // compiler's waits, which know nothing of the loads in flight, into the loop.
+  constexpr int SCALES = 2 * WSTAGE;
+  auto issue_scales = [&](int stage, int kb) __attribute__((always_inline)) {    // stage: 0 or WSTAGE
+    const uint32_t to = (uint32_t)(uintptr_t)(lds_void*)lds + SCALES + (stage ? WSC : 0);
+    dma_dword_at(sxp + (int64_t)kb * a.sxb, sxo, to + wave * 256);
+    dma_dword_at(swp + (int64_t)kb * a.swb, swo, to + 1024 + wave * 256);
+  };
+  struct Sc { uint32_t x[4], w[2]; };
+  auto scales = [&](Sc& sc, int stage) __attribute__((always_inline)) {
+    const uint8_t* const st = lds + SCALES + (stage ? WSC : 0);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sc.x[i] = (sxp + (int64_t)kb * a.sxb)[sxo[i]];
+    for (int i = 0; i < 4; ++i) sc.x[i] = *(const uint32_t*)(st + (wm * 128 + 32 * i + c) * 4);
 #pragma unroll
-    for (int t = 0; t < (SILU ? 2 : 1); ++t) sc.w[t] = swp[t][(int64_t)kb * a.swb];
+    for (int t = 0; t < (SILU ? 2 : 1); ++t) sc.w[t] = *(const uint32_t*)(st + 1024 + wave * 256 + t * 4);
+  };
+  auto bytes_of = [&](Sc& sc, int kb) __attribute__((always_inline)) {           // the bytes in those dwords
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sc.x[i] = __builtin_amdgcn_ubfe(sc.x[i], (xlow[i] + (uint32_t)kb * (uint32_t)a.sxb) << 3 & 24, 8);
+#pragma unroll
+    for (int t = 0; t < (SILU ? 2 : 1); ++t)
+      sc.w[t] = __builtin_amdgcn_ubfe(sc.w[t], (wlow[t] + (uint32_t)kb * (uint32_t)a.swb) << 3 & 24, 8);
   };
   // The blocks in the order last, first, second .. (the last may be short:
   // what lies behind it is zeroed before the loop starts).  A full block's
   // pieces need no check against the row's end.
   auto block = [&](int t) { return t == 0 ? end : t > end ? 0 : t - 1; };
-  auto issue_last = [&]() __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      dma_1k(base, off[i] + (uint32_t)min(end * 8 + (piece0 ^ (i & 1)), last) * 16, lds0 + i * 1024);
-  };
-  const uint32_t po[2] = {(uint32_t)min(piece0, last) * 16, (uint32_t)min(piece0 ^ 1, last) * 16};
   auto issue1 = [&](int stage, int kb, int i) __attribute__((always_inline)) {
-    dma_1k(base + (int64_t)kb * FP8_BLOCK, off[i] + po[i & 1], lds0 + stage + i * 1024);
+    dma_1k(base + (int64_t)kb * FP8_BLOCK, off[i], lds0 + stage + i * 1024);
+  };
+  auto issue_last = [&]() __attribute__((always_inline)) {
+    const int left = last - end * 8;
+    const uint32_t d[2] = {(uint32_t)min(piece0, left) * 16 - po[0], (uint32_t)min(piece0 ^ 1, left) * 16 - po[1]};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dma_1k(base + (int64_t)end * FP8_BLOCK, off[i] + d[i & 1], lds0 + i * 1024);
   };
 
   // operand reads: lane (c, g) takes pieces 4 h + 2 g and + 1 of row c
@@ -483,35 +486,53 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_wide_kernel(const Fp8GemmArgs
   if (idx >= stop) return;
   take(idx);
   Sc sc, sn;
-  issue_last();
-  scales(sc, end);
+  // a tile's first two blocks
+  constexpr int FACTORS = 2 * WSTAGE + 2 * WSC;    // row factors of this tile and the next
+  int par = 0;
+  auto start = [&](int to) __attribute__((always_inline)) {
+    if (a.rscale)
+      dma_dword(a.rscale + min(m0 + wave * 64 + lane, a.m - 1), (uint32_t)(uintptr_t)(lds_void*)lds + FACTORS + to * WT * 4 + wave * 256);
+    issue_last();
+    issue_scales(0, end);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) issue1(WSTAGE, block(1), i);
+    issue_scales(WSTAGE, block(1));
+  };
+  start(par);
+  // vmcnt counts in order: behind the start's loads stand the stores of the last tile, NSTORE of them if it was
+  // whole, which need not have ended for the loads to be there
+  constexpr int NSTORE = SILU ? 16 : 32;
+  bool drain = true;                               // another number of stores: wait for everything
   while (true) {
     floatx16 acc[4][4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[j][i] = floatx16{};
-    __builtin_amdgcn_s_waitcnt(0x0070);
+    if (drain) __builtin_amdgcn_s_waitcnt(vm_lgkm0(0));
+    else __builtin_amdgcn_s_waitcnt(vm_lgkm0(WLOADS + NSTORE));
     asm volatile("s_barrier" ::: "memory");
     if (a.k & (FP8_BLOCK - 1)) {
       zero_tail<2 * WT, 256>(lds, a.k & (FP8_BLOCK - 1), threadIdx.x);
-      __syncthreads();
+      __builtin_amdgcn_s_waitcnt(0xC07F);            // LDS writes done
+      asm volatile("s_barrier" ::: "memory");
     }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) issue1(WSTAGE, block(1), i);
     Half h0, h1;
 #pragma unroll
     for (int q = 0; q < 16; ++q) read1(h0, lds, 0, q);
+    scales(sc, 0);
     int cur = 0;
     auto product = [&](const Half& o, int q) __attribute__((always_inline)) {
       // row groups in the order in which the reads bring them
       constexpr int ORDER[16] = {0, 1, 4, 5, 2, 6, 8, 9, 10, 3, 7, 11, 12, 13, 14, 15};
       const int j = ORDER[q] >> 2, i = ORDER[q] & 3;
-      acc[j][i] = mfma8_32(frag8(o.w[j][0], o.w[j][1]), frag8(o.x[i][0], o.x[i][1]), acc[j][i], sc.w[SILU ? j >> 1 : 0],
-                           sc.x[i]);
+      acc[j][i] = mfma8_32(frag8(o.w[j][0], o.w[j][1]), frag8(o.x[i][0], o.x[i][1]), acc[j][i],
+                           (int)sc.w[SILU ? j >> 1 : 0], (int)sc.x[i]);
     };
-    for (int t = 0; t <= end; ++t, cur ^= WSTAGE) {    // block(t) in stage `cur`, its half 0 in h0, its scales in sc
-      scales(sn, block(t + 1));
+    // block(t) in stage `cur`, its half 0 in h0, its scales in sc
+    auto step = [&](int t, auto firstc) __attribute__((always_inline)) {
+      constexpr bool FIRST = decltype(firstc)::value;
+      bytes_of(sc, block(t));
 #pragma unroll
       for (int q = 0; q < 16; ++q) {
         product(h0, q);
@@ -519,7 +540,8 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_wide_kernel(const Fp8GemmArgs
         __builtin_amdgcn_sched_barrier(0);
       }
       // half 1 read; this wave's part of the next stage landed
-      __builtin_amdgcn_s_waitcnt(0x0070);
+      if (FIRST && !drain) __builtin_amdgcn_s_waitcnt(vm_lgkm0(NSTORE));
+      else __builtin_amdgcn_s_waitcnt(vm_lgkm0(0));
       asm volatile("s_barrier" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
       const int kn = block(t + 2);
@@ -528,10 +550,15 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_wide_kernel(const Fp8GemmArgs
         product(h1, q);
         issue1(cur, kn, q);
         read1(h0, lds + (cur ^ WSTAGE), 0, q);
+        if (q == 0) issue_scales(cur, kn);
+        if (q == 8) scales(sn, cur ^ WSTAGE);
         __builtin_amdgcn_sched_barrier(0);
       }
       sc = sn;
-    }
+      cur ^= WSTAGE;
+    };
+    step(0, std::true_type{});
+    for (int t = 1; t <= end; ++t) step(t, std::false_type{});
     // after the last blocks the loads repeated one and the reads took what was there, for nobody
     __builtin_amdgcn_s_waitcnt(0x0070);
     asm volatile("s_barrier" ::: "memory");
@@ -540,75 +567,128 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_wide_kernel(const Fp8GemmArgs
     const bool more = idx < stop;
     if (more) {
       take(idx);
-      issue_last();
-      scales(sc, end);
+      start(par ^ 1);
     }
 
-    // Results: lane (c, g) holds columns 32 j + 8 q + 4 g .. + 3 of row 32 i + c of acc[j][i].  Two accumulators
-    // (SILU: gate and up) go through the wave's own part of LDS at a time, 32 rows of 256 bytes, 16-byte piece p of
-    // row r at p ^ (r & 15).  One copy of the code that finishes and stores them serves all: a tile's stores are run
-    // once, and unrolled they came from memory instruction by instruction (48 KB of code: 25 us a tile).
-    uint8_t* const ob = lds + 2 * WSTAGE + wave * WOUT;
-    const int ncol = SILU ? a.half : a.n;
+    // Results, 32 rows x 64 columns at a time: lane (c, g) holds columns 32 j + 8 q + 4 g .. + 3 of row 32 i + c in
+    // acc[j][i].  They are finished and rounded there and go through the wave's own part of LDS, so that whole
+    // 128-byte lines leave; a residual comes the same way.  16-byte piece p of row r lies at p ^ (r & 7).  One copy
+    // of the code serves all chunks: unrolled it came from memory instruction by instruction (48 KB of code: 25 us a
+    // tile).  Stores are non-temporal: results of this many bytes would push operands out of L2 (8192 x 8192, k
+    // 16384: 890 -> 785 us).
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    uint8_t* const ob = lds + FACTORS + 2 * WT * 4 + wave * WOUT;
+    const int ncol = SILU ? a.half : a.n, lr0 = lane >> 3, rc = lane & 7;
+    const bool quick = a.vec_out >= 2 && on + (SILU ? 64 : 128) <= ncol;      // whole pieces in every row
+    const bool whole = quick && om + 128 <= a.m;
+    drain = !whole;
+    auto slot = [&](int r, int p) __attribute__((always_inline)) { return ob + r * 128 + ((p ^ (r & 7)) << 4); };
 #pragma unroll 1
-    for (int ch = 0; ch < 8; ++ch) {
-      auto put = [&](auto chc) __attribute__((always_inline)) {
-        constexpr int C = decltype(chc)::value, I = C >> 1, J = C & 1;
+    for (int ch = 0; ch < (SILU ? 4 : 8); ++ch) {
+      const int row0 = om + 32 * (SILU ? ch : ch >> 1), col = on + (SILU ? 0 : 64 * (ch & 1)) + 8 * rc;
+      if (!SILU && a.res) {
+        if (quick) {
+          uint4 v[4];
 #pragma unroll
-        for (int jj = 0; jj < 2; ++jj)
+          for (int t = 0; t < 4; ++t)
+            v[t] = *(const uint4*)((const O*)a.res + (int64_t)min(row0 + lr0 + 8 * t, a.m - 1) * a.rs + col);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const floatx16& v = acc[SILU ? J + 2 * jj : 2 * J + jj][I];
-            *(floatx4*)(ob + c * 256 + (((8 * jj + 2 * q + g) ^ (c & 15)) << 4)) =
-                floatx4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+          for (int t = 0; t < 4; ++t) *(uint4*)slot(lr0 + 8 * t, rc) = v[t];
+        } else {
+#pragma unroll 1
+          for (int lr = lr0; lr < 32; lr += 8) {
+            O v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              v[e] = row0 + lr < a.m && col + e < ncol ? ((const O*)a.res)[(int64_t)(row0 + lr) * a.rs + col + e] : (O)0.f;
+            uint4 u;
+            __builtin_memcpy(&u, v, 16);
+            *(uint4*)slot(lr, rc) = u;
           }
+        }
+      }
+      asm volatile("" ::: "memory");               // other lanes read what this one wrote
+      // the chunk's accumulators (SILU: gate columns, then the up columns)
+      int cl = c;
+      asm volatile("" : "+v"(cl));                 // addresses are formed here, not kept over the tile
+      floatx16 v[SILU ? 4 : 2];
+      auto pick = [&](auto chc) __attribute__((always_inline)) {
+        constexpr int C = decltype(chc)::value;
+#pragma unroll
+        for (int j = 0; j < (SILU ? 4 : 2); ++j) v[j] = SILU ? acc[j][C & 3] : acc[2 * (C & 1) + j][C >> 1];
       };
       switch (ch) {
-        case 0: put(std::integral_constant<int, 0>{}); break;
-        case 1: put(std::integral_constant<int, 1>{}); break;
-        case 2: put(std::integral_constant<int, 2>{}); break;
-        case 3: put(std::integral_constant<int, 3>{}); break;
-        case 4: put(std::integral_constant<int, 4>{}); break;
-        case 5: put(std::integral_constant<int, 5>{}); break;
-        case 6: put(std::integral_constant<int, 6>{}); break;
-        default: put(std::integral_constant<int, 7>{}); break;
+        case 0: pick(std::integral_constant<int, 0>{}); break;
+        case 1: pick(std::integral_constant<int, 1>{}); break;
+        case 2: pick(std::integral_constant<int, 2>{}); break;
+        case 3: pick(std::integral_constant<int, 3>{}); break;
+        case 4: pick(std::integral_constant<int, SILU ? 0 : 4>{}); break;
+        case 5: pick(std::integral_constant<int, SILU ? 0 : 5>{}); break;
+        case 6: pick(std::integral_constant<int, SILU ? 0 : 6>{}); break;
+        default: pick(std::integral_constant<int, SILU ? 0 : 7>{}); break;
       }
-      // eight columns a lane: 8 lanes to a row of 64 columns, or 4 to a row of 32 gate and 32 up columns
-      constexpr int LPR = SILU ? 4 : 8, RPI = 64 / LPR;
-      const int rc = lane & (LPR - 1);
-      const int col = on + (ch & 1) * (SILU ? 32 : 64) + 8 * rc;
-#pragma unroll 1
-      for (int lr = lane / LPR; lr < 32; lr += RPI) {
-        const int row = om + 32 * (ch >> 1) + lr;
-        const uint8_t* p = ob + lr * 256;
-        const int sw = lr & 15;
-        const floatx4 u0 = *(const floatx4*)(p + (((2 * rc) ^ sw) << 4)), u1 = *(const floatx4*)(p + (((2 * rc + 1) ^ sw) << 4));
-        if (row >= a.m || col >= ncol) continue;
-        const float r = a.rscale ? a.rscale[row] : 1.f;
-        float v[8];
-        if constexpr (SILU) {
-          const floatx4 w0 = *(const floatx4*)(p + (((2 * rc + 8) ^ sw) << 4)), w1 = *(const floatx4*)(p + (((2 * rc + 9) ^ sw) << 4));
+      const float r = a.rscale ? *(const float*)(lds + FACTORS + par * WT * 4 + (row0 - om + wm * 128 + c) * 4) : 1.f;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            v[e] = silu_mul_f32(r * u0[e], r * w0[e]);
-            v[4 + e] = silu_mul_f32(r * u1[e], r * w1[e]);
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint2* const p = (uint2*)(slot(cl, 4 * j + q) + 8 * g);
+          float f[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            f[e] = SILU ? silu_mul_f32(r * v[j][4 * q + e], r * v[SILU ? j + 2 : j][4 * q + e]) : r * v[j][4 * q + e];
+          O w[4];
+          if (!SILU && a.res) {
+            const uint2 u = *p;
+            __builtin_memcpy(w, &u, 8);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] += (float)w[e];
           }
-        } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) { v[e] = r * u0[e]; v[4 + e] = r * u1[e]; }
+          for (int e = 0; e < 4; ++e) w[e] = (O)f[e];
+          uint2 u;
+          __builtin_memcpy(&u, w, 8);
+          *p = u;
         }
-        store8<O>(a, row, col, ncol - col, v);
+      asm volatile("" ::: "memory");
+      if (quick) {
+        uint4 o[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) o[t] = *(const uint4*)slot(lr0 + 8 * t, rc);
+        O* const out = (O*)a.out + (int64_t)(row0 + lr0) * a.os + col;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const uint4 u = o[t];
+          if (whole || row0 + lr0 + 8 * t < a.m)
+            __builtin_nontemporal_store(u32x4{u.x, u.y, u.z, u.w}, (u32x4*)(out + (int64_t)(8 * t) * a.os));
+        }
+      } else {
+#pragma unroll 1
+        for (int lr = lr0; lr < 32; lr += 8) {
+          const uint4 u = *(const uint4*)slot(lr, rc);
+          O w[8];
+          __builtin_memcpy(w, &u, 16);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (row0 + lr < a.m && col + e < ncol) ((O*)a.out)[(int64_t)(row0 + lr) * a.os + col + e] = w[e];
+        }
       }
+      asm volatile("" ::: "memory");
     }
+    par ^= 1;
     if (!more) break;
   }
 }
 
-// Which kernel and tile, by modelled time: rounds of resident workgroups times
-// the k blocks times what a block takes with one and with two workgroups on a
-// CU (microseconds, measured at n 4096 and 7376, k 1640 to 11008, 8 to 8192
-// rows: the model picks the fastest of them within 10 %).  Small tiles fill
-// the chip with few rows; large ones read less per product.
+// Which kernel and tile, by modelled time: for each round of resident
+// workgroups a fixed part and a part for each k block (microseconds), with one
+// workgroup on a CU and with two; a 256 x 256 workgroup has its CU alone, and
+// its blocks go faster while others idle.  Fitted to 182 times of each tile at
+// n 1640 to 22016, k 512 to 11008, 48 to 4096 rows: the tile picked is the
+// fastest or within 7 % of it at all but one of them (12 %).  Small tiles fill the
+// chip with few rows; large ones read less per product: 4096 x 4096, k 4096
+// takes 178, 135, 98, 80 and 61 us on the tiles below; 256 rows 16, 16, 21,
+// 29 and 44.
 //   few rows  16 weight rows a workgroup, no LDS (m <= 16; to 32 rows while a
 //             second group of rows costs less than the tiles' fixed 4 us:
 //             n 4096, k 4096: 9.2 against 9.7 us; k 11008: 18.2 against 17.4)
@@ -624,15 +704,23 @@ Fp8Plan plan_fp8_gemm(int m, int n, int kb, bool silu, bool exact, bool pow2, in
     p.bn = silu ? 32 : 16;
     return p;
   }
-  struct Shape { int bm, bn; float one, two, fixed; };
-  static const Shape shapes[] = {{64, 32, 0.20f, 0.30f, 0.f}, {64, 64, 0.37f, 0.45f, 0.f}, {64, 128, 0.52f, 0.80f, 0.f},
-                                 {128, 128, 0.75f, 1.25f, 0.f}, {256, 256, 1.45f, 2.90f, 12.f}};
+  struct Shape { int bm, bn; float one, two, fix1, fix2; };        // 256 x 256: one of the only CU in use, two of all
+  static const Shape fast[] = {{64, 32, 0.14f, 0.27f, 2.f, 2.f}, {64, 64, 0.28f, 0.37f, 2.f, 3.5f},
+                               {64, 128, 0.42f, 0.575f, 2.f, 4.f}, {128, 128, 0.65f, 0.85f, 4.f, 7.4f},
+                               {256, 256, 1.05f, 1.40f, 8.f, 11.f}};
+  // the sums of a block scaled apart
+  static const Shape part[] = {{64, 32, 0.18f, 0.30f, 1.f, 1.3f}, {64, 64, 0.36f, 0.40f, 0.f, 2.4f},
+                               {64, 128, 0.48f, 0.65f, 2.3f, 2.6f}, {128, 128, 0.72f, 1.07f, 4.5f, 3.3f}};
+  const bool scaled = exact || !pow2;
   float best = 0.f;
-  for (const Shape& h : shapes) {
-    if ((h.bn == 32 && silu) || (h.bm == 256 && (exact || !pow2))) continue;
-    const int64_t tiles = ceil_div(m, h.bm) * ceil_div(n, h.bn), pairs = tiles / (2 * cus), rest = tiles - pairs * 2 * cus;
-    const float rest_t = rest == 0 ? 0.f : rest <= cus ? h.one : h.two;
-    const float t = kb * (pairs * h.two + rest_t) + h.fixed * (float)ceil_div(tiles, cus);
+  for (int i = 0; i < (scaled ? 4 : 5); ++i) {
+    const Shape& h = scaled ? part[i] : fast[i];
+    if (h.bn == 32 && silu) continue;
+    const int64_t tiles = ceil_div(m, h.bm) * ceil_div(n, h.bn), slots = h.bm == 256 ? cus : 2 * cus;
+    const int64_t rounds = tiles / slots, rest = tiles - rounds * slots;
+    float t = rounds * (kb * h.two + h.fix2);
+    if (rest && h.bm == 256) t += kb * (h.one + (h.two - h.one) * rest / cus) + h.fix1;
+    else if (rest) t += rest <= cus ? kb * h.one + h.fix1 : kb * h.two + h.fix2;
     if (p.bm == 0 || t < best) {
       best = t;
       p.bm = h.bm;

@@ -272,6 +272,46 @@ def test_large_tiles():
         assert torch.isfinite(out.float()).all()
 
 
+@pytest.mark.parametrize("epilogue,rms", [("none", None), ("none", 1e-5), ("residual", None), ("residual", 1e-5),
+                                          ("silu_mul", None), ("silu_mul", 1e-5)])
+@pytest.mark.parametrize("m,n,k", [(8192, 4608, 128), (4300, 8448, 264), (6000, 5888, 1000)])
+def test_every_tile_of_a_workgroup(m, n, k, epilogue, rms):
+    """Workgroups that take two and three tiles, whole and ragged ones: every result against the fp32 output of the
+    same product (another kernel, checked above on its own), odd rows into a wider buffer whose rest stays."""
+    _flush(f"[tiles] {m} {n} {k} {epilogue} {rms}")
+    n -= 0 if epilogue == "silu_mul" else m % 8          # (ragged columns, too, where m is)
+    c = make(m, n, k, BF16, BF16, E8, epilogue)
+    kw = {} if rms is None else dict(rms_eps=rms)
+    wide = n // 2 if epilogue == "silu_mul" else n
+    buf = torch.full((m + 1, wide + 8), 7.0, dtype=BF16, device="cuda")
+    out = buf[:m, :wide]
+    if c["res"] is not None:
+        out.copy_(c["res"])
+        c["res"] = out                                    # in place
+    want = call(c | dict(res=None if c["res"] is None else c["res"].float()), out_dtype=F32, **kw).double()
+    got = call(c, out=out, out_dtype=None, **kw)
+    assert got.data_ptr() == out.data_ptr()
+    torch.cuda.synchronize()
+    assert bool((buf[m] == 7.0).all()) and bool((buf[:, wide:] == 7.0).all())
+    # the instruction's 7 * 2^-13 of sum |x||w| (test_product's bound), by a product of magnitudes in fp32
+    from starkv import fp8_quantize
+    q, s = fp8_quantize(c["x"], E8)
+    xa = (q.float() * s.float().repeat_interleave(128, 1)[:, :k]).abs()
+    wa = (c["w"].float() * c["ws"].float().repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)[:, :k]).abs()
+    mag = (xa @ wa.t().contiguous()).double()
+    if rms is not None:
+        mag = mag / torch.sqrt(c["x"].double().square().mean(-1, keepdim=True) + rms)
+    bound = mag * (7 * 2.0 ** -13 + 2.0 ** -20)
+    if epilogue == "silu_mul":
+        # d(silu(g) u): |silu'| <= 1.1 and |silu(g)| <= |g| <= mag
+        bg, bu = bound[:, :wide], bound[:, wide:]
+        bound = 1.1 * bg * mag[:, wide:] + mag[:, :wide] * bu + 1.1 * bg * bu
+    lim = bound + (want.abs() + bound) * torch.finfo(BF16).eps / 2
+    worst = float(((out.double() - want).abs() / lim.clamp_min(1e-30)).max())
+    _flush(f"   worst error / bound = {worst:.3f}")
+    assert worst <= 1.0
+
+
 @pytest.mark.parametrize("m", [5, 40])
 def test_layouts_and_in_place(m):
     """Activations at odd offsets, a padded output whose other columns and rows stay, the residual in place, leading dims."""

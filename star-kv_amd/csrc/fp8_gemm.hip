@@ -55,7 +55,9 @@ __device__ inline void dma_dword_at(const uint8_t* base, uint32_t off, uint32_t 
 }
 // Wait until at most n stages of LOADS loads each are on their way (n is uniform, at most NST - 2), and for this
 // wave's LDS reads.
-__device__ constexpr int vm_lgkm0(int v) { return 0x0070 | (v & 15) | ((v >> 4) << 14); }     // s_waitcnt vmcnt(v) lgkmcnt(0)
+// s_waitcnt vmcnt(v) lgkmcnt(l)
+__device__ constexpr int vm_lgkm(int v, int l) { return 0x0070 | (v & 15) | ((v >> 4) << 14) | l << 8; }
+__device__ constexpr int vm_lgkm0(int v) { return vm_lgkm(v, 0); }
 template <int NST, int LOADS> __device__ inline void wait_stages(int n) {
   constexpr auto code = vm_lgkm0;
   static_assert(NST <= 7, "cases");
@@ -99,16 +101,15 @@ template <int WM, int WN, int I, int J, int KS, int NST, typename S, typename O,
 __global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN * KS + 3) / 4 * (KS * NST * (WM * I + WN * J) * 4096 <= 78000 ? 2 : 1))
 void fp8_gemm_kernel(const Fp8GemmArgs a) {
   constexpr int NW = WM * WN, TM = 32 * I, TN = 32 * J, BM = WM * TM, BN = WN * TN;
-  constexpr int LOADS = (BM + BN) / 8 / NW, LW = LOADS + 1;  // 1 KB loads (and one of scales) per wave and stage
+  constexpr int LOADS = (BM + BN) / 8 / NW;         // 1 KB loads per wave and stage
   static_assert(LOADS * 8 * NW == BM + BN, "whole loads");
   static_assert(!SILU || J % 2 == 0, "gate and up halves");
-  static_assert(NST >= 2 && (NST - 2) * LW < 64, "vmcnt");
   constexpr bool EXACT = __is_same(O, float);      // 16-bit instructions (see half_of)
   constexpr bool PART = EXACT || !S::pow2;         // a block's sums are scaled afterwards
   // a stage: rows, then a dword with the scale of each activation row and of two weight blocks
   constexpr int SLOTS = (BM + 2 + 63) / 64 * 64, ROWS = (BM + BN) * 128, STAGE = ROWS + SLOTS * 4;
-  constexpr int SLW = SLOTS / 64;                  // loads that fill the scales' slots
-  static_assert(SLW <= NW, "one load of scales per wave");
+  constexpr int SLW = SLOTS / 64, SL = (SLW + NW - 1) / NW, LW = LOADS + SL;       // loads that fill those slots, a wave's of them
+  static_assert(NST >= 2 && (NST - 2) * LW < 64, "vmcnt");
   __shared__ __attribute__((aligned(16))) uint8_t lds_all[KS * NST * STAGE];
   static_assert((KS - 1) * NW * I * J * 4096 <= KS * NST * STAGE, "the groups' sums fit");
 
@@ -148,16 +149,23 @@ void fp8_gemm_kernel(const Fp8GemmArgs a) {
     const int64_t r = row < BM ? min(m0 + row, a.m - 1) - m0 : min(wrow_of(row - BM), a.n - 1) - n0;
     off[i] = (uint32_t)(r * (row < BM ? a.xs : a.ws));
   }
-  // Scales go the same way, a dword a lane: this wave's load takes slots 64 (wave % SLW) .., which hold the scale
-  // of activation row slot, then of the tile's two weight blocks (the gate and the up rows', or 128 rows each).
+  // Scales go the same way, a dword a lane: this wave's loads take 64 slots each, which hold the scale of activation
+  // row slot, then of the tile's two weight blocks (the gate and the up rows', or 128 rows each).
   // (Power-of-two scales are bytes: the aligned dword that holds it is loaded, and the byte taken from it at the end.)
   typedef typename S::T ST;
-  const int slot0 = (wave % SLW) * 64, slot = slot0 + lane;
-  const bool xslot = slot < BM;
   auto wblock = [&](int u) { return min(SILU ? n0 + u * a.half : n0 + u * FP8_BLOCK, a.n - 1) >> 7; };
-  const ST* const sptr = xslot ? (const ST*)a.sx + (int64_t)min(m0 + slot, a.m - 1) * a.sxr
-                               : (const ST*)a.sw + (int64_t)wblock(slot == BM + 1) * a.swr;
-  const int64_t sstep = xslot ? a.sxb : a.swb;
+  const ST* sptr[SL];
+  int64_t sstep[SL];
+  int slot0[SL];
+#pragma unroll
+  for (int u = 0; u < SL; ++u) {
+    slot0[u] = (wave + u * NW) % SLW * 64;
+    const int slot = slot0[u] + lane;
+    const bool xslot = slot < BM;
+    sptr[u] = xslot ? (const ST*)a.sx + (int64_t)min(m0 + slot, a.m - 1) * a.sxr
+                    : (const ST*)a.sw + (int64_t)wblock(slot == BM + 1) * a.swr;
+    sstep[u] = xslot ? a.sxb : a.swb;
+  }
   const int last = (a.k - 1) >> 4;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)lds_all + kg * NST * STAGE;
   // load number i < LW of a stage for block kb
@@ -167,7 +175,8 @@ void fp8_gemm_kernel(const Fp8GemmArgs a) {
       const int p = min(kb * 8 + (q8 ^ rs ^ ((row >> 3) & 1)), last);
       dma_1k(row < BM ? xbase : wbase, off[i] + (uint32_t)p * 16, lds0 + stage + row * 128);
     } else {
-      dma_dword((const void*)((uintptr_t)(sptr + kb * sstep) & ~(uintptr_t)3), lds0 + stage + ROWS + slot0 * 4);
+      const int u = i - LOADS;
+      dma_dword((const void*)((uintptr_t)(sptr[u] + kb * sstep[u]) & ~(uintptr_t)3), lds0 + stage + ROWS + slot0[u] * 4);
     }
   };
   // the scale in slot `s` of a stage, p its address: as the instruction takes it (its byte in a register) or in fp32
@@ -495,8 +504,10 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_wide_kernel(const Fp8GemmArgs
     issue_last();
     issue_scales(0, end);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) issue1(WSTAGE, block(1), i);
+    for (int i = 0; i < 8; ++i) issue1(WSTAGE, block(1), i);
     issue_scales(WSTAGE, block(1));
+#pragma unroll
+    for (int i = 8; i < 16; ++i) issue1(WSTAGE, block(1), i);
   };
   start(par);
   // vmcnt counts in order: behind the start's loads stand the stores of the last tile, NSTORE of them if it was
@@ -533,26 +544,32 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_wide_kernel(const Fp8GemmArgs
     auto step = [&](int t, auto firstc) __attribute__((always_inline)) {
       constexpr bool FIRST = decltype(firstc)::value;
       bytes_of(sc, block(t));
+      const int kn = block(t + 2);
+      // a wait that leaves v loads on their way (and the first block's: the last tile's stores), and four reads
+      auto sync = [&](auto vc) __attribute__((always_inline)) {
+        constexpr int V = decltype(vc)::value;
+        if (FIRST && !drain) __builtin_amdgcn_s_waitcnt(vm_lgkm(V + NSTORE, 4));
+        else __builtin_amdgcn_s_waitcnt(vm_lgkm(V, 4));
+        asm volatile("s_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+      };
 #pragma unroll
       for (int q = 0; q < 16; ++q) {
         product(h0, q);
+        if (q == 12) issue_scales(cur, kn);
+        if (q >= 12) issue1(cur, kn, q - 12);
         read1(h1, lds + cur, 1, q);
         __builtin_amdgcn_sched_barrier(0);
+        if (q == 11) sync(std::integral_constant<int, 8>{});
       }
-      // half 1 read; this wave's part of the next stage landed
-      if (FIRST && !drain) __builtin_amdgcn_s_waitcnt(vm_lgkm0(NSTORE));
-      else __builtin_amdgcn_s_waitcnt(vm_lgkm0(0));
-      asm volatile("s_barrier" ::: "memory");
-      __builtin_amdgcn_sched_barrier(0);
-      const int kn = block(t + 2);
 #pragma unroll
       for (int q = 0; q < 16; ++q) {
         product(h1, q);
-        issue1(cur, kn, q);
+        if (q < 12) issue1(cur, kn, q + 4);
         read1(h0, lds + (cur ^ WSTAGE), 0, q);
-        if (q == 0) issue_scales(cur, kn);
         if (q == 8) scales(sn, cur ^ WSTAGE);
         __builtin_amdgcn_sched_barrier(0);
+        if (q == 3) sync(std::integral_constant<int, 10>{});
       }
       sc = sn;
       cur ^= WSTAGE;

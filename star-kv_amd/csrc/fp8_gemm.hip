@@ -48,27 +48,30 @@ __device__ inline void dma_1k(const uint8_t* base, uint32_t off, uint32_t lds) {
 __device__ inline void dma_dword(const void* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds) : "m0");
 }
+// The same where go is not 0: the branch stands inside the statement, so that a loop stays one block of code, within
+// which the compiler keeps the order given (it moved products over a branch of its own, away from the reads that
+// they are to cover).
+__device__ inline void dma_1k_if(int go, const uint8_t* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_cmp_eq_u32 %3, 0\n\ts_cbranch_scc1 1f\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1\n1:"
+               ::"v"(off), "s"(base), "s"(lds), "s"(go) : "m0", "scc");
+}
+__device__ inline void dma_dword_if(int go, const void* src, uint32_t lds) {
+  asm volatile("s_cmp_eq_u32 %2, 0\n\ts_cbranch_scc1 1f\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off\n1:"
+               ::"v"(src), "s"(lds), "s"(go) : "m0", "scc");
+}
+// Wait for LDS reads, and until at most LOADS loads are on their way (go not 0) or none.
+template <int LOADS> __device__ inline void wait_one_stage(int go) {
+  asm volatile("s_cmp_lg_u32 %0, 0\n\ts_cbranch_scc1 1f\n\ts_waitcnt vmcnt(0)\n1:\ts_waitcnt vmcnt(%1) lgkmcnt(0)"
+               ::"s"(go), "n"(LOADS) : "scc", "memory");
+}
 // the aligned dword with the byte at base + the lane's offset
 __device__ inline void dma_dword_at(const uint8_t* base, uint32_t off, uint32_t lds) {
   const uint32_t low = (uint32_t)(uintptr_t)base & 3;
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"((off + low) & ~3u), "s"(base - low), "s"(lds) : "m0");
 }
-// Wait until at most n stages of LOADS loads each are on their way (n is uniform, at most NST - 2), and for this
-// wave's LDS reads.
 // s_waitcnt vmcnt(v) lgkmcnt(l)
 __device__ constexpr int vm_lgkm(int v, int l) { return 0x0070 | (v & 15) | ((v >> 4) << 14) | l << 8; }
 __device__ constexpr int vm_lgkm0(int v) { return vm_lgkm(v, 0); }
-template <int NST, int LOADS> __device__ inline void wait_stages(int n) {
-  constexpr auto code = vm_lgkm0;
-  static_assert(NST <= 7, "cases");
-  if (NST > 6 && n == 5) __builtin_amdgcn_s_waitcnt(code(NST > 6 ? 5 * LOADS : 0));
-  else if (NST > 5 && n == 4) __builtin_amdgcn_s_waitcnt(code(NST > 5 ? 4 * LOADS : 0));
-  else if (NST > 4 && n == 3) __builtin_amdgcn_s_waitcnt(code(NST > 4 ? 3 * LOADS : 0));
-  else if (NST > 3 && n == 2) __builtin_amdgcn_s_waitcnt(code(NST > 3 ? 2 * LOADS : 0));
-  else if (NST > 2 && n == 1) __builtin_amdgcn_s_waitcnt(code(NST > 2 ? LOADS : 0));
-  else __builtin_amdgcn_s_waitcnt(code(0));
-}
-
 // Tile number -> (tm, tn): down eight row tiles before the next column, so that an XCD's L2 serves most reads of a
 // contiguous run of tiles.
 __device__ inline void tile_at(const Fp8GemmArgs& a, int tl, int& tm, int& tn) {
@@ -109,7 +112,7 @@ void fp8_gemm_kernel(const Fp8GemmArgs a) {
   // a stage: rows, then a dword with the scale of each activation row and of two weight blocks
   constexpr int SLOTS = (BM + 2 + 63) / 64 * 64, ROWS = (BM + BN) * 128, STAGE = ROWS + SLOTS * 4;
   constexpr int SLW = SLOTS / 64, SL = (SLW + NW - 1) / NW, LW = LOADS + SL;       // loads that fill those slots, a wave's of them
-  static_assert(NST >= 2 && (NST - 2) * LW < 64, "vmcnt");
+  static_assert(NST == 2 || (NST == 3 && LW < 32), "waits");
   __shared__ __attribute__((aligned(16))) uint8_t lds_all[KS * NST * STAGE];
   static_assert((KS - 1) * NW * I * J * 4096 <= KS * NST * STAGE, "the groups' sums fit");
 
@@ -168,15 +171,15 @@ void fp8_gemm_kernel(const Fp8GemmArgs a) {
   }
   const int last = (a.k - 1) >> 4;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)lds_all + kg * NST * STAGE;
-  // load number i < LW of a stage for block kb
-  auto issue1 = [&](int stage, int kb, int i) __attribute__((always_inline)) {
+  // load number i < LW of a stage for block kb, where go is not 0
+  auto issue1 = [&](int stage, int kb, int i, int go) __attribute__((always_inline)) {
     if (i < LOADS) {
       const int row = (wave * LOADS + i) * 8;      // uniform; the lane's piece of its row is q8 ^ swz(row + rs)
       const int p = min(kb * 8 + (q8 ^ rs ^ ((row >> 3) & 1)), last);
-      dma_1k(row < BM ? xbase : wbase, off[i] + (uint32_t)p * 16, lds0 + stage + row * 128);
+      dma_1k_if(go, row < BM ? xbase : wbase, off[i] + (uint32_t)p * 16, lds0 + stage + row * 128);
     } else {
       const int u = i - LOADS;
-      dma_dword((const void*)((uintptr_t)(sptr[u] + kb * sstep[u]) & ~(uintptr_t)3), lds0 + stage + ROWS + slot0[u] * 4);
+      dma_dword_if(go, (const void*)((uintptr_t)(sptr[u] + kb * sstep[u]) & ~(uintptr_t)3), lds0 + stage + ROWS + slot0[u] * 4);
     }
   };
   // the scale in slot `s` of a stage, p its address: as the instruction takes it (its byte in a register) or in fp32
@@ -208,12 +211,17 @@ void fp8_gemm_kernel(const Fp8GemmArgs a) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) rd[h][t] = c * 128 + (((4 * h + 2 * g + t) ^ f) << 4);
   struct Half { intx8 x[I], w[J]; };
-  auto read = [&](Half& o, const uint8_t* st, int h) __attribute__((always_inline)) {
-    auto get = [&](int row) { return frag8(*(const uint4*)(st + row * 128 + rd[h][0]), *(const uint4*)(st + row * 128 + rd[h][1])); };
-#pragma unroll
-    for (int i = 0; i < I; ++i) o.x[i] = get(wm * TM + 32 * i);
-#pragma unroll
-    for (int j = 0; j < J; ++j) o.w[j] = get(BM + wn * TN + 32 * j);
+  auto get = [&](const uint8_t* st, int h, int row) __attribute__((always_inline)) {
+    return frag8(*(const uint4*)(st + row * 128 + rd[h][0]), *(const uint4*)(st + row * 128 + rd[h][1]));
+  };
+  // operand e of a half: activations and weights in turn, as the products ask for them
+  constexpr int NR = I + J, NP = I * J;
+  auto read1 = [&](Half& o, const uint8_t* st, int h, int e) __attribute__((always_inline)) {
+    constexpr int L = 2 * (I < J ? I : J);
+    const bool isx = e < L ? (e & 1) == 0 : I > J;
+    const int k = e < L ? e >> 1 : e - L / 2;
+    if (isx) o.x[k] = get(st, h, wm * TM + 32 * k);
+    else o.w[k] = get(st, h, BM + wn * TN + 32 * k);
   };
 
   floatx16 acc[J][I], part[PART ? J : 1][PART ? I : 1];
@@ -221,35 +229,27 @@ void fp8_gemm_kernel(const Fp8GemmArgs a) {
   for (int j = 0; j < J; ++j)
 #pragma unroll
     for (int i = 0; i < I; ++i) acc[j][i] = floatx16{};
-  auto products = [&](const Half& o, const Sc& sc, auto h) __attribute__((always_inline)) {
+  auto product = [&](const Half& o, const Sc& sc, auto h, int q) __attribute__((always_inline)) {
     constexpr bool FIRST = decltype(h)::value == 0;
+    const int j = q % J, i = q / J;
+    if constexpr (EXACT) {
+      floatx16 p = FIRST ? floatx16{} : part[j][i];
 #pragma unroll
-    for (int j = 0; j < J; ++j)
-#pragma unroll
-      for (int i = 0; i < I; ++i) {
-        if constexpr (EXACT) {
-          floatx16 p = FIRST ? floatx16{} : part[j][i];
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            p = __builtin_amdgcn_mfma_f32_32x32x16_f16(half_of(o.w[j], q), half_of(o.x[i], q), p, 0, 0, 0);
-          part[j][i] = p;
-        } else if constexpr (PART) {
-          part[j][i] = mfma8_32(o.w[j], o.x[i], FIRST ? floatx16{} : part[j][i], E8_ONE, E8_ONE);
-        } else {
-          acc[j][i] = mfma8_32(o.w[j], o.x[i], acc[j][i], sc.w[SILU ? j / (J / 2) : 0], sc.x[i]);
-        }
-      }
+      for (int u = 0; u < 4; ++u)
+        p = __builtin_amdgcn_mfma_f32_32x32x16_f16(half_of(o.w[j], u), half_of(o.x[i], u), p, 0, 0, 0);
+      part[j][i] = p;
+    } else if constexpr (PART) {
+      part[j][i] = mfma8_32(o.w[j], o.x[i], FIRST ? floatx16{} : part[j][i], E8_ONE, E8_ONE);
+    } else {
+      acc[j][i] = mfma8_32(o.w[j], o.x[i], acc[j][i], sc.w[SILU ? j / (J / 2) : 0], sc.x[i]);
+    }
   };
-  auto rescale = [&](const Sc& sc) __attribute__((always_inline)) {
+  auto rescale = [&](const Sc& sc, int q) __attribute__((always_inline)) {
     if constexpr (PART) {
+      const int j = q % J, i = q / J;
+      const float s = scale_f32((ST)sc.x[i]) * scale_f32((ST)sc.w[SILU ? j / (J / 2) : 0]);
 #pragma unroll
-      for (int j = 0; j < J; ++j)
-#pragma unroll
-        for (int i = 0; i < I; ++i) {
-          const float s = scale_f32((ST)sc.x[i]) * scale_f32((ST)sc.w[SILU ? j / (J / 2) : 0]);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[j][i][e] = fmaf(part[j][i][e], s, acc[j][i][e]);
-        }
+      for (int e = 0; e < 16; ++e) acc[j][i][e] = fmaf(part[j][i][e], s, acc[j][i][e]);
     }
   };
 
@@ -261,8 +261,11 @@ void fp8_gemm_kernel(const Fp8GemmArgs a) {
 #pragma unroll 1
   for (int t = 0; t < min(n, NST); ++t)
 #pragma unroll
-    for (int i = 0; i < LW; ++i) issue1(t * STAGE, block(t), i);
-  wait_stages<NST + 1, LW>(max(0, min(n, NST) - 1));
+    for (int i = 0; i < LW; ++i) issue1(t * STAGE, block(t), i, 1);
+  // the first stage landed
+  if (n >= NST) __builtin_amdgcn_s_waitcnt(vm_lgkm0((NST - 1) * LW));
+  else if (NST > 2 && n > 1) __builtin_amdgcn_s_waitcnt(vm_lgkm0(LW));
+  else __builtin_amdgcn_s_waitcnt(vm_lgkm0(0));
   asm volatile("s_barrier" ::: "memory");
   if (a.k & (FP8_BLOCK - 1)) {
     if (kg == 0) zero_tail<BM + BN, 64 * NW>(lds, a.k & (FP8_BLOCK - 1), wave * 64 + lane);
@@ -273,27 +276,40 @@ void fp8_gemm_kernel(const Fp8GemmArgs a) {
   const std::integral_constant<int, 1> second{};
   Half h0, h1;
   Sc sc, sn;
-  read(h0, lds, 0);
+#pragma unroll
+  for (int e = 0; e < NR; ++e) read1(h0, lds, 0, e);
   scales(sc, lds, block(0));
   int cur = 0;
   for (int t = 0; t < n; ++t) {                    // block(t) in stage `cur`, its half 0 in h0, its scales in sc
-    read(h1, lds + cur, 1);
-    products(h0, sc, first);
-    __builtin_amdgcn_sched_barrier(0);
-    // half 1 read; this wave's part of the next stage landed (those of up to NST - 2 more may be on their way)
-    wait_stages<NST, LW>(max(0, min(n - 2 - t, NST - 2)));
+#pragma unroll
+    for (int q = 0; q < NP; ++q) {
+      product(h0, sc, first, q);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int e = q * NR / NP; e < (q + 1) * NR / NP; ++e) read1(h1, lds + cur, 1, e);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // half 1 read; this wave's part of the next stage landed (with three stages, that of one more may be on its way)
+    if constexpr (NST == 2) __builtin_amdgcn_s_waitcnt(vm_lgkm0(0));
+    else wait_one_stage<LW>(max(0, n - 2 - t));
     asm volatile("s_barrier" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
     const int nxt = cur == (NST - 1) * STAGE ? 0 : cur + STAGE;
     // (behind the last block: reads of what is there, for nobody)
-    read(h0, lds + nxt, 0);
     scales(sn, lds + nxt, block(t + 1));
-    if (t + NST < n) {
+    const int more = max(0, n - NST - t), kn = block(t + NST);
 #pragma unroll
-      for (int i = 0; i < LW; ++i) issue1(cur, block(t + NST), i);
+    for (int q = 0; q < NP; ++q) {
+      product(h1, sc, second, q);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = q * LW / NP; i < (q + 1) * LW / NP; ++i) issue1(cur, kn, i, more);
+#pragma unroll
+      for (int e = q * NR / NP; e < (q + 1) * NR / NP; ++e) read1(h0, lds + nxt, 0, e);
+      if (q) rescale(sc, q - 1);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    products(h1, sc, second);
-    rescale(sc);
+    rescale(sc, NP - 1);
     sc = sn;
     cur = nxt;
   }

@@ -493,7 +493,8 @@ int starkv_skinny_gemm(const starkv_skinny_gemm_desc* d, void* stream);
  * each block of the row, weights [n][k] one for each block of 128 rows x 128
  * columns.  Scales are STARKV_E8M0 (powers of two, one byte) or STARKV_F32,
  * scale (r, b) at scale + r * scale_stride_r + b * scale_stride_b elements,
- * r the row of an activation and row / 128 of a weight.
+ * r the row of an activation and row / 128 of a weight.  The aligned dword
+ * that holds a one-byte scale may be read whole.
  *
  * starkv_fp8_quantize: x (dtype F16 or BF16, row r at x + r * x_stride
  * elements) to e4m3 rows at q + r * q_stride bytes and their scales.  With
@@ -521,7 +522,8 @@ int starkv_fp8_quantize(const starkv_fp8_quantize_desc* d, void* stream);
 
 /* starkv_fp8_gemm: nn.Linear by an e4m3 weight,
  *   y[i][j] = r_i * sum_b sx[i][b] sw[j / 128][b] sum_{k in b} qx[i][k] qw[j][k]
- * accumulated in fp32 and rounded once to out_dtype (the act dtypes or F32):
+ * accumulated in fp32 (sx sw too is formed in fp32 or exactly) and rounded
+ * once to out_dtype (the act dtypes or F32):
  *   out[i][j] = y[i][j] (+ residual[i][j])                        j < n
  *   silu_mul: out[i][j] = y[i][j] / (1 + exp(-y[i][j])) * y[i][n/2 + j]   j < n/2
  *             (LlamaMLP over the gate rows followed by the up rows of one

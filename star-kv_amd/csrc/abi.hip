@@ -1569,7 +1569,7 @@ int starkv_fp8_gemm(const starkv_fp8_gemm_desc* d, void* workspace, size_t works
   if (!sp.plan.few) {
     const int64_t lim = ((int64_t)1 << 32) - 1, wr = 256 + (d->silu_mul ? d->n / 2 : 0);
     if ((q ? round_up(d->k, 16) : d->x_stride) > (lim - d->k) / 256 || d->w_stride > (lim - d->k) / wr ||
-        (!q && d->x_scale_stride_r > lim / 1024))
+        (!q && d->x_scale_stride_r > lim / 1024) || (d->silu_mul && d->w_scale_stride_r > lim / (d->n / 256 + 8)))
       return STARKV_ERR_LIMIT;
   }
   Fp8GemmArgs a = {};

@@ -621,12 +621,12 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_wide_kernel(const Fp8GemmArgs
       const int row0 = om + 32 * (SILU ? ch : ch >> 1), col = on + (SILU ? 0 : 64 * (ch & 1)) + 8 * rc;
       if (!SILU && a.res) {
         if (quick) {
-          uint4 v[4];
+          u32x4 v[4];
 #pragma unroll
           for (int t = 0; t < 4; ++t)
-            v[t] = *(const uint4*)((const O*)a.res + (int64_t)min(row0 + lr0 + 8 * t, a.m - 1) * a.rs + col);
+            v[t] = *(const u32x4*)((const O*)a.res + (int64_t)min(row0 + lr0 + 8 * t, a.m - 1) * a.rs + col);
 #pragma unroll
-          for (int t = 0; t < 4; ++t) *(uint4*)slot(lr0 + 8 * t, rc) = v[t];
+          for (int t = 0; t < 4; ++t) *(u32x4*)slot(lr0 + 8 * t, rc) = v[t];
         } else {
 #pragma unroll 1
           for (int lr = lr0; lr < 32; lr += 8) {
@@ -685,15 +685,14 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_wide_kernel(const Fp8GemmArgs
         }
       asm volatile("" ::: "memory");
       if (quick) {
-        uint4 o[4];
+        u32x4 o[4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) o[t] = *(const uint4*)slot(lr0 + 8 * t, rc);
+        for (int t = 0; t < 4; ++t) o[t] = *(const u32x4*)slot(lr0 + 8 * t, rc);
         O* const out = (O*)a.out + (int64_t)(row0 + lr0) * a.os + col;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          const uint4 u = o[t];
           if (whole || row0 + lr0 + 8 * t < a.m)
-            __builtin_nontemporal_store(u32x4{u.x, u.y, u.z, u.w}, (u32x4*)(out + (int64_t)(8 * t) * a.os));
+            __builtin_nontemporal_store(o[t], (u32x4*)(out + (int64_t)(8 * t) * a.os));
         }
       } else {
 #pragma unroll 1

@@ -27,7 +27,7 @@ import torch.nn.functional as F
 from ._lib import StarKVError
 from .cache import LatentCache
 from .fp8 import fp8_linear, fp8_quantize_weight
-from .logprobs import TokenLogprobs, token_logprobs
+from .logprobs import MAX_TOP, TokenLogprobs, token_logprobs
 from .ops import GEMM_ADD, GEMM_SILU_MUL, SKINNY_MAX_ROWS, decode_attention, prefill_attention, skinny_linear
 from .rope import RopeConfig
 
@@ -501,6 +501,13 @@ def attention_layers(model) -> List[LatentAttention]:
     return [layer.self_attn for layer in model.model.layers]
 
 
+def _check_top(model, top: Optional[int]) -> None:
+    """Refuse a number of alternatives before anything has run (the caches would have moved on)."""
+    most = min(MAX_TOP, model.lm_head.weight.shape[0])
+    if top is not None and not 0 <= top <= most:
+        raise StarKVError(f"the number of alternatives must be 0 .. {most}, got {top}")
+
+
 @torch.no_grad()
 def generate(model, prompt: torch.Tensor, steps: int, reference: bool = False,
              forced: Optional[torch.Tensor] = None, logprobs: Optional[int] = None):
@@ -510,6 +517,7 @@ def generate(model, prompt: torch.Tensor, steps: int, reference: bool = False,
     Returns (tokens [B, steps + 1], logits of the last position per forward)
     and, where ``logprobs`` is a number of alternatives (0 .. 64), the
     ``TokenLogprobs`` [B, steps + 1] of the tokens returned."""
+    _check_top(model, logprobs)
     for att in attention_layers(model):
         att.reference = reference
     model.model.norm.starkv_reference = reference
@@ -551,6 +559,7 @@ def score(model, tokens: torch.Tensor, top: int = 0, reference: bool = False) ->
         raise StarKVError(f"score: tokens must be [B, T] with T at least 1, got shape {tuple(tokens.shape)}")
     if tokens.dtype != torch.int64:
         raise StarKVError(f"score: tokens must be int64, got {tokens.dtype}")
+    _check_top(model, top)
     atts = attention_layers(model)
     B, T = tokens.shape
     V = model.lm_head.weight.shape[0]
@@ -579,6 +588,7 @@ def generate_graphed(model, prompt: torch.Tensor, steps: int, keep_logits: bool 
     (``decode_graphed``).  Returns (tokens [B, steps + 1], logits of the last
     position per forward, or [] when ``keep_logits`` is False) and, where
     ``logprobs`` is given, the ``TokenLogprobs`` as ``generate`` does."""
+    _check_top(model, logprobs)
     for att in attention_layers(model):
         att.reference = False
     model.model.norm.starkv_reference = False
@@ -610,6 +620,7 @@ def decode_graphed(model, tok: torch.Tensor, steps: int, keep_logits: bool = Tru
     (tokens [B, steps], logits per step or []) and, where ``logprobs`` is a
     number of alternatives, the ``TokenLogprobs`` [B, steps] of the tokens,
     computed inside the graph."""
+    _check_top(model, logprobs)
     atts = attention_layers(model)
     B = tok.shape[0]
     dev = tok.device

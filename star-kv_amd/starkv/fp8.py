@@ -23,6 +23,7 @@ __all__ = ["fp8_quantize", "fp8_quantize_weight", "fp8_matmul", "fp8_linear"]
 
 BLOCK = 128
 E4M3_MAX = 448.0
+MAX_DIM = 1 << 30                    # rows and columns of one call
 _ACT = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 _OUT = {**_ACT, torch.float32: _lib.F32}
 _SCALE = {torch.float8_e8m0fnu: _lib.E8M0, torch.float32: _lib.F32}
@@ -52,6 +53,8 @@ def _rows2d(t: torch.Tensor, name: str) -> Tuple[torch.Tensor, int, int, int]:
             raise StarKVError(f"{name} rows must be addressable with one row stride") from None
         shape, stride = t.shape, t.stride()
     m = shape[0]
+    if m > MAX_DIM or w > MAX_DIM:
+        raise StarKVError(f"{name} has more than {MAX_DIM} rows or columns: {tuple(shape)}")
     return t, m, w, (stride[0] if m > 1 else -(-w // 16) * 16)
 
 

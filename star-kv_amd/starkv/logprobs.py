@@ -13,6 +13,7 @@ from .ops import _dt, _launch, _out
 __all__ = ["TokenLogprobs", "token_logprobs", "MAX_TOP"]
 
 MAX_TOP = 64                         # STARKV_MAX_TOP
+MAX_ROWS = 1 << 30                   # of one call (fewer where rows are many: the library says)
 
 
 class TokenLogprobs(NamedTuple):
@@ -32,6 +33,8 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise StarKVError(f"logits must be [..., V], got shape {tuple(logits.shape)}")
     dev, v, lead = logits.device, logits.shape[-1], logits.shape[:-1]
+    if lead.numel() > MAX_ROWS:
+        raise StarKVError(f"logits have more than {MAX_ROWS} rows: {tuple(logits.shape)}")
     if dev.type != "cuda":
         raise StarKVError("libstarkv operators take device tensors (there is no CPU path)")
     if not 0 <= top <= min(MAX_TOP, v):

@@ -155,3 +155,19 @@ def test_quantize_weight_norm_zero_and_nan():
                 lambda: fp8_quantize_weight(w, torch.float16), lambda: fp8_quantize_weight(w, norm_weight=nw[:3])):
         with pytest.raises(StarKVError):
             bad()
+
+
+def test_dimensions_that_pass_32_bits_are_refused():
+    """A row count that the C interface's int cannot hold is an error, not its low bits."""
+    from starkv import StarKVError, fp8_quantize, token_logprobs
+    many = torch.zeros(1, 1, dtype=torch.float16).expand(2 ** 32 + 5, 1)
+    with pytest.raises(StarKVError, match="rows or columns"):
+        fp8_quantize(many)
+    with pytest.raises(StarKVError, match="rows"):
+        token_logprobs(many)
+
+
+def test_gemm_refuses_weight_scales_too_far_apart():
+    """With SiLU-multiply a tile's up rows' scales are reached by a 32-bit offset from its gate rows'."""
+    d = _set(_gemm(), m=512, n=4096, out_stride=4096, silu_mul=1, w_scale_stride_r=2 ** 29)
+    assert L.lib().starkv_fp8_gemm(ctypes.byref(d), FAKE, 1 << 40, None) == LIMIT

@@ -26,8 +26,16 @@ def test_fuse_layers_refuses_before_it_changes_anything():
 
 def test_score_refuses():
     from starkv import StarKVError
-    from starkv.e2e import score
+    from starkv.e2e import decode_graphed, generate, generate_graphed, score
     model = _model()
+    ids = torch.zeros(1, 4, dtype=torch.int64)
+    for top in (-1, 65):                                 # before any forward: the caches stay where they are
+        for call in (lambda: score(model, ids, top=top), lambda: generate(model, ids, 1, logprobs=top),
+                     lambda: generate_graphed(model, ids, 1, logprobs=top),
+                     lambda: decode_graphed(model, ids[:, :1], 1, logprobs=top)):
+            with pytest.raises(StarKVError, match="alternatives"):
+                call()
+        assert model.model.layers[0].self_attn.cache.length == 0
     for tokens in (torch.zeros(4, dtype=torch.int64), torch.zeros(1, 0, dtype=torch.int64),
                    torch.zeros(1, 4, dtype=torch.int32)):
         with pytest.raises(StarKVError, match="score"):

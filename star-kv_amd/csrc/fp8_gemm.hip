@@ -713,20 +713,23 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_wide_kernel(const Fp8GemmArgs
 }
 
 // Which kernel and tile, by modelled time: for each round of resident
-// workgroups a fixed part and a part for each k block (microseconds), with one
-// workgroup on a CU and with two; a 256 x 256 workgroup has its CU alone, and
-// its blocks go faster while others idle.  Fitted to 182 times of each tile at
-// n 1640 to 22016, k 512 to 11008, 48 to 4096 rows: the tile picked is the
-// fastest or within 7 % of it at all but one of them (12 %).  Small tiles fill the
-// chip with few rows; large ones read less per product: 4096 x 4096, k 4096
-// takes 178, 135, 98, 80 and 61 us on the tiles below; 256 rows 16, 16, 21,
-// 29 and 44.
-//   few rows  16 weight rows a workgroup, no LDS (m <= 16; to 32 rows while a
-//             second group of rows costs less than the tiles' fixed 4 us:
-//             n 4096, k 4096: 9.2 against 9.7 us; k 11008: 18.2 against 17.4)
-//   64 x 32   4 k groups of waves, one workgroup a CU; 2 k groups, two
-//   64 x 64   2 k groups      64 x 128, 128 x 128   one
-//   256 x 256 power-of-two scales and 16-bit outputs
+// workgroups a fixed part and a part for each k block (microseconds).  Tiles
+// of 64 and 128 columns run with one workgroup on a CU or two, the larger ones
+// alone, and their blocks go the faster the more CUs idle.  Fitted to the
+// times of every tile in 196 products of n 1640 to 22016, k 512 to 11008, 48
+// to 8192 rows: the tile picked is the fastest or within 6 % of it in all but
+// two (13 % of 7.7 us).  Small tiles fill the chip with few rows, large ones
+// read less per product: powers of two, 4096 x 4096, k 4096 takes 177, 136,
+// 96, 80, 80 and 60 us on the tiles below, 256 rows of it 16, 16, 21, 29, 39
+// and 44.
+//   few rows   16 weight rows a workgroup, no LDS (m <= 16; to 32 rows while a
+//              second group of rows costs less than the tiles' fixed 4 us:
+//              n 4096, k 4096: 9.2 against 9.7 us; k 11008: 18.2 against 17.4)
+//   64 x 32    4 k groups of waves, one workgroup a CU; 2 k groups, two
+//   64 x 64    2 k groups      64 x 128, 128 x 128   one
+//   128 x 256  eight waves, three stages (fp32 scales, 2048 x 4096, k 11008:
+//              109 us on 128 x 128, 97 on these)
+//   256 x 256  power-of-two scales and 16-bit outputs
 Fp8Plan plan_fp8_gemm(int m, int n, int kb, bool silu, bool exact, bool pow2, int cus) {
   Fp8Plan p = {};
   p.cus = cus;
@@ -736,22 +739,24 @@ Fp8Plan plan_fp8_gemm(int m, int n, int kb, bool silu, bool exact, bool pow2, in
     p.bn = silu ? 32 : 16;
     return p;
   }
-  struct Shape { int bm, bn; float one, two, fix1, fix2; };        // 256 x 256: one of the only CU in use, two of all
-  static const Shape fast[] = {{64, 32, 0.14f, 0.27f, 2.f, 2.f}, {64, 64, 0.28f, 0.37f, 2.f, 3.5f},
-                               {64, 128, 0.42f, 0.575f, 2.f, 4.f}, {128, 128, 0.65f, 0.85f, 4.f, 7.4f},
-                               {256, 256, 1.05f, 1.40f, 8.f, 11.f}};
+  struct Shape { int bm, bn; float one, two, fix1, fix2; };        // 256 columns: one of the only CU in use, two of all
+  static const Shape fast[] = {{64, 32, 0.15f, 0.27f, 1.8f, 2.3f},  {64, 64, 0.29f, 0.37f, 1.8f, 3.5f},
+                               {64, 128, 0.36f, 0.58f, 2.1f, 3.7f}, {128, 128, 0.62f, 0.87f, 3.8f, 8.3f},
+                               {128, 256, 0.60f, 0.83f, 4.8f, 9.0f}, {256, 256, 0.92f, 1.37f, 8.2f, 8.9f}};
   // the sums of a block scaled apart
-  static const Shape part[] = {{64, 32, 0.18f, 0.30f, 1.f, 1.3f}, {64, 64, 0.36f, 0.40f, 0.f, 2.4f},
-                               {64, 128, 0.48f, 0.65f, 2.3f, 2.6f}, {128, 128, 0.72f, 1.07f, 4.5f, 3.3f}};
+  static const Shape part[] = {{64, 32, 0.15f, 0.27f, 1.8f, 2.3f},  {64, 64, 0.31f, 0.37f, 1.8f, 3.6f},
+                               {64, 128, 0.43f, 0.62f, 2.0f, 3.8f}, {128, 128, 0.64f, 0.94f, 4.2f, 8.2f},
+                               {128, 256, 0.62f, 0.88f, 4.8f, 9.2f}};
   const bool scaled = exact || !pow2;
   float best = 0.f;
-  for (int i = 0; i < (scaled ? 4 : 5); ++i) {
+  for (int i = 0; i < (scaled ? 5 : 6); ++i) {
     const Shape& h = scaled ? part[i] : fast[i];
     if (h.bn == 32 && silu) continue;
-    const int64_t tiles = ceil_div(m, h.bm) * ceil_div(n, h.bn), slots = h.bm == 256 ? cus : 2 * cus;
+    const bool alone = h.bn == 256;
+    const int64_t tiles = ceil_div(m, h.bm) * ceil_div(n, h.bn), slots = alone ? cus : 2 * cus;
     const int64_t rounds = tiles / slots, rest = tiles - rounds * slots;
     float t = rounds * (kb * h.two + h.fix2);
-    if (rest && h.bm == 256) t += kb * (h.one + (h.two - h.one) * rest / cus) + h.fix1;
+    if (rest && alone) t += kb * (h.one + (h.two - h.one) * rest / cus) + h.fix1;
     else if (rest) t += rest <= cus ? kb * h.one + h.fix1 : kb * h.two + h.fix2;
     if (p.bm == 0 || t < best) {
       best = t;
@@ -782,6 +787,7 @@ template <typename O, bool SILU> static int launch_wide(Fp8GemmArgs a, int cus, 
 template <typename S, typename O, bool SILU> static int launch_shape(const Fp8GemmArgs& a, const Fp8Plan& p, hipStream_t st) {
   if constexpr (!__is_same(O, float) && S::pow2)
     if (p.bm == 256) return launch_wide<O, SILU>(a, p.cus, st);
+  if (p.bn == 256) return launch_tile<2, 4, 2, 2, 1, 3, S, O, SILU>(a, st);
   if (p.bm == 128) return launch_tile<2, 2, 2, 2, 1, 2, S, O, SILU>(a, st);
   if (p.bn == 128) return launch_tile<2, 2, 1, 2, 1, 3, S, O, SILU>(a, st);
   if constexpr (!SILU)

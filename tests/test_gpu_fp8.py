@@ -272,6 +272,22 @@ def test_large_tiles():
         assert torch.isfinite(out.float()).all()
 
 
+@pytest.mark.parametrize("scale,out,epilogue", [(E8, BF16, "none"), (F32, BF16, "residual"), (F32, F32, "none"),
+                                                (E8, F16, "silu_mul"), (F32, F16, "silu_mul")])
+def test_long_products_of_some_rows(scale, out, epilogue):
+    """A tile for nearly every compute unit and many blocks (eight waves to a workgroup), ragged at every edge:
+    checked on rows at the tiles' edges, every column."""
+    m, n, k = 2000, 4096 if epilogue == "silu_mul" else 4092, 5000
+    _flush(f"[long] {scale} {out} {epilogue}")
+    c = make(m, n, k, BF16, out, scale, epilogue)
+    got = call(c)
+    assert torch.isfinite(got.float()).all()
+    rows = torch.tensor([0, 1, 31, 32, 127, 128, 1023, 1024, 1919, 1920, 1998, 1999])
+    sub = dict(c, m=len(rows), x=c["x"][rows.cuda()], res=None if c["res"] is None else c["res"][rows.cuda()])
+    check(got[rows.cuda()], sub)
+    assert torch.equal(got, call(c))
+
+
 @pytest.mark.parametrize("epilogue,rms", [("none", None), ("none", 1e-5), ("residual", None), ("residual", 1e-5),
                                           ("silu_mul", None), ("silu_mul", 1e-5)])
 @pytest.mark.parametrize("m,n,k", [(8192, 4608, 128), (4300, 8448, 264), (6000, 5888, 1000)])

@@ -380,17 +380,26 @@ void fp8_gemm_kernel(const Fp8GemmArgs a) {
 // 128 KB of LDS reads and 64 KB of writes per block, 1536 cycles at 128
 // bytes, where eight waves of 64 x 128 would take all of the 2048.
 //
-// A block is two halves of 64 columns, each with operand registers of its own:
-//   * half 0's products run while half 1's operands are read;
-//   * then every wave has read this stage and (its loads have landed and) the
-//     next stage is whole: the one barrier of the block;
-//   * half 1's products run while the next block's half 0 is read, and the
-//     block after that is loaded into the stage just freed.
-// So neither the barrier nor an LDS read is waited for with the matrix cores
-// idle.  A workgroup takes tile after tile: the next tile's first blocks load
-// while this one's results are stored, by way of LDS so that whole 128-byte
-// lines leave (straight from the accumulators' layout, 16 bytes a row, the
-// stores of a tile took as long as 1600 columns of products).
+// A block is two halves of 64 columns, each with operand registers of its own,
+// 16 products to a half:
+//   * half 0's products run while half 1's operands are read, those of the
+//     first two row groups first;
+//   * behind product 12 these have been read: all waves meet, and the first
+//     half of the stage's rows is loaded anew, for the block after next;
+//   * behind product 20 (the fourth of half 1) the rest has been read: they
+//     meet again, and the other half is loaded;
+//   * half 1's products run while the next block's half 0 is read.
+// At each meeting a wave waits for the loads it issued 24 products ago, not for
+// the last ones, and for all but its last four reads: nothing is waited for
+// with the matrix cores idle unless memory is late.  (One meeting, after half
+// 0: loads in a burst of 16 products, 16 products to land: 2 % slower.)
+// Measured: 1.4 us a block on all CUs, where products alone take 1.0; without
+// the loads 1.2, without the reads 1.24.  8192 x 22016 x 4096 with SiLU: 565 us,
+// 2610 TFLOP/s.
+//
+// A workgroup takes tile after tile: the next tile's first two blocks load
+// while this one's results are stored, and the stores drain behind the next
+// tile's first block.
 // ---------------------------------------------------------------------------
 constexpr int WT = 256;                            // tile rows and columns
 constexpr int WSTAGE = 2 * WT * 128;               // bytes of a stage

@@ -378,6 +378,40 @@ def test_linear_is_quantize_then_matmul(m, scale):
     assert torch.equal(fp8_linear(c["x"], c["w"], c["ws"]), fp8_matmul(q, s, c["w"], c["ws"], out_dtype=F16))
 
 
+def test_offsets_past_32_bits():
+    """Activations, weights and results of more than 2^31 elements: the rows and columns at their ends."""
+    from starkv import fp8_linear, fp8_matmul, fp8_quantize
+    g = torch.Generator(device="cuda").manual_seed(9)
+    # quantiser: 2^20 + 3 rows of 4096
+    m, k = (1 << 20) + 3, 4096
+    x = torch.zeros(m, k, dtype=F16, device="cuda")
+    rows = torch.tensor([0, (1 << 19) - 1, 1 << 19, m - 2, m - 1])
+    x[rows.cuda()] = torch.randn(len(rows), k, generator=g, device="cuda").half()
+    q, s = fp8_quantize(x)
+    rq, rs = ref_quantize(x[rows.cuda()], E8)
+    assert _eq(q[rows.cuda()].double().cpu(), rq) and _eq(s[rows.cuda()].double().cpu(), rs)
+    del x, q, s
+    # weight: 4.3 GB, by the stream (m 3) and by tiles (m 40)
+    n = (1 << 20) + 130
+    w = torch.zeros(n, 4096, dtype=torch.uint8, device="cuda").view(E4M3)
+    ws = torch.ones(-(-n // 128), 32, device="cuda").to(E8)
+    n0 = (n - 300) // 128 * 128
+    w[n0:] = (torch.randn(n - n0, 4096, generator=g, device="cuda") * 20).to(E4M3)
+    for m in (3, 40):
+        x = torch.randn(m, 4096, generator=g, device="cuda").half()
+        out = fp8_linear(x, w, ws)
+        assert int(out[:, :n0].count_nonzero()) == 0
+        check(out[:, n0:], dict(m=m, n=n - n0, k=4096, x=x, w=w[n0:], ws=ws[n0 // 128:], dtype=F16, out=F16, scale=E8,
+                                res=None, epilogue="none"))
+    del w, ws, out
+    # results: 70001 x 32768
+    m, n, k = 70001, 32768, 128
+    c = make(m, n, k, BF16, BF16, E8, "none")
+    out = call(c)
+    rows = torch.tensor([0, 32767, 32768, 65535, 65536, 69999, 70000])
+    check(out[rows.cuda()], dict(c, m=len(rows), x=c["x"][rows.cuda()]))
+
+
 def test_streams_and_graphs():
     """On another stream, and captured once and replayed with new inputs beside eager calls of other sizes."""
     from starkv import fp8_linear, fp8_quantize

@@ -221,3 +221,20 @@ def test_score_after_a_shared_prefix():
     rel = float((part.logprob - whole.logprob[:, 17:]).abs().mean() / whole.logprob.abs().mean())
     print(f"   logprob mean_rel={rel:.2e}", flush=True)
     assert rel <= 1e-3
+
+
+def test_one_token_prompts_and_texts():
+    """A prompt of one token (every forward is a decode step), a text of two, one sequence."""
+    import starkv.e2e as e2e
+    kw = dict(KW, batch=1)
+    model = e2e.build_model(**kw, fmt="int8_g64", seed=8, fp8=F32)
+    prompt = _prompt(3)[:1, :1]
+    toks, logits, probs = e2e.generate(model, prompt, 3, logprobs=0)
+    assert toks.shape == probs.logprob.shape == (1, 4) and probs.top_ids.shape == (1, 4, 0)
+    for i, row in enumerate(logits):
+        probabilities.check(row, toks[:, i], 0, type(probs)(*(t[:, i] for t in probs)))
+    for a in e2e.attention_layers(model):
+        a.cache.length = 0
+    s = e2e.score(model, torch.cat([prompt, toks[:, :1]], 1), top=64)
+    assert s.logprob.shape == (1, 1) and s.top_ids.shape == (1, 1, 64)
+    assert bool((s.top_logprobs[..., :-1] >= s.top_logprobs[..., 1:]).all())

@@ -202,6 +202,21 @@ def test_rows_beyond_are_left_alone():
             assert all(torch.equal(p, q) for p, q in zip(r, e))
 
 
+def test_offsets_past_32_bits():
+    """More than 2^31 logits: rows on both sides of the border and the last one; and rows a long stride apart."""
+    from starkv import token_logprobs
+    V, rows = 32000, 70001
+    x = torch.zeros(rows, V, dtype=BF16, device="cuda")
+    at = torch.tensor([0, 67107, 67108, 67109, 70000])
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x[at.cuda()] = (torch.randn(len(at), V, generator=g, device="cuda") * 3).bfloat16()
+    tok = torch.randint(0, V, (rows,), generator=g, device="cuda")
+    res = token_logprobs(x, tok, top=3)
+    check(x[at.cuda()], tok[at.cuda()], 3, type(res)(*(t[at.cuda()] for t in res)))
+    far = torch.as_strided(x, (2, V), (67109 * V, 1))
+    check(far, tok[:2], 5, token_logprobs(far, tok[:2], top=5))
+
+
 def test_refusals():
     from starkv import StarKVError, token_logprobs
     x = torch.zeros(2, 100, device="cuda")

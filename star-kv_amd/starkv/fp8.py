@@ -38,32 +38,35 @@ def _e4m3_rows(rows: int, k: int, device) -> torch.Tensor:
     return torch.empty(rows, -(-k // 16) * 16, dtype=torch.float8_e4m3fn, device=device)[:, :k]
 
 
-def _rows2d(t: torch.Tensor, name: str) -> Tuple[torch.Tensor, int, int, int]:
-    """(t as [rows, width], rows, width, row stride); one row has any stride, 16 * ceil(width / 16) is given."""
+def _rows2d(t: torch.Tensor, name: str) -> Tuple[int, int, int]:
+    """(rows, width, row stride) of t as [rows, width]; one row has any stride, 16 * ceil(width / 16) is given."""
     shape, stride = t.shape, t.stride()
-    w = shape[-1] if shape else 0
+    if len(shape) == 2:
+        m, w = shape
+    else:
+        w = shape[-1] if shape else 0
+        m = shape[:-1].numel()
     if w < 1:
         raise StarKVError(f"{name} must have rows of at least one value, got shape {tuple(shape)}")
     if w > 1 and stride[-1] != 1:
         raise StarKVError(f"{name} must have a contiguous last dim")
-    if len(shape) != 2:
+    if len(shape) != 2 and m > 1:
         try:
-            t = t.view(-1, w) if t.numel() else t.reshape(0, w)
+            t = t.view(-1, w)
         except RuntimeError:
             raise StarKVError(f"{name} rows must be addressable with one row stride") from None
-        shape, stride = t.shape, t.stride()
-    m = shape[0]
+        stride = t.stride()
     if m > MAX_DIM or w > MAX_DIM:
         raise StarKVError(f"{name} has more than {MAX_DIM} rows or columns: {tuple(shape)}")
-    return t, m, w, (stride[0] if m > 1 else -(-w // 16) * 16)
+    return m, w, (stride[0] if m > 1 else -(-w // 16) * 16)
 
 
-def _on(device, **ts: Optional[torch.Tensor]) -> None:
+def _on(device, *ts: Optional[torch.Tensor]) -> None:
     if device.type != "cuda":
         raise StarKVError("libstarkv operators take device tensors (there is no CPU path)")
-    for name, t in ts.items():
+    for t in ts:
         if t is not None and t.device != device:
-            raise StarKVError(f"{name} is on {t.device}, the activations on {device}")
+            raise StarKVError(f"a {t.dtype} {tuple(t.shape)} is on {t.device}, the activations on {device}")
 
 
 def _scale_code(dtype) -> int:
@@ -82,7 +85,7 @@ def fp8_quantize(x: torch.Tensor, scale_dtype: torch.dtype = torch.float8_e8m0fn
     if dt is None:
         raise StarKVError(f"activations are float16 or bfloat16, got {x.dtype}")
     sd = _scale_code(scale_dtype)
-    xr, m, k, xs = _rows2d(x, "x")
+    m, k, xs = _rows2d(x, "x")
     dev = x.device
     _on(dev)
     kb, lead, pitch = -(-k // BLOCK), x.shape[:-1], -(-k // 16) * 16
@@ -98,7 +101,7 @@ def fp8_quantize(x: torch.Tensor, scale_dtype: torch.dtype = torch.float8_e8m0fn
     scale = torch.empty_strided((*lead, kb), strides, dtype=scale_dtype, device=dev)
     if ops.POISON:
         _poison(scale.movedim(-1, 0))
-    _launch("starkv_fp8_quantize", Fp8QuantizeDesc(m, k, dt, xr.data_ptr(), xs, q.data_ptr(), pitch, scale.data_ptr(),
+    _launch("starkv_fp8_quantize", Fp8QuantizeDesc(m, k, dt, x.data_ptr(), xs, q.data_ptr(), pitch, scale.data_ptr(),
                                                    sd, 1, m), dev)
     return (q if pitch == k else q[..., :k]), scale
 
@@ -141,55 +144,59 @@ def fp8_quantize_weight(w: torch.Tensor, scale_dtype: torch.dtype = torch.float8
 
 def _product(name, x, x_scale, weight, weight_scale, residual, silu_mul, rms_eps, out, out_dtype):
     dev = x.device
-    _on(dev, x_scale=x_scale, weight=weight, weight_scale=weight_scale, residual=residual, out=out)
+    _on(dev, weight, weight_scale, x_scale, residual, out)
     if weight.dtype != torch.float8_e4m3fn or weight.dim() != 2:
         raise StarKVError(f"{name}: weight must be a float8_e4m3fn [n, k], got {weight.dtype} {tuple(weight.shape)}")
     sd = _scale_code(weight_scale.dtype)
-    _, n, k, ws = _rows2d(weight, "weight")
-    xr, m, xw, xs = _rows2d(x, "x")
+    n, k, ws = _rows2d(weight, "weight")
+    m, xw, xs = _rows2d(x, "x")
     if xw != k:
         raise StarKVError(f"{name}: x has {xw} columns, the weight {k}")
-    kb = -(-k // BLOCK)
-    if weight_scale.shape != (-(-n // BLOCK), kb):
-        raise StarKVError(f"{name}: weight_scale must be [{-(-n // BLOCK)}, {kb}], got {tuple(weight_scale.shape)}")
+    kb = (k + BLOCK - 1) // BLOCK
+    if weight_scale.shape != ((n + BLOCK - 1) // BLOCK, kb):
+        raise StarKVError(f"{name}: weight_scale must be [{_blocks(n)}, {kb}], got {tuple(weight_scale.shape)}")
+    n_out = n
     if silu_mul:
+        n_out = n // 2
         if n % (2 * BLOCK):
             raise StarKVError(f"{name}: the gate and the up half of a merged weight are whole blocks of {BLOCK} rows "
                               f"each, got n = {n}")
         if residual is not None:
             raise StarKVError(f"{name}: silu_mul takes no residual")
-    n_out = n // 2 if silu_mul else n
-    shape = (*x.shape[:-1], n_out)
+    lead = x.shape[:-1]
+    shape = (*lead, n_out)
     if out is None:
-        out = _out(*shape, dtype=out_dtype, device=dev)
-    elif out.shape != shape or (out_dtype is not None and out.dtype != out_dtype):
-        raise StarKVError(f"{name}: out must be {shape} of {out_dtype}, got {tuple(out.shape)} of {out.dtype}")
+        out, os_ = _out(*shape, dtype=out_dtype, device=dev), n_out
+    else:
+        if out.shape != shape or (out_dtype is not None and out.dtype != out_dtype):
+            raise StarKVError(f"{name}: out must be {shape} of {out_dtype}, got {tuple(out.shape)} of {out.dtype}")
+        os_ = _rows2d(out, "out")[2]
     od = _OUT.get(out.dtype)
     if od is None:
         raise StarKVError(f"{name}: outputs are float16, bfloat16 or float32, got {out.dtype}")
-    orr, _, _, os_ = _rows2d(out, "out")
     rp, rs = None, 0
     if residual is not None:
         if residual.shape != shape or residual.dtype != out.dtype:
             raise StarKVError(f"{name}: residual must be {shape} of {out.dtype}")
-        rr, _, _, rs = _rows2d(residual, "residual")
-        rp = rr.data_ptr()
+        rp, rs = residual.data_ptr(), _rows2d(residual, "residual")[2]
     if x_scale is None:
         xd, xp, xsr, xsb = _ACT[x.dtype], None, 0, 0
     else:
-        if x_scale.shape != (*x.shape[:-1], kb) or x_scale.dtype != weight_scale.dtype:
-            raise StarKVError(f"{name}: x_scale must be {(*x.shape[:-1], kb)} of {weight_scale.dtype} like weight_scale")
+        if x_scale.shape != (*lead, kb) or x_scale.dtype != weight_scale.dtype:
+            raise StarKVError(f"{name}: x_scale must be {(*lead, kb)} of {weight_scale.dtype} like weight_scale")
         sr = x_scale
-        if sr.dim() != 2:
+        if len(lead) != 1:
             try:
                 sr = sr.view(-1, kb) if m else sr.reshape(0, kb)
             except RuntimeError:
                 raise StarKVError(f"{name}: x_scale rows must be addressable with one row stride") from None
-        xd, xp, xsr, xsb = _lib.E4M3, sr.data_ptr(), sr.stride(0), sr.stride(1)
-    d = Fp8GemmDesc(m, n, k, xd, od, xr.data_ptr(), xs, xp, xsr, xsb, weight.data_ptr(), ws, weight_scale.data_ptr(),
-                    weight_scale.stride(0), weight_scale.stride(1), sd, rp, rs, 1 if silu_mul else 0,
-                    0 if rms_eps is None else 1, rms_eps or 0.0, orr.data_ptr(), os_)
-    _launch("starkv_fp8_gemm", d, dev, workspace=True)
+        xd, xp, (xsr, xsb) = _lib.E4M3, sr.data_ptr(), sr.stride()
+    wsr, wsb = weight_scale.stride()
+    d = Fp8GemmDesc(m, n, k, xd, od, x.data_ptr(), xs, xp, xsr, xsb, weight.data_ptr(), ws, weight_scale.data_ptr(),
+                    wsr, wsb, sd, rp, rs, 1 if silu_mul else 0, 0 if rms_eps is None else 1, rms_eps or 0.0,
+                    out.data_ptr(), os_)
+    # e4m3 activations need no workspace
+    _launch("starkv_fp8_gemm", d, dev, workspace=x_scale is None)
     return out
 
 

@@ -8,11 +8,12 @@ import torch
 
 from . import _lib
 from ._lib import LogprobsDesc, StarKVError
-from .ops import _dt, _launch, _out
+from .ops import _launch, _out
 
 __all__ = ["TokenLogprobs", "token_logprobs", "MAX_TOP"]
 
 MAX_TOP = 64                         # STARKV_MAX_TOP
+_TYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
 MAX_ROWS = 1 << 30                   # of one call (fewer where rows are many: the library says)
 
 
@@ -30,36 +31,44 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     logits (fp16, bf16 or fp32; rows at any alignment).  Logits of -inf are
     barred tokens.  A token outside [0, V) has the log probability NaN, and so
     has everything of a row without a finite logit or with a NaN or +inf."""
-    if logits.dim() < 1 or logits.shape[-1] < 1:
-        raise StarKVError(f"logits must be [..., V], got shape {tuple(logits.shape)}")
-    dev, v, lead = logits.device, logits.shape[-1], logits.shape[:-1]
-    if lead.numel() > MAX_ROWS:
-        raise StarKVError(f"logits have more than {MAX_ROWS} rows: {tuple(logits.shape)}")
+    shape, dev, dt = logits.shape, logits.device, _TYPES.get(logits.dtype)
+    if not shape or shape[-1] < 1:
+        raise StarKVError(f"logits must be [..., V], got shape {tuple(shape)}")
+    v, lead, stride = shape[-1], shape[:-1], logits.stride()
+    n = lead.numel()
+    if n > MAX_ROWS:
+        raise StarKVError(f"logits have more than {MAX_ROWS} rows: {tuple(shape)}")
     if dev.type != "cuda":
         raise StarKVError("libstarkv operators take device tensors (there is no CPU path)")
-    if not 0 <= top <= min(MAX_TOP, v):
+    if dt is None:
+        raise StarKVError(f"unsupported dtype {logits.dtype}")
+    if not 0 <= top <= MAX_TOP or top > v:
         raise StarKVError(f"top must be 0 .. min({MAX_TOP}, V = {v}), got {top}")
-    if v > 1 and logits.stride(-1) != 1:
+    if v > 1 and stride[-1] != 1:
         raise StarKVError("logits must have a contiguous last dim")
-    rows = logits
-    if rows.dim() != 2:
+    if len(lead) == 1:
+        step = stride[0]
+    elif n < 2:
+        step = v
+    else:
         try:
-            rows = rows.view(-1, v) if rows.numel() else rows.reshape(0, v)
+            step = logits.view(-1, v).stride(0)
         except RuntimeError:
             raise StarKVError("logits rows must be addressable with one row stride") from None
-    n = rows.shape[0]
+    tp = lp = lpp = None
+    size = lead or ((),)
     if tokens is not None:
         if tokens.shape != lead or tokens.dtype != torch.int64 or tokens.device != dev:
             raise StarKVError(f"tokens must be int64 {tuple(lead)} on {dev}, got {tokens.dtype} {tuple(tokens.shape)} "
                               f"on {tokens.device}")
         if not tokens.is_contiguous():
             tokens = tokens.contiguous()
-    lp = _out(lead, dtype=torch.float32, device=dev) if tokens is not None else None
-    ent = _out(lead, dtype=torch.float32, device=dev)
+        lp = _out(*size, dtype=torch.float32, device=dev)
+        tp, lpp = tokens.data_ptr(), lp.data_ptr()
+    ent = _out(*size, dtype=torch.float32, device=dev)
     tops = _out(*lead, top, dtype=torch.float32, device=dev)
     ids = _out(*lead, top, dtype=torch.int64, device=dev)
-    d = LogprobsDesc(n, v, _dt(logits), top, rows.data_ptr(), rows.stride(0) if n > 1 else v,
-                     None if tokens is None else tokens.data_ptr(), None if lp is None else lp.data_ptr(),
-                     ent.data_ptr(), tops.data_ptr(), ids.data_ptr())
+    d = LogprobsDesc(n, v, dt, top, logits.data_ptr(), step if n > 1 else v, tp, lpp, ent.data_ptr(), tops.data_ptr(),
+                     ids.data_ptr())
     _launch("starkv_token_logprobs", d, dev, workspace=True)
     return TokenLogprobs(lp, ent, tops, ids)

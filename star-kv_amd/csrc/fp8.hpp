@@ -86,22 +86,22 @@ __device__ inline uint4 keep_bytes(uint4 v, int nv) {
 // wholly past k are not read).
 template <typename T>
 __device__ inline void load16(const uint8_t* row, int c0, int k, bool vec, uint32_t (&w)[8]) {
-  if (vec) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int c = c0 + 8 * h, nv = k - c;
-      uint4 v = make_uint4(0, 0, 0, 0);
+  for (int h = 0; h < 2; ++h) {
+    const int c = c0 + 8 * h, nv = k - c;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (vec) {
       if (nv > 0) v = *(const uint4*)(row + 2 * (int64_t)c);
       if (nv < 8) v = keep_bytes(v, 2 * nv);
-      w[4 * h] = v.x; w[4 * h + 1] = v.y; w[4 * h + 2] = v.z; w[4 * h + 3] = v.w;
-    }
-  } else {
-    const uint16_t* p = (const uint16_t*)row;
+    } else if (nv >= 8) {
+      __builtin_memcpy(&v, row + 2 * (int64_t)c, 16);      // one load at any alignment (2157 x 15550: 62 us by elements, 21)
+    } else {
+      uint16_t e[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t lo = c0 + 2 * i < k ? p[c0 + 2 * i] : 0u, hi = c0 + 2 * i + 1 < k ? p[c0 + 2 * i + 1] : 0u;
-      w[i] = lo | (hi << 16);
+      for (int i = 0; i < 8; ++i) e[i] = i < nv ? ((const uint16_t*)row)[c + i] : (uint16_t)0;
+      __builtin_memcpy(&v, e, 16);
     }
+    w[4 * h] = v.x; w[4 * h + 1] = v.y; w[4 * h + 2] = v.z; w[4 * h + 3] = v.w;
   }
 }
 

@@ -1577,11 +1577,6 @@ int starkv_fp8_gemm(const starkv_fp8_gemm_desc* d, void* workspace, size_t works
   a.w = (const uint8_t*)d->w; a.ws = d->w_stride; a.sw = d->w_scale; a.swr = d->w_scale_stride_r; a.swb = d->w_scale_stride_b;
   a.res = d->residual; a.rs = d->residual_stride; a.out = d->out; a.os = d->out_stride;
   a.m = d->m; a.n = d->n; a.k = d->k; a.kb = (int)ceil_div(d->k, FP8_BLOCK); a.half = d->n / 2;
-  auto vec = [&](int n) {
-    return al(d->out, n * os) && d->out_stride % n == 0 &&
-           (!d->residual || (al(d->residual, n * os) && d->residual_stride % n == 0));
-  };
-  a.vec_out = os == 2 && vec(8) ? 2 : vec(4);
   hipStream_t s = (hipStream_t)stream;
   if (q) {
     char* ws = (char*)workspace;

@@ -310,7 +310,6 @@ struct Fp8GemmArgs {
   const void* res; int64_t rs;                     // optional, of the output's type
   void* out; int64_t os;
   int m, n, k, kb, half;                           // half = n / 2 (SiLU-multiply)
-  int vec_out;                                     // out and res allow loads / stores of 4 (1) or 8 (2) columns
   int tiles_m, tiles_n;
 };
 struct LogprobArgs {

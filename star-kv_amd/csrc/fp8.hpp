@@ -203,35 +203,24 @@ __device__ inline floatx4 mfma8_exact(intx8 a, intx8 b) {
   return c;
 }
 
-// store four consecutive outputs of type O; the vector form needs 4-element alignment
-template <typename O> __device__ inline void store4(O* p, const float (&v)[4], int nv, bool vec) {
-  if (vec && nv >= 4) {
-    if constexpr (sizeof(O) == 4) {
-      *(float4*)p = make_float4(v[0], v[1], v[2], v[3]);
-    } else {
-      const O t[4] = {(O)v[0], (O)v[1], (O)v[2], (O)v[3]};
-      uint2 u;
-      __builtin_memcpy(&u, t, 8);
-      *(uint2*)p = u;
-    }
+// Four consecutive outputs of type O, nv of them inside the row, at any alignment: whole ones go in one access, which
+// the hardware takes at any address (8192 x 8191 outputs by elements cost 35 to 65 % of the product more).
+template <typename O> __device__ inline void store4(O* p, const float (&v)[4], int nv) {
+  const O t[4] = {(O)v[0], (O)v[1], (O)v[2], (O)v[3]};
+  if (nv >= 4) {
+    __builtin_memcpy(p, t, sizeof(t));
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (e < nv) p[e] = (O)v[e];
+      if (e < nv) p[e] = t[e];
   }
 }
-template <typename O> __device__ inline void load4(const O* p, float (&v)[4], int nv, bool vec) {
-  if (vec && nv >= 4) {
-    if constexpr (sizeof(O) == 4) {
-      const float4 t = *(const float4*)p;
-      v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
-    } else {
-      const uint2 u = *(const uint2*)p;
-      O t[4];
-      __builtin_memcpy(t, &u, 8);
+template <typename O> __device__ inline void load4(const O* p, float (&v)[4], int nv) {
+  if (nv >= 4) {
+    O t[4];
+    __builtin_memcpy(t, p, sizeof(t));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = (float)t[e];
-    }
+    for (int e = 0; e < 4; ++e) v[e] = (float)t[e];
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = e < nv ? (float)p[e] : 0.f;

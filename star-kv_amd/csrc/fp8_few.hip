@@ -156,11 +156,11 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(const Fp8GemmArgs a) {
     for (int e = 0; e < 4; ++e) v[e] = SILU ? silu_mul_f32(r * s[e], r * u[e]) : r * s[e];
     if (!SILU && a.res) {
       float x[4];
-      load4<O>((const O*)a.res + (int64_t)row * a.rs + col, x, nv, a.vec_out != 0);
+      load4<O>((const O*)a.res + (int64_t)row * a.rs + col, x, nv);
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] += x[e];
     }
-    store4<O>((O*)a.out + (int64_t)row * a.os + col, v, nv, a.vec_out != 0);
+    store4<O>((O*)a.out + (int64_t)row * a.os + col, v, nv);
   }
 }
 

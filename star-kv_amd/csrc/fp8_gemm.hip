@@ -364,11 +364,11 @@ void fp8_gemm_kernel(const Fp8GemmArgs a) {
                       : r * acc[j][i][4 * q + e];
         if (!SILU && a.res) {
           float t[4];
-          load4<O>((const O*)a.res + (int64_t)row * a.rs + col, t, nv, a.vec_out != 0);
+          load4<O>((const O*)a.res + (int64_t)row * a.rs + col, t, nv);
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[e] += t[e];
         }
-        store4<O>((O*)a.out + (int64_t)row * a.os + col, v, nv, a.vec_out != 0);
+        store4<O>((O*)a.out + (int64_t)row * a.os + col, v, nv);
       }
   }
 }
@@ -619,9 +619,10 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_wide_kernel(const Fp8GemmArgs
     // tile).  Stores are non-temporal: results of this many bytes would push operands out of L2 (8192 x 8192, k
     // 16384: 890 -> 785 us).
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    typedef u32x4 __attribute__((aligned(2))) u32x4_any;
     uint8_t* const ob = lds + FACTORS + 2 * WT * 4 + wave * WOUT;
     const int ncol = SILU ? a.half : a.n, lr0 = lane >> 3, rc = lane & 7;
-    const bool quick = a.vec_out >= 2 && on + (SILU ? 64 : 128) <= ncol;      // whole pieces in every row
+    const bool quick = on + (SILU ? 64 : 128) <= ncol;      // whole pieces in every row (at any alignment)
     const bool whole = quick && om + 128 <= a.m;
     drain = !whole;
     auto slot = [&](int r, int p) __attribute__((always_inline)) { return ob + r * 128 + ((p ^ (r & 7)) << 4); };
@@ -633,7 +634,7 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_wide_kernel(const Fp8GemmArgs
           u32x4 v[4];
 #pragma unroll
           for (int t = 0; t < 4; ++t)
-            v[t] = *(const u32x4*)((const O*)a.res + (int64_t)min(row0 + lr0 + 8 * t, a.m - 1) * a.rs + col);
+            v[t] = *(const u32x4_any*)((const O*)a.res + (int64_t)min(row0 + lr0 + 8 * t, a.m - 1) * a.rs + col);
 #pragma unroll
           for (int t = 0; t < 4; ++t) *(u32x4*)slot(lr0 + 8 * t, rc) = v[t];
         } else {
@@ -701,7 +702,7 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_wide_kernel(const Fp8GemmArgs
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           if (whole || row0 + lr0 + 8 * t < a.m)
-            __builtin_nontemporal_store(o[t], (u32x4*)(out + (int64_t)(8 * t) * a.os));
+            __builtin_nontemporal_store(o[t], (u32x4_any*)(out + (int64_t)(8 * t) * a.os));
         }
       } else {
 #pragma unroll 1

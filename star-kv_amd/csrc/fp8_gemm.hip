@@ -98,6 +98,91 @@ __device__ inline floatx16 mfma8_32(intx8 a, intx8 b, floatx16 c, int scale_a, i
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, scale_a, 0, scale_b);
 }
 
+// The results of 32 rows and 32 G columns from (row0, col0) on: lane (c, g) holds columns 32 j + 8 q + 4 g .. + 3 of row
+// c in v[j] (SILU: gate columns, then the same up columns).  They are finished and rounded there and go through the
+// wave's own part of LDS, so that whole rows of 64 bytes and more leave (8 bytes of each of 32 rows at a time, as the
+// accumulators hold them, 128 x 128 tiles spent 8 us of a round on it); a residual comes the same way.  16-byte
+// piece p of row r lies at p ^ r (of the row's pieces).  quick: all columns are inside the row; whole: the rows, too.
+template <typename O, int G, bool SILU, bool NONTEMPORAL>
+__device__ inline void finish_chunk(const Fp8GemmArgs& a, uint8_t* ob, int row0, int col0, const floatx16 (&v)[SILU ? 2 * G : G],
+                                    float r, bool quick, bool whole) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  typedef u32x4 __attribute__((aligned(2))) u32x4_any;
+  constexpr int RB = 32 * G * sizeof(O), PP = RB / 16, PC = 16 / sizeof(O);     // bytes and pieces of a row, columns of a piece
+  constexpr int RPI = 64 / PP, NR = 32 / RPI;      // rows at a time
+  const int lane = threadIdx.x & 63, g = lane >> 5;
+  int c = lane & 31;
+  asm volatile("" : "+v"(c));                      // addresses are formed here, not kept over a tile
+  const int ncol = SILU ? a.half : a.n, lr0 = lane / PP, rc = lane % PP, col = col0 + PC * rc;
+  auto slot = [&](int row, int p) __attribute__((always_inline)) { return ob + row * RB + ((p ^ (row & (PP - 1))) << 4); };
+  if (!SILU && a.res) {
+    if (quick) {
+      u32x4 t[NR];
+#pragma unroll
+      for (int i = 0; i < NR; ++i)
+        t[i] = *(const u32x4_any*)((const O*)a.res + (int64_t)min(row0 + lr0 + RPI * i, a.m - 1) * a.rs + col);
+#pragma unroll
+      for (int i = 0; i < NR; ++i) *(u32x4*)slot(lr0 + RPI * i, rc) = t[i];
+    } else {
+#pragma unroll 1
+      for (int lr = lr0; lr < 32; lr += RPI) {
+        O e[PC];
+#pragma unroll
+        for (int i = 0; i < PC; ++i)
+          e[i] = row0 + lr < a.m && col + i < ncol ? ((const O*)a.res)[(int64_t)(row0 + lr) * a.rs + col + i] : (O)0.f;
+        u32x4 u;
+        __builtin_memcpy(&u, e, 16);
+        *(u32x4*)slot(lr, rc) = u;
+      }
+    }
+  }
+  asm volatile("" ::: "memory");                   // other lanes read what this one wrote
+#pragma unroll
+  for (int j = 0; j < G; ++j)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint8_t* const p = sizeof(O) == 2 ? slot(c, 4 * j + q) + 8 * g : slot(c, 8 * j + 2 * q + g);
+      float f[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        f[e] = SILU ? silu_mul_f32(r * v[j][4 * q + e], r * v[SILU ? j + G : j][4 * q + e]) : r * v[j][4 * q + e];
+      O w[4];
+      if (!SILU && a.res) {
+        __builtin_memcpy(w, __builtin_assume_aligned(p, 4 * sizeof(O)), sizeof(w));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] += (float)w[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = (O)f[e];
+      __builtin_memcpy(__builtin_assume_aligned(p, 4 * sizeof(O)), w, sizeof(w));
+    }
+  asm volatile("" ::: "memory");
+  if (quick) {
+    u32x4 o[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) o[i] = *(const u32x4*)slot(lr0 + RPI * i, rc);
+    O* const out = (O*)a.out + (int64_t)(row0 + lr0) * a.os + col;
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+      if (whole || row0 + lr0 + RPI * i < a.m) {
+        u32x4_any* const to = (u32x4_any*)(out + (int64_t)(RPI * i) * a.os);
+        if (NONTEMPORAL) __builtin_nontemporal_store(o[i], to);
+        else *to = o[i];
+      }
+  } else {
+#pragma unroll 1
+    for (int lr = lr0; lr < 32; lr += RPI) {
+      const u32x4 u = *(const u32x4*)slot(lr, rc);
+      O e[PC];
+      __builtin_memcpy(e, &u, 16);
+#pragma unroll
+      for (int i = 0; i < PC; ++i)
+        if (row0 + lr < a.m && col + i < ncol) ((O*)a.out)[(int64_t)(row0 + lr) * a.os + col + i] = e[i];
+    }
+  }
+  asm volatile("" ::: "memory");
+}
+
 // WM x WN waves of 32 I x 32 J, NST stages; KS such groups of waves take every KS-th block, each with stages of its
 // own, and meet in LDS at the end; SILU: a wave's columns are half gate columns and half the same up columns
 template <int WM, int WN, int I, int J, int KS, int NST, typename S, typename O, bool SILU>
@@ -344,32 +429,20 @@ void fp8_gemm_kernel(const Fp8GemmArgs a) {
           }
   }
 
-  // lane (c, g): columns 32 j + 8 q + 4 g .. + 3 of row 32 i + c of the wave's tile
+  // results by way of LDS, behind what the groups' sums take
+  constexpr int G = SILU ? J / 2 : J, OB = 32 * 32 * G * sizeof(O), SUMS = (KS - 1) * NW * I * J * 4096;
+  static_assert(SUMS + NW * OB <= KS * NST * STAGE, "the results fit");
+  if constexpr (KS == 1) __syncthreads();          // the other waves' operands
+  const int col0 = n0 + wn * 32 * G;
+  const bool quick = col0 + 32 * G <= (SILU ? a.half : a.n);
 #pragma unroll
   for (int i = 0; i < I; ++i) {
-    const int row = m0 + wm * TM + 32 * i + c;
-    if (row >= a.m) continue;
-    const float r = a.rscale ? a.rscale[row] : 1.f;
+    const int row0 = m0 + wm * TM + 32 * i;
+    floatx16 v[J];
 #pragma unroll
-    for (int j = 0; j < (SILU ? J / 2 : J); ++j)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int col = n0 + wn * (SILU ? TN / 2 : TN) + 32 * j + 8 * q + 4 * g;
-        const int nv = (SILU ? a.half : a.n) - col;
-        if (nv <= 0) continue;
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          v[e] = SILU ? silu_mul_f32(r * acc[j][i][4 * q + e], r * acc[SILU ? j + J / 2 : j][i][4 * q + e])
-                      : r * acc[j][i][4 * q + e];
-        if (!SILU && a.res) {
-          float t[4];
-          load4<O>((const O*)a.res + (int64_t)row * a.rs + col, t, nv);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] += t[e];
-        }
-        store4<O>((O*)a.out + (int64_t)row * a.os + col, v, nv);
-      }
+    for (int j = 0; j < J; ++j) v[j] = acc[j][i];
+    finish_chunk<O, G, SILU, false>(a, lds_all + SUMS + wave * OB, row0, col0, v,
+                                    a.rscale ? a.rscale[min(row0 + c, a.m - 1)] : 1.f, quick, row0 + 32 <= a.m);
   }
 }
 
@@ -612,48 +685,15 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_wide_kernel(const Fp8GemmArgs
       start(par ^ 1);
     }
 
-    // Results, 32 rows x 64 columns at a time: lane (c, g) holds columns 32 j + 8 q + 4 g .. + 3 of row 32 i + c in
-    // acc[j][i].  They are finished and rounded there and go through the wave's own part of LDS, so that whole
-    // 128-byte lines leave; a residual comes the same way.  16-byte piece p of row r lies at p ^ (r & 7).  One copy
-    // of the code serves all chunks: unrolled it came from memory instruction by instruction (48 KB of code: 25 us a
-    // tile).  Stores are non-temporal: results of this many bytes would push operands out of L2 (8192 x 8192, k
-    // 16384: 890 -> 785 us).
-    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    typedef u32x4 __attribute__((aligned(2))) u32x4_any;
+    // Results, 32 rows x 64 columns at a time.  One copy of the code serves all chunks: unrolled it came from memory
+    // instruction by instruction (48 KB of code: 25 us a tile).  Stores are non-temporal: results of this many bytes
+    // would push operands out of L2 (8192 x 8192, k 16384: 890 -> 785 us).
     uint8_t* const ob = lds + FACTORS + 2 * WT * 4 + wave * WOUT;
-    const int ncol = SILU ? a.half : a.n, lr0 = lane >> 3, rc = lane & 7;
-    const bool quick = on + (SILU ? 64 : 128) <= ncol;      // whole pieces in every row (at any alignment)
-    const bool whole = quick && om + 128 <= a.m;
+    const bool quick = on + (SILU ? 64 : 128) <= (SILU ? a.half : a.n), whole = quick && om + 128 <= a.m;
     drain = !whole;
-    auto slot = [&](int r, int p) __attribute__((always_inline)) { return ob + r * 128 + ((p ^ (r & 7)) << 4); };
 #pragma unroll 1
     for (int ch = 0; ch < (SILU ? 4 : 8); ++ch) {
-      const int row0 = om + 32 * (SILU ? ch : ch >> 1), col = on + (SILU ? 0 : 64 * (ch & 1)) + 8 * rc;
-      if (!SILU && a.res) {
-        if (quick) {
-          u32x4 v[4];
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-            v[t] = *(const u32x4_any*)((const O*)a.res + (int64_t)min(row0 + lr0 + 8 * t, a.m - 1) * a.rs + col);
-#pragma unroll
-          for (int t = 0; t < 4; ++t) *(u32x4*)slot(lr0 + 8 * t, rc) = v[t];
-        } else {
-#pragma unroll 1
-          for (int lr = lr0; lr < 32; lr += 8) {
-            O v[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              v[e] = row0 + lr < a.m && col + e < ncol ? ((const O*)a.res)[(int64_t)(row0 + lr) * a.rs + col + e] : (O)0.f;
-            uint4 u;
-            __builtin_memcpy(&u, v, 16);
-            *(uint4*)slot(lr, rc) = u;
-          }
-        }
-      }
-      asm volatile("" ::: "memory");               // other lanes read what this one wrote
-      // the chunk's accumulators (SILU: gate columns, then the up columns)
-      int cl = c;
-      asm volatile("" : "+v"(cl));                 // addresses are formed here, not kept over the tile
+      const int row0 = om + 32 * (SILU ? ch : ch >> 1), col0 = on + (SILU ? 0 : 64 * (ch & 1));
       floatx16 v[SILU ? 4 : 2];
       auto pick = [&](auto chc) __attribute__((always_inline)) {
         constexpr int C = decltype(chc)::value;
@@ -671,51 +711,7 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_wide_kernel(const Fp8GemmArgs
         default: pick(std::integral_constant<int, SILU ? 0 : 7>{}); break;
       }
       const float r = a.rscale ? *(const float*)(lds + FACTORS + par * WT * 4 + (row0 - om + wm * 128 + c) * 4) : 1.f;
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint2* const p = (uint2*)(slot(cl, 4 * j + q) + 8 * g);
-          float f[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            f[e] = SILU ? silu_mul_f32(r * v[j][4 * q + e], r * v[SILU ? j + 2 : j][4 * q + e]) : r * v[j][4 * q + e];
-          O w[4];
-          if (!SILU && a.res) {
-            const uint2 u = *p;
-            __builtin_memcpy(w, &u, 8);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) f[e] += (float)w[e];
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = (O)f[e];
-          uint2 u;
-          __builtin_memcpy(&u, w, 8);
-          *p = u;
-        }
-      asm volatile("" ::: "memory");
-      if (quick) {
-        u32x4 o[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) o[t] = *(const u32x4*)slot(lr0 + 8 * t, rc);
-        O* const out = (O*)a.out + (int64_t)(row0 + lr0) * a.os + col;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          if (whole || row0 + lr0 + 8 * t < a.m)
-            __builtin_nontemporal_store(o[t], (u32x4_any*)(out + (int64_t)(8 * t) * a.os));
-        }
-      } else {
-#pragma unroll 1
-        for (int lr = lr0; lr < 32; lr += 8) {
-          const uint4 u = *(const uint4*)slot(lr, rc);
-          O w[8];
-          __builtin_memcpy(w, &u, 16);
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (row0 + lr < a.m && col + e < ncol) ((O*)a.out)[(int64_t)(row0 + lr) * a.os + col + e] = w[e];
-        }
-      }
-      asm volatile("" ::: "memory");
+      finish_chunk<O, 2, SILU, true>(a, ob, row0, col0, v, r, quick, whole);
     }
     par ^= 1;
     if (!more) break;

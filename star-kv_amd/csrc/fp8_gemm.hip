@@ -722,37 +722,38 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_wide_kernel(const Fp8GemmArgs
 // workgroups a fixed part and a part for each k block (microseconds).  Tiles
 // of 64 and 128 columns run with one workgroup on a CU or two, the larger ones
 // alone, and their blocks go the faster the more CUs idle.  Fitted to the
-// times of every tile in 196 products of n 1640 to 22016, k 512 to 11008, 48
-// to 8192 rows: the tile picked is the fastest or within 6 % of it in all but
-// two (13 % of 7.7 us).  Small tiles fill the chip with few rows, large ones
-// read less per product: powers of two, 4096 x 4096, k 4096 takes 177, 136,
-// 96, 80, 80 and 60 us on the tiles below, 256 rows of it 16, 16, 21, 29, 39
-// and 44.
+// times of every tile in 252 products of n 1640 to 22016, k 320 to 11008, 48
+// to 8192 rows: the tile picked is the fastest or within 8 % of it in all but
+// three (10 to 16 %).  Small tiles fill the chip with few rows, large ones
+// read less per product: powers of two, 2048 x 4096, k 4096 takes 89, 62, 47,
+// 38, 37 and 49 us on the tiles below, 256 rows of it 15, 14, 17, 21, 27 and
+// 43, 4096 rows 59 on the last and 70 on the one before it.
 //   few rows   16 weight rows a workgroup, no LDS (m <= 16; to 32 rows while a
-//              second group of rows costs less than the tiles' fixed 4 us:
-//              n 4096, k 4096: 9.2 against 9.7 us; k 11008: 18.2 against 17.4)
+//              second group of rows costs less than the tiles' start: 32 rows,
+//              n 1640, k 1024: 4.7 against 5.4 us; n 2048, k 4096: 8.6 against
+//              8.5; n 7376, k 2048: 8.9 against 7.0)
 //   64 x 32    4 k groups of waves, one workgroup a CU; 2 k groups, two
 //   64 x 64    2 k groups      64 x 128, 128 x 128   one
 //   128 x 256  eight waves, three stages (fp32 scales, 2048 x 4096, k 11008:
-//              109 us on 128 x 128, 97 on these)
+//              100 us on 128 x 128, 90 on these)
 //   256 x 256  power-of-two scales and 16-bit outputs
 Fp8Plan plan_fp8_gemm(int m, int n, int kb, bool silu, bool exact, bool pow2, int cus) {
   Fp8Plan p = {};
   p.cus = cus;
-  if (m <= 16 || (m <= 32 && (int64_t)n * kb <= 131072)) {
+  if (m <= 16 || (m <= 32 && (int64_t)m * n * kb <= 1 << 21)) {
     p.few = true;
     p.bm = m <= 16 ? 16 : 32;
     p.bn = silu ? 32 : 16;
     return p;
   }
   struct Shape { int bm, bn; float one, two, fix1, fix2; };        // 256 columns: one of the only CU in use, two of all
-  static const Shape fast[] = {{64, 32, 0.15f, 0.27f, 1.8f, 2.3f},  {64, 64, 0.29f, 0.37f, 1.8f, 3.5f},
-                               {64, 128, 0.36f, 0.58f, 2.1f, 3.7f}, {128, 128, 0.62f, 0.87f, 3.8f, 8.3f},
-                               {128, 256, 0.60f, 0.83f, 4.8f, 9.0f}, {256, 256, 0.92f, 1.37f, 8.2f, 8.9f}};
+  static const Shape fast[] = {{64, 32, 0.15f, 0.26f, 1.3f, 2.1f},  {64, 64, 0.29f, 0.34f, 1.4f, 3.0f},
+                               {64, 128, 0.37f, 0.55f, 1.0f, 3.2f}, {128, 128, 0.55f, 0.87f, 3.2f, 4.2f},
+                               {128, 256, 0.59f, 0.81f, 2.9f, 6.2f}, {256, 256, 0.87f, 1.28f, 9.6f, 12.9f}};
   // the sums of a block scaled apart
-  static const Shape part[] = {{64, 32, 0.15f, 0.27f, 1.8f, 2.3f},  {64, 64, 0.31f, 0.37f, 1.8f, 3.6f},
-                               {64, 128, 0.43f, 0.62f, 2.0f, 3.8f}, {128, 128, 0.64f, 0.94f, 4.2f, 8.2f},
-                               {128, 256, 0.62f, 0.88f, 4.8f, 9.2f}};
+  static const Shape part[] = {{64, 32, 0.14f, 0.26f, 1.7f, 2.3f},  {64, 64, 0.29f, 0.34f, 1.3f, 2.8f},
+                               {64, 128, 0.38f, 0.57f, 2.2f, 3.3f}, {128, 128, 0.58f, 0.99f, 3.3f, 5.1f},
+                               {128, 256, 0.80f, 0.80f, 2.7f, 7.9f}};
   const bool scaled = exact || !pow2;
   float best = 0.f;
   for (int i = 0; i < (scaled ? 5 : 6); ++i) {

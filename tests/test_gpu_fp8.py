@@ -328,6 +328,27 @@ def test_every_tile_of_a_workgroup(m, n, k, epilogue, rms):
     assert worst <= 1.0
 
 
+@pytest.mark.parametrize("m,n,k,scale,epilogue", [(4300, 8443, 264, E8, "residual"), (2000, 4091, 5000, E8, "none"),
+                                                 (2000, 4091, 5000, F32, "residual"), (700, 4093, 1000, F32, "residual"),
+                                                 (4300, 8448, 264, E8, "silu_mul"), (300, 1025, 640, F32, "residual")])
+@pytest.mark.parametrize("out", [F16, F32], ids=["f16", "f32"])
+def test_odd_rows_of_large_tiles(m, n, k, scale, epilogue, out):
+    """Results, and the residual in place, whose rows start at every alignment of their elements: the same bits as
+    into rows that are aligned, and nothing beside them."""
+    c = make(m, n, k, F16, out, scale, epilogue)
+    want = call(c)
+    wide = want.shape[1]
+    buf = torch.full((m + 2, wide + 3 + wide % 2), 7.0, dtype=out, device="cuda")     # an odd pitch
+    to = buf[1:m + 1, 1:wide + 1]
+    if c["res"] is not None:
+        to.copy_(c["res"])
+        c["res"] = to
+    got = call(c, out=to, out_dtype=None)
+    assert got.data_ptr() == to.data_ptr() and torch.equal(got, want)
+    to.fill_(7.0)
+    assert bool((buf == 7.0).all())
+
+
 @pytest.mark.parametrize("m", [5, 40])
 def test_layouts_and_in_place(m):
     """Activations at odd offsets, a padded output whose other columns and rows stay, the residual in place, leading dims."""

@@ -7,13 +7,19 @@
 // (both terms of the entropy are >= 0: nothing cancels).  Every thread keeps
 // its own m, Z and S over 16-byte pieces of the row, in units of log 2: with
 // c = log2 e and M = fl(m c), y = fma(x, c, -M) and 2^y replace x - m and
-// e^(x - m), S sums 2^y y.  The rounding of M is the same for all terms and is
-// taken back once (ln Z - (m c - M) ln 2).  y stops at -150, where 2^y is 0,
-// so that -inf adds 0 and not 0 * inf.  A larger maximum rescales the sums,
-// which soon gets rare.  That leaves nine and a half issue slots an element,
-// four of them the exponential: 16-bit logits are bound by those nearly as
-// much as by HBM.  Rows whose maximum is beyond +-1e30 (where x c may
-// overflow) are summed again with x - m formed first.
+// e^(x - m), S sums 2^y y.  The rounding of M, e = m c - M, is the same for all
+// terms and is taken back at the end (Z 2^-e; S - e Z likewise).  y stops at
+// -150, where 2^y is 0, so that -inf adds 0 and not 0 * inf.  A larger maximum
+// rescales the sums, which soon gets rare.  That leaves nine and a half issue
+// slots an element, four of them the exponential: 16-bit logits are bound by
+// those nearly as much as by HBM.
+//
+// This holds while 2^e is near 1: |e| is up to half a unit of M's last place,
+// 0.07 for |m| = 2^20, but 64 for 1e9 and 440 for 1e10, where 2^e is infinite.
+// So a thread's maximum starts at -2^20 (logits far below it, finite masks
+// among them, add 0 as -inf does), and rows, or pieces of rows, whose maximum
+// is outside +-2^20 are summed again with x - m formed first.  fp16 logits are
+// all inside.
 //
 // Top alternatives: keys are (logit, lowest index first) as one 64-bit number
 // in a total order.  Each thread knows its greatest logit and the first piece
@@ -38,7 +44,7 @@ constexpr int LP_WIDE = 1024;                      // rows of 16 KB and more whi
 constexpr int LP_MAX_PIECES = 64;                  // of a row (a lane each in the join)
 constexpr int LP_BATCH = 4;                        // 16-byte pieces a thread asks for at a time
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-constexpr float START = -1e30f, HUGE_X = 1e30f;    // maxima in between take the fast sums
+constexpr float START = -0x1p20f, HUGE_X = 0x1p20f;   // maxima in between take the fast sums
 constexpr float FAR = -150.f;                      // 2^FAR is 0 in fp32
 
 // logits ordered as unsigned integers: -0 = +0, a NaN above everything
@@ -53,7 +59,8 @@ __device__ inline float unorder32(uint32_t k) {
 }
 __device__ inline uint64_t make_key(float f, uint32_t idx) { return ((uint64_t)order32(f) << 32) | (uint32_t)~idx; }
 
-// Sums over some elements: z = sum 2^y, s = sum 2^y y with y = x log2 e - fl(m log2 e)
+// Sums over some elements: z = sum 2^y, s = sum 2^y y, while they are taken with y = x log2 e - fl(m log2 e), in the end
+// (exact_sums) with y = (x - m) log2 e
 struct Stat { float m, z, s; };
 // (rounded, wherever it is used: a product fused into a difference would leave what the rounding took)
 __device__ inline float log2_of(float m) {
@@ -66,6 +73,12 @@ __device__ inline void rebase(Stat& a, float to) {
   a.s = f * fmaf(a.z, d, a.s);
   a.z *= f;
   a.m = to;
+}
+// sums with y = x log2 e - fl(m log2 e) -> with y = (x - m) log2 e, less by what the rounding took
+__device__ inline void exact_sums(Stat& a) {
+  const float e = fmaf(a.m, LOG2E, -log2_of(a.m)), f = __builtin_amdgcn_exp2f(-e);
+  a.s = f * fmaf(-e, a.z, a.s);
+  a.z *= f;
 }
 
 // wave reductions by lane shifts inside rows of 16 and broadcasts between them; lane 63 ends with the result
@@ -151,11 +164,10 @@ template <typename T> __device__ inline float token_logit(const LogprobArgs& a, 
 }
 __device__ inline float finish_row(const LogprobArgs& a, int64_t row, float xt, const Stat& st, bool nan, bool write) {
   const float none = __uint_as_float(0x7fc00000u);
-  const float eps = fmaf(st.m, LOG2E, -log2_of(st.m));       // what fl(m log2 e) is short of m log2 e
-  const float lnz = nan ? none : logf(st.z) - (fabsf(st.m) < HUGE_X ? eps * LN2 : 0.f);
+  const float lnz = nan ? none : logf(st.z);
   if (write) {
     if (a.tok) a.lp[row] = (xt - st.m) - lnz;
-    if (a.ent) a.ent[row] = nan ? none : logf(st.z) - LN2 * (st.s / st.z);
+    if (a.ent) a.ent[row] = nan ? none : lnz - LN2 * (st.s / st.z);
   }
   return lnz;
 }
@@ -330,9 +342,11 @@ template <typename T, int NT, bool TOP> __global__ __launch_bounds__(NT) void lo
   bool any_nan = false;
 #pragma unroll
   for (int v = 0; v < NW; ++v) any_nan |= wnan[v] != 0;
-  if (!any_nan && !(st.m > START && st.m < HUGE_X)) {
-    // x log2 e may overflow: the maximum itself (START was none of the elements) and then x - m, exactly as the
-    // definition has it.  No finite element: z = 0.  +inf: not a number.
+  if (st.m > START && st.m < HUGE_X) {
+    exact_sums(st);
+  } else if (!any_nan) {
+    // the maximum itself (START was none of the elements) and then x - m, exactly as the definition has it.  No finite
+    // element: z = 0.  +inf: not a number.
     float m = -__builtin_inff();
     each([&](float v, int) { m = fmaxf(m, v); });
     m = wave_maxf(m);
@@ -484,13 +498,10 @@ template <typename T> __global__ __launch_bounds__(LP_NT) void logprobs_join_ker
   const float m = wave_maxf(ps.x);
   Stat st = {ps.x, ps.y, ps.z};
   const bool nan = __any(st.z != st.z) || m == __builtin_inff();
-  if (m > START && m < HUGE_X) {
-    rebase(st, m);                                 // (pieces without an element above START end at 0)
-  } else {
-    const float d = fmaxf((st.m - m) * LOG2E, FAR), f = __builtin_amdgcn_exp2f(d);
-    st.s = f * fmaf(st.z, d, st.s);
-    st.z = st.m == m ? st.z : st.z * f;
-  }
+  // pieces of either way of summing are given over their own maximum, x - m exactly (a piece without a finite element: 0)
+  const float d = fmaxf((st.m - m) * LOG2E, FAR), f = __builtin_amdgcn_exp2f(d);
+  st.s = f * fmaf(st.z, d, st.s);
+  st.z *= f;
   st = Stat{m, wave_sumf(st.z), wave_sumf(st.s)};
   const float lnz = finish_row(a, row, xt, st, nan, tid == 0);
   __syncthreads();

@@ -47,14 +47,16 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float START = -0x1p20f, HUGE_X = 0x1p20f;   // maxima in between take the fast sums
 constexpr float FAR = -150.f;                      // 2^FAR is 0 in fp32
 
-// logits ordered as unsigned integers: -0 = +0, a NaN above everything
+// logits ordered as unsigned integers: -0 = +0, a NaN above everything, and none all ones (a key that every other one
+// is below starts the search by rounds)
+constexpr uint32_t ORDER_NAN = 0xfffffffeu;
 __device__ inline uint32_t order32(float f) {
-  if (f != f) return 0xffffffffu;
+  if (f != f) return ORDER_NAN;
   const uint32_t u = __float_as_uint(f + 0.0f);    // -0 + 0 = +0
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 __device__ inline float unorder32(uint32_t k) {
-  if (k == 0xffffffffu) return __uint_as_float(0x7fc00000u);
+  if (k == ORDER_NAN) return __uint_as_float(0x7fc00000u);
   return __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
 }
 __device__ inline uint64_t make_key(float f, uint32_t idx) { return ((uint64_t)order32(f) << 32) | (uint32_t)~idx; }

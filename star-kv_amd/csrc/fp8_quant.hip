@@ -10,7 +10,10 @@
 // product with the rounded reciprocal instead of a division per value.
 //
 // With `rscale` (the GEMM's RMS-normalised input) a workgroup takes one row
+// (of more than 2^22 rows, every 2^22-th: a launch has less than 2^32 threads)
 // and also sums its squares: rscale = rsqrt(mean x^2 + eps).
+#include <algorithm>
+
 #include "fp8.hpp"
 
 namespace starkv {
@@ -18,6 +21,7 @@ namespace starkv {
 namespace {
 constexpr int QT = 256;                            // threads per workgroup
 constexpr int QB = QT / 8;                         // blocks of 128 a workgroup holds at a time
+constexpr int QROWS = 1 << 22;                     // workgroups of a launch that take rows
 }  // namespace
 
 // block `kb` of row `row`, this thread's 16 of its 128 values; returns them for the sum of squares
@@ -49,27 +53,30 @@ __global__ __launch_bounds__(QT) void fp8_quant_kernel(const Fp8QuantArgs a) {
 
 template <typename T, typename S>
 __global__ __launch_bounds__(QT) void fp8_quant_rms_kernel(const Fp8QuantArgs a) {
-  __shared__ float part[QT / 64];
-  const int64_t row = blockIdx.x;
-  float ss = 0.f;
-  for (int kb = threadIdx.x >> 3; kb < a.kb; kb += QB) {
-    uint32_t w[8];
-    quant_block<T, S>(a, row, kb, threadIdx.x & 7, w);
-    ss = sumsq16<T>(w, ss);
-  }
+  __shared__ float parts[2][QT / 64];              // of this row and the next: one barrier a row
+  int odd = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, odd ^= 1) {
+    float* const part = parts[odd];
+    float ss = 0.f;
+    for (int kb = threadIdx.x >> 3; kb < a.kb; kb += QB) {
+      uint32_t w[8];
+      quant_block<T, S>(a, row, kb, threadIdx.x & 7, w);
+      ss = sumsq16<T>(w, ss);
+    }
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) ss += __shfl_xor(ss, o, 64);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = ss;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    const float tot = (part[0] + part[1]) + (part[2] + part[3]);
-    a.rscale[row] = rsqrtf(tot / (float)a.k + a.rms_eps);
+    for (int o = 32; o >= 1; o >>= 1) ss += __shfl_xor(ss, o, 64);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = ss;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      const float tot = (part[0] + part[1]) + (part[2] + part[3]);
+      a.rscale[row] = rsqrtf(tot / (float)a.k + a.rms_eps);
+    }
   }
 }
 
 template <typename T, typename S> static int launch_q(const Fp8QuantArgs& a, hipStream_t st) {
   if (a.rscale)
-    hipLaunchKernelGGL((fp8_quant_rms_kernel<T, S>), dim3((unsigned)a.rows), dim3(QT), 0, st, a);
+    hipLaunchKernelGGL((fp8_quant_rms_kernel<T, S>), dim3((unsigned)std::min(a.rows, QROWS)), dim3(QT), 0, st, a);
   else
     hipLaunchKernelGGL((fp8_quant_kernel<T, S>), dim3((unsigned)ceil_div((int64_t)a.rows * a.kb, QB)), dim3(QT), 0, st, a);
   return (int)hipGetLastError();

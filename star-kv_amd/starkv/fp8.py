@@ -106,6 +106,7 @@ def fp8_quantize(x: torch.Tensor, scale_dtype: torch.dtype = torch.float8_e8m0fn
     return (q if pitch == k else q[..., :k]), scale
 
 
+@torch.no_grad()
 def fp8_quantize_weight(w: torch.Tensor, scale_dtype: torch.dtype = torch.float8_e8m0fnu,
                         norm_weight: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """An nn.Linear weight [n, k] (any float type, any device) as e4m3 with one
@@ -113,7 +114,7 @@ def fp8_quantize_weight(w: torch.Tensor, scale_dtype: torch.dtype = torch.float8
     ceil(k / 128)]), by the same rule as ``fp8_quantize``.  ``norm_weight`` [k]:
     the weight of an RMSNorm applied to the input first, folded in for
     ``fp8_linear(..., rms_eps=...)``.  Run once when a model is loaded (torch
-    operations)."""
+    operations, none of them recorded for gradients)."""
     _scale_code(scale_dtype)
     if w.dim() != 2 or not w.numel():
         raise StarKVError(f"a weight is [n, k], got shape {tuple(w.shape)}")

@@ -2,8 +2,12 @@
 // weight (the definition is in starkv.h).
 //
 // One matrix instruction (16 x 16 x 128) is one block of 128 columns of 16
-// weight rows against 16 activation rows; its partial sums are scaled by sx sw
-// in fp32.  A workgroup owns NT groups of 16 weight rows (SiLU-multiply: 16
+// weight rows against 16 activation rows.  Power-of-two scales ride in the
+// instruction, exactly, and it adds to the accumulators; fp32 scales, and any
+// of fp32 outputs, multiply a block's sums as sx sw, formed in fp32.  (Formed
+// so for power-of-two scales too, a product of scales past 2^127 made NaN of
+// blocks of zeros, which the tiles of fp8_gemm.hip add as zeros.)  A workgroup
+// owns NT groups of 16 weight rows (SiLU-multiply: 16
 // gate rows and their 16 up rows) and MT groups of 16 activation rows; its
 // waves split the blocks of k and meet in LDS at the end.  Weight and
 // activation bytes go from memory to the matrix operand registers directly,
@@ -100,15 +104,18 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(const Fp8GemmArgs a) {
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const intx8 xf = frag8(d.x[i][0], d.x[i][1]);
-      const float sx = scale_f32(d.sx[i]);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const intx8 wf = frag8(d.w[t][0], d.w[t][1]);
-        const floatx4 p = __is_same(O, float) ? mfma8_exact(wf, xf)
-                                              : mfma8(wf, xf, floatx4{0.f, 0.f, 0.f, 0.f}, E8_ONE, E8_ONE);
-        const float sc = sx * scale_f32(d.sw[t]);
+        if constexpr (S::pow2 && !__is_same(O, float)) {
+          acc[t][i] = mfma8(wf, xf, acc[t][i], d.sw[t], d.sx[i]);
+        } else {
+          const floatx4 p = __is_same(O, float) ? mfma8_exact(wf, xf)
+                                                : mfma8(wf, xf, floatx4{0.f, 0.f, 0.f, 0.f}, E8_ONE, E8_ONE);
+          const float sc = scale_f32(d.sx[i]) * scale_f32(d.sw[t]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[t][i][e] = fmaf(p[e], sc, acc[t][i][e]);
+          for (int e = 0; e < 4; ++e) acc[t][i][e] = fmaf(p[e], sc, acc[t][i][e]);
+        }
       }
     }
   };

@@ -326,13 +326,13 @@ void fp8_gemm_kernel(const Fp8GemmArgs a) {
     } else if constexpr (PART) {
       part[j][i] = mfma8_32(o.w[j], o.x[i], FIRST ? floatx16{} : part[j][i], E8_ONE, E8_ONE);
     } else {
-      acc[j][i] = mfma8_32(o.w[j], o.x[i], acc[j][i], sc.w[SILU ? j / (J / 2) : 0], sc.x[i]);
+      acc[j][i] = mfma8_32(o.w[j], o.x[i], acc[j][i], sc.w[SILU ? 2 * j / J : 0], sc.x[i]);
     }
   };
   auto rescale = [&](const Sc& sc, int q) __attribute__((always_inline)) {
     if constexpr (PART) {
       const int j = q % J, i = q / J;
-      const float s = scale_f32((ST)sc.x[i]) * scale_f32((ST)sc.w[SILU ? j / (J / 2) : 0]);
+      const float s = scale_f32((ST)sc.x[i]) * scale_f32((ST)sc.w[SILU ? 2 * j / J : 0]);
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[j][i][e] = fmaf(part[j][i][e], s, acc[j][i][e]);
     }

@@ -2,16 +2,16 @@
 // weight (the definition is in starkv.h).
 //
 // One matrix instruction (16 x 16 x 128) is one block of 128 columns of 16
-// weight rows against 16 activation rows.  Power-of-two scales ride in the
-// instruction, exactly, and it adds to the accumulators; fp32 scales, and any
-// of fp32 outputs, multiply a block's sums as sx sw, formed in fp32.  (Formed
-// so for power-of-two scales too, a product of scales past 2^127 made NaN of
-// blocks of zeros, which the tiles of fp8_gemm.hip add as zeros.)  A workgroup
-// owns NT groups of 16 weight rows (SiLU-multiply: 16
-// gate rows and their 16 up rows) and MT groups of 16 activation rows; its
-// waves split the blocks of k and meet in LDS at the end.  Weight and
-// activation bytes go from memory to the matrix operand registers directly,
-// without LDS: FW blocks in flight per wave and as many waves as fit.
+// weight rows against 16 activation rows, added up in fp32.  Power-of-two
+// scales ride in the instruction, exactly; fp32 scales, and any of fp32
+// outputs, multiply a block's sums as sx sw, formed in fp32.  (Formed so for
+// power-of-two scales too, a product of scales past 2^127 made NaN of blocks of
+// zeros, which the tiles of fp8_gemm.hip add as zeros.)  A workgroup owns NT
+// groups of 16 weight rows (SiLU-multiply: 16 gate rows and their 16 up rows)
+// and MT groups of 16 activation rows; its waves split the blocks of k and meet
+// in LDS at the end.  Weight and activation bytes go from memory to the matrix
+// operand registers directly, without LDS: a block or two in flight per wave
+// and as many waves as fit.
 //
 // Bound by the weight stream for few rows (6.5 TB/s beside 3.4 us of launch
 // and first loads: m 1, n 22016, k 4096 in 17.3 us), by the reads of the
@@ -29,7 +29,7 @@
 namespace starkv {
 
 namespace {
-constexpr int FW = 2;                              // k blocks a wave loads at a time (1: the same; 4: 5 to 15 % slower)
+constexpr int FW_PART = 2;                         // k blocks a wave loads at a time, sums scaled apart (1: the same; 4: 5 to 15 % slower)
 }  // namespace
 
 // O: output type; NT: groups of weight rows (SILU: 2, gate and up); MT: groups of activation rows
@@ -65,6 +65,10 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(const Fp8GemmArgs a) {
     xsc[i] = (const typename S::T*)a.sx + (int64_t)r * a.sxr;
   }
 
+  // Scales that the instruction takes are asked for before the bytes they go with: behind them, or behind the first
+  // product (where the compiler put one, or two blocks at a time), m 8, n 22016, k 4096 with SiLU took 2 % more.
+  constexpr bool SCALED = S::pow2 && !__is_same(O, float);
+  constexpr int FW = SCALED ? 1 : FW_PART;
   floatx4 acc[NT][MT];
 #pragma unroll
   for (int t = 0; t < NT; ++t)
@@ -75,7 +79,17 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(const Fp8GemmArgs a) {
     typename S::T sx[MT], sw[NT];
   };
   // block bb's bytes; SHORT: pieces behind column k repeat the last one
+  auto scales = [&](Block& d, int bb) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i) d.sx[i] = xsc[i][(int64_t)bb * a.sxb];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) d.sw[t] = wsc[t][(int64_t)bb * a.swb];
+  };
   auto load = [&](auto short_c, Block& d, int bb) __attribute__((always_inline)) {
+    if constexpr (SCALED) {
+      scales(d, bb);
+      __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       int64_t at = (int64_t)bb * FP8_BLOCK + 64 * h;
@@ -85,12 +99,10 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(const Fp8GemmArgs a) {
 #pragma unroll
       for (int i = 0; i < MT; ++i) d.x[i][h] = *(const uint4*)(xrow[i] + at);
     }
-#pragma unroll
-    for (int i = 0; i < MT; ++i) d.sx[i] = xsc[i][(int64_t)bb * a.sxb];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) d.sw[t] = wsc[t][(int64_t)bb * a.swb];
+    if constexpr (!SCALED) scales(d, bb);
   };
   auto use = [&](auto short_c, Block& d, int bb) __attribute__((always_inline)) {
+    if constexpr (SCALED) __builtin_amdgcn_sched_barrier(0);       // all that a block needs is asked for first
     if constexpr (decltype(short_c)::value) {      // columns past k: any value in either operand
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -107,8 +119,8 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(const Fp8GemmArgs a) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const intx8 wf = frag8(d.w[t][0], d.w[t][1]);
-        if constexpr (S::pow2 && !__is_same(O, float)) {
-          acc[t][i] = mfma8(wf, xf, acc[t][i], d.sw[t], d.sx[i]);
+        if constexpr (SCALED) {
+          acc[t][i] += mfma8(wf, xf, floatx4{0.f, 0.f, 0.f, 0.f}, d.sw[t], d.sx[i]);
         } else {
           const floatx4 p = __is_same(O, float) ? mfma8_exact(wf, xf)
                                                 : mfma8(wf, xf, floatx4{0.f, 0.f, 0.f, 0.f}, E8_ONE, E8_ONE);

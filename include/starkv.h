@@ -522,8 +522,7 @@ int starkv_fp8_quantize(const starkv_fp8_quantize_desc* d, void* stream);
 
 /* starkv_fp8_gemm: nn.Linear by an e4m3 weight,
  *   y[i][j] = r_i * sum_b sx[i][b] sw[j / 128][b] sum_{k in b} qx[i][k] qw[j][k]
- * accumulated in fp32 (sx sw too is formed in fp32 or exactly) and rounded
- * once to out_dtype (the act dtypes or F32):
+ * summed in fp32 and rounded once to out_dtype (the act dtypes or F32):
  *   out[i][j] = y[i][j] (+ residual[i][j])                        j < n
  *   silu_mul: out[i][j] = y[i][j] / (1 + exp(-y[i][j])) * y[i][n/2 + j]   j < n/2
  *             (LlamaMLP over the gate rows followed by the up rows of one
@@ -536,7 +535,18 @@ int starkv_fp8_quantize(const starkv_fp8_quantize_desc* d, void* stream);
  * that are multiples of 16 (STARKV_ERR_ALIGN); they are read in whole 16-byte
  * pieces that hold at least one byte of a row, and what lies behind column k
  * never reaches a result.  residual (row stride residual_stride elements, of
- * out_dtype) may be out itself.  Any m >= 0, n >= 1, k >= 1.
+ * out_dtype) may be out itself.  Any m >= 0, n >= 1, k >= 1 up to 2^30, 2^30
+ * and 2^24, m ceil(k / 128) below 2^28, about 2^22 tiles of output (64 x 32 to
+ * 256 x 256 by the size; 16 columns a tile for few rows): STARKV_ERR_LIMIT.
+ * Precision.  For F32 outputs every product enters the sums exactly.  For
+ * 16-bit outputs the matrix instruction adds each eight consecutive columns'
+ * products with 13 bits or more below the largest of them: a result is off by
+ * at most 7 * 2^-13 sum |x||w| before it is rounded (1.5e-5 of the results in
+ * the norm, so that a few rounded values in a hundred (F16) or a thousand
+ * (BF16) are neighbours of those that an fp32 product rounds to).
+ * E8M0 scales with 16-bit outputs are applied exactly; F32 scales, and either
+ * type with F32 outputs, as sx * sw formed in fp32 (where that is infinite, the
+ * block's sums are infinite or NaN, also of zeros).
  * Workspace: the quantised activations (0 for e4m3 ones).
  * Results do not depend on the order of atomics; the same call gives the
  * same bits.

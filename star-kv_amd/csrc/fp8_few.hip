@@ -78,13 +78,13 @@ __global__ __launch_bounds__(512) void fp8_few_kernel(const Fp8GemmArgs a) {
     uint4 x[MT][2], w[NT][2];
     typename S::T sx[MT], sw[NT];
   };
-  // block bb's bytes; SHORT: pieces behind column k repeat the last one
   auto scales = [&](Block& d, int bb) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < MT; ++i) d.sx[i] = xsc[i][(int64_t)bb * a.sxb];
 #pragma unroll
     for (int t = 0; t < NT; ++t) d.sw[t] = wsc[t][(int64_t)bb * a.swb];
   };
+  // block bb's bytes; SHORT: pieces behind column k repeat the last one
   auto load = [&](auto short_c, Block& d, int bb) __attribute__((always_inline)) {
     if constexpr (SCALED) {
       scales(d, bb);

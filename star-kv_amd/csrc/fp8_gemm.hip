@@ -467,8 +467,8 @@ void fp8_gemm_kernel(const Fp8GemmArgs a) {
 // with the matrix cores idle unless memory is late.  (One meeting, after half
 // 0: loads in a burst of 16 products, 16 products to land: 2 % slower.)
 // Measured: 1.4 us a block on all CUs, where products alone take 1.0; without
-// the loads 1.2, without the reads 1.24.  8192 x 22016 x 4096 with SiLU: 565 us,
-// 2610 TFLOP/s.
+// the loads 1.2, without the reads 1.24.  8192 x 22016 x 4096 with SiLU: 565 to
+// 600 us by the card, 2610 to 2460 TFLOP/s.
 //
 // A workgroup takes tile after tile: the next tile's first two blocks load
 // while this one's results are stored, and the stores drain behind the next
@@ -723,8 +723,10 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_wide_kernel(const Fp8GemmArgs
 // of 64 and 128 columns run with one workgroup on a CU or two, the larger ones
 // alone, and their blocks go the faster the more CUs idle.  Fitted to the
 // times of every tile in 252 products of n 1640 to 22016, k 320 to 11008, 48
-// to 8192 rows: the tile picked is the fastest or within 8 % of it in all but
-// three (10 to 16 %).  Small tiles fill the chip with few rows, large ones
+// to 8192 rows, all with bf16 outputs: the tile picked is the fastest or within
+// 8 % of it in all but three (10 to 16 %).  (fp32 outputs, whose blocks take 16-bit
+// instructions, go by the table of sums scaled apart; their tiles have not been
+// timed one against the other.)  Small tiles fill the chip with few rows, large ones
 // read less per product: powers of two, 2048 x 4096, k 4096 takes 89, 62, 47,
 // 38, 37 and 49 us on the tiles below, 256 rows of it 15, 14, 17, 21, 27 and
 // 43, 4096 rows 59 on the last and 70 on the one before it.

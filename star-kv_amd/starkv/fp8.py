@@ -206,9 +206,11 @@ def fp8_matmul(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, wei
                out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """x W^T of quantised activations (``fp8_quantize``: e4m3 x [..., k] with
     x_scale [..., ceil(k / 128)], rows whole 16-byte pieces apart) and a
-    quantised weight [n, k], accumulated in fp32 and rounded once (to bfloat16
-    unless ``out_dtype`` or ``out`` says otherwise).  The scales of both are of
-    one type.  ``residual`` [..., n] is added (``out`` may be it); with
+    quantised weight [n, k], summed in fp32 and rounded once (to bfloat16
+    unless ``out_dtype`` or ``out`` says otherwise).  For 16-bit results the
+    matrix instruction keeps 13 bits or more below the largest of each eight
+    products (1.5e-5 of the results in the norm); ``out_dtype=torch.float32``
+    adds exact products, at half the rate.  The scales of both are of one type.  ``residual`` [..., n] is added (``out`` may be it); with
     ``silu_mul`` the weight holds gate rows then up rows and the result is
     SiLU(x Wg^T) * (x Wu^T) [..., n / 2], each half whole blocks of 128 rows."""
     if x.dtype != torch.float8_e4m3fn:

@@ -597,6 +597,124 @@ typedef struct {
 size_t starkv_token_logprobs_workspace_bytes(const starkv_logprobs_desc* d);
 int starkv_token_logprobs(const starkv_logprobs_desc* d, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------
+ * Attention weights summed by position, and caches bounded by them.  No
+ * counterpart in the reference, whose caches only grow (HF:cache_utils.py:127-146).
+ *
+ * starkv_attention_scores:
+ *   scores[b][p] (+)= sum_h softmax_p(logits[b][h])[p],  p < seq_len
+ * in fp32 (add != 0: onto what is there).  logits: dtype F16, BF16 or F32,
+ * element (b, h, p) at logits + b*stride_b + h*stride_h + p, any alignment of
+ * whole elements.  A row of nothing but -inf adds nothing; a row with a NaN or
+ * +inf adds NaN at every position.  n_heads <= 1024, batch <= 65535, seq_len <=
+ * 2^24.  The sums are the same on every run.
+ *
+ * starkv_decode_attention_scores: starkv_decode_attention (the same output)
+ * that also adds each position's weights of all query heads onto
+ * scores[b * scores_stride_b + p], p < seq_len (the same workspace).
+ * ------------------------------------------------------------------- */
+typedef struct {
+  int batch, n_heads, seq_len, dtype;
+  const void* logits; int64_t stride_b, stride_h;
+  int add;
+  float* scores; int64_t scores_stride_b;
+} starkv_scores_desc;
+
+size_t starkv_attention_scores_workspace_bytes(const starkv_scores_desc* d);
+int starkv_attention_scores(const starkv_scores_desc* d, void* workspace, size_t workspace_bytes, void* stream);
+int starkv_decode_attention_scores(const starkv_decode_desc* d, float* scores, int64_t scores_stride_b, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------
+ * starkv_select_positions: the `keep` of a row's `length` positions that a
+ * bounded cache keeps, in ascending order: the first `sinks`, the last
+ * `recent`, and of those between the keep - sinks - recent with the largest
+ * scores (equal ones: the lowest positions; NaN counts as -infinity).
+ * 0 <= sinks + recent <= keep <= length <= 2^24.
+ * scores (b, p) at scores + b*scores_stride_b + p; positions (b, i) at
+ * positions + b*positions_stride_b + i.
+ *
+ * starkv_keep_positions: rows positions[b][i] of the K and V latents (with
+ * their scales and zero points) and scores become rows i < keep, in place;
+ * rows from keep on stay as they are, scores[b][keep .. length) become 0.
+ * Needs i <= positions[b][i] < length, as starkv_select_positions writes them:
+ * a position that breaks it leaves row i as it is and sets *error_flag
+ * (optional device int, never cleared by the library) to 1.  The keys are
+ * stored before rotation, so a moved row takes the angle of its new place.
+ * B_k's fields of k are not read.  dtype: of dense latents.  batch <= 65535;
+ * rows of different positions, heads or sequences must not overlap.
+ * ------------------------------------------------------------------- */
+typedef struct {
+  int batch, length, keep, sinks, recent;
+  const float* scores; int64_t scores_stride_b;
+  int* positions; int64_t positions_stride_b;
+} starkv_select_desc;
+
+int starkv_select_positions(const starkv_select_desc* d, void* stream);
+
+typedef struct {
+  int batch, length, keep, dtype;
+  const int* positions; int64_t positions_stride_b;
+  starkv_klatent k;
+  starkv_vlatent v;
+  float* scores; int64_t scores_stride_b;      /* optional */
+  int* error_flag;                             /* optional */
+} starkv_keep_desc;
+
+int starkv_keep_positions(const starkv_keep_desc* d, void* stream);
+
+/* ---------------------------------------------------------------------
+ * Decode of a batch whose sequences share a prefix (a system prompt, the
+ * prompt of several samples): attention over the prefix is computed once for
+ * all.  No counterpart in the reference, which holds a copy of the prefix for
+ * each sequence.
+ *
+ * starkv_prefix_pack lays out one sequence's dense latents (positions [0,
+ * length) of k and v, whose stride_b is not read) and B_k for
+ * starkv_prefix_decode, once; prefix: starkv_prefix_bytes, 256-byte aligned.
+ * attention_scaling: the rotation table's (rope_build).
+ *
+ * starkv_prefix_decode: out[b, q] = U_v[q / gs] (softmax over the prefix's and
+ * the sequence's own positions of the logits, times their value latents), with
+ *   prefix position p: scale * RoPE_length(q[b,q]) . RoPE_p(X_k[p] B_k)
+ *   own position s:    scale * q[b,q] . RoPE_s(x_k[b,s] B_k) (+ mask)
+ * that is, own.q is rotated at its position behind the sequence's own first one
+ * (as the cache writer does, whose positions are the cache's), and the prefix
+ * lies before that one.  own: as for starkv_decode_attention; own.seq_len 0:
+ * no own positions (k, v, mask and last_pos_device are not read).  A sequence
+ * whose mask leaves none of its own positions attends to the prefix alone.
+ * turn_cos / turn_sin: host arrays [64], the (unscaled) rotation of frequency i
+ * by `length` positions.  The prefix's rank, v_rank, length and dtype are those
+ * it was packed with; rope_max_positions >= round_up(length, 64).  scores
+ * (optional): the weights of own positions, summed over the query heads, are
+ * added onto scores[b * scores_stride_b + s].
+ * Keys over the prefix are fp16 between the reconstruction and the logits,
+ * weights fp16 relative to a strip of 64 positions, sums fp32.
+ * Results do not depend on the order of atomics.
+ * ------------------------------------------------------------------- */
+typedef struct {
+  int length, dtype;
+  starkv_klatent k;
+  starkv_vlatent v;
+  float attention_scaling;
+  void* prefix; size_t prefix_bytes;
+} starkv_prefix_pack_desc;
+
+size_t starkv_prefix_bytes(const starkv_prefix_pack_desc* d);          /* 0: invalid */
+int starkv_prefix_pack(const starkv_prefix_pack_desc* d, void* stream);
+
+typedef struct {
+  starkv_decode_desc own;
+  int n_kv_heads, v_rank, length;
+  const int* rank;                             /* host [n_kv_heads] */
+  const void* prefix; size_t prefix_bytes;
+  const float* turn_cos; const float* turn_sin;
+  float* scores; int64_t scores_stride_b;
+} starkv_prefix_decode_desc;
+
+size_t starkv_prefix_decode_workspace_bytes(const starkv_prefix_decode_desc* d);   /* 0: invalid */
+int starkv_prefix_decode(const starkv_prefix_decode_desc* d, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -4,6 +4,7 @@
 // before any HIP call so that every argument error is reported without a GPU.
 #include <algorithm>
 #include <climits>
+#include <cmath>
 #include <mutex>
 #include <vector>
 
@@ -1049,19 +1050,11 @@ size_t starkv_decode_workspace_bytes(const starkv_decode_desc* d) {
                     d->dtype == STARKV_F16).total;
 }
 
-static int decode_impl(const starkv_decode_desc* d, void* workspace, size_t workspace_bytes, void* stream,
-                       void* const* events) {
-  int gs = 0, n_wg = 0, k1pc = 1, vq = 0, st;
-  if ((st = validate_decode(d, &gs, &n_wg, &k1pc, &vq))) return st;
-  const DecodeLayout L =
-      decode_layout(d->batch, d->n_q_heads, d->k.n_kv_heads, d->seq_len, d->v.rank, n_wg, k1pc, vq, v_row_bytes(d->v),
-                    d->dtype == STARKV_F16);
-  if (!workspace || workspace_bytes < L.total) return STARKV_ERR_WORKSPACE;
-  if (!al(workspace, 256)) return STARKV_ERR_ALIGN;
-  char* ws = (char*)workspace;
-  hipStream_t s = (hipStream_t)stream;
+// the logits and P.V of a validated decode call, into its workspace
+static int decode_sums(const starkv_decode_desc* d, const DecodeLayout& L, int gs, char* ws, hipStream_t s,
+                       void* const* events, PVArgs& pa) {
   const int B = d->batch, Hq = d->n_q_heads;
-
+  int vq = 0, st;
   KArgs ka;
   KPlan plan;
   if ((st = build_k_plan(d->k, Hq, gs, d->dtype, d->seq_len, ka, plan, false, true))) return st;
@@ -1083,7 +1076,7 @@ static int decode_impl(const starkv_decode_desc* d, void* workspace, size_t work
   if ((st = launch_k_logits(ka, d->dtype, d->k.format, true, STARKV_F32, kfast, B, s))) return st;
   if (events && (st = (int)hipEventRecord((hipEvent_t)events[1], s))) return st;
 
-  PVArgs pa = {};
+  pa = PVArgs{};
   if ((st = validate_v(d->v, pa, &vq))) return st;
   vq = pv_storage(pa, vq, d->v.rank, true, d->seq_len);
   pa.logits = (const float*)(ws + L.off_logits); pa.l_sb = ka.o_sb; pa.l_st = ka.o_st; pa.l_sh = ka.o_sh;
@@ -1093,6 +1086,41 @@ static int decode_impl(const starkv_decode_desc* d, void* workspace, size_t work
   pa.n_cb = L.pv.n_cb; pa.n_c2 = L.pv.n_c2; pa.c2_len = L.pv.c2_len;
   if ((st = launch_pv(pa, d->dtype, vq, true, v_fast(d->v, pa), B, s))) return st;
   if (events && (st = (int)hipEventRecord((hipEvent_t)events[2], s))) return st;
+  return STARKV_OK;
+}
+
+// weights of a decode call's logits by position, from its maxima and sums
+static int decode_scores(const starkv_decode_desc* d, const DecodeLayout& L, const char* ws, const float* rmax, int n_max,
+                         const float* rsum, int n_sum, float* scores, int64_t stride, hipStream_t s) {
+  ScoreArgs a = {};
+  a.x = ws + L.off_logits; a.x_sb = (int64_t)d->n_q_heads * L.S_pad; a.x_st = (int64_t)d->n_q_heads * TILE; a.x_sh = TILE;
+  a.B = d->batch; a.H = d->n_q_heads; a.S = d->seq_len; a.add = 1;
+  a.rmax = rmax; a.n_max = n_max; a.rsum = rsum; a.n_sum = n_sum; a.n_hg = L.n_hg;
+  a.out = scores; a.o_sb = stride;
+  return launch_scores(a, STARKV_F32, true, s);
+}
+
+static int check_scores(const starkv_decode_desc* d, const float* scores, int64_t stride) {
+  if (!al(scores, 4)) return STARKV_ERR_ALIGN;
+  if (d->batch > 65535) return STARKV_ERR_LIMIT;
+  return d->batch > 1 && stride < d->seq_len ? STARKV_ERR_SHAPE : STARKV_OK;
+}
+
+static int decode_impl(const starkv_decode_desc* d, void* workspace, size_t workspace_bytes, void* stream,
+                       void* const* events, float* scores = nullptr, int64_t scores_stride = 0) {
+  int gs = 0, n_wg = 0, k1pc = 1, vq = 0, st;
+  if ((st = validate_decode(d, &gs, &n_wg, &k1pc, &vq))) return st;
+  if (scores && (st = check_scores(d, scores, scores_stride))) return st;
+  const DecodeLayout L =
+      decode_layout(d->batch, d->n_q_heads, d->k.n_kv_heads, d->seq_len, d->v.rank, n_wg, k1pc, vq, v_row_bytes(d->v),
+                    d->dtype == STARKV_F16);
+  if (!workspace || workspace_bytes < L.total) return STARKV_ERR_WORKSPACE;
+  if (!al(workspace, 256)) return STARKV_ERR_ALIGN;
+  char* ws = (char*)workspace;
+  hipStream_t s = (hipStream_t)stream;
+  const int B = d->batch, Hq = d->n_q_heads;
+  PVArgs pa;
+  if ((st = decode_sums(d, L, gs, ws, s, events, pa))) return st;
 
   UPArgs ua;
   ua.part = pa.part; ua.psum = pa.psum; ua.part16 = L.part16; ua.n_c2 = L.pv.n_c2; ua.Rvp = L.pv.Rvp;
@@ -1105,6 +1133,7 @@ static int decode_impl(const starkv_decode_desc* d, void* workspace, size_t work
   const bool ufast = al(d->uv, 16) && al64(d->uv_row_stride * 2, 16);
   if ((st = launch_up_proj(ua, d->dtype, ufast, s))) return st;
   if (events && (st = (int)hipEventRecord((hipEvent_t)events[3], s))) return st;
+  if (scores) return decode_scores(d, L, ws, pa.chunkmax, L.n_c1, pa.psum, L.pv.n_c2, scores, scores_stride, s);
   return STARKV_OK;
 }
 
@@ -1638,6 +1667,322 @@ int starkv_token_logprobs(const starkv_logprobs_desc* d, void* workspace, size_t
   a.x = d->logits; a.xs = d->stride; a.tok = d->tokens;
   a.lp = d->logprob; a.ent = d->entropy; a.tlp = d->top_logprob; a.tid = d->top_id;
   return launch_logprobs(a, wide, d->dtype, (hipStream_t)stream);
+}
+
+
+// ---------------------------------------------------------------------------
+// Bounded caches
+// ---------------------------------------------------------------------------
+static int check_scores_desc(const starkv_scores_desc* d) {
+  if (!d) return STARKV_ERR_NULL;
+  if (d->batch < 1 || d->n_heads < 1 || d->seq_len < 1) return STARKV_ERR_SHAPE;
+  if (d->batch > 65535 || d->n_heads > SCORE_MAX_H || d->seq_len > MAX_S) return STARKV_ERR_LIMIT;
+  if (!act16(d->dtype) && d->dtype != STARKV_F32) return STARKV_ERR_DTYPE;
+  // one workgroup of 256 threads a piece
+  if ((int64_t)d->batch * d->n_heads * score_pieces(d->seq_len) * 256 > MAX_THREADS_1D) return STARKV_ERR_LIMIT;
+  return STARKV_OK;
+}
+
+size_t starkv_attention_scores_workspace_bytes(const starkv_scores_desc* d) {
+  return check_scores_desc(d) ? 0 : (size_t)d->batch * d->n_heads * score_pieces(d->seq_len) * 8;
+}
+
+int starkv_attention_scores(const starkv_scores_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
+  const int st = check_scores_desc(d);
+  if (st) return st;
+  if (!d->logits || !d->scores) return STARKV_ERR_NULL;
+  if (d->stride_b < 0 || d->stride_h < 0 || (d->batch > 1 && d->scores_stride_b < d->seq_len)) return STARKV_ERR_SHAPE;
+  if (!al(d->logits, esize(d->dtype)) || !al(d->scores, 4)) return STARKV_ERR_ALIGN;
+  if (!workspace || workspace_bytes < starkv_attention_scores_workspace_bytes(d)) return STARKV_ERR_WORKSPACE;
+  if (!al(workspace, 256)) return STARKV_ERR_ALIGN;
+  ScoreArgs a = {};
+  a.x = d->logits; a.x_sb = d->stride_b; a.x_st = 32; a.x_sh = d->stride_h;
+  a.B = d->batch; a.H = d->n_heads; a.S = d->seq_len; a.add = d->add != 0;
+  a.stat = (float2*)workspace; a.n_max = score_pieces(d->seq_len);
+  a.out = d->scores; a.o_sb = d->scores_stride_b;
+  return launch_scores(a, d->dtype, false, (hipStream_t)stream);
+}
+
+int starkv_decode_attention_scores(const starkv_decode_desc* d, float* scores, int64_t scores_stride_b, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  if (!scores) return STARKV_ERR_NULL;
+  return decode_impl(d, workspace, workspace_bytes, stream, nullptr, scores, scores_stride_b);
+}
+
+int starkv_select_positions(const starkv_select_desc* d, void* stream) {
+  if (!d) return STARKV_ERR_NULL;
+  if (d->batch < 0 || d->length < 0 || d->sinks < 0 || d->recent < 0 || d->keep > d->length ||
+      (int64_t)d->sinks + d->recent > d->keep)
+    return STARKV_ERR_SHAPE;
+  if (d->length > MAX_S || d->batch > (1 << 20)) return STARKV_ERR_LIMIT;
+  if (d->batch == 0 || d->keep == 0) return STARKV_OK;
+  if (!d->scores || !d->positions) return STARKV_ERR_NULL;
+  if (d->batch > 1 && (d->scores_stride_b < 0 || d->positions_stride_b < d->keep)) return STARKV_ERR_SHAPE;
+  if (!al(d->scores, 4) || !al(d->positions, 4)) return STARKV_ERR_ALIGN;
+  SelectArgs a = {d->scores, d->scores_stride_b, d->positions, d->positions_stride_b, d->length, d->keep, d->sinks, d->recent};
+  return launch_select(a, d->batch, (hipStream_t)stream);
+}
+
+int starkv_keep_positions(const starkv_keep_desc* d, void* stream) {
+  if (!d) return STARKV_ERR_NULL;
+  if (d->batch < 1 || d->length < 0 || d->keep < 0 || d->keep > d->length) return STARKV_ERR_SHAPE;
+  if (d->length > MAX_S || d->batch > 65535) return STARKV_ERR_LIMIT;
+  const starkv_klatent& k = d->k;
+  const starkv_vlatent& v = d->v;
+  PVArgs pv = {};
+  int vq = 0, st;
+  if ((st = validate_klayout(k, d->dtype)) || (st = validate_v(v, pv, &vq))) return st;
+  if (d->length == 0) return STARKV_OK;
+  if (!d->positions && d->keep) return STARKV_ERR_NULL;
+  const bool many = d->batch > 1, dense = k.format == STARKV_FMT_DENSE, two = k.format == STARKV_FMT_INT4_REF && k.split > 0;
+  if (many && (d->positions_stride_b < d->keep || (d->scores && d->scores_stride_b < d->length))) return STARKV_ERR_SHAPE;
+  if (!al(d->positions, 4) || !al(d->scores, 4)) return STARKV_ERR_ALIGN;
+  MoveArgs a = {};
+  a.pos = d->positions; a.p_sb = d->positions_stride_b; a.keep = d->keep; a.length = d->length; a.err = d->error_flag;
+  const int es = dense ? 2 : 1, H = k.n_kv_heads, split = two ? k.split : 128;
+  const bool a8 = two ? k.split_format == STARKV_FMT_INT8_SYM : k.format == STARKV_FMT_INT8_SYM;
+  a.k1 = (uint8_t*)k.data; a.k1_sb = k.stride_b * es;
+  a.k2 = (uint8_t*)k.data2; a.k2_sb = k.stride2_b;
+  bool lower = false;
+  for (int h = 0; h < H; ++h) {
+    const int r = k.rank[h], up = std::min(r, split);
+    a.off1[h] = k.head_offset[h] * es; a.pitch1[h] = k.pos_stride[h] * es;
+    a.nb1[h] = dense ? 2 * r : a8 ? up : (up + 1) / 2;
+    if (!two || r <= split) continue;
+    lower = true;
+    a.off2[h] = k.head_offset2[h]; a.pitch2[h] = k.pos_stride2[h]; a.nb2[h] = (r - split + 1) / 2;
+  }
+  a.units[MOVE_K1] = H;
+  a.units[MOVE_K2] = lower ? H : 0;
+  if (!dense) {
+    a.ks1 = (uint8_t*)k.scale; a.ks1_sb = 2 * k.scale_stride_b; a.ks1_sh = 2 * k.scale_stride_h;
+    a.units[MOVE_KS1] = H;
+  }
+  if (lower) {
+    a.ks2 = (uint8_t*)k.scale2; a.ks2_sb = 2 * k.scale2_stride_b; a.ks2_sh = 2 * k.scale2_stride_h;
+    a.units[MOVE_KS2] = H;
+  }
+  if (many && (!a.k1_sb || (lower && !a.k2_sb) || (!dense && !a.ks1_sb) || (lower && !a.ks2_sb))) return STARKV_ERR_SHAPE;
+  if (H > 1 && ((!dense && !a.ks1_sh) || (lower && !a.ks2_sh))) return STARKV_ERR_SHAPE;
+  // V rows, the lower block's, their scales and zero points
+  const int vs = vq == VQ_DENSE ? 2 : 1, groups = vq == VQ_G64 ? (v.rank + 63) / 64 : 1;
+  a.v[0] = {(uint8_t*)v.data, v.stride_b * vs, v.stride_s * vs, vq == VQ_DENSE ? 2 * v.rank : pv.xnb};
+  if (pv.x2) a.v[1] = {(uint8_t*)v.data2, v.stride2_b, v.stride2_s, pv.x2nb};
+  if (vq != VQ_DENSE) a.v[2] = {(uint8_t*)v.scale, 2 * v.scale_stride_b, 2 * v.scale_stride_s, 2 * groups};
+  if (pv.x2) a.v[3] = {(uint8_t*)v.scale2, 2 * v.scale2_stride_b, 2 * v.scale2_stride_s, 2};
+  if (vq == VQ_G64) a.v[4] = {(uint8_t*)v.zero, 2 * v.scale_stride_b, 2 * v.scale_stride_s, 2 * groups};
+  for (int i = 0; i < MOVE_SCORES - MOVE_V; ++i) {
+    a.units[MOVE_V + i] = (int)ceil_div(a.v[i].nb, MOVE_SLICE);
+    if (a.v[i].nb && (a.v[i].pitch < a.v[i].nb || (many && !a.v[i].sb))) return STARKV_ERR_SHAPE;
+  }
+  if (d->scores) { a.scores = d->scores; a.scores_sb = d->scores_stride_b; a.units[MOVE_SCORES] = 1; }
+  return launch_move(a, d->batch, (hipStream_t)stream);
+}
+
+// ---------------------------------------------------------------------------
+// Decode over a shared prefix
+// ---------------------------------------------------------------------------
+namespace {
+
+constexpr int64_t PX_MAX_ROWS = 1 << 20;           // (sequence, query head) rows of a call
+
+// offsets of a packed prefix
+struct PrefixSpace {
+  int strips, Rvp, ks_max;
+  int64_t xkoff[K_MAX_KV], xboff[K_MAX_KV];
+  size_t off_xk, off_xb, off_xv, total;
+};
+
+int prefix_space(int n_kv, const int* rank, int Rv, int P, PrefixSpace& s) {
+  if (n_kv < 1 || P < 1) return STARKV_ERR_SHAPE;
+  if (n_kv > K_MAX_KV || P > MAX_S) return STARKV_ERR_LIMIT;
+  if (!rank) return STARKV_ERR_NULL;
+  if (Rv < 1 || Rv > MAX_RV) return STARKV_ERR_RANK;
+  s = PrefixSpace{};
+  s.strips = (int)ceil_div(P, PX_STRIP);
+  s.Rvp = (int)round_up(Rv, 32);
+  int64_t k = 0, b = 0;
+  for (int h = 0; h < n_kv; ++h) {
+    if (rank[h] < 1 || rank[h] > 128) return STARKV_ERR_RANK;
+    s.xkoff[h] = k; s.xboff[h] = b;
+    const int nc = (rank[h] + 7) / 8;
+    k += (int64_t)s.strips * 2 * nc * 512;
+    b += (int64_t)((nc + 1) / 2) * 4096;
+    s.ks_max = std::max(s.ks_max, (nc + 1) / 2);
+  }
+  s.off_xk = PX_HEAD_BYTES;
+  s.off_xb = s.off_xk + (size_t)k;
+  s.off_xv = s.off_xb + (size_t)b;
+  s.total = s.off_xv + (size_t)s.strips * PX_STRIP * s.Rvp * 2;
+  return STARKV_OK;
+}
+
+int check_pack(const starkv_prefix_pack_desc* d, PrefixSpace& s) {
+  if (!d) return STARKV_ERR_NULL;
+  if (!act16(d->dtype)) return STARKV_ERR_DTYPE;
+  if (d->k.format != STARKV_FMT_DENSE || d->v.format != STARKV_FMT_DENSE) return STARKV_ERR_FORMAT;
+  PVArgs pv = {};
+  int vq = 0, st;
+  if ((st = validate_klayout(d->k, d->dtype)) || (st = validate_v(d->v, pv, &vq))) return st;
+  if (!d->k.bk || !d->k.bk_head_offset) return STARKV_ERR_NULL;
+  if (d->k.bk_row_stride < HEAD_DIM) return STARKV_ERR_SHAPE;
+  return prefix_space(d->k.n_kv_heads, d->k.rank, d->v.rank, d->length, s);
+}
+
+struct PrefixLayout {
+  DecodeLayout own;
+  PrefixSpace space;
+  bool has_own;
+  int gs, M, Mp, bm, tiles_m, tiles_n, n_split, sp_len, n_ch, ch_len, n_hg, sw, n_sl;
+  size_t off_p, off_stat, off_cmax, off_rmax, off_part, off_lsum, off_jpart, off_jsum, off_jmax, off_ypart, total;
+};
+
+int prefix_layout(const starkv_prefix_decode_desc* d, PrefixLayout& L) {
+  if (!d) return STARKV_ERR_NULL;
+  const starkv_decode_desc& o = d->own;
+  L = PrefixLayout{};
+  int st;
+  if ((st = prefix_space(d->n_kv_heads, d->rank, d->v_rank, d->length, L.space))) return st;
+  L.has_own = o.seq_len != 0;
+  if (L.has_own) {
+    int n_wg = 0, k1pc = 1, vq = 0;
+    if ((st = validate_decode(&o, &L.gs, &n_wg, &k1pc, &vq))) return st;
+    if (o.k.n_kv_heads != d->n_kv_heads || o.v.rank != d->v_rank) return STARKV_ERR_SHAPE;
+    for (int h = 0; h < d->n_kv_heads; ++h)
+      if (o.k.rank[h] != d->rank[h]) return STARKV_ERR_SHAPE;
+    L.own = decode_layout(o.batch, o.n_q_heads, d->n_kv_heads, o.seq_len, o.v.rank, n_wg, k1pc, vq, v_row_bytes(o.v),
+                          o.dtype == STARKV_F16);
+  } else {
+    if (o.batch < 1 || o.head_dim != HEAD_DIM || o.n_q_heads < 1 || o.n_q_heads % d->n_kv_heads) return STARKV_ERR_SHAPE;
+    if (!act16(o.dtype)) return STARKV_ERR_DTYPE;
+    if (o.n_q_heads > K2_MAX_H) return STARKV_ERR_LIMIT;
+    if (!o.q || !o.uv || !o.out || !o.rope_table) return STARKV_ERR_NULL;
+    if (o.uv_row_stride < d->v_rank) return STARKV_ERR_SHAPE;
+    if (o.out_dtype != 0 && o.out_dtype != o.dtype && o.out_dtype != STARKV_F32) return STARKV_ERR_DTYPE;
+    L.gs = o.n_q_heads / d->n_kv_heads;
+  }
+  const int B = o.batch, Hq = o.n_q_heads, cus = device_cus(), strips = L.space.strips, Rvp = L.space.Rvp;
+  if ((int64_t)B * Hq > PX_MAX_ROWS || B > 65535) return STARKV_ERR_LIMIT;
+  L.M = B * Hq;
+  L.bm = L.M <= 32 ? 32 : L.M <= 64 ? 64 : L.M <= 128 ? 128 : 256;
+  L.tiles_m = (int)ceil_div(L.M, L.bm);
+  L.Mp = L.tiles_m * L.bm;
+  L.tiles_n = (int)ceil_div(Rvp, PX_BN);
+  const int tiles = L.tiles_m * L.tiles_n;
+  L.n_split = choose_splits(tiles, cus, strips, 256, 3.0, 0.004);
+  L.sp_len = (int)ceil_div(strips, L.n_split);
+  L.n_split = (int)ceil_div(strips, L.sp_len);
+  // logits: two workgroups a CU, each of its four waves a strip at a time
+  const int zb = (int)ceil_div((int64_t)B * L.gs, 32 * PX_GROUPS);
+  const int64_t want = std::max<int64_t>(1, 2 * cus / ((int64_t)d->n_kv_heads * zb));
+  L.ch_len = (int)round_up(ceil_div(strips, want), 4);
+  L.n_ch = (int)ceil_div(strips, L.ch_len);
+  L.n_hg = head_groups(Hq);
+  L.sw = up_slice_width(d->n_kv_heads, d->v_rank, cus);
+  L.n_sl = (int)ceil_div(d->v_rank, L.sw);
+  const size_t BQ = (size_t)B * L.n_hg, Mp = L.Mp;
+  size_t off = L.has_own ? L.own.total : 0;
+  auto take = [&](size_t& at, size_t n) { at = off; off = a256(off + n); };
+  take(L.off_p, (size_t)strips * 8 * Mp * 16);
+  take(L.off_stat, (size_t)strips * Mp * 8);
+  take(L.off_cmax, (size_t)L.n_ch * Mp * 4);
+  take(L.off_rmax, Mp * 4);
+  take(L.off_part, (size_t)L.n_split * L.M * Rvp * 2);
+  take(L.off_lsum, (size_t)L.n_split * Mp * 4);
+  take(L.off_jpart, BQ * 32 * Rvp * 4);
+  take(L.off_jsum, BQ * 32 * 4);
+  take(L.off_jmax, (size_t)L.M * 4);
+  take(L.off_ypart, (size_t)d->n_kv_heads * L.n_sl * ((size_t)B * L.gs) * HEAD_DIM * 4);
+  L.total = off;
+  return STARKV_OK;
+}
+
+}  // namespace
+
+size_t starkv_prefix_bytes(const starkv_prefix_pack_desc* d) {
+  PrefixSpace s;
+  return check_pack(d, s) ? 0 : s.total;
+}
+
+int starkv_prefix_pack(const starkv_prefix_pack_desc* d, void* stream) {
+  PrefixSpace s;
+  const int st = check_pack(d, s);
+  if (st) return st;
+  if (!d->prefix) return STARKV_ERR_NULL;
+  if (d->prefix_bytes < s.total) return STARKV_ERR_WORKSPACE;
+  if (!al(d->prefix, 256) || !al(d->k.data, 2) || !al(d->v.data, 2) || !al(d->k.bk, 2)) return STARKV_ERR_ALIGN;
+  PrefixPackArgs a = {};
+  a.k = d->k.data; a.bk = d->k.bk; a.v = d->v.data;
+  a.bk_rs = d->k.bk_row_stride; a.v_ss = d->v.stride_s;
+  a.Hkv = d->k.n_kv_heads; a.P = d->length; a.strips = s.strips; a.Rv = d->v.rank; a.Rvp = s.Rvp;
+  a.scale_v = d->dtype == STARKV_BF16;
+  int rmax = 1;
+  for (int h = 0; h < a.Hkv; ++h) {
+    a.koff[h] = d->k.head_offset[h]; a.kpitch[h] = d->k.pos_stride[h]; a.bkoff[h] = d->k.bk_head_offset[h];
+    a.rank[h] = d->k.rank[h]; a.xkoff[h] = s.xkoff[h]; a.xboff[h] = s.xboff[h];
+    rmax = std::max(rmax, a.rank[h]);
+  }
+  a.bound = 1.4143 * rmax * std::max(1.0, std::fabs((double)d->attention_scaling));
+  char* p = (char*)d->prefix;
+  a.head = (float*)p; a.xk = (uint8_t*)p + s.off_xk; a.xb = (uint8_t*)p + s.off_xb; a.xv = (uint4*)(p + s.off_xv);
+  return launch_prefix_pack(a, d->dtype, (hipStream_t)stream);
+}
+
+size_t starkv_prefix_decode_workspace_bytes(const starkv_prefix_decode_desc* d) {
+  PrefixLayout L;
+  return prefix_layout(d, L) ? 0 : L.total;
+}
+
+int starkv_prefix_decode(const starkv_prefix_decode_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
+  PrefixLayout L;
+  int st = prefix_layout(d, L);
+  if (st) return st;
+  const starkv_decode_desc& o = d->own;
+  if (!d->prefix || !d->turn_cos || !d->turn_sin) return STARKV_ERR_NULL;
+  if (d->prefix_bytes < L.space.total || round_up(d->length, PX_STRIP) > o.rope_max_positions) return STARKV_ERR_SHAPE;
+  if (!al(d->prefix, 256) || !al(o.q, 2)) return STARKV_ERR_ALIGN;
+  const bool score = d->scores && L.has_own;
+  if (score && (st = check_scores(&o, d->scores, d->scores_stride_b))) return st;
+  if (!workspace || workspace_bytes < L.total) return STARKV_ERR_WORKSPACE;
+  if (!al(workspace, 256)) return STARKV_ERR_ALIGN;
+  char* ws = (char*)workspace;
+  hipStream_t s = (hipStream_t)stream;
+  PrefixArgs a = {};
+  const char* p = (const char*)d->prefix;
+  a.head = (const float*)p; a.xk = (const uint8_t*)p + L.space.off_xk; a.xb = (const uint8_t*)p + L.space.off_xb;
+  a.xv = (const uint4*)(p + L.space.off_xv);
+  for (int h = 0; h < d->n_kv_heads; ++h) {
+    a.xkoff[h] = L.space.xkoff[h]; a.xboff[h] = L.space.xboff[h]; a.nc[h] = (d->rank[h] + 7) / 8;
+  }
+  for (int i = 0; i < 64; ++i) { a.cos_p[i] = d->turn_cos[i]; a.sin_p[i] = d->turn_sin[i]; }
+  a.rope = (const uint4*)o.rope_table;
+  a.q = o.q; a.q_sb = o.q_stride_b; a.q_sh = o.q_stride_h;
+  a.scale_log2 = o.scale * 1.4426950408889634f;
+  a.P = d->length; a.strips = L.space.strips; a.B = o.batch; a.Hq = o.n_q_heads; a.Hkv = d->n_kv_heads; a.gs = L.gs;
+  a.Rvp = L.space.Rvp; a.ks_max = L.space.ks_max; a.M = L.M; a.Mp = L.Mp;
+  a.p = (uint4*)(ws + L.off_p); a.stat = (float2*)(ws + L.off_stat);
+  a.cmax = (float*)(ws + L.off_cmax); a.n_ch = L.n_ch; a.ch_len = L.ch_len; a.rmax = (float*)(ws + L.off_rmax);
+  a.bm = L.bm; a.tiles_m = L.tiles_m; a.tiles_n = L.tiles_n; a.n_split = L.n_split; a.sp_len = L.sp_len;
+  a.part = (_Float16*)(ws + L.off_part); a.lsum = (float*)(ws + L.off_lsum);
+  a.n_hg = L.n_hg; a.jpart = (float*)(ws + L.off_jpart); a.jsum = (float*)(ws + L.off_jsum);
+  a.jmax = score ? (float*)(ws + L.off_jmax) : nullptr;
+  if (L.has_own) {
+    PVArgs pa;
+    if ((st = decode_sums(&o, L.own, L.gs, ws, s, nullptr, pa))) return st;
+    a.own_max = pa.chunkmax; a.own_sum = pa.psum; a.own_part = pa.part;
+    a.n_c1 = L.own.n_c1; a.n_c2 = L.own.pv.n_c2; a.own_Rvp = L.own.pv.Rvp; a.own_part16 = L.own.part16;
+  }
+  if ((st = launch_prefix(a, o.dtype, s)) || (st = launch_prefix_join(a, s))) return st;
+  UPArgs ua;
+  ua.part = a.jpart; ua.psum = a.jsum; ua.part16 = 0; ua.n_c2 = 1; ua.Rvp = a.Rvp; ua.n_hg = L.n_hg;
+  ua.uv = o.uv; ua.uv_rs = o.uv_row_stride;
+  ua.out = o.out; ua.o_sb = o.out_stride_b; ua.o_sh = o.out_stride_h;
+  ua.B = o.batch; ua.Hq = o.n_q_heads; ua.gs = L.gs; ua.Rv = d->v_rank;
+  ua.sw = L.sw; ua.n_sl = L.n_sl; ua.n_cs = 1; ua.ypart = (float*)(ws + L.off_ypart);
+  ua.out_f32 = o.out_dtype == STARKV_F32;
+  if ((st = launch_up_proj(ua, o.dtype, al(o.uv, 16) && al64(o.uv_row_stride * 2, 16), s))) return st;
+  if (score) return decode_scores(&o, L.own, ws, a.jmax, 1, a.jsum, 1, d->scores, d->scores_stride_b, s);
+  return STARKV_OK;
 }
 
 }  // extern "C"

@@ -321,6 +321,82 @@ struct LogprobArgs {
   float* pstat; uint64_t* ptop;                    // pieces > 1: [rows][pieces][4] statistics, [rows][pieces][top] keys
 };
 
+// ---------------------------------------------------------------------------
+// Bounded caches (bounded.hip): attention weights summed by position, the
+// positions kept, and their rows moved together.
+// ---------------------------------------------------------------------------
+constexpr int SCORE_MAX_H = 1024;
+struct ScoreArgs {
+  // logit (b, h, s) at x + b*x_sb + (s / 32)*x_st + h*x_sh + s % 32 (rows: x_st = 32)
+  const void* x; int64_t x_sb, x_st, x_sh;
+  int B, H, S, add;                                // add: onto out, else in its place
+  float2* stat;                                    // [B][H][n_max] (maximum, sum) of the row's pieces
+  // or a decode call's: maxima [B][H][n_max], sums relative to the largest [B*n_hg][n_sum][32]
+  const float* rmax; const float* rsum;
+  int n_max, n_sum, n_hg;
+  float* out; int64_t o_sb;
+};
+struct SelectArgs {
+  const float* scores; int64_t s_sb;
+  int* out; int64_t o_sb;
+  int length, keep, sinks, recent;
+};
+constexpr int MOVE_SLICE = 256;                    // bytes of a row per workgroup
+// what a workgroup moves: K rows (both blocks) and their scales by head, V rows and their scales by slice, scores
+constexpr int MOVE_K1 = 0, MOVE_K2 = 1, MOVE_KS1 = 2, MOVE_KS2 = 3, MOVE_V = 4, MOVE_SCORES = 9, MOVE_KINDS = 10;
+struct MoveRows { uint8_t* base; int64_t sb, pitch; int nb; };           // bytes
+struct MoveArgs {
+  const int* pos; int64_t p_sb;
+  int keep, length;
+  int* err;                                        // optional: set to 1 where a position is none
+  uint8_t* k1; int64_t k1_sb;
+  uint8_t* k2; int64_t k2_sb;
+  uint8_t* ks1; int64_t ks1_sb, ks1_sh;
+  uint8_t* ks2; int64_t ks2_sb, ks2_sh;
+  int64_t off1[K_MAX_KV], pitch1[K_MAX_KV], off2[K_MAX_KV], pitch2[K_MAX_KV];
+  int nb1[K_MAX_KV], nb2[K_MAX_KV];
+  MoveRows v[MOVE_SCORES - MOVE_V];                // data, data2, scale, scale2, zero
+  float* scores; int64_t scores_sb;
+  int units[MOVE_KINDS];                           // workgroups of each kind
+};
+
+// ---------------------------------------------------------------------------
+// Decode over a shared prefix (prefix.hip)
+// ---------------------------------------------------------------------------
+constexpr int PX_STRIP = 64;                       // positions of a strip
+constexpr int PX_GROUPS = 4;                       // groups of 32 query rows that a logits workgroup holds
+constexpr int PX_BN = 256;                         // columns of a P V workgroup
+constexpr int PX_HEAD_BYTES = 256;                 // (K multiplier, V multiplier), largest magnitudes
+struct PrefixPackArgs {
+  const void* k; const void* bk; const void* v;    // dense latents of one sequence, act dtype, strides in elements
+  int64_t koff[K_MAX_KV], kpitch[K_MAX_KV], bkoff[K_MAX_KV], bk_rs, v_ss;
+  int rank[K_MAX_KV];
+  int P, strips, Hkv, Rv, Rvp, scale_v;
+  double bound;                                    // of |key| over |latent| |B_k|
+  float* head; uint8_t* xk; uint8_t* xb; uint4* xv;
+  int64_t xkoff[K_MAX_KV], xboff[K_MAX_KV];        // bytes
+};
+struct PrefixArgs {
+  const float* head; const uint8_t* xk; const uint8_t* xb; const uint4* xv;
+  int64_t xkoff[K_MAX_KV], xboff[K_MAX_KV];
+  int nc[K_MAX_KV];                                // chunks of 8 ranks
+  float cos_p[64], sin_p[64];                      // the rotation by P positions
+  const uint4* rope;
+  const void* q; int64_t q_sb, q_sh;
+  float scale_log2;
+  int P, strips, B, Hq, Hkv, gs, Rvp, ks_max;
+  int M, Mp;                                       // rows (KV head, sequence, head of its group); padded to the tile
+  uint4* p; float2* stat;                          // weights [8 positions][row][8]; strips' (maximum, sum) [strip][row]
+  float* cmax; int n_ch, ch_len;                   // maxima [chunk][row], strips of a logits chunk
+  float* rmax;                                     // [row]
+  int bm, tiles_m, tiles_n, n_split, sp_len;       // P V: tile rows, tiles, splits and their strips
+  _Float16* part; float* lsum;                     // [split][M][Rvp] means / 2, [split][Mp] sums
+  // own positions (n_c1 = 0: none): the decode kernels' maxima, sums and partials
+  const float* own_max; const float* own_sum; const void* own_part;
+  int n_c1, n_c2, n_hg, own_Rvp, own_part16;
+  float* jpart; float* jsum; float* jmax;          // joined [B*n_hg][32][Rvp], [B*n_hg][32], optional [B][Hq]
+};
+
 // A decode step's cache writes and query rotation in one launch (quant.hip)
 struct StepAppendArgs {
   KAppendArgs k;
@@ -331,7 +407,8 @@ struct StepAppendArgs {
 };
 
 // these are passed by value as kernel arguments (at most 4 KiB)
-static_assert(sizeof(KArgs) <= 4096 && sizeof(PFArgs) <= 4096 && sizeof(StepAppendArgs) <= 4096,
+static_assert(sizeof(KArgs) <= 4096 && sizeof(PFArgs) <= 4096 && sizeof(StepAppendArgs) <= 4096 && sizeof(MoveArgs) <= 4096 &&
+                  sizeof(PrefixPackArgs) <= 4096 && sizeof(PrefixArgs) <= 4096,
               "kernel argument size");
 
 // ---------------------------------------------------------------------------
@@ -482,6 +559,13 @@ constexpr int pv_wg_per_cu(int ntw, int vq) { return ntw >= 8 && vq == VQ_DENSE 
 int launch_up_proj(const UPArgs& a, int dtype, bool fast, hipStream_t st);
 int up_slice_width(int n_kv, int Rv, int cus);        // V-rank columns per up-projection workgroup
 int up_chunk_sets(int n_kv, int n_sl, int n_c2, int cus);   // chunk sets per (slice, KV head)
+int score_pieces(int S);                              // pieces of a logit row: their statistics are 8 bytes each
+int launch_scores(const ScoreArgs& a, int dtype, bool fused, hipStream_t st);
+int launch_select(const SelectArgs& a, int B, hipStream_t st);
+int launch_move(const MoveArgs& a, int B, hipStream_t st);
+int launch_prefix_pack(const PrefixPackArgs& a, int dtype, hipStream_t st);
+int launch_prefix(const PrefixArgs& a, int dtype, hipStream_t st);
+int launch_prefix_join(const PrefixArgs& a, hipStream_t st);
 int launch_fill_i32(int* p, int n, int v, hipStream_t st);
 int launch_k_append(const KAppendArgs& a, int dtype, hipStream_t st);
 int launch_v_append(const VAppendArgs& a, int dtype, hipStream_t st);

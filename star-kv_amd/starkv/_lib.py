@@ -222,6 +222,56 @@ class LogprobsDesc(ctypes.Structure):
     ]
 
 
+class ScoresDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int), ("n_heads", ctypes.c_int), ("seq_len", ctypes.c_int), ("dtype", ctypes.c_int),
+        ("logits", ctypes.c_void_p), ("stride_b", ctypes.c_int64), ("stride_h", ctypes.c_int64),
+        ("add", ctypes.c_int),
+        ("scores", ctypes.c_void_p), ("scores_stride_b", ctypes.c_int64),
+    ]
+
+
+class SelectDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int), ("length", ctypes.c_int), ("keep", ctypes.c_int), ("sinks", ctypes.c_int),
+        ("recent", ctypes.c_int),
+        ("scores", ctypes.c_void_p), ("scores_stride_b", ctypes.c_int64),
+        ("positions", ctypes.c_void_p), ("positions_stride_b", ctypes.c_int64),
+    ]
+
+
+class KeepDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int), ("length", ctypes.c_int), ("keep", ctypes.c_int), ("dtype", ctypes.c_int),
+        ("positions", ctypes.c_void_p), ("positions_stride_b", ctypes.c_int64),
+        ("k", KLatent),
+        ("v", VLatent),
+        ("scores", ctypes.c_void_p), ("scores_stride_b", ctypes.c_int64),
+        ("error_flag", ctypes.c_void_p),
+    ]
+
+
+class PrefixPackDesc(ctypes.Structure):
+    _fields_ = [
+        ("length", ctypes.c_int), ("dtype", ctypes.c_int),
+        ("k", KLatent),
+        ("v", VLatent),
+        ("attention_scaling", ctypes.c_float),
+        ("prefix", ctypes.c_void_p), ("prefix_bytes", ctypes.c_size_t),
+    ]
+
+
+class PrefixDecodeDesc(ctypes.Structure):
+    _fields_ = [
+        ("own", DecodeDesc),
+        ("n_kv_heads", ctypes.c_int), ("v_rank", ctypes.c_int), ("length", ctypes.c_int),
+        ("rank", c_intp),
+        ("prefix", ctypes.c_void_p), ("prefix_bytes", ctypes.c_size_t),
+        ("turn_cos", ctypes.POINTER(ctypes.c_float)), ("turn_sin", ctypes.POINTER(ctypes.c_float)),
+        ("scores", ctypes.c_void_p), ("scores_stride_b", ctypes.c_int64),
+    ]
+
+
 EXPORTS = (
     "starkv_abi_version", "starkv_status_string",
     "starkv_rope_table_bytes", "starkv_rope_build", "starkv_rope_apply",
@@ -234,6 +284,9 @@ EXPORTS = (
     "starkv_rms_norm", "starkv_silu_mul", "starkv_skinny_gemm",
     "starkv_fp8_quantize", "starkv_fp8_gemm_workspace_bytes", "starkv_fp8_gemm",
     "starkv_token_logprobs_workspace_bytes", "starkv_token_logprobs",
+    "starkv_attention_scores_workspace_bytes", "starkv_attention_scores", "starkv_decode_attention_scores",
+    "starkv_select_positions", "starkv_keep_positions",
+    "starkv_prefix_bytes", "starkv_prefix_pack", "starkv_prefix_decode_workspace_bytes", "starkv_prefix_decode",
 )
 
 ABI_VERSION = 5          # STARKV_ABI_VERSION of include/starkv.h that these structs mirror
@@ -297,7 +350,16 @@ def lib() -> ctypes.CDLL:
     L.starkv_skinny_gemm.argtypes = [ctypes.POINTER(SkinnyGemmDesc), ctypes.c_void_p]
     L.starkv_fp8_quantize.restype = ctypes.c_int
     L.starkv_fp8_quantize.argtypes = [ctypes.POINTER(Fp8QuantizeDesc), ctypes.c_void_p]
-    for name, desc in (("fp8_gemm", Fp8GemmDesc), ("token_logprobs", LogprobsDesc)):
+    L.starkv_decode_attention_scores.restype = ctypes.c_int
+    L.starkv_decode_attention_scores.argtypes = [ctypes.POINTER(DecodeDesc), ctypes.c_void_p, ctypes.c_int64,
+                                                 ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+    L.starkv_prefix_bytes.restype = ctypes.c_size_t
+    L.starkv_prefix_bytes.argtypes = [ctypes.POINTER(PrefixPackDesc)]
+    for name, desc in (("select_positions", SelectDesc), ("keep_positions", KeepDesc), ("prefix_pack", PrefixPackDesc)):
+        f = getattr(L, f"starkv_{name}")
+        f.restype, f.argtypes = ctypes.c_int, [ctypes.POINTER(desc), ctypes.c_void_p]
+    for name, desc in (("fp8_gemm", Fp8GemmDesc), ("token_logprobs", LogprobsDesc), ("attention_scores", ScoresDesc),
+                       ("prefix_decode", PrefixDecodeDesc)):
         wsf, f = getattr(L, f"starkv_{name}_workspace_bytes"), getattr(L, f"starkv_{name}")
         wsf.restype, f.restype = ctypes.c_size_t, ctypes.c_int
         wsf.argtypes = [ctypes.POINTER(desc)]

@@ -28,7 +28,9 @@ from typing import List, Optional, Sequence
 import torch
 
 from ._lib import FMT_DENSE, FMT_INT4_REF, FMT_INT8_SYM, StarKVError
+from .bounded import keep_positions, select_positions
 from .ops import KLatentSpec, VLatentSpec, decode_append
+from .prefix import SharedPrefix
 from .rope import RopeConfig
 
 __all__ = ["LatentCache"]
@@ -223,3 +225,38 @@ class LatentCache:
         decode_append(src, ks, vsrc, self.v_spec, self.length, self.cap, q=q, rope=rope or RopeConfig())
         self.length += T
         return ks, self.v_spec, self.length
+
+    def share(self, bk: torch.Tensor, rope: Optional[RopeConfig] = None, length: Optional[int] = None,
+              row: int = 0) -> SharedPrefix:
+        """The first ``length`` positions of sequence ``row`` as a prefix that
+        a batch can share (``prefix_decode_attention``): a copy, dequantised
+        once, in the act dtype."""
+        n = self.length if length is None else int(length)
+        if not 1 <= n <= self.length or not 0 <= row < self.B:
+            raise StarKVError(f"sequence {row} of {self.B} does not hold {n} positions: the cache has {self.length}")
+        ks = [x[row] for x in self.dequant_k(n)]
+        data = torch.cat([x.reshape(-1) for x in ks])[None]
+        offsets = [n * sum(self.ranks[:h]) for h in range(len(self.ranks))]
+        k = KLatentSpec(data, self.ranks, offsets, self.ranks, data.stride(0), bk,
+                        [h * bk.stride(0) for h in range(len(self.ranks))], bk.stride(1))
+        return SharedPrefix(k, self.dequant_v(n)[row:row + 1], n, rope or RopeConfig())
+
+    def keep(self, positions: torch.Tensor, scores: Optional[torch.Tensor] = None,
+             error_flag: Optional[torch.Tensor] = None) -> None:
+        """Keep the rows ``positions`` [B, n] (int32, ascending) alone, moved
+        to the front in place; the next token goes to position n.  ``scores``
+        and ``error_flag`` as in ``keep_positions``."""
+        bk = self.k_data.new_empty(1, 1, HEAD_DIM).expand(len(self.ranks), 1, HEAD_DIM)    # not read
+        keep_positions(self.k_spec(bk), self.v_spec, positions, self.length, scores, error_flag)
+        self.length = positions.shape[1]
+
+    def bound(self, keep: int, scores: torch.Tensor, sinks: int = 0, recent: int = 0) -> torch.Tensor:
+        """Keep ``keep`` positions: the first ``sinks``, the last ``recent``
+        and those of the largest ``scores`` [B, >= length] between, which move
+        along.  Returns the positions kept.  (A cache that holds no more than
+        ``keep`` is left as it is.)"""
+        n = min(int(keep), self.length)
+        positions = select_positions(scores, n, self.length, min(sinks, n), min(recent, n - min(sinks, n)))
+        if n < self.length:
+            self.keep(positions, scores)
+        return positions

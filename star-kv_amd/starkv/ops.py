@@ -414,26 +414,16 @@ def pv_latent(p: torch.Tensor, xv) -> torch.Tensor:
     return out
 
 
-def decode_attention(q: torch.Tensor, k: KLatentSpec, xv: torch.Tensor, uv_weight: torch.Tensor,
-                     rope: RopeConfig = RopeConfig(), seq_len: Optional[int] = None,
-                     mask: Optional[torch.Tensor] = None, scale: Optional[float] = None,
-                     out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
-                     events: Optional[Sequence] = None, noalloc: bool = False,
-                     last_pos: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Fused decode attention core (model.py:450-487): [B, Hq, 128] in q's dtype
-    (or float32 with out_dtype=torch.float32).  ``events``: four
-    torch.cuda.Event recorded around the three kernels (timing).
-    ``noalloc``: run starkv_decode_attention_noalloc, whose workspace is the
-    library's own device array (no workspace allocation; with ``out`` given
-    the call allocates nothing at all).
-    ``last_pos``: an int32 device tensor whose first element is read by the
-    kernels: positions after it take the logit -1e30, as an additive -1e30
-    mask would give them (a context length kept on the device for graph
-    replay; the caller keeps it alive while the call or a captured graph runs).
+def _check_scores(scores: torch.Tensor, B: int, S: int, device) -> None:
+    """fp32 sums of B rows of at least S positions."""
+    if scores.dtype != torch.float32 or scores.dim() != 2 or scores.shape[0] != B or scores.shape[1] < S or \
+            (scores.shape[1] > 1 and scores.stride(1) != 1) or scores.device != device:
+        raise StarKVError(f"scores must be float32 [{B}, >= {S}] on {device} with a contiguous last dim, got "
+                          f"{scores.dtype} {tuple(scores.shape)} on {scores.device}")
 
-    q: rotated query [B, Hq, 128]; k: key-latent spec; xv: V latent [B, S, Rv]
-    (dense tensor) or a VLatentSpec; uv_weight: v_proj.U.weight [Hkv*128, Rv];
-    seq_len defaults to the V latent's position count."""
+
+def _decode_desc(q, k, xv, uv_weight, rope, seq_len, mask, scale, out, out_dtype, last_pos):
+    """(the checked descriptor of a decode call, its output, what has to live until the call returns)."""
     q = _q3(q)
     v = _vspec(xv)
     _require_cuda(q, uv_weight, mask, last_pos, *k.tensors, *v.tensors)
@@ -466,7 +456,46 @@ def decode_attention(q: torch.Tensor, k: KLatentSpec, xv: torch.Tensor, uv_weigh
     d.out, d.out_stride_b, d.out_stride_h = out.data_ptr(), out.stride(0), out.stride(1)
     d.out_dtype = F32 if out.dtype == torch.float32 else 0
     d.last_pos_device = last_pos.data_ptr() if last_pos is not None else None
+    return d, out, (keep, m, table)
+
+
+def decode_attention(q: torch.Tensor, k: KLatentSpec, xv: torch.Tensor, uv_weight: torch.Tensor,
+                     rope: RopeConfig = RopeConfig(), seq_len: Optional[int] = None,
+                     mask: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                     out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+                     events: Optional[Sequence] = None, noalloc: bool = False,
+                     last_pos: Optional[torch.Tensor] = None,
+                     scores: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Fused decode attention core (model.py:450-487): [B, Hq, 128] in q's dtype
+    (or float32 with out_dtype=torch.float32).  ``events``: four
+    torch.cuda.Event recorded around the three kernels (timing).
+    ``noalloc``: run starkv_decode_attention_noalloc, whose workspace is the
+    library's own device array (no workspace allocation; with ``out`` given
+    the call allocates nothing at all).
+    ``last_pos``: an int32 device tensor whose first element is read by the
+    kernels: positions after it take the logit -1e30, as an additive -1e30
+    mask would give them (a context length kept on the device for graph
+    replay; the caller keeps it alive while the call or a captured graph runs).
+    ``scores``: fp32 [B, >= S], onto which each position's attention weights,
+    summed over the query heads, are added (``starkv.select_positions`` picks
+    the positions that a bounded cache keeps by them).
+
+    q: rotated query [B, Hq, 128]; k: key-latent spec; xv: V latent [B, S, Rv]
+    (dense tensor) or a VLatentSpec; uv_weight: v_proj.U.weight [Hkv*128, Rv];
+    seq_len defaults to the V latent's position count."""
+    d, out, keep = _decode_desc(q, k, xv, uv_weight, rope, seq_len, mask, scale, out, out_dtype, last_pos)
+    q = _q3(q)
     L = _lib.lib()
+    if scores is not None:
+        if noalloc or events is not None:
+            raise StarKVError("scores need the ordinary decode: neither noalloc nor events")
+        _check_scores(scores, d.batch, d.seq_len, q.device)
+        nb = L.starkv_decode_workspace_bytes(ctypes.byref(d))
+        ws = _workspace(q.device, nb) if nb else None
+        check(L.starkv_decode_attention_scores(ctypes.byref(d), _ptr(scores), scores.stride(0), _ptr(ws),
+                                               ws.numel() if nb else 0, _stream(q.device)),
+              "starkv_decode_attention_scores")
+        return out
     if noalloc:
         if events is not None:
             raise StarKVError("the allocation-free decode has no timed form")

@@ -1050,11 +1050,10 @@ size_t starkv_decode_workspace_bytes(const starkv_decode_desc* d) {
                     d->dtype == STARKV_F16).total;
 }
 
-// the logits and P.V of a validated decode call, into its workspace
-static int decode_sums(const starkv_decode_desc* d, const DecodeLayout& L, int gs, char* ws, hipStream_t s,
-                       void* const* events, PVArgs& pa) {
+// the logits of a validated decode call, into its workspace
+static int decode_logits(const starkv_decode_desc* d, const DecodeLayout& L, int gs, char* ws, hipStream_t s) {
   const int B = d->batch, Hq = d->n_q_heads;
-  int vq = 0, st;
+  int st;
   KArgs ka;
   KPlan plan;
   if ((st = build_k_plan(d->k, Hq, gs, d->dtype, d->seq_len, ka, plan, false, true))) return st;
@@ -1072,21 +1071,22 @@ static int decode_sums(const starkv_decode_desc* d, const DecodeLayout& L, int g
   ka.S = d->seq_len; ka.Hq = Hq; ka.n_chunks = L.n_c1; ka.tiles_per_chunk = L.tiles_per_chunk;
   ka.wscale = d->scale;
   const bool kfast = k_fast(d->k, d->dtype, d->q, d->q_stride_b, d->q_stride_h);
-  if (events && (st = (int)hipEventRecord((hipEvent_t)events[0], s))) return st;
-  if ((st = launch_k_logits(ka, d->dtype, d->k.format, true, STARKV_F32, kfast, B, s))) return st;
-  if (events && (st = (int)hipEventRecord((hipEvent_t)events[1], s))) return st;
+  return launch_k_logits(ka, d->dtype, d->k.format, true, STARKV_F32, kfast, B, s);
+}
 
+// P.V over them
+static int decode_pv(const starkv_decode_desc* d, const DecodeLayout& L, char* ws, hipStream_t s, PVArgs& pa) {
+  const int B = d->batch, Hq = d->n_q_heads;
+  int vq = 0, st;
   pa = PVArgs{};
   if ((st = validate_v(d->v, pa, &vq))) return st;
   vq = pv_storage(pa, vq, d->v.rank, true, d->seq_len);
-  pa.logits = (const float*)(ws + L.off_logits); pa.l_sb = ka.o_sb; pa.l_st = ka.o_st; pa.l_sh = ka.o_sh;
+  pa.logits = (const float*)(ws + L.off_logits); pa.l_sb = (int64_t)Hq * L.S_pad; pa.l_st = (int64_t)Hq * TILE; pa.l_sh = TILE;
   pa.chunkmax = (const float*)(ws + L.off_cmax); pa.n_chunk1 = L.n_c1;
   pa.part = (float*)(ws + L.off_part); pa.psum = (float*)(ws + L.off_psum); pa.part16 = L.part16;
   pa.S = d->seq_len; pa.H = Hq; pa.n_hg = L.n_hg; pa.Rv = d->v.rank; pa.Rvp = L.pv.Rvp;
   pa.n_cb = L.pv.n_cb; pa.n_c2 = L.pv.n_c2; pa.c2_len = L.pv.c2_len;
-  if ((st = launch_pv(pa, d->dtype, vq, true, v_fast(d->v, pa), B, s))) return st;
-  if (events && (st = (int)hipEventRecord((hipEvent_t)events[2], s))) return st;
-  return STARKV_OK;
+  return launch_pv(pa, d->dtype, vq, true, v_fast(d->v, pa), B, s);
 }
 
 // weights of a decode call's logits by position, from its maxima and sums
@@ -1120,7 +1120,11 @@ static int decode_impl(const starkv_decode_desc* d, void* workspace, size_t work
   hipStream_t s = (hipStream_t)stream;
   const int B = d->batch, Hq = d->n_q_heads;
   PVArgs pa;
-  if ((st = decode_sums(d, L, gs, ws, s, events, pa))) return st;
+  if (events && (st = (int)hipEventRecord((hipEvent_t)events[0], s))) return st;
+  if ((st = decode_logits(d, L, gs, ws, s))) return st;
+  if (events && (st = (int)hipEventRecord((hipEvent_t)events[1], s))) return st;
+  if ((st = decode_pv(d, L, ws, s, pa))) return st;
+  if (events && (st = (int)hipEventRecord((hipEvent_t)events[2], s))) return st;
 
   UPArgs ua;
   ua.part = pa.part; ua.psum = pa.psum; ua.part16 = L.part16; ua.n_c2 = L.pv.n_c2; ua.Rvp = L.pv.Rvp;
@@ -1829,11 +1833,14 @@ int check_pack(const starkv_prefix_pack_desc* d, PrefixSpace& s) {
   return prefix_space(d->k.n_kv_heads, d->k.rank, d->v.rank, d->length, s);
 }
 
+// Whether a call's own logits are formed beside the prefix's
+bool own_logits_here(const starkv_decode_desc& o) { return o.k.format == STARKV_FMT_DENSE; }
+
 struct PrefixLayout {
   DecodeLayout own;
   PrefixSpace space;
-  bool has_own;
-  int gs, M, Mp, bm, tiles_m, tiles_n, n_split, sp_len, n_ch, ch_len, n_hg, sw, n_sl;
+  bool has_own, own_here;
+  int oc_len, gs, M, Mp, bm, tiles_m, tiles_n, n_split, sp_len, n_ch, ch_len, n_hg, sw, n_sl;
   size_t off_p, off_stat, off_cmax, off_rmax, off_part, off_lsum, off_jpart, off_jsum, off_jmax, off_ypart, total;
 };
 
@@ -1852,6 +1859,14 @@ int prefix_layout(const starkv_prefix_decode_desc* d, PrefixLayout& L) {
       if (o.k.rank[h] != d->rank[h]) return STARKV_ERR_SHAPE;
     L.own = decode_layout(o.batch, o.n_q_heads, d->n_kv_heads, o.seq_len, o.v.rank, n_wg, k1pc, vq, v_row_bytes(o.v),
                           o.dtype == STARKV_F16);
+    L.own_here = own_logits_here(o);
+    if (L.own_here) {
+      // chunks of at least one strip a wave, two workgroups a CU
+      const int strips = (int)ceil_div(o.seq_len, PX_STRIP);
+      const int64_t want = std::max<int64_t>(1, 2 * device_cus() / ((int64_t)o.batch * d->n_kv_heads));
+      L.oc_len = (int)round_up(ceil_div(strips, want), 4);
+      L.own.n_c1 = (int)ceil_div(strips, L.oc_len);
+    }
   } else {
     if (o.batch < 1 || o.head_dim != HEAD_DIM || o.n_q_heads < 1 || o.n_q_heads % d->n_kv_heads) return STARKV_ERR_SHAPE;
     if (!act16(o.dtype)) return STARKV_ERR_DTYPE;
@@ -1864,12 +1879,12 @@ int prefix_layout(const starkv_prefix_decode_desc* d, PrefixLayout& L) {
   const int B = o.batch, Hq = o.n_q_heads, cus = device_cus(), strips = L.space.strips, Rvp = L.space.Rvp;
   if ((int64_t)B * Hq > PX_MAX_ROWS || B > 65535) return STARKV_ERR_LIMIT;
   L.M = B * Hq;
-  L.bm = L.M <= 32 ? 32 : L.M <= 64 ? 64 : L.M <= 128 ? 128 : 256;
+  L.bm = L.M <= 64 ? 64 : L.M <= 128 ? 128 : 256;
   L.tiles_m = (int)ceil_div(L.M, L.bm);
   L.Mp = L.tiles_m * L.bm;
   L.tiles_n = (int)ceil_div(Rvp, PX_BN);
   const int tiles = L.tiles_m * L.tiles_n;
-  L.n_split = choose_splits(tiles, cus, strips, 256, 3.0, 0.004);
+  L.n_split = std::max(choose_splits(tiles, cus, strips, 256, 3.0, 0.004), (int)ceil_div(strips, PX_SPLIT_STRIPS));
   L.sp_len = (int)ceil_div(strips, L.n_split);
   L.n_split = (int)ceil_div(strips, L.sp_len);
   // logits: two workgroups a CU, each of its four waves a strip at a time
@@ -1883,6 +1898,7 @@ int prefix_layout(const starkv_prefix_decode_desc* d, PrefixLayout& L) {
   const size_t BQ = (size_t)B * L.n_hg, Mp = L.Mp;
   size_t off = L.has_own ? L.own.total : 0;
   auto take = [&](size_t& at, size_t n) { at = off; off = a256(off + n); };
+  if (L.own_here) take(L.own.off_cmax, (size_t)B * Hq * L.own.n_c1 * 4);
   take(L.off_p, (size_t)strips * 8 * Mp * 16);
   take(L.off_stat, (size_t)strips * Mp * 8);
   take(L.off_cmax, (size_t)L.n_ch * Mp * 4);
@@ -1952,12 +1968,12 @@ int starkv_prefix_decode(const starkv_prefix_decode_desc* d, void* workspace, si
   a.head = (const float*)p; a.xk = (const uint8_t*)p + L.space.off_xk; a.xb = (const uint8_t*)p + L.space.off_xb;
   a.xv = (const uint4*)(p + L.space.off_xv);
   for (int h = 0; h < d->n_kv_heads; ++h) {
-    a.xkoff[h] = L.space.xkoff[h]; a.xboff[h] = L.space.xboff[h]; a.nc[h] = (d->rank[h] + 7) / 8;
+    a.xkoff[h] = L.space.xkoff[h]; a.xboff[h] = L.space.xboff[h]; a.rank[h] = d->rank[h];
   }
   for (int i = 0; i < 64; ++i) { a.cos_p[i] = d->turn_cos[i]; a.sin_p[i] = d->turn_sin[i]; }
   a.rope = (const uint4*)o.rope_table;
   a.q = o.q; a.q_sb = o.q_stride_b; a.q_sh = o.q_stride_h;
-  a.scale_log2 = o.scale * 1.4426950408889634f;
+  a.scale = o.scale;
   a.P = d->length; a.strips = L.space.strips; a.B = o.batch; a.Hq = o.n_q_heads; a.Hkv = d->n_kv_heads; a.gs = L.gs;
   a.Rvp = L.space.Rvp; a.ks_max = L.space.ks_max; a.M = L.M; a.Mp = L.Mp;
   a.p = (uint4*)(ws + L.off_p); a.stat = (float2*)(ws + L.off_stat);
@@ -1967,12 +1983,25 @@ int starkv_prefix_decode(const starkv_prefix_decode_desc* d, void* workspace, si
   a.n_hg = L.n_hg; a.jpart = (float*)(ws + L.off_jpart); a.jsum = (float*)(ws + L.off_jsum);
   a.jmax = score ? (float*)(ws + L.off_jmax) : nullptr;
   if (L.has_own) {
-    PVArgs pa;
-    if ((st = decode_sums(&o, L.own, L.gs, ws, s, nullptr, pa))) return st;
-    a.own_max = pa.chunkmax; a.own_sum = pa.psum; a.own_part = pa.part;
+    a.own_max = (float*)(ws + L.own.off_cmax); a.own_sum = (const float*)(ws + L.own.off_psum);
+    a.own_part = ws + L.own.off_part;
     a.n_c1 = L.own.n_c1; a.n_c2 = L.own.pv.n_c2; a.own_Rvp = L.own.pv.Rvp; a.own_part16 = L.own.part16;
+    a.S = o.seq_len;
+    if (L.own_here) {
+      a.own_wg = o.batch * d->n_kv_heads * L.own.n_c1; a.oc_len = L.oc_len;
+      a.ox = o.k.data; a.ox_sb = o.k.stride_b;
+      for (int h = 0; h < d->n_kv_heads; ++h) { a.oxoff[h] = o.k.head_offset[h]; a.oxpitch[h] = o.k.pos_stride[h]; }
+      a.mask = o.mask; a.m_sb = o.mask_stride_b; a.m_sh = o.mask_stride_h; a.mask_dtype = o.mask_dtype;
+      a.last_pos = o.last_pos_device;
+      a.ol = (float*)(ws + L.own.off_logits); a.ol_sb = (int64_t)o.n_q_heads * L.own.S_pad; a.ol_st = (int64_t)o.n_q_heads * TILE;
+    } else if ((st = decode_logits(&o, L.own, L.gs, ws, s))) {
+      return st;
+    }
   }
-  if ((st = launch_prefix(a, o.dtype, s)) || (st = launch_prefix_join(a, s))) return st;
+  if ((st = launch_prefix_logits(a, o.dtype, s))) return st;
+  PVArgs pa;
+  if (L.has_own && (st = decode_pv(&o, L.own, ws, s, pa))) return st;
+  if ((st = launch_prefix_pv(a, s)) || (st = launch_prefix_join(a, s))) return st;
   UPArgs ua;
   ua.part = a.jpart; ua.psum = a.jsum; ua.part16 = 0; ua.n_c2 = 1; ua.Rvp = a.Rvp; ua.n_hg = L.n_hg;
   ua.uv = o.uv; ua.uv_rs = o.uv_row_stride;

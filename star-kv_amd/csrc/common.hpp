@@ -364,7 +364,8 @@ struct MoveArgs {
 // Decode over a shared prefix (prefix.hip)
 // ---------------------------------------------------------------------------
 constexpr int PX_STRIP = 64;                       // positions of a strip
-constexpr int PX_GROUPS = 4;                       // groups of 32 query rows that a logits workgroup holds
+constexpr int PX_GROUPS = 2;                       // groups of 32 query rows that a logits workgroup holds
+constexpr int PX_SPLIT_STRIPS = 56;                // most strips of a P V split: their factors lie in LDS
 constexpr int PX_BN = 256;                         // columns of a P V workgroup
 constexpr int PX_HEAD_BYTES = 256;                 // (K multiplier, V multiplier), largest magnitudes
 struct PrefixPackArgs {
@@ -379,11 +380,11 @@ struct PrefixPackArgs {
 struct PrefixArgs {
   const float* head; const uint8_t* xk; const uint8_t* xb; const uint4* xv;
   int64_t xkoff[K_MAX_KV], xboff[K_MAX_KV];
-  int nc[K_MAX_KV];                                // chunks of 8 ranks
+  int rank[K_MAX_KV];
   float cos_p[64], sin_p[64];                      // the rotation by P positions
   const uint4* rope;
   const void* q; int64_t q_sb, q_sh;
-  float scale_log2;
+  float scale;
   int P, strips, B, Hq, Hkv, gs, Rvp, ks_max;
   int M, Mp;                                       // rows (KV head, sequence, head of its group); padded to the tile
   uint4* p; float2* stat;                          // weights [8 positions][row][8]; strips' (maximum, sum) [strip][row]
@@ -392,8 +393,14 @@ struct PrefixArgs {
   int bm, tiles_m, tiles_n, n_split, sp_len;       // P V: tile rows, tiles, splits and their strips
   _Float16* part; float* lsum;                     // [split][M][Rvp] means / 2, [split][Mp] sums
   // own positions (n_c1 = 0: none): the decode kernels' maxima, sums and partials
-  const float* own_max; const float* own_sum; const void* own_part;
+  float* own_max; const float* own_sum; const void* own_part;
   int n_c1, n_c2, n_hg, own_Rvp, own_part16;
+  // ... whose logits (dense latents) the first own_wg workgroups of the logits kernel form
+  int own_wg, S, oc_len;                           // strips of one of their n_c1 chunks
+  const void* ox; int64_t ox_sb, oxoff[K_MAX_KV], oxpitch[K_MAX_KV];       // elements
+  const void* mask; int64_t m_sb, m_sh; int mask_dtype;
+  const int* last_pos;
+  float* ol; int64_t ol_sb, ol_st;                 // logits [b][32 positions][Hq][32]
   float* jpart; float* jsum; float* jmax;          // joined [B*n_hg][32][Rvp], [B*n_hg][32], optional [B][Hq]
 };
 
@@ -564,7 +571,8 @@ int launch_scores(const ScoreArgs& a, int dtype, bool fused, hipStream_t st);
 int launch_select(const SelectArgs& a, int B, hipStream_t st);
 int launch_move(const MoveArgs& a, int B, hipStream_t st);
 int launch_prefix_pack(const PrefixPackArgs& a, int dtype, hipStream_t st);
-int launch_prefix(const PrefixArgs& a, int dtype, hipStream_t st);
+int launch_prefix_logits(const PrefixArgs& a, int dtype, hipStream_t st);
+int launch_prefix_pv(const PrefixArgs& a, hipStream_t st);
 int launch_prefix_join(const PrefixArgs& a, hipStream_t st);
 int launch_fill_i32(int* p, int n, int v, hipStream_t st);
 int launch_k_append(const KAppendArgs& a, int dtype, hipStream_t st);

@@ -34,7 +34,7 @@
 // to [2^14, 2^15); each is undone in fp32.
 #include <algorithm>
 
-#include "common.hpp"
+#include "fp8.hpp"
 
 namespace starkv {
 
@@ -85,10 +85,26 @@ __global__ __launch_bounds__(256) void px_amax_kernel(const PrefixPackArgs a) {
   const XT* base = (const XT*)(is_v ? a.v : is_b ? a.bk : a.k) + (is_v ? 0 : is_b ? a.bkoff[h] : a.koff[h]);
   uint32_t m = 0;
   for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)gridDim.x * 4)
-    for (int c = threadIdx.x & 63; c < cols; c += 64) m = max(m, __float_as_uint(to_f32(base[r * pitch + c])) & 0x7fffffffu);
+    for (int c = 8 * (threadIdx.x & 63); c < cols; c += 512) {
+      XT e[8];
+      if (c + 8 <= cols) {
+        __builtin_memcpy(e, base + r * pitch + c, 16);           // any alignment
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = base[r * pitch + min(c + j, cols - 1)];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(to_f32(e[j])) & 0x7fffffffu);
+    }
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
-  if ((threadIdx.x & 63) == 0 && m) atomicMax((uint32_t*)a.head + 2 + (is_v ? 2 : is_b ? 1 : 0), m);
+  // one atomic a workgroup, and none where the maximum is there already: thousands on one word took 3 ms
+  __shared__ uint32_t red[4];
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = max(max(red[0], red[1]), max(red[2], red[3]));
+  uint32_t* to = (uint32_t*)a.head + 2 + (is_v ? 2 : is_b ? 1 : 0);
+  if (threadIdx.x == 0 && m > __hip_atomic_load(to, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(to, m);
 }
 
 // 2^e, |e| <= 126
@@ -120,6 +136,7 @@ __global__ __launch_bounds__(256) void px_pack_kernel(const PrefixPackArgs a) {
   if (u == 0 && i0 == 0) {
     a.head[0] = pow2f(px_k_exp(a));
     a.head[1] = pow2f(px_v_exp(a));
+    a.head[5] = (float)((double)a.head[3] * a.bound);            // of |key| over |latent|
   }
   if (u < a.Hkv) {
     const int h = u, r = a.rank[h], nc = (r + 7) / 8;
@@ -176,32 +193,79 @@ __global__ __launch_bounds__(256) void px_pack_kernel(const PrefixPackArgs a) {
 // ---------------------------------------------------------------------------
 // Logits and weights
 // ---------------------------------------------------------------------------
-template <typename XT>
-__global__ __launch_bounds__(256, 2) void prefix_logits_kernel(const PrefixArgs a) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t px_lds[];
+// NG: groups of 32 query rows per workgroup.  A tile of B_k^T (32 dims) at a
+// time: its keys are rotated and at once multiplied with the queries' same dims,
+// so no more than a tile's keys are held; the next tile's rotation and the next
+// strip's latents are asked for ahead.
+// OWN: a sequence's own positions instead: dense latents where they lie (rows at
+// any alignment), the queries of one KV head and sequence, and the logits go out
+// in fp32 as the decode's P.V kernels read them.
+template <typename XT, int NG, bool OWN>
+__device__ __forceinline__ void px_logits(const PrefixArgs& a, uint8_t* px_lds, int bx) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5, n = lane & 31;
-  // workgroups of one chunk of strips on one XCD: its L2 serves the rotation table to all heads
-  const int bx = blockIdx.x, chunk = (bx & 7) + 8 * ((bx >> 3) / a.Hkv), h = (bx >> 3) % a.Hkv;
-  if (chunk >= a.n_ch) return;
-  const int nr = a.B * a.gs, r0 = blockIdx.y * PX_GROUPS * 32, ng = min(PX_GROUPS, (nr - r0 + 31) / 32);
-  const int nc = a.nc[h], ks_n = (nc + 1) / 2;
+  int chunk, h, b = 0;
+  if constexpr (OWN) {
+    chunk = bx % a.n_c1;
+    h = bx / a.n_c1 % a.Hkv;
+    b = bx / a.n_c1 / a.Hkv;
+  } else {
+    // workgroups of one chunk of strips on one XCD: its L2 serves the rotation table to all heads
+    chunk = (bx & 7) + 8 * ((bx >> 3) / a.Hkv);
+    h = (bx >> 3) % a.Hkv;
+    if (chunk >= a.n_ch) return;
+  }
+  const int nr = OWN ? a.gs : a.B * a.gs, r0 = OWN ? 0 : blockIdx.y * NG * 32;
+  const int rank = a.rank[h], nc = (rank + 7) / 8, ks_n = (nc + 1) / 2;
+  const int len = OWN ? a.S : a.P, strips = OWN ? (a.S + PX_STRIP - 1) / PX_STRIP : a.strips;
+  const int per = OWN ? a.oc_len : a.ch_len;
   uint4* bl = (uint4*)px_lds;                      // [k step][tile w][lane]
   uint4* ql = bl + a.ks_max * 256;                 // [group][4 tiles x 2 halves][lane]
-  float* mul = (float*)(ql + PX_GROUPS * 512);     // [group * 32 + row]
-  float* wm = mul + PX_GROUPS * 32;                // [wave][group * 32 + row]
+  float* mul = (float*)(ql + NG * 512);            // [group * 32 + row]
+  float* wm = mul + NG * 32;                       // [wave][group * 32 + row]
+  const int pn = px_pos(n), s_end = min(strips, (chunk + 1) * per);
+  int s = chunk * per + wave;
+  uint4 xf[2][8];
+  const uint4* xk = (const uint4*)(a.xk + a.xkoff[h]) + pn;
+  const XT* xo = OWN ? (const XT*)a.ox + b * a.ox_sb + a.oxoff[h] : nullptr;
+  const int64_t xpitch = OWN ? a.oxpitch[h] : 0;
+  auto fetch = [&](int at) {
+#pragma unroll
+    for (int pt = 0; pt < 2; ++pt) {
+      const XT* row = OWN ? xo + min(64 * at + 32 * pt + pn, len - 1) * xpitch : nullptr;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (k < ks_n) {
+          const int c = min(2 * k + hh, nc - 1);
+          if constexpr (!OWN) {
+            xf[pt][k] = xk[((int64_t)(2 * at + pt) * nc + c) * 32];
+          } else if (rank >= 8) {                  // a last chunk of fewer ranks ends with the row
+            __builtin_memcpy(&xf[pt][k], row + min(8 * c, rank - 8), 16);
+          } else {
+            XT e[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) e[j] = row[min(j, rank - 1)];
+            __builtin_memcpy(&xf[pt][k], e, 16);
+          }
+        }
+      }
+    }
+  };
+  if (s < s_end) fetch(s);
   {
     const uint4* src = (const uint4*)(a.xb + a.xboff[h]);
     for (int i = tid; i < ks_n * 256; i += 256) bl[i] = src[i];
   }
-  // queries turned by P positions, scaled to [1, 2) by row, in the operand's order
-  const float cs = a.cos_p[lane], sn = a.sin_p[lane], kmul = a.head[0];
-  for (int r = wave; r < ng * 32; r += 4) {
+  // queries (the prefix's: turned by P positions), scaled to [1, 2) by row, in the operand's order
+  const float cs = OWN ? 1.f : a.cos_p[lane], sn = OWN ? 0.f : a.sin_p[lane];
+  const float kmul = OWN ? a.scale : a.scale * LOG2E * a.head[0];
+  for (int r = wave; r < NG * 32; r += 4) {
     float y0 = 0.f, y1 = 0.f;
     if (r0 + r < nr) {
-      const XT* q = (const XT*)a.q + (r0 + r) / a.gs * a.q_sb + (h * a.gs + (r0 + r) % a.gs) * a.q_sh;
+      const int qb = OWN ? b : (r0 + r) / a.gs, qg = OWN ? r : (r0 + r) % a.gs;
+      const XT* q = (const XT*)a.q + qb * a.q_sb + (h * a.gs + qg) * a.q_sh;
       const float x0 = to_f32(q[lane]), x1 = to_f32(q[lane + 64]);
-      y0 = x0 * cs - x1 * sn;
-      y1 = x1 * cs + x0 * sn;
+      y0 = OWN ? x0 : x0 * cs - x1 * sn;
+      y1 = OWN ? x1 : x1 * cs + x0 * sn;
     }
     const float m = px_wave_max(fmaxf(fabsf(y0), fabsf(y1)));
     const int e = m < INFINITY && m > 0.f ? min(max((int)(__float_as_uint(m) >> 23), 1), 253) - 127 : 0;
@@ -210,137 +274,229 @@ __global__ __launch_bounds__(256, 2) void prefix_logits_kernel(const PrefixArgs 
                     4 * ((lane >> 3) & 1) + (lane & 3);
     dst[0] = (_Float16)(y0 * f);
     dst[64 * 8] = (_Float16)(y1 * f);
-    if (lane == 0) mul[r] = a.scale_log2 * kmul * pow2f(e);
+    if (lane == 0) mul[r] = kmul * pow2f(e);
   }
   __syncthreads();
 
-  float top[PX_GROUPS];
+  float top[NG];
 #pragma unroll
-  for (int g = 0; g < PX_GROUPS; ++g) top[g] = -INFINITY;
-  const int pn = px_pos(n);
-  const int s_end = min(a.strips, (chunk + 1) * a.ch_len);
-  for (int s = chunk * a.ch_len + wave; s < s_end; s += 4) {
-    uint4 xf[2][8], kf[2][4][2];
+  for (int g = 0; g < NG; ++g) top[g] = -INFINITY;
+  const int last_pos = OWN && a.last_pos ? *a.last_pos : INT32_MAX;
+  const int tail = OWN ? rank & 7 : 0;             // ranks of a last chunk that is not whole
+  for (; s < s_end; s += 4) {
+    floatx16 acc[NG][2] = {};
+    // the last k step: a partial chunk's ranks to its front, zeros behind the rank
 #pragma unroll
-    for (int pt = 0; pt < 2; ++pt) {
-      const uint4* x = (const uint4*)(a.xk + a.xkoff[h]) + (int64_t)(2 * s + pt) * nc * 32 + pn;
+    for (int k = 0; k < 8; ++k) {
+      if (k != ks_n - 1) continue;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (k < ks_n) {
-          const int c = 2 * k + hh;
-          xf[pt][k] = x[min(c, nc - 1) * 32];
-          if (c >= nc) xf[pt][k] = make_uint4(0, 0, 0, 0);
+      for (int pt = 0; pt < 2; ++pt) {
+        if (OWN && tail) {
+          const uint4 v = xf[pt][k];
+          uint64_t lo = v.x | ((uint64_t)v.y << 32), hi = v.z | ((uint64_t)v.w << 32);
+          if (rank >= 8) {
+            const int sh = 16 * (8 - tail);
+            lo = sh >= 64 ? hi >> (sh - 64) : (lo >> sh) | (hi << (64 - sh));
+            hi = sh >= 64 ? 0 : hi >> sh;
+          }
+          // (of a row of fewer than 8 ranks the last was repeated)
+          const uint64_t ml = tail >= 4 ? ~0ull : (1ull << (16 * tail)) - 1, mh = tail <= 4 ? 0 : (1ull << (16 * (tail - 4))) - 1;
+          lo &= ml;
+          hi &= mh;
+          if (min(2 * k + hh, nc - 1) == nc - 1)
+            xf[pt][k] = make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
         }
+        if (2 * k + hh >= nc) xf[pt][k] = make_uint4(0, 0, 0, 0);
       }
     }
+    // bf16 keys of own positions can pass fp16's range: scaled by what bounds them (the prefix's were when it was packed)
+    int ke = 0;
+    if constexpr (OWN && __is_same(XT, __bf16)) {
+      uint32_t big = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (k >= ks_n) continue;
+#pragma unroll
+        for (int pt = 0; pt < 2; ++pt)
+          big = max2_u16(max2_u16(max2_u16(big, xf[pt][k].x & 0x7fff7fffu), xf[pt][k].y & 0x7fff7fffu),
+                         max2_u16(xf[pt][k].z & 0x7fff7fffu, xf[pt][k].w & 0x7fff7fffu));
+      }
+      const float bound = px_wave_max(fmaxf(__uint_as_float(big << 16), __uint_as_float(big & 0xffff0000u))) * a.head[5];
+      if (bound > 32768.f && bound < INFINITY) ke = min((int)(__float_as_uint(bound) >> 23) - 141, 100);
+      ke = __builtin_amdgcn_readfirstlane(ke);
+    }
+    const float kdown = pow2f(-ke);
+    uint4 rt[2][2][2];
+    auto turn = [&](int w) {
+#pragma unroll
+      for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+          rt[w & 1][pt][g] = a.rope[((int64_t)min(2 * s + pt, (len - 1) >> 5) * 8 + 2 * w + g) * 64 + hh * 32 + pn];
+    };
+    turn(0);
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      floatx16 acc[2] = {};
+      if (w < 3) turn(w + 1);
+      floatx16 kx[2] = {};
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         if (k < ks_n) {
-          const uint4 b = bl[(k * 4 + w) * 64 + lane];
-          acc[0] = px_mfma<XT>(b, xf[0][k], acc[0]);
-          acc[1] = px_mfma<XT>(b, xf[1][k], acc[1]);
+          const uint4 bf = bl[(k * 4 + w) * 64 + lane];
+          kx[0] = px_mfma<XT>(bf, xf[0][k], kx[0]);
+          kx[1] = px_mfma<XT>(bf, xf[1][k], kx[1]);
         }
       }
+      if (OWN && ke) {
+#pragma unroll
+        for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) kx[pt][r] *= kdown;
+      }
+      uint4 kf[2][2];
 #pragma unroll
       for (int pt = 0; pt < 2; ++pt) {
         half8 lo, hi;
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          const half8 t = __builtin_bit_cast(half8, a.rope[((int64_t)(2 * s + pt) * 8 + 2 * w + g) * 64 + hh * 32 + pn]);
+          const half8 t = __builtin_bit_cast(half8, rt[w & 1][pt][g]);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float k0 = acc[pt][4 * g + j], k1 = acc[pt][8 + 4 * g + j], c = (float)t[2 * j], sp = (float)t[2 * j + 1];
+            const float k0 = kx[pt][4 * g + j], k1 = kx[pt][8 + 4 * g + j], c = (float)t[2 * j], sp = (float)t[2 * j + 1];
             lo[4 * g + j] = (_Float16)(k0 * c - k1 * sp);
             hi[4 * g + j] = (_Float16)(k1 * c + k0 * sp);
           }
         }
-        kf[pt][w][0] = __builtin_bit_cast(uint4, lo);
-        kf[pt][w][1] = __builtin_bit_cast(uint4, hi);
+        kf[pt][0] = __builtin_bit_cast(uint4, lo);
+        kf[pt][1] = __builtin_bit_cast(uint4, hi);
       }
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+          const uint4 q = ql[(g * 8 + 2 * w + f) * 64 + lane];
+          acc[g][0] = px_mfma<_Float16>(kf[0][f], q, acc[g][0]);
+          acc[g][1] = px_mfma<_Float16>(kf[1][f], q, acc[g][1]);
+        }
+      __builtin_amdgcn_sched_barrier(0);           // loads hoisted across tiles cost a hundred spills
     }
+    const int cur = s;
+    if (s + 4 < s_end) fetch(s + 4);
 #pragma unroll
-    for (int g = 0; g < PX_GROUPS; ++g) {
-      if (g >= ng) break;
-      floatx16 acc[2] = {};
+    for (int g = 0; g < NG; ++g) {
+      const float f = OWN ? mul[g * 32 + n] * pow2f(ke) : mul[g * 32 + n];
+      const int rl = r0 + g * 32 + n, p0 = 64 * cur + 16 * hh;
 #pragma unroll
-      for (int f = 0; f < 8; ++f) {
-        const uint4 q = ql[(g * 8 + f) * 64 + lane];
-        acc[0] = px_mfma<_Float16>(kf[0][f >> 1][f & 1], q, acc[0]);
-        acc[1] = px_mfma<_Float16>(kf[1][f >> 1][f & 1], q, acc[1]);
+      for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[g][pt][r] *= f;
+      if (OWN && a.mask != nullptr && rl < nr) {
+        const int64_t at = b * a.m_sb + (h * a.gs + rl) * a.m_sh;
+#pragma unroll
+        for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[g][pt][r] += load_elem_f32(a.mask, a.mask_dtype, at + min(p0 + 32 * pt + r, len - 1));
       }
-      const float f = mul[g * 32 + n];
+      if (64 * (cur + 1) > min(len, last_pos + (last_pos < INT32_MAX ? 1 : 0))) {
+#pragma unroll
+        for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            if (p0 + 32 * pt + r > last_pos) acc[g][pt][r] = -1e30f;
+            if (p0 + 32 * pt + r >= len) acc[g][pt][r] = -INFINITY;
+          }
+      }
       float m = -INFINITY;
 #pragma unroll
       for (int pt = 0; pt < 2; ++pt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[pt][r] *= f;
-      if (64 * (s + 1) > a.P) {
+        for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[g][pt][r]);
+      m = max_halves(m);
+      if constexpr (OWN) {
+        top[g] = fmaxf(top[g], m);
+        if (rl < nr) {
 #pragma unroll
-        for (int pt = 0; pt < 2; ++pt)
+          for (int pt = 0; pt < 2; ++pt) {
+            float4* o = (float4*)(a.ol + b * a.ol_sb + (2 * cur + pt) * a.ol_st + (h * a.gs + rl) * 32 + 16 * hh);
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (64 * s + 32 * pt + 16 * hh + r >= a.P) acc[pt][r] = -INFINITY;
+            for (int r = 0; r < 4; ++r) o[r] = make_float4(acc[g][pt][4 * r], acc[g][pt][4 * r + 1], acc[g][pt][4 * r + 2], acc[g][pt][4 * r + 3]);
+          }
+        }
+        continue;
       }
-#pragma unroll
-      for (int pt = 0; pt < 2; ++pt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[pt][r]);
-      m = fmaxf(max_halves(m), -3.0e38f);          // a strip of -inf alone: weights 0
+      m = fmaxf(m, -3.0e38f);                      // a strip of -inf alone: weights 0
       top[g] = fmaxf(top[g], m);
       float l = 0.f;
-      uint4 p[4];
+      const int64_t row = (int64_t)h * nr + rl;
+      uint4* o = a.p + (int64_t)(8 * cur + 2 * hh) * a.Mp + row;
 #pragma unroll
       for (int pt = 0; pt < 2; ++pt) {
         half8 v[2];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) v[r >> 3][r & 7] = (_Float16)__builtin_amdgcn_exp2f(acc[pt][r] - m);
+        for (int r = 0; r < 16; ++r) v[r >> 3][r & 7] = (_Float16)__builtin_amdgcn_exp2f(acc[g][pt][r] - m);
 #pragma unroll
         for (int r = 0; r < 16; ++r) l += (float)v[r >> 3][r & 7];
-        p[2 * pt] = __builtin_bit_cast(uint4, v[0]);
-        p[2 * pt + 1] = __builtin_bit_cast(uint4, v[1]);
+        if (rl < nr) {
+          o[4 * pt * (int64_t)a.Mp] = __builtin_bit_cast(uint4, v[0]);
+          o[(4 * pt + 1) * (int64_t)a.Mp] = __builtin_bit_cast(uint4, v[1]);
+        }
       }
       l = add_halves(l);
-      const int rl = r0 + g * 32 + n;
-      if (rl < nr) {
-        const int64_t row = (int64_t)h * nr + rl;
-        uint4* o = a.p + (int64_t)(8 * s + 2 * hh) * a.Mp + row;
-        o[0] = p[0];
-        o[a.Mp] = p[1];
-        o[4 * (int64_t)a.Mp] = p[2];
-        o[5 * (int64_t)a.Mp] = p[3];
-        if (hh == 0) a.stat[(int64_t)s * a.Mp + row] = make_float2(m, l);
-      }
+      if (rl < nr && hh == 0) a.stat[(int64_t)cur * a.Mp + row] = make_float2(m, l);
     }
   }
   // the chunk's maximum of each row
 #pragma unroll
-  for (int g = 0; g < PX_GROUPS; ++g)
-    if (g < ng && hh == 0) wm[wave * PX_GROUPS * 32 + g * 32 + n] = top[g];
+  for (int g = 0; g < NG; ++g)
+    if (hh == 0) wm[wave * NG * 32 + g * 32 + n] = top[g];
   __syncthreads();
-  for (int r = tid; r < ng * 32; r += 256) {
+  for (int r = tid; r < NG * 32; r += 256) {
     if (r0 + r >= nr) continue;
     float m = wm[r];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) m = fmaxf(m, wm[w * PX_GROUPS * 32 + r]);
-    a.cmax[(int64_t)chunk * a.Mp + (int64_t)h * nr + r0 + r] = m;
+    for (int w = 1; w < 4; ++w) m = fmaxf(m, wm[w * NG * 32 + r]);
+    if constexpr (OWN) a.own_max[((int64_t)b * a.Hq + h * a.gs + r) * a.n_c1 + chunk] = m;
+    else a.cmax[(int64_t)chunk * a.Mp + (int64_t)h * nr + r0 + r] = m;
   }
+}
+
+// The first own_wg workgroups: own positions (while they wait for their few latents the prefix's compute).
+template <typename XT, int NG>
+__global__ __launch_bounds__(256, 2) void prefix_logits_kernel(const PrefixArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t px_lds[];
+  const int bx = blockIdx.x;
+  if (bx >= a.own_wg) px_logits<XT, NG, false>(a, px_lds, bx - a.own_wg);
+  else if (blockIdx.y == 0) px_logits<XT, NG, true>(a, px_lds, bx);
 }
 
 // ---------------------------------------------------------------------------
 // P V
 // ---------------------------------------------------------------------------
-// Workgroup = (split of the strips, 32 WM RM rows, 32 WN RN columns); wave (wm, wn)
-// of WM x WN owns RM x RN MFMA tiles.
+// One 1 KB global -> LDS copy, 16 bytes per lane from base + off to LDS address
+// `lds` + 16 lane (as inline assembly: the compiler then adds no waits of its own
+// before reads of other stages; m0 needs a wait state before the copy).
+__device__ inline void px_dma(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
+}
+// all but the last N copies of this wave have landed, its LDS reads are done; then the workgroup's
+template <int N> __device__ inline void px_stage_ready() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// Workgroup of 8 waves = (split of the strips, BM rows, 256 columns), wave (wm, wn)
+// of WM x WN: RM x RN MFMA tiles, two waves a SIMD.  Steps of 32 positions go
+// through a ring of four LDS stages, three of them in flight.  The factors of the
+// split's strips are formed once, before the loop.
 template <int RM, int RN, int WM, int WN>
-__global__ __launch_bounds__(256, RM * RN >= 16 ? 1 : 2) void prefix_pv_kernel(const PrefixArgs a) {
-  constexpr int BM = 32 * RM * WM, BN = 32 * RN * WN, AU = BM * 8 / 256, BU = BN * 8 / 256;
-  static_assert(WM * WN == 4 && BN == PX_BN, "four waves");
-  __shared__ uint4 sa[2][8 * BM], sb[2][8 * BN];
-  __shared__ float row_f[BM];                      // row maximum, then 1 / (2 sum)
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5, n = lane & 31;
+__global__ __launch_bounds__(512, 2) void prefix_pv_kernel(const PrefixArgs a) {
+  constexpr int BM = 32 * RM * WM, BN = 32 * RN * WN, RING = 4;
+  constexpr int AI = (BM * 4 / 64 + 7) / 8, BI = BN * 4 / 64 / 8, NI = AI + BI;     // copies per wave and stage
+  constexpr int STAGE = 4 * (BM + BN);             // 16-byte pieces
+  static_assert(WM * WN == 8 && BN == PX_BN, "eight waves");
+  __shared__ uint4 ring[RING * STAGE];
+  __shared__ _Float16 fac[PX_SPLIT_STRIPS * BM];   // [strip][row]
+  __shared__ float row_f[BM];                      // 1 / (2 sum)
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5, n = lane & 31;
   const int wm = wave / WN, wn = wave % WN;
   // consecutive (split, tile) pairs on one XCD: a split's tiles share its weights and latents in that L2
   const int tiles = a.tiles_m * a.tiles_n, total = a.n_split * tiles, per = (total + 7) / 8;
@@ -349,100 +505,94 @@ __global__ __launch_bounds__(256, RM * RN >= 16 ? 1 : 2) void prefix_pv_kernel(c
   const int split = at / tiles, m0 = (at % tiles) / a.tiles_n * BM, n0 = (at % tiles) % a.tiles_n * BN;
   const int s0 = split * a.sp_len, s1 = min(a.strips, s0 + a.sp_len);
 
-  const uint4* asrc[AU];
-  const uint4* bsrc[BU];
+  // this wave's copies: instruction i brings 64 rows (columns) of one group of 8 positions
+  uint32_t off[NI], dst[NI];
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint4*)ring;
 #pragma unroll
-  for (int u = 0; u < AU; ++u) asrc[u] = a.p + (int64_t)(8 * s0 + (tid + 256 * u) / BM) * a.Mp + m0 + (tid + 256 * u) % BM;
+  for (int i = 0; i < AI; ++i) {
+    const int j = (wave * AI + i) % (BM / 16), k8 = j / (BM / 64), r = j % (BM / 64) * 64;   // fewer than 8: some twice
+    off[i] = (uint32_t)(k8 * a.Mp + r + lane) * 16;
+    dst[i] = lds0 + (k8 * BM + r) * 16;
+  }
 #pragma unroll
-  for (int u = 0; u < BU; ++u)
-    bsrc[u] = a.xv + (int64_t)(8 * s0 + (tid + 256 * u) / BN) * a.Rvp + min(n0 + (tid + 256 * u) % BN, a.Rvp - 1);
-  uint4 ra[AU], rb[BU];
-  auto fetch = [&]() {
+  for (int i = 0; i < BI; ++i) {
+    const int j = wave * BI + i, k8 = j / (BN / 64), c = j % (BN / 64) * 64;
+    off[AI + i] = (uint32_t)(k8 * a.Rvp + min(n0 + c + lane, a.Rvp - 1)) * 16;
+    dst[AI + i] = lds0 + (4 * BM + k8 * BN + c) * 16;
+  }
+  const uint4* pa = a.p + (int64_t)8 * s0 * a.Mp + m0;
+  const uint4* pb = a.xv + (int64_t)8 * s0 * a.Rvp;
+  const int steps = 2 * (s1 - s0);
+  int issued = 0;
+  auto issue = [&](int slot) {                     // past the end the last step again (never read): the counts stay
 #pragma unroll
-    for (int u = 0; u < AU; ++u) { ra[u] = *asrc[u]; asrc[u] += 8 * (int64_t)a.Mp; }
-#pragma unroll
-    for (int u = 0; u < BU; ++u) { rb[u] = *bsrc[u]; bsrc[u] += 8 * (int64_t)a.Rvp; }
+    for (int i = 0; i < NI; ++i) px_dma(i < AI ? pa : pb, off[i], dst[i] + slot * STAGE * 16);
+    if (++issued < steps) { pa += 4 * (int64_t)a.Mp; pb += 4 * (int64_t)a.Rvp; }
   };
-  auto place = [&](int st) {
-#pragma unroll
-    for (int u = 0; u < AU; ++u) sa[st][tid + 256 * u] = ra[u];
-#pragma unroll
-    for (int u = 0; u < BU; ++u) sb[st][tid + 256 * u] = rb[u];
-  };
-  fetch();
+  // strips' factors and sums, a row per thread
+  float lsum = 0.f;
   if (tid < BM) {
     float m = -INFINITY;
-    for (int c = 0; c < a.n_ch; ++c) m = fmaxf(m, a.cmax[(int64_t)c * a.Mp + m0 + tid]);
-    row_f[tid] = m;
+    const float* cm = a.cmax + m0 + tid;
+#pragma unroll 8
+    for (int c = 0; c < a.n_ch; ++c) m = fmaxf(m, cm[(int64_t)c * a.Mp]);
     if (split == 0 && n0 == 0) a.rmax[m0 + tid] = m;
-  }
-  __syncthreads();
-  float rmx[RM], lsum[RM];
-  const float2* st_src[RM];
-  float2 st[RM];
-#pragma unroll
-  for (int i = 0; i < RM; ++i) {
-    const int r = (wm * RM + i) * 32 + n;
-    rmx[i] = row_f[r];
-    lsum[i] = 0.f;
-    st_src[i] = a.stat + (int64_t)s0 * a.Mp + m0 + r;
-    st[i] = *st_src[i];
+    const float2* st = a.stat + (int64_t)s0 * a.Mp + m0 + tid;
+#pragma unroll 8
+    for (int s = 0; s < s1 - s0; ++s) {
+      const float2 v = st[(int64_t)s * a.Mp];
+      const _Float16 f = (_Float16)__builtin_amdgcn_exp2f((v.x - m) + PX_LIFT);
+      fac[s * BM + tid] = f;
+      lsum = fmaf(v.y, (float)f, lsum);
+    }
+    row_f[tid] = lsum == 0.f ? 0.f : 0.5f / lsum;
+    if (n0 == 0) a.lsum[(int64_t)split * a.Mp + m0 + tid] = lsum;
   }
   floatx16 acc[RM][RN];
 #pragma unroll
   for (int i = 0; i < RM; ++i)
 #pragma unroll
     for (int j = 0; j < RN; ++j) acc[i][j] = floatx16{};
-  place(0);
-  __syncthreads();
-  for (int s = s0; s < s1; ++s) {
-    const int cur = (s - s0) & 1;
-    kh2 fac[RM];
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // only copies are counted from here on
 #pragma unroll
-    for (int i = 0; i < RM; ++i) {
-      const _Float16 f = (_Float16)__builtin_amdgcn_exp2f((st[i].x - rmx[i]) + PX_LIFT);
-      fac[i] = kh2{f, f};
-      lsum[i] = fmaf(st[i].y, (float)f, lsum[i]);
-    }
-    const bool more = s + 1 < s1;
-    if (more) {
-      fetch();
+  for (int i = 0; i < RING - 1; ++i) issue(i);
+  kh2 fc[RM];
+  for (int t0 = 0; t0 < steps; t0 += RING) {
 #pragma unroll
-      for (int i = 0; i < RM; ++i) { st_src[i] += a.Mp; st[i] = *st_src[i]; }
-    }
+    for (int u = 0; u < RING; ++u) {
+      if (t0 + u >= steps) break;
+      px_stage_ready<(RING - 2) * NI>();
+      issue((u + RING - 1) % RING);
+      if (u % 2 == 0) {
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      uint4 fa[RM], fb[RN];
-#pragma unroll
-      for (int i = 0; i < RM; ++i) {
-        const uint4 v = sa[cur][(2 * kk + hh) * BM + (wm * RM + i) * 32 + n];
-        fa[i].x = __builtin_bit_cast(uint32_t, __builtin_bit_cast(kh2, v.x) * fac[i]);
-        fa[i].y = __builtin_bit_cast(uint32_t, __builtin_bit_cast(kh2, v.y) * fac[i]);
-        fa[i].z = __builtin_bit_cast(uint32_t, __builtin_bit_cast(kh2, v.z) * fac[i]);
-        fa[i].w = __builtin_bit_cast(uint32_t, __builtin_bit_cast(kh2, v.w) * fac[i]);
+        for (int i = 0; i < RM; ++i) {
+          const _Float16 f = fac[((t0 + u) >> 1) * BM + (wm * RM + i) * 32 + n];
+          fc[i] = kh2{f, f};
+        }
       }
+      const uint4* sa = ring + u * STAGE + (wm * RM) * 32 + n;
+      const uint4* sb = ring + u * STAGE + 4 * BM + (wn * RN) * 32 + n;
 #pragma unroll
-      for (int j = 0; j < RN; ++j) fb[j] = sb[cur][(2 * kk + hh) * BN + (wn * RN + j) * 32 + n];
+      for (int kk = 0; kk < 2; ++kk) {
+        uint4 fa[RM], fb[RN];
 #pragma unroll
-      for (int i = 0; i < RM; ++i)
+        for (int j = 0; j < RN; ++j) fb[j] = sb[(2 * kk + hh) * BN + 32 * j];
 #pragma unroll
-        for (int j = 0; j < RN; ++j) acc[i][j] = px_mfma<_Float16>(fa[i], fb[j], acc[i][j]);
-    }
-    if (more) {
-      place(cur ^ 1);
-      __syncthreads();
+        for (int i = 0; i < RM; ++i) {
+          const uint4 v = sa[(2 * kk + hh) * BM + 32 * i];
+          fa[i].x = __builtin_bit_cast(uint32_t, __builtin_bit_cast(kh2, v.x) * fc[i]);
+          fa[i].y = __builtin_bit_cast(uint32_t, __builtin_bit_cast(kh2, v.y) * fc[i]);
+          fa[i].z = __builtin_bit_cast(uint32_t, __builtin_bit_cast(kh2, v.z) * fc[i]);
+          fa[i].w = __builtin_bit_cast(uint32_t, __builtin_bit_cast(kh2, v.w) * fc[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < RM; ++i)
+#pragma unroll
+          for (int j = 0; j < RN; ++j) acc[i][j] = px_mfma<_Float16>(fa[i], fb[j], acc[i][j]);
+      }
     }
   }
-  __syncthreads();
-  if (wn == 0 && hh == 0) {
-#pragma unroll
-    for (int i = 0; i < RM; ++i) {
-      const int r = (wm * RM + i) * 32 + n;
-      row_f[r] = lsum[i] == 0.f ? 0.f : 0.5f / lsum[i];
-      if (n0 == 0) a.lsum[(int64_t)split * a.Mp + m0 + r] = lsum[i];
-    }
-  }
-  __syncthreads();
+  px_stage_ready<0>();                             // the last copies, before the workgroup's LDS is another's
   _Float16* out = a.part + ((int64_t)split * a.M + m0) * a.Rvp + n0;
 #pragma unroll
   for (int i = 0; i < RM; ++i)
@@ -462,47 +612,70 @@ __global__ __launch_bounds__(256, RM * RN >= 16 ? 1 : 2) void prefix_pv_kernel(c
 // ---------------------------------------------------------------------------
 // Join: row (b, q)'s sums over the prefix's splits and over its own positions' chunks
 // ---------------------------------------------------------------------------
+// Workgroup = (row, 512 columns), a lane 8 columns, wave w splits and chunks w, w + 4, ...
 __global__ __launch_bounds__(256) void prefix_join_kernel(const PrefixArgs a) {
+  __shared__ float red[3][64][9];
   const int row = blockIdx.x, nr = a.B * a.gs, h = row / nr, b = row % nr / a.gs, q = h * a.gs + row % a.gs;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t bq = (int64_t)b * a.n_hg + (q >> 5);
   const float mp = a.rmax[row];
   float ms = -INFINITY;                            // in units of log 2, as the prefix's
   for (int c = 0; c < a.n_c1; ++c) ms = fmaxf(ms, a.own_max[((int64_t)b * a.Hq + q) * a.n_c1 + c] * LOG2E);
   const float m = fmaxf(mp, ms);
-  const float wp = __builtin_amdgcn_exp2f(mp - m - PX_LIFT);
+  const float wp = __builtin_amdgcn_exp2f((mp - m) - PX_LIFT);
   const float wo = ms > -INFINITY ? __builtin_amdgcn_exp2f(ms - m) : 0.f;
   const float vmul = 2.f * a.head[1];
   const float* psum = a.own_sum + (bq * a.n_c2) * 32 + (q & 31);
   const int n_own = wo > 0.f ? a.n_c2 : 0;         // own positions without weight are not looked at (their sums may be NaN)
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 0 && blockIdx.y == 0) {
     float l = 0.f, o = 0.f;
+#pragma unroll 8
     for (int s = 0; s < a.n_split; ++s) l += a.lsum[(int64_t)s * a.Mp + row];
+#pragma unroll 8
     for (int c = 0; c < n_own; ++c) o += psum[(int64_t)c * 32];
     a.jsum[bq * 32 + (q & 31)] = n_own ? l * wp + o * wo : l * wp;
     if (a.jmax) a.jmax[(int64_t)b * a.Hq + q] = m * (1.f / LOG2E);
   }
-  for (int c0 = 4 * threadIdx.x; c0 < a.Rvp; c0 += 1024) {
-    float v[4] = {};
+  const int c0 = blockIdx.y * 512 + 8 * lane;
+  float v[8] = {};
+  if (c0 < a.Rvp) {
     const _Float16* p = a.part + (int64_t)row * a.Rvp + c0;
 #pragma unroll 8
-    for (int s = 0; s < a.n_split; ++s) {
-      const half4 e = *(const half4*)(p + (int64_t)s * a.M * a.Rvp);
+    for (int s = wave; s < a.n_split; s += 4) {
+      const half8 e = *(const half8*)(p + (int64_t)s * a.M * a.Rvp);
       const float f = a.lsum[(int64_t)s * a.Mp + row];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = fmaf((float)e[i], f, v[i]);
+      for (int i = 0; i < 8; ++i) v[i] = fmaf((float)e[i], f, v[i]);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] *= wp * vmul;
-    for (int c = 0; c < n_own; ++c) {
+    for (int i = 0; i < 8; ++i) v[i] *= wp * vmul;
+#pragma unroll 2
+    for (int c = wave; c < n_own; c += 4) {
       const int64_t at = ((bq * a.n_c2 + c) * 32 + (q & 31)) * a.own_Rvp + c0;
-      float f = wo;
-      if (a.own_part16) f *= psum[(int64_t)c * 32];
+      if (a.own_part16) {
+        const half8 e = *(const half8*)((const _Float16*)a.own_part + at);
+        const float f = wo * psum[(int64_t)c * 32];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v[i] = fmaf(a.own_part16 ? (float)((const _Float16*)a.own_part)[at + i] : ((const float*)a.own_part)[at + i], f, v[i]);
+        for (int i = 0; i < 8; ++i) v[i] = fmaf((float)e[i], f, v[i]);
+      } else {
+        const float4* e = (const float4*)((const float*)a.own_part + at);
+        const float4 x = e[0], y = e[1];
+        v[0] = fmaf(x.x, wo, v[0]); v[1] = fmaf(x.y, wo, v[1]); v[2] = fmaf(x.z, wo, v[2]); v[3] = fmaf(x.w, wo, v[3]);
+        v[4] = fmaf(y.x, wo, v[4]); v[5] = fmaf(y.y, wo, v[5]); v[6] = fmaf(y.z, wo, v[6]); v[7] = fmaf(y.w, wo, v[7]);
+      }
     }
-    *(float4*)(a.jpart + (bq * 32 + (q & 31)) * a.Rvp + c0) = make_float4(v[0], v[1], v[2], v[3]);
   }
+  if (wave) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) red[wave - 1][lane][i] = v[i];
+  }
+  __syncthreads();
+  if (wave || c0 >= a.Rvp) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] += (red[0][lane][i] + red[1][lane][i]) + red[2][lane][i];
+  float4* o = (float4*)(a.jpart + (bq * 32 + (q & 31)) * a.Rvp + c0);
+  o[0] = make_float4(v[0], v[1], v[2], v[3]);
+  o[1] = make_float4(v[4], v[5], v[6], v[7]);
 }
 
 }  // namespace
@@ -510,7 +683,7 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(const PrefixArgs a) {
 int launch_prefix_pack(const PrefixPackArgs& a, int dtype, hipStream_t st) {
   int e = launch_fill_i32((int*)a.head, 8, 0, st);
   if (e) return e;
-  const dim3 rows((unsigned)std::min<int64_t>(ceil_div(std::max(a.P, 128), 4), 512), 2 * a.Hkv + 1);
+  const dim3 rows((unsigned)std::min<int64_t>(ceil_div(std::max(a.P, 128), 32), 512), 2 * a.Hkv + 1);
   const dim3 pieces((unsigned)std::min<int64_t>((int64_t)a.strips * 4, 2048), 2 * a.Hkv + 1);
   if (dtype == STARKV_F16) {
     hipLaunchKernelGGL(px_amax_kernel<_Float16>, rows, dim3(256), 0, st, a);
@@ -522,22 +695,34 @@ int launch_prefix_pack(const PrefixPackArgs& a, int dtype, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
-int launch_prefix(const PrefixArgs& a, int dtype, hipStream_t st) {
+template <typename XT, int NG> static void launch_logits(const PrefixArgs& a, int groups, hipStream_t st) {
+  const size_t lds = (size_t)a.ks_max * 4096 + NG * 8192 + NG * 32 * 4 * 5;
+  const dim3 grid((unsigned)(round_up(a.n_ch, 8) * a.Hkv + a.own_wg), (unsigned)ceil_div(groups, NG));
+  hipLaunchKernelGGL((prefix_logits_kernel<XT, NG>), grid, dim3(256), lds, st, a);
+}
+
+int launch_prefix_logits(const PrefixArgs& a, int dtype, hipStream_t st) {
   const int groups = (int)ceil_div((int64_t)a.B * a.gs, 32);
-  const size_t lds = (size_t)a.ks_max * 4096 + PX_GROUPS * 8192 + PX_GROUPS * 32 * 4 * 5;
-  const dim3 g1((unsigned)(round_up(a.n_ch, 8) * a.Hkv), (unsigned)ceil_div(groups, PX_GROUPS));
-  if (dtype == STARKV_F16) hipLaunchKernelGGL(prefix_logits_kernel<_Float16>, g1, dim3(256), lds, st, a);
-  else hipLaunchKernelGGL(prefix_logits_kernel<__bf16>, g1, dim3(256), lds, st, a);
-  const dim3 g2((unsigned)(8 * ceil_div((int64_t)a.n_split * a.tiles_m * a.tiles_n, 8)));
-  if (a.bm == 256) hipLaunchKernelGGL((prefix_pv_kernel<4, 4, 2, 2>), g2, dim3(256), 0, st, a);
-  else if (a.bm == 128) hipLaunchKernelGGL((prefix_pv_kernel<2, 4, 2, 2>), g2, dim3(256), 0, st, a);
-  else if (a.bm == 64) hipLaunchKernelGGL((prefix_pv_kernel<2, 2, 1, 4>), g2, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((prefix_pv_kernel<1, 2, 1, 4>), g2, dim3(256), 0, st, a);
+  if (groups == 1) {
+    if (dtype == STARKV_F16) launch_logits<_Float16, 1>(a, groups, st);
+    else launch_logits<__bf16, 1>(a, groups, st);
+  } else {
+    if (dtype == STARKV_F16) launch_logits<_Float16, PX_GROUPS>(a, groups, st);
+    else launch_logits<__bf16, PX_GROUPS>(a, groups, st);
+  }
+  return (int)hipGetLastError();
+}
+
+int launch_prefix_pv(const PrefixArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)(8 * ceil_div((int64_t)a.n_split * a.tiles_m * a.tiles_n, 8)));
+  if (a.bm == 256) hipLaunchKernelGGL((prefix_pv_kernel<2, 4, 4, 2>), grid, dim3(512), 0, st, a);
+  else if (a.bm == 128) hipLaunchKernelGGL((prefix_pv_kernel<2, 2, 2, 4>), grid, dim3(512), 0, st, a);
+  else hipLaunchKernelGGL((prefix_pv_kernel<2, 1, 1, 8>), grid, dim3(512), 0, st, a);
   return (int)hipGetLastError();
 }
 
 int launch_prefix_join(const PrefixArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL(prefix_join_kernel, dim3((unsigned)a.M), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(prefix_join_kernel, dim3((unsigned)a.M, (unsigned)ceil_div(a.Rvp, 512)), dim3(256), 0, st, a);
   return (int)hipGetLastError();
 }
 

@@ -1844,6 +1844,20 @@ struct PrefixLayout {
   size_t off_p, off_stat, off_cmax, off_rmax, off_part, off_lsum, off_jpart, off_jsum, off_jmax, off_ypart, total;
 };
 
+// Strips per P V split: the least modelled time, rounds of one workgroup a CU, each its strips and a fixed time, times the
+// share of the splits' partials (a round of workgroups that is hardly begun costs as much as a full one: 65536 positions of
+// 512 rows in 19 splits of 14 tiles ran 198 us, in 36 161, in 18 SPLIT18).
+int prefix_split_len(int tiles, int cus, int strips) {
+  int best = 0;
+  double least = 0;
+  for (int len = 1; len <= strips; ++len) {
+    const int64_t n = ceil_div(strips, len);
+    const double t = (double)ceil_div(tiles * n, cus) * (len + 3.0) * (1.0 + 0.004 * std::min<int64_t>(n, 64));
+    if (!best || t < least * 0.9999) { best = len; least = t; }
+  }
+  return best;
+}
+
 int prefix_layout(const starkv_prefix_decode_desc* d, PrefixLayout& L) {
   if (!d) return STARKV_ERR_NULL;
   const starkv_decode_desc& o = d->own;
@@ -1861,11 +1875,11 @@ int prefix_layout(const starkv_prefix_decode_desc* d, PrefixLayout& L) {
                           o.dtype == STARKV_F16);
     L.own_here = own_logits_here(o);
     if (L.own_here) {
-      // chunks of at least one strip a wave, two workgroups a CU
-      const int strips = (int)ceil_div(o.seq_len, PX_STRIP);
+      // chunks of at least one tile a wave, two workgroups a CU
+      const int tiles = (int)ceil_div(o.seq_len, TILE);
       const int64_t want = std::max<int64_t>(1, 2 * device_cus() / ((int64_t)o.batch * d->n_kv_heads));
-      L.oc_len = (int)round_up(ceil_div(strips, want), 4);
-      L.own.n_c1 = (int)ceil_div(strips, L.oc_len);
+      L.oc_len = (int)round_up(ceil_div(tiles, want), 8);
+      L.own.n_c1 = (int)ceil_div(tiles, L.oc_len);
     }
   } else {
     if (o.batch < 1 || o.head_dim != HEAD_DIM || o.n_q_heads < 1 || o.n_q_heads % d->n_kv_heads) return STARKV_ERR_SHAPE;
@@ -1884,13 +1898,12 @@ int prefix_layout(const starkv_prefix_decode_desc* d, PrefixLayout& L) {
   L.Mp = L.tiles_m * L.bm;
   L.tiles_n = (int)ceil_div(Rvp, PX_BN);
   const int tiles = L.tiles_m * L.tiles_n;
-  L.n_split = std::max(choose_splits(tiles, cus, strips, 256, 3.0, 0.004), (int)ceil_div(strips, PX_SPLIT_STRIPS));
-  L.sp_len = (int)ceil_div(strips, L.n_split);
+  L.sp_len = prefix_split_len(tiles, cus, strips);
   L.n_split = (int)ceil_div(strips, L.sp_len);
-  // logits: two workgroups a CU, each of its four waves a strip at a time
+  // logits: two workgroups a CU, each of its eight waves a strip at a time
   const int zb = (int)ceil_div((int64_t)B * L.gs, 32 * PX_GROUPS);
   const int64_t want = std::max<int64_t>(1, 2 * cus / ((int64_t)d->n_kv_heads * zb));
-  L.ch_len = (int)round_up(ceil_div(strips, want), 4);
+  L.ch_len = (int)round_up(ceil_div(strips, want), 8);
   L.n_ch = (int)ceil_div(strips, L.ch_len);
   L.n_hg = head_groups(Hq);
   L.sw = up_slice_width(d->n_kv_heads, d->v_rank, cus);
@@ -1988,12 +2001,13 @@ int starkv_prefix_decode(const starkv_prefix_decode_desc* d, void* workspace, si
     a.n_c1 = L.own.n_c1; a.n_c2 = L.own.pv.n_c2; a.own_Rvp = L.own.pv.Rvp; a.own_part16 = L.own.part16;
     a.S = o.seq_len;
     if (L.own_here) {
-      a.own_wg = o.batch * d->n_kv_heads * L.own.n_c1; a.oc_len = L.oc_len;
+      a.oc_len = L.oc_len;
       a.ox = o.k.data; a.ox_sb = o.k.stride_b;
       for (int h = 0; h < d->n_kv_heads; ++h) { a.oxoff[h] = o.k.head_offset[h]; a.oxpitch[h] = o.k.pos_stride[h]; }
       a.mask = o.mask; a.m_sb = o.mask_stride_b; a.m_sh = o.mask_stride_h; a.mask_dtype = o.mask_dtype;
       a.last_pos = o.last_pos_device;
       a.ol = (float*)(ws + L.own.off_logits); a.ol_sb = (int64_t)o.n_q_heads * L.own.S_pad; a.ol_st = (int64_t)o.n_q_heads * TILE;
+      if ((st = launch_own_logits(a, o.dtype, s))) return st;
     } else if ((st = decode_logits(&o, L.own, L.gs, ws, s))) {
       return st;
     }

@@ -365,7 +365,6 @@ struct MoveArgs {
 // ---------------------------------------------------------------------------
 constexpr int PX_STRIP = 64;                       // positions of a strip
 constexpr int PX_GROUPS = 2;                       // groups of 32 query rows that a logits workgroup holds
-constexpr int PX_SPLIT_STRIPS = 56;                // most strips of a P V split: their factors lie in LDS
 constexpr int PX_BN = 256;                         // columns of a P V workgroup
 constexpr int PX_HEAD_BYTES = 256;                 // (K multiplier, V multiplier), largest magnitudes
 struct PrefixPackArgs {
@@ -395,8 +394,8 @@ struct PrefixArgs {
   // own positions (n_c1 = 0: none): the decode kernels' maxima, sums and partials
   float* own_max; const float* own_sum; const void* own_part;
   int n_c1, n_c2, n_hg, own_Rvp, own_part16;
-  // ... whose logits (dense latents) the first own_wg workgroups of the logits kernel form
-  int own_wg, S, oc_len;                           // strips of one of their n_c1 chunks
+  // ... for own_logits_kernel (dense latents)
+  int S, oc_len;                                   // positions; tiles of 32 in one of their n_c1 chunks
   const void* ox; int64_t ox_sb, oxoff[K_MAX_KV], oxpitch[K_MAX_KV];       // elements
   const void* mask; int64_t m_sb, m_sh; int mask_dtype;
   const int* last_pos;
@@ -572,6 +571,7 @@ int launch_select(const SelectArgs& a, int B, hipStream_t st);
 int launch_move(const MoveArgs& a, int B, hipStream_t st);
 int launch_prefix_pack(const PrefixPackArgs& a, int dtype, hipStream_t st);
 int launch_prefix_logits(const PrefixArgs& a, int dtype, hipStream_t st);
+int launch_own_logits(const PrefixArgs& a, int dtype, hipStream_t st);
 int launch_prefix_pv(const PrefixArgs& a, hipStream_t st);
 int launch_prefix_join(const PrefixArgs& a, hipStream_t st);
 int launch_fill_i32(int* p, int n, int v, hipStream_t st);

@@ -61,6 +61,14 @@ __device__ inline float px_wave_max(float v) {
   return v;
 }
 
+// two fp32 values as fp16, nearest even (an instruction for both; left to itself the compiler joins each conversion to
+// the sum before it, in a form that takes twice as long)
+__device__ inline uint32_t px_pack(float a, float b) {
+  uint32_t r;
+  asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+
 // position within a 32-position tile of MFMA row m: lane half hh of the result
 // then holds positions 16 hh .. 16 hh + 15 in register order
 __device__ inline int px_pos(int m) { return ((m >> 2) & 1) * 16 + (m >> 3) * 4 + (m & 3); }
@@ -193,80 +201,106 @@ __global__ __launch_bounds__(256) void px_pack_kernel(const PrefixPackArgs a) {
 // ---------------------------------------------------------------------------
 // Logits and weights
 // ---------------------------------------------------------------------------
-// NG: groups of 32 query rows per workgroup.  A tile of B_k^T (32 dims) at a
-// time: its keys are rotated and at once multiplied with the queries' same dims,
-// so no more than a tile's keys are held; the next tile's rotation and the next
-// strip's latents are asked for ahead.
-// OWN: a sequence's own positions instead: dense latents where they lie (rows at
-// any alignment), the queries of one KV head and sequence, and the logits go out
-// in fp32 as the decode's P.V kernels read them.
-template <typename XT, int NG, bool OWN>
-__device__ __forceinline__ void px_logits(const PrefixArgs& a, uint8_t* px_lds, int bx) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5, n = lane & 31;
-  int chunk, h, b = 0;
-  if constexpr (OWN) {
-    chunk = bx % a.n_c1;
-    h = bx / a.n_c1 % a.Hkv;
-    b = bx / a.n_c1 / a.Hkv;
-  } else {
-    // workgroups of one chunk of strips on one XCD: its L2 serves the rotation table to all heads
-    chunk = (bx & 7) + 8 * ((bx >> 3) / a.Hkv);
-    h = (bx >> 3) % a.Hkv;
-    if (chunk >= a.n_ch) return;
-  }
-  const int nr = OWN ? a.gs : a.B * a.gs, r0 = OWN ? 0 : blockIdx.y * NG * 32;
-  const int rank = a.rank[h], nc = (rank + 7) / 8, ks_n = (nc + 1) / 2;
-  const int len = OWN ? a.S : a.P, strips = OWN ? (a.S + PX_STRIP - 1) / PX_STRIP : a.strips;
-  const int per = OWN ? a.oc_len : a.ch_len;
-  uint4* bl = (uint4*)px_lds;                      // [k step][tile w][lane]
-  uint4* ql = bl + a.ks_max * 256;                 // [group][4 tiles x 2 halves][lane]
-  float* mul = (float*)(ql + NG * 512);            // [group * 32 + row]
-  float* wm = mul + NG * 32;                       // [wave][group * 32 + row]
-  const int pn = px_pos(n), s_end = min(strips, (chunk + 1) * per);
-  int s = chunk * per + wave;
-  uint4 xf[2][8];
-  const uint4* xk = (const uint4*)(a.xk + a.xkoff[h]) + pn;
-  const XT* xo = OWN ? (const XT*)a.ox + b * a.ox_sb + a.oxoff[h] : nullptr;
-  const int64_t xpitch = OWN ? a.oxpitch[h] : 0;
-  auto fetch = [&](int at) {
+// A wave takes 32 positions at a time, and of them 32 dims: those keys are rotated
+// and at once multiplied with the queries' same dims, so few registers are held and
+// four waves a SIMD cover each other's waits.  KP: pairs of 16 ranks, so that the
+// operand reads and products of a tile are one block of code (a test of the rank
+// before each product left every one waiting for its own read); the dims are a
+// rolled loop (unrolled, a wave that runs through it once or twice waited for
+// instructions: 33 us for 4 x 1024 positions of 8 heads, now 8).
+//
+// NG: groups of 32 query rows.  acc[g][r] += the logits of query row n of group g
+// and positions px_pos, in register order, of the tile whose latents are in xf.
+// PIPE: the next 32 dims' keys are formed under this one's rotation, in code of
+// their own (registers for both; three waves a SIMD).  `between` runs when xf has
+// been used for the last time.
+template <typename XT, int NG, int KP, bool PIPE, typename F>
+__device__ __forceinline__ void px_tile(const uint4* bl, const uint4* ql, const uint4* rope, const uint4 (&xf)[2 * KP], float down,
+                                        floatx16 (&acc)[NG], F between) {
+  const int lane = threadIdx.x & 63;
+  auto keys = [&](int w) {
+    floatx16 kx = px_mfma<XT>(bl[w * 64 + lane], xf[0], floatx16{});
 #pragma unroll
-    for (int pt = 0; pt < 2; ++pt) {
-      const XT* row = OWN ? xo + min(64 * at + 32 * pt + pn, len - 1) * xpitch : nullptr;
+    for (int k = 1; k < 2 * KP; ++k) kx = px_mfma<XT>(bl[(k * 4 + w) * 64 + lane], xf[k], kx);
+    return kx;
+  };
+  auto turn = [&](int w, const floatx16& kx, const uint4 (&rt)[2]) {
+    uint32_t lo[4], hi[4];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (k < ks_n) {
-          const int c = min(2 * k + hh, nc - 1);
-          if constexpr (!OWN) {
-            xf[pt][k] = xk[((int64_t)(2 * at + pt) * nc + c) * 32];
-          } else if (rank >= 8) {                  // a last chunk of fewer ranks ends with the row
-            __builtin_memcpy(&xf[pt][k], row + min(8 * c, rank - 8), 16);
-          } else {
-            XT e[8];
+    for (int g = 0; g < 2; ++g) {
+      const half8 t = __builtin_bit_cast(half8, rt[g]);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) e[j] = row[min(j, rank - 1)];
-            __builtin_memcpy(&xf[pt][k], e, 16);
-          }
+      for (int j = 0; j < 4; j += 2) {
+        float l[2], u[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float k0 = kx[4 * g + j + i], k1 = kx[8 + 4 * g + j + i];
+          const float c = (float)t[2 * (j + i)], sp = (float)t[2 * (j + i) + 1];
+          if constexpr (!PIPE && __is_same(XT, __bf16)) { k0 *= down; k1 *= down; }
+          // (k sin + 0 takes the table's fp16 as it is; a plain product would convert it first)
+          l[i] = fmaf(c, k0, -fmaf(sp, k1, 0.f));
+          u[i] = fmaf(c, k1, fmaf(sp, k0, 0.f));
         }
+        lo[2 * g + j / 2] = px_pack(l[0], l[1]);
+        hi[2 * g + j / 2] = px_pack(u[0], u[1]);
       }
     }
-  };
-  if (s < s_end) fetch(s);
-  {
-    const uint4* src = (const uint4*)(a.xb + a.xboff[h]);
-    for (int i = tid; i < ks_n * 256; i += 256) bl[i] = src[i];
-  }
-  // queries (the prefix's: turned by P positions), scaled to [1, 2) by row, in the operand's order
-  const float cs = OWN ? 1.f : a.cos_p[lane], sn = OWN ? 0.f : a.sin_p[lane];
-  const float kmul = OWN ? a.scale : a.scale * LOG2E * a.head[0];
-  for (int r = wave; r < NG * 32; r += 4) {
-    float y0 = 0.f, y1 = 0.f;
-    if (r0 + r < nr) {
-      const int qb = OWN ? b : (r0 + r) / a.gs, qg = OWN ? r : (r0 + r) % a.gs;
-      const XT* q = (const XT*)a.q + qb * a.q_sb + (h * a.gs + qg) * a.q_sh;
-      const float x0 = to_f32(q[lane]), x1 = to_f32(q[lane + 64]);
-      y0 = OWN ? x0 : x0 * cs - x1 * sn;
-      y1 = OWN ? x1 : x1 * cs + x0 * sn;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      acc[g] = px_mfma<_Float16>(make_uint4(lo[0], lo[1], lo[2], lo[3]), ql[(g * 8 + 2 * w) * 64 + lane], acc[g]);
+      acc[g] = px_mfma<_Float16>(make_uint4(hi[0], hi[1], hi[2], hi[3]), ql[(g * 8 + 2 * w + 1) * 64 + lane], acc[g]);
     }
+  };
+  if constexpr (PIPE) {
+    uint4 rt[2][2] = {{rope[0], rope[64]}, {}};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      if (w < 3) {
+        rt[(w + 1) & 1][0] = rope[128 * (w + 1)];
+        rt[(w + 1) & 1][1] = rope[128 * (w + 1) + 64];
+      }
+      const floatx16 kx = keys(w);
+      if (w == 3) between();
+      turn(w, kx, rt[w & 1]);
+      __builtin_amdgcn_sched_barrier(0);           // loads hoisted across the dims' tiles cost registers
+    }
+  } else {
+    uint4 next[2] = {rope[0], rope[64]};
+#pragma unroll 1
+    for (int w = 0; w < 4; ++w) {
+      const uint4 rt[2] = {next[0], next[1]};
+      const int more = w < 3 ? 128 * (w + 1) : 0;  // (the last reads the first again)
+      next[0] = rope[more];
+      next[1] = rope[more + 64];
+      turn(w, keys(w), rt);
+    }
+    between();
+  }
+}
+
+// B_k's operands of one head and the query rows r0 .. of it into LDS: the rows of (sequence, head of the group) from
+// sequence b0 on, turned by (cos, sin), scaled to [1, 2) by a power of two each, in the operand's order
+template <typename XT, int NG, int KP, int NW>
+__device__ __forceinline__ void px_stage(const PrefixArgs& a, int h, int b0, int r0, int nr, float cs, float sn, float kmul, uint4* bl,
+                                         uint4* ql, float* mul) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, ks_n = ((a.rank[h] + 7) / 8 + 1) / 2;
+  const uint4* src = (const uint4*)(a.xb + a.xboff[h]);
+  constexpr int RW = 32 * NG / NW;
+  XT q0[RW], q1[RW];
+#pragma unroll
+  for (int i = 0; i < RW; ++i) {                   // (rows past the last repeat it)
+    const int r = min(r0 + wave + NW * i, nr - 1);
+    const XT* q = (const XT*)a.q + (b0 + r / a.gs) * a.q_sb + (h * a.gs + r % a.gs) * a.q_sh;
+    q0[i] = q[lane];
+    q1[i] = q[lane + 64];
+  }
+#pragma unroll
+  for (int i = 0; i < 8 * KP / NW; ++i)
+    bl[tid + 64 * NW * i] = tid + 64 * NW * i < ks_n * 256 ? src[tid + 64 * NW * i] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int i = 0; i < RW; ++i) {
+    const int r = wave + NW * i;
+    const float x0 = to_f32(q0[i]), x1 = to_f32(q1[i]), y0 = x0 * cs - x1 * sn, y1 = x1 * cs + x0 * sn;
     const float m = px_wave_max(fmaxf(fabsf(y0), fabsf(y1)));
     const int e = m < INFINITY && m > 0.f ? min(max((int)(__float_as_uint(m) >> 23), 1), 253) - 127 : 0;
     const float f = pow2f(-e);
@@ -276,197 +310,245 @@ __device__ __forceinline__ void px_logits(const PrefixArgs& a, uint8_t* px_lds, 
     dst[64 * 8] = (_Float16)(y1 * f);
     if (lane == 0) mul[r] = kmul * pow2f(e);
   }
-  __syncthreads();
+}
 
+// the largest over the workgroup's waves of each row's maximum, in wm[row]
+template <int NG, int NW> __device__ __forceinline__ void px_row_max(const float (&top)[NG], float* wm) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+#pragma unroll
+  for (int g = 0; g < NG; ++g)
+    if (lane < 32) wm[wave * NG * 32 + g * 32 + lane] = top[g];
+  __syncthreads();
+  if (tid >= NG * 32) return;
+  float m = wm[tid];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) m = fmaxf(m, wm[w * NG * 32 + tid]);
+  wm[tid] = m;
+}
+
+// Workgroup of eight waves = (chunk of strips, KV head, NG groups of rows), a wave a strip at a time.
+template <typename XT, int NG, int KP>
+__device__ __forceinline__ void px_prefix_logits(const PrefixArgs& a, uint8_t* lds, int chunk, int h) {
+  constexpr int KS = 2 * KP;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5, n = lane & 31;
+  const int nr = a.B * a.gs, r0 = blockIdx.y * NG * 32, nc = (a.rank[h] + 7) / 8;
+  uint4* bl = (uint4*)lds;                         // [k step][tile w][lane]
+  uint4* ql = bl + KS * 256;                       // [group][4 tiles x 2 halves][lane]
+  float* mul = (float*)(ql + NG * 512);            // [group * 32 + row]
+  float* wm = mul + NG * 32;                       // [wave][group * 32 + row]
+  const int at_lane = 32 * hh + px_pos(n), s_end = min(a.strips, (chunk + 1) * a.ch_len);
+  int s = chunk * a.ch_len + wave;
+  uint4 xf[KS];
+  // (of an odd number of chunks the last one's upper lanes, and of an odd number of k steps the last, read what lies
+  // behind: the packed B_k at most, and replaced by zeros)
+  auto fetch = [&](int tile) {
+    const uint4* x = (const uint4*)(a.xk + a.xkoff[h]) + (int64_t)tile * nc * 32;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) xf[k] = x[at_lane + 64 * min(k, (nc - 1) / 2)];
+  };
+  auto clear = [&]() {
+#pragma unroll
+    for (int k = KS - 2; k < KS; ++k)
+      if (2 * k + hh >= nc) xf[k] = make_uint4(0, 0, 0, 0);
+  };
+  if (s < s_end) fetch(2 * s);
+  px_stage<XT, NG, KP, 8>(a, h, 0, r0, nr, a.cos_p[lane], a.sin_p[lane], a.scale * LOG2E * a.head[0], bl, ql, mul);
+  __syncthreads();
   float top[NG];
 #pragma unroll
   for (int g = 0; g < NG; ++g) top[g] = -INFINITY;
-  const int last_pos = OWN && a.last_pos ? *a.last_pos : INT32_MAX;
-  const int tail = OWN ? rank & 7 : 0;             // ranks of a last chunk that is not whole
-  for (; s < s_end; s += 4) {
-    floatx16 acc[NG][2] = {};
-    // the last k step: a partial chunk's ranks to its front, zeros behind the rank
+  for (; s < s_end; s += 8) {
+    floatx16 acc[2][NG] = {};
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if (k != ks_n - 1) continue;
-#pragma unroll
-      for (int pt = 0; pt < 2; ++pt) {
-        if (OWN && tail) {
-          const uint4 v = xf[pt][k];
-          uint64_t lo = v.x | ((uint64_t)v.y << 32), hi = v.z | ((uint64_t)v.w << 32);
-          if (rank >= 8) {
-            const int sh = 16 * (8 - tail);
-            lo = sh >= 64 ? hi >> (sh - 64) : (lo >> sh) | (hi << (64 - sh));
-            hi = sh >= 64 ? 0 : hi >> sh;
-          }
-          // (of a row of fewer than 8 ranks the last was repeated)
-          const uint64_t ml = tail >= 4 ? ~0ull : (1ull << (16 * tail)) - 1, mh = tail <= 4 ? 0 : (1ull << (16 * (tail - 4))) - 1;
-          lo &= ml;
-          hi &= mh;
-          if (min(2 * k + hh, nc - 1) == nc - 1)
-            xf[pt][k] = make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
-        }
-        if (2 * k + hh >= nc) xf[pt][k] = make_uint4(0, 0, 0, 0);
-      }
+    for (int pt = 0; pt < 2; ++pt) {
+      clear();
+      px_tile<XT, NG, KP, true>(bl, ql, a.rope + (int64_t)(2 * s + pt) * 512 + at_lane, xf, 1.f, acc[pt],
+                                [&]() { fetch(pt == 0 ? 2 * s + 1 : 2 * min(s + 8, s_end - 1)); });
     }
-    // bf16 keys of own positions can pass fp16's range: scaled by what bounds them (the prefix's were when it was packed)
-    int ke = 0;
-    if constexpr (OWN && __is_same(XT, __bf16)) {
-      uint32_t big = 0;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (k >= ks_n) continue;
-#pragma unroll
-        for (int pt = 0; pt < 2; ++pt)
-          big = max2_u16(max2_u16(max2_u16(big, xf[pt][k].x & 0x7fff7fffu), xf[pt][k].y & 0x7fff7fffu),
-                         max2_u16(xf[pt][k].z & 0x7fff7fffu, xf[pt][k].w & 0x7fff7fffu));
-      }
-      const float bound = px_wave_max(fmaxf(__uint_as_float(big << 16), __uint_as_float(big & 0xffff0000u))) * a.head[5];
-      if (bound > 32768.f && bound < INFINITY) ke = min((int)(__float_as_uint(bound) >> 23) - 141, 100);
-      ke = __builtin_amdgcn_readfirstlane(ke);
-    }
-    const float kdown = pow2f(-ke);
-    uint4 rt[2][2][2];
-    auto turn = [&](int w) {
-#pragma unroll
-      for (int pt = 0; pt < 2; ++pt)
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-          rt[w & 1][pt][g] = a.rope[((int64_t)min(2 * s + pt, (len - 1) >> 5) * 8 + 2 * w + g) * 64 + hh * 32 + pn];
-    };
-    turn(0);
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      if (w < 3) turn(w + 1);
-      floatx16 kx[2] = {};
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (k < ks_n) {
-          const uint4 bf = bl[(k * 4 + w) * 64 + lane];
-          kx[0] = px_mfma<XT>(bf, xf[0][k], kx[0]);
-          kx[1] = px_mfma<XT>(bf, xf[1][k], kx[1]);
-        }
-      }
-      if (OWN && ke) {
-#pragma unroll
-        for (int pt = 0; pt < 2; ++pt)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) kx[pt][r] *= kdown;
-      }
-      uint4 kf[2][2];
-#pragma unroll
-      for (int pt = 0; pt < 2; ++pt) {
-        half8 lo, hi;
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const half8 t = __builtin_bit_cast(half8, rt[w & 1][pt][g]);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float k0 = kx[pt][4 * g + j], k1 = kx[pt][8 + 4 * g + j], c = (float)t[2 * j], sp = (float)t[2 * j + 1];
-            lo[4 * g + j] = (_Float16)(k0 * c - k1 * sp);
-            hi[4 * g + j] = (_Float16)(k1 * c + k0 * sp);
-          }
-        }
-        kf[pt][0] = __builtin_bit_cast(uint4, lo);
-        kf[pt][1] = __builtin_bit_cast(uint4, hi);
-      }
-#pragma unroll
-      for (int g = 0; g < NG; ++g)
-#pragma unroll
-        for (int f = 0; f < 2; ++f) {
-          const uint4 q = ql[(g * 8 + 2 * w + f) * 64 + lane];
-          acc[g][0] = px_mfma<_Float16>(kf[0][f], q, acc[g][0]);
-          acc[g][1] = px_mfma<_Float16>(kf[1][f], q, acc[g][1]);
-        }
-      __builtin_amdgcn_sched_barrier(0);           // loads hoisted across tiles cost a hundred spills
-    }
-    const int cur = s;
-    if (s + 4 < s_end) fetch(s + 4);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      const float f = OWN ? mul[g * 32 + n] * pow2f(ke) : mul[g * 32 + n];
-      const int rl = r0 + g * 32 + n, p0 = 64 * cur + 16 * hh;
-#pragma unroll
-      for (int pt = 0; pt < 2; ++pt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[g][pt][r] *= f;
-      if (OWN && a.mask != nullptr && rl < nr) {
-        const int64_t at = b * a.m_sb + (h * a.gs + rl) * a.m_sh;
-#pragma unroll
-        for (int pt = 0; pt < 2; ++pt)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) acc[g][pt][r] += load_elem_f32(a.mask, a.mask_dtype, at + min(p0 + 32 * pt + r, len - 1));
-      }
-      if (64 * (cur + 1) > min(len, last_pos + (last_pos < INT32_MAX ? 1 : 0))) {
-#pragma unroll
-        for (int pt = 0; pt < 2; ++pt)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            if (p0 + 32 * pt + r > last_pos) acc[g][pt][r] = -1e30f;
-            if (p0 + 32 * pt + r >= len) acc[g][pt][r] = -INFINITY;
-          }
-      }
+      const float f = mul[g * 32 + n];
+      const int rl = r0 + g * 32 + n, row = h * nr + rl;
       float m = -INFINITY;
 #pragma unroll
       for (int pt = 0; pt < 2; ++pt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[g][pt][r]);
-      m = max_halves(m);
-      if constexpr (OWN) {
-        top[g] = fmaxf(top[g], m);
-        if (rl < nr) {
+        for (int r = 0; r < 16; ++r) acc[pt][g][r] *= f;
+      if (64 * (s + 1) > a.P) {
 #pragma unroll
-          for (int pt = 0; pt < 2; ++pt) {
-            float4* o = (float4*)(a.ol + b * a.ol_sb + (2 * cur + pt) * a.ol_st + (h * a.gs + rl) * 32 + 16 * hh);
+        for (int pt = 0; pt < 2; ++pt)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] = make_float4(acc[g][pt][4 * r], acc[g][pt][4 * r + 1], acc[g][pt][4 * r + 2], acc[g][pt][4 * r + 3]);
-          }
-        }
-        continue;
+          for (int r = 0; r < 16; ++r)
+            if (64 * s + 32 * pt + 16 * hh + r >= a.P) acc[pt][g][r] = -INFINITY;
       }
-      m = fmaxf(m, -3.0e38f);                      // a strip of -inf alone: weights 0
+#pragma unroll
+      for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[pt][g][r]);
+      m = fmaxf(max_halves(m), -3.0e38f);          // a strip of -inf alone: weights 0
       top[g] = fmaxf(top[g], m);
       float l = 0.f;
-      const int64_t row = (int64_t)h * nr + rl;
-      uint4* o = a.p + (int64_t)(8 * cur + 2 * hh) * a.Mp + row;
+      uint8_t* o = (uint8_t*)(a.p + (int64_t)8 * s * a.Mp);
+      const uint32_t at = (uint32_t)(2 * hh * a.Mp + row) * 16, step = (uint32_t)a.Mp * 16;
 #pragma unroll
       for (int pt = 0; pt < 2; ++pt) {
         half8 v[2];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) v[r >> 3][r & 7] = (_Float16)__builtin_amdgcn_exp2f(acc[g][pt][r] - m);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) l += (float)v[r >> 3][r & 7];
+        for (int r = 0; r < 16; ++r) {
+          const float e = __builtin_amdgcn_exp2f(acc[pt][g][r] - m);
+          l += e;
+          v[r >> 3][r & 7] = (_Float16)e;
+        }
         if (rl < nr) {
-          o[4 * pt * (int64_t)a.Mp] = __builtin_bit_cast(uint4, v[0]);
-          o[(4 * pt + 1) * (int64_t)a.Mp] = __builtin_bit_cast(uint4, v[1]);
+          *(uint4*)(o + (at + 4 * pt * step)) = __builtin_bit_cast(uint4, v[0]);
+          *(uint4*)(o + (at + (4 * pt + 1) * step)) = __builtin_bit_cast(uint4, v[1]);
         }
       }
       l = add_halves(l);
-      if (rl < nr && hh == 0) a.stat[(int64_t)cur * a.Mp + row] = make_float2(m, l);
+      if (rl < nr && hh == 0) *(float2*)((uint8_t*)(a.stat + (int64_t)s * a.Mp) + (uint32_t)row * 8) = make_float2(m, l);
     }
   }
-  // the chunk's maximum of each row
-#pragma unroll
-  for (int g = 0; g < NG; ++g)
-    if (hh == 0) wm[wave * NG * 32 + g * 32 + n] = top[g];
-  __syncthreads();
-  for (int r = tid; r < NG * 32; r += 256) {
-    if (r0 + r >= nr) continue;
-    float m = wm[r];
-#pragma unroll
-    for (int w = 1; w < 4; ++w) m = fmaxf(m, wm[w * NG * 32 + r]);
-    if constexpr (OWN) a.own_max[((int64_t)b * a.Hq + h * a.gs + r) * a.n_c1 + chunk] = m;
-    else a.cmax[(int64_t)chunk * a.Mp + (int64_t)h * nr + r0 + r] = m;
-  }
+  px_row_max<NG, 8>(top, wm);
+  if (tid < NG * 32 && r0 + tid < nr) a.cmax[(int64_t)chunk * a.Mp + (int64_t)h * nr + r0 + tid] = wm[tid];
 }
 
-// The first own_wg workgroups: own positions (while they wait for their few latents the prefix's compute).
 template <typename XT, int NG>
-__global__ __launch_bounds__(256, 2) void prefix_logits_kernel(const PrefixArgs a) {
+__global__ __launch_bounds__(512, NG == 1 ? 4 : 2) void prefix_logits_kernel(const PrefixArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t px_lds[];
-  const int bx = blockIdx.x;
-  if (bx >= a.own_wg) px_logits<XT, NG, false>(a, px_lds, bx - a.own_wg);
-  else if (blockIdx.y == 0) px_logits<XT, NG, true>(a, px_lds, bx);
+  // workgroups of one chunk of strips on one XCD: its L2 serves the rotation table to all heads
+  const int bx = blockIdx.x, chunk = (bx & 7) + 8 * ((bx >> 3) / a.Hkv), h = (bx >> 3) % a.Hkv, kp = (a.rank[h] + 31) / 32;
+  if (chunk >= a.n_ch) return;
+  if (kp == 1) px_prefix_logits<XT, NG, 1>(a, px_lds, chunk, h);
+  else if (kp == 2) px_prefix_logits<XT, NG, 2>(a, px_lds, chunk, h);
+  else if (kp == 3) px_prefix_logits<XT, NG, 3>(a, px_lds, chunk, h);
+  else px_prefix_logits<XT, NG, 4>(a, px_lds, chunk, h);
+}
+
+// A sequence's own positions: dense latents where they lie (rows at any alignment),
+// the queries of one KV head and sequence, and the logits go out in fp32 as the
+// decode's P.V kernels read them.  Workgroup = (sequence, KV head, chunk of tiles
+// of 32 positions), a wave a tile at a time.
+template <typename XT, int NG, int KP>
+__device__ __forceinline__ void px_own_logits(const PrefixArgs& a, uint8_t* lds, int chunk, int h, int b) {
+  constexpr int KS = 2 * KP;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5, n = lane & 31;
+  const int rank = a.rank[h], nc = (rank + 7) / 8, tail = rank & 7, pn = px_pos(n);
+  uint4* bl = (uint4*)lds;
+  uint4* ql = bl + KS * 256;
+  float* mul = (float*)(ql + NG * 512);
+  float* wm = mul + NG * 32;
+  const int t_end = min((a.S + 31) / 32, (chunk + 1) * a.oc_len);
+  int t = chunk * a.oc_len + wave;
+  uint4 xf[KS];
+  const XT* x = (const XT*)a.ox + b * a.ox_sb + a.oxoff[h];
+  auto fetch = [&](int tile) {
+    const XT* row = x + min(32 * tile + pn, a.S - 1) * a.oxpitch[h];
+    if (KP == 1 && rank < 8) {
+      XT e[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) e[j] = row[min(j, rank - 1)];
+      __builtin_memcpy(&xf[0], e, 16);
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < KS; ++k) __builtin_memcpy(&xf[k], row + min(8 * (2 * k + hh), rank - 8), 16);   // the last ends with the row
+  };
+  if (t < t_end) fetch(t);
+  px_stage<XT, NG, KP, 8>(a, h, b, 0, a.gs, 1.f, 0.f, a.scale, bl, ql, mul);
+  __syncthreads();
+  const int last_pos = a.last_pos ? *a.last_pos : INT32_MAX;
+  // a last chunk of fewer than 8 ranks: to its front (of a row of fewer in all the last was repeated), zeros behind
+  const int sh = rank >= 8 && tail ? 16 * (8 - tail) : 0;
+  const uint64_t ml = tail == 0 || tail >= 4 ? ~0ull : (1ull << (16 * tail)) - 1;
+  const uint64_t mh = tail == 0 ? ~0ull : tail <= 4 ? 0 : (1ull << (16 * (tail - 4))) - 1;
+  float top[NG];
+#pragma unroll
+  for (int g = 0; g < NG; ++g) top[g] = -INFINITY;
+#pragma unroll 1
+  for (; t < t_end; t += 8) {
+#pragma unroll
+    for (int k = KS - 2; k < KS; ++k) {
+      uint64_t lo = xf[k].x | ((uint64_t)xf[k].y << 32), hi = xf[k].z | ((uint64_t)xf[k].w << 32);
+      if (2 * k + hh == nc - 1) {
+        if (sh >= 64) {
+          lo = hi >> (sh - 64);
+          hi = 0;
+        } else if (sh) {
+          lo = (lo >> sh) | (hi << (64 - sh));
+          hi >>= sh;
+        }
+        lo &= ml;
+        hi &= mh;
+      }
+      if (2 * k + hh >= nc) lo = hi = 0;
+      xf[k] = make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
+    }
+    // bf16 keys can pass fp16's range: scaled by what bounds them (the prefix's were when it was packed)
+    float up = 1.f, down = 1.f;
+    if constexpr (__is_same(XT, __bf16)) {
+      uint32_t big = 0;
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+        big = max2_u16(max2_u16(max2_u16(big, xf[k].x & 0x7fff7fffu), xf[k].y & 0x7fff7fffu),
+                       max2_u16(xf[k].z & 0x7fff7fffu, xf[k].w & 0x7fff7fffu));
+      const float bound = px_wave_max(fmaxf(__uint_as_float(big << 16), __uint_as_float(big & 0xffff0000u))) * a.head[5];
+      if (bound > 32768.f && bound < INFINITY) {
+        const int e = min((int)(__float_as_uint(bound) >> 23) - 141, 100);
+        up = pow2f(e);
+        down = pow2f(-e);
+      }
+    }
+    floatx16 acc[NG] = {};
+    px_tile<XT, NG, KP, false>(bl, ql, a.rope + (int64_t)t * 512 + 32 * hh + pn, xf, down, acc,
+                               [&]() { if (t + 8 < t_end) fetch(t + 8); });
+    const int p0 = 32 * t + 16 * hh;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const float f = mul[g * 32 + n] * up;
+      const int rl = g * 32 + n;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[g][r] *= f;
+      if (a.mask != nullptr && rl < a.gs) {
+        const int64_t at = b * a.m_sb + (h * a.gs + rl) * a.m_sh;
+        if (a.mask_dtype == STARKV_F32) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[g][r] += ((const float*)a.mask)[at + min(p0 + r, a.S - 1)];
+        } else {
+          const uint16_t* mk = (const uint16_t*)a.mask + at;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const uint16_t v = mk[min(p0 + r, a.S - 1)];
+            acc[g][r] += a.mask_dtype == STARKV_F16 ? (float)__builtin_bit_cast(_Float16, v) : bf16_bits_to_float(v);
+          }
+        }
+      }
+      float m = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        if (p0 + r > last_pos) acc[g][r] = -1e30f;
+        if (p0 + r >= a.S) acc[g][r] = -INFINITY;
+        m = fmaxf(m, acc[g][r]);
+      }
+      top[g] = fmaxf(top[g], max_halves(m));
+      if (rl < a.gs) {
+        float4* o = (float4*)(a.ol + b * a.ol_sb + t * a.ol_st + (h * a.gs + rl) * 32 + 16 * hh);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = make_float4(acc[g][4 * r], acc[g][4 * r + 1], acc[g][4 * r + 2], acc[g][4 * r + 3]);
+      }
+    }
+  }
+  px_row_max<NG, 8>(top, wm);
+  if (tid < a.gs) a.own_max[((int64_t)b * a.Hq + h * a.gs + tid) * a.n_c1 + chunk] = wm[tid];
+}
+
+template <typename XT, int NG>
+__global__ __launch_bounds__(512, NG == 1 ? 4 : 3) void own_logits_kernel(const PrefixArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t px_lds[];
+  const int bx = blockIdx.x, chunk = bx % a.n_c1, h = bx / a.n_c1 % a.Hkv, b = bx / a.n_c1 / a.Hkv, kp = (a.rank[h] + 31) / 32;
+  if (kp == 1) px_own_logits<XT, NG, 1>(a, px_lds, chunk, h, b);
+  else if (kp == 2) px_own_logits<XT, NG, 2>(a, px_lds, chunk, h, b);
+  else if (kp == 3) px_own_logits<XT, NG, 3>(a, px_lds, chunk, h, b);
+  else px_own_logits<XT, NG, 4>(a, px_lds, chunk, h, b);
 }
 
 // ---------------------------------------------------------------------------
@@ -485,16 +567,18 @@ template <int N> __device__ inline void px_stage_ready() {
 
 // Workgroup of 8 waves = (split of the strips, BM rows, 256 columns), wave (wm, wn)
 // of WM x WN: RM x RN MFMA tiles, two waves a SIMD.  Steps of 32 positions go
-// through a ring of four LDS stages, three of them in flight.  The factors of the
-// split's strips are formed once, before the loop.
+// through a ring of four LDS stages, three of them in flight; the strips' factors
+// are formed 56 strips at a time.
 template <int RM, int RN, int WM, int WN>
 __global__ __launch_bounds__(512, 2) void prefix_pv_kernel(const PrefixArgs a) {
   constexpr int BM = 32 * RM * WM, BN = 32 * RN * WN, RING = 4;
   constexpr int AI = (BM * 4 / 64 + 7) / 8, BI = BN * 4 / 64 / 8, NI = AI + BI;     // copies per wave and stage
   constexpr int STAGE = 4 * (BM + BN);             // 16-byte pieces
+  constexpr int FS = 56;                           // strips whose factors lie in LDS (what the ring of BM 256 leaves)
+  static_assert(2 * FS % RING == 0, "whole rounds of the ring");
   static_assert(WM * WN == 8 && BN == PX_BN, "eight waves");
   __shared__ uint4 ring[RING * STAGE];
-  __shared__ _Float16 fac[PX_SPLIT_STRIPS * BM];   // [strip][row]
+  __shared__ _Float16 fac[FS * BM];                // [strip][row]
   __shared__ float row_f[BM];                      // 1 / (2 sum)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5, n = lane & 31;
   const int wm = wave / WN, wn = wave % WN;
@@ -529,25 +613,26 @@ __global__ __launch_bounds__(512, 2) void prefix_pv_kernel(const PrefixArgs a) {
     for (int i = 0; i < NI; ++i) px_dma(i < AI ? pa : pb, off[i], dst[i] + slot * STAGE * 16);
     if (++issued < steps) { pa += 4 * (int64_t)a.Mp; pb += 4 * (int64_t)a.Rvp; }
   };
-  // strips' factors and sums, a row per thread
-  float lsum = 0.f;
+  // the row's maximum; its strips' factors and sum, FS strips at a time, a row per thread
+  float row_max = -INFINITY, lsum = 0.f;
   if (tid < BM) {
-    float m = -INFINITY;
     const float* cm = a.cmax + m0 + tid;
 #pragma unroll 8
-    for (int c = 0; c < a.n_ch; ++c) m = fmaxf(m, cm[(int64_t)c * a.Mp]);
-    if (split == 0 && n0 == 0) a.rmax[m0 + tid] = m;
-    const float2* st = a.stat + (int64_t)s0 * a.Mp + m0 + tid;
+    for (int c = 0; c < a.n_ch; ++c) row_max = fmaxf(row_max, cm[(int64_t)c * a.Mp]);
+    if (split == 0 && n0 == 0) a.rmax[m0 + tid] = row_max;
+  }
+  auto factors = [&](int from) {
+    if (tid >= BM) return;
+    const float2* st = a.stat + (int64_t)(s0 + from) * a.Mp + m0 + tid;
 #pragma unroll 8
-    for (int s = 0; s < s1 - s0; ++s) {
+    for (int s = 0; s < min(FS, s1 - s0 - from); ++s) {
       const float2 v = st[(int64_t)s * a.Mp];
-      const _Float16 f = (_Float16)__builtin_amdgcn_exp2f((v.x - m) + PX_LIFT);
+      const _Float16 f = (_Float16)__builtin_amdgcn_exp2f((v.x - row_max) + PX_LIFT);
       fac[s * BM + tid] = f;
       lsum = fmaf(v.y, (float)f, lsum);
     }
-    row_f[tid] = lsum == 0.f ? 0.f : 0.5f / lsum;
-    if (n0 == 0) a.lsum[(int64_t)split * a.Mp + m0 + tid] = lsum;
-  }
+  };
+  factors(0);
   floatx16 acc[RM][RN];
 #pragma unroll
   for (int i = 0; i < RM; ++i)
@@ -558,6 +643,11 @@ __global__ __launch_bounds__(512, 2) void prefix_pv_kernel(const PrefixArgs a) {
   for (int i = 0; i < RING - 1; ++i) issue(i);
   kh2 fc[RM];
   for (int t0 = 0; t0 < steps; t0 += RING) {
+    if (t0 && t0 % (2 * FS) == 0) {
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");        // the last ones have been used
+      factors(t0 / 2);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
 #pragma unroll
     for (int u = 0; u < RING; ++u) {
       if (t0 + u >= steps) break;
@@ -566,7 +656,7 @@ __global__ __launch_bounds__(512, 2) void prefix_pv_kernel(const PrefixArgs a) {
       if (u % 2 == 0) {
 #pragma unroll
         for (int i = 0; i < RM; ++i) {
-          const _Float16 f = fac[((t0 + u) >> 1) * BM + (wm * RM + i) * 32 + n];
+          const _Float16 f = fac[((t0 + u) / 2 % FS) * BM + (wm * RM + i) * 32 + n];
           fc[i] = kh2{f, f};
         }
       }
@@ -592,7 +682,11 @@ __global__ __launch_bounds__(512, 2) void prefix_pv_kernel(const PrefixArgs a) {
       }
     }
   }
-  px_stage_ready<0>();                             // the last copies, before the workgroup's LDS is another's
+  if (tid < BM) {
+    row_f[tid] = lsum == 0.f ? 0.f : 0.5f / lsum;
+    if (n0 == 0) a.lsum[(int64_t)split * a.Mp + m0 + tid] = lsum;
+  }
+  px_stage_ready<0>();                             // the sums, and the last copies before the LDS is another's
   _Float16* out = a.part + ((int64_t)split * a.M + m0) * a.Rvp + n0;
 #pragma unroll
   for (int i = 0; i < RM; ++i)
@@ -695,21 +789,28 @@ int launch_prefix_pack(const PrefixPackArgs& a, int dtype, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
-template <typename XT, int NG> static void launch_logits(const PrefixArgs& a, int groups, hipStream_t st) {
-  const size_t lds = (size_t)a.ks_max * 4096 + NG * 8192 + NG * 32 * 4 * 5;
-  const dim3 grid((unsigned)(round_up(a.n_ch, 8) * a.Hkv + a.own_wg), (unsigned)ceil_div(groups, NG));
-  hipLaunchKernelGGL((prefix_logits_kernel<XT, NG>), grid, dim3(256), lds, st, a);
+static size_t px_logits_lds(const PrefixArgs& a, int ng) { return (size_t)round_up(a.ks_max, 2) * 4096 + ng * (8192 + 32 * 4 * 9); }
+
+template <typename XT> static void launch_logits(const PrefixArgs& a, hipStream_t st) {
+  const int groups = (int)ceil_div((int64_t)a.B * a.gs, 32);
+  const dim3 grid((unsigned)(round_up(a.n_ch, 8) * a.Hkv), (unsigned)ceil_div(groups, groups == 1 ? 1 : PX_GROUPS));
+  if (groups == 1) hipLaunchKernelGGL((prefix_logits_kernel<XT, 1>), grid, dim3(512), px_logits_lds(a, 1), st, a);
+  else hipLaunchKernelGGL((prefix_logits_kernel<XT, PX_GROUPS>), grid, dim3(512), px_logits_lds(a, PX_GROUPS), st, a);
+}
+int launch_prefix_logits(const PrefixArgs& a, int dtype, hipStream_t st) {
+  if (dtype == STARKV_F16) launch_logits<_Float16>(a, st);
+  else launch_logits<__bf16>(a, st);
+  return (int)hipGetLastError();
 }
 
-int launch_prefix_logits(const PrefixArgs& a, int dtype, hipStream_t st) {
-  const int groups = (int)ceil_div((int64_t)a.B * a.gs, 32);
-  if (groups == 1) {
-    if (dtype == STARKV_F16) launch_logits<_Float16, 1>(a, groups, st);
-    else launch_logits<__bf16, 1>(a, groups, st);
-  } else {
-    if (dtype == STARKV_F16) launch_logits<_Float16, PX_GROUPS>(a, groups, st);
-    else launch_logits<__bf16, PX_GROUPS>(a, groups, st);
-  }
+template <typename XT> static void launch_own(const PrefixArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)(a.B * a.Hkv * a.n_c1));
+  if (a.gs <= 32) hipLaunchKernelGGL((own_logits_kernel<XT, 1>), grid, dim3(512), px_logits_lds(a, 1), st, a);
+  else hipLaunchKernelGGL((own_logits_kernel<XT, 2>), grid, dim3(512), px_logits_lds(a, 2), st, a);
+}
+int launch_own_logits(const PrefixArgs& a, int dtype, hipStream_t st) {
+  if (dtype == STARKV_F16) launch_own<_Float16>(a, st);
+  else launch_own<__bf16>(a, st);
   return (int)hipGetLastError();
 }
 

@@ -630,7 +630,8 @@ int starkv_decode_attention_scores(const starkv_decode_desc* d, float* scores, i
  * bounded cache keeps, in ascending order: the first `sinks`, the last
  * `recent`, and of those between the keep - sinks - recent with the largest
  * scores (equal ones: the lowest positions; NaN counts as -infinity).
- * 0 <= sinks + recent <= keep <= length <= 2^24.
+ * 0 <= sinks + recent <= keep <= length <= 2^24, batch <= 65535.  Workspace:
+ * only for rows of more than 32768 positions between (0 otherwise).
  * scores (b, p) at scores + b*scores_stride_b + p; positions (b, i) at
  * positions + b*positions_stride_b + i.
  *
@@ -650,7 +651,8 @@ typedef struct {
   int* positions; int64_t positions_stride_b;
 } starkv_select_desc;
 
-int starkv_select_positions(const starkv_select_desc* d, void* stream);
+size_t starkv_select_positions_workspace_bytes(const starkv_select_desc* d);   /* 0: none needed, or invalid */
+int starkv_select_positions(const starkv_select_desc* d, void* workspace, size_t workspace_bytes, void* stream);
 
 typedef struct {
   int batch, length, keep, dtype;

@@ -1713,18 +1713,44 @@ int starkv_decode_attention_scores(const starkv_decode_desc* d, float* scores, i
   return decode_impl(d, workspace, workspace_bytes, stream, nullptr, scores, scores_stride_b);
 }
 
-int starkv_select_positions(const starkv_select_desc* d, void* stream) {
+static int check_select(const starkv_select_desc* d, SelectArgs& a, size_t& bytes) {
   if (!d) return STARKV_ERR_NULL;
   if (d->batch < 0 || d->length < 0 || d->sinks < 0 || d->recent < 0 || d->keep > d->length ||
       (int64_t)d->sinks + d->recent > d->keep)
     return STARKV_ERR_SHAPE;
-  if (d->length > MAX_S || d->batch > (1 << 20)) return STARKV_ERR_LIMIT;
+  if (d->length > MAX_S || d->batch > 65535) return STARKV_ERR_LIMIT;
+  a = SelectArgs{d->scores, d->scores_stride_b, d->positions, d->positions_stride_b, d->length, d->keep, d->sinks, d->recent, d->batch};
+  const int fixed = d->sinks + d->recent, n = d->length - fixed;
+  a.piece_len = select_piece(n, d->keep - fixed);
+  bytes = 0;
+  if (!a.piece_len || !d->batch) return STARKV_OK;
+  a.pieces = (int)ceil_div(n, a.piece_len);
+  bytes = a256((size_t)3 * d->batch * a.pieces * 2048 * 4) + (size_t)d->batch * 3 * 8;
+  return STARKV_OK;
+}
+
+size_t starkv_select_positions_workspace_bytes(const starkv_select_desc* d) {
+  SelectArgs a;
+  size_t bytes;
+  return check_select(d, a, bytes) ? 0 : bytes;
+}
+
+int starkv_select_positions(const starkv_select_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
+  SelectArgs a;
+  size_t bytes;
+  const int st = check_select(d, a, bytes);
+  if (st) return st;
   if (d->batch == 0 || d->keep == 0) return STARKV_OK;
   if (!d->scores || !d->positions) return STARKV_ERR_NULL;
   if (d->batch > 1 && (d->scores_stride_b < 0 || d->positions_stride_b < d->keep)) return STARKV_ERR_SHAPE;
   if (!al(d->scores, 4) || !al(d->positions, 4)) return STARKV_ERR_ALIGN;
-  SelectArgs a = {d->scores, d->scores_stride_b, d->positions, d->positions_stride_b, d->length, d->keep, d->sinks, d->recent};
-  return launch_select(a, d->batch, (hipStream_t)stream);
+  if (bytes) {
+    if (!workspace || workspace_bytes < bytes) return STARKV_ERR_WORKSPACE;
+    if (!al(workspace, 256)) return STARKV_ERR_ALIGN;
+    a.hist = (uint32_t*)workspace;
+    a.state = (int2*)((char*)workspace + a256((size_t)3 * a.B * a.pieces * 2048 * 4));
+  }
+  return launch_select(a, (hipStream_t)stream);
 }
 
 int starkv_keep_positions(const starkv_keep_desc* d, void* stream) {
@@ -1756,8 +1782,7 @@ int starkv_keep_positions(const starkv_keep_desc* d, void* stream) {
     lower = true;
     a.off2[h] = k.head_offset2[h]; a.pitch2[h] = k.pos_stride2[h]; a.nb2[h] = (r - split + 1) / 2;
   }
-  a.units[MOVE_K1] = H;
-  a.units[MOVE_K2] = lower ? H : 0;
+  a.Hk = H;
   if (!dense) {
     a.ks1 = (uint8_t*)k.scale; a.ks1_sb = 2 * k.scale_stride_b; a.ks1_sh = 2 * k.scale_stride_h;
     a.units[MOVE_KS1] = H;
@@ -1775,12 +1800,18 @@ int starkv_keep_positions(const starkv_keep_desc* d, void* stream) {
   if (vq != VQ_DENSE) a.v[2] = {(uint8_t*)v.scale, 2 * v.scale_stride_b, 2 * v.scale_stride_s, 2 * groups};
   if (pv.x2) a.v[3] = {(uint8_t*)v.scale2, 2 * v.scale2_stride_b, 2 * v.scale2_stride_s, 2};
   if (vq == VQ_G64) a.v[4] = {(uint8_t*)v.zero, 2 * v.scale_stride_b, 2 * v.scale_stride_s, 2 * groups};
+  int nk1 = 0, nk2 = 0;
+  for (int h = 0; h < H; ++h) { nk1 = std::max(nk1, a.nb1[h]); nk2 = std::max(nk2, a.nb2[h]); }
+  a.units[MOVE_K1] = H * (int)ceil_div(nk1, MOVE_SLICE);
+  a.units[MOVE_K2] = lower ? H * (int)ceil_div(nk2, MOVE_SLICE) : 0;
+  for (int i = 0; i < MOVE_SCORES - MOVE_V; ++i) a.units[MOVE_V + i] = (int)ceil_div(a.v[i].nb, MOVE_SLICE);
   for (int i = 0; i < MOVE_SCORES - MOVE_V; ++i) {
-    a.units[MOVE_V + i] = (int)ceil_div(a.v[i].nb, MOVE_SLICE);
     if (a.v[i].nb && (a.v[i].pitch < a.v[i].nb || (many && !a.v[i].sb))) return STARKV_ERR_SHAPE;
   }
   if (d->scores) { a.scores = d->scores; a.scores_sb = d->scores_stride_b; a.units[MOVE_SCORES] = 1; }
-  return launch_move(a, d->batch, (hipStream_t)stream);
+  a.B = d->batch;
+  for (int k = 0; k < MOVE_KINDS; ++k) a.per_row += a.units[k];
+  return launch_move(a, (hipStream_t)stream);
 }
 
 // ---------------------------------------------------------------------------

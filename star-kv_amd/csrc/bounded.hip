@@ -20,6 +20,7 @@
 //    chunk's own rows are in registers before its first write.  So the move is in
 //    place without a copy of the cache, and slices run side by side.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.hpp"
 
@@ -160,6 +161,8 @@ __device__ inline uint32_t score_key(float x) {
   return u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
 }
 
+constexpr uint32_t ZERO_KEY = 0x80000000u;
+
 // inclusive sum over the wave's lanes
 __device__ inline int wave_scan(int v) {
   const int lane = threadIdx.x & 63;
@@ -171,127 +174,245 @@ __device__ inline int wave_scan(int v) {
   return v;
 }
 
-// NT: tiles of 4096 candidates held in registers (0: read again in each pass)
-template <int NT>
-__global__ __launch_bounds__(SEL_T) void select_kernel(const SelectArgs a) {
-  // four copies of each bin, a lane's by its number: equal scores (positions that
-  // never got any weight) otherwise queue 64 deep
-  __shared__ uint32_t hist[2048 * 4];
-  __shared__ int tot[2][16];
-  __shared__ int found[2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const float* x = a.scores + blockIdx.x * a.s_sb + a.sinks;
-  int* out = a.out + blockIdx.x * a.o_sb;
-  const int n = a.length - a.sinks - a.recent, need0 = a.keep - a.sinks - a.recent;
-  for (int i = tid; i < a.sinks; i += SEL_T) out[i] = i;
-  for (int i = tid; i < a.recent; i += SEL_T) out[a.keep - a.recent + i] = a.length - a.recent + i;
-  if (need0 == 0) return;
-  const int tiles = (n + SEL_TILE - 1) / SEL_TILE;
-  uint32_t held[NT ? NT : 1][4];
-  auto fetch = [&](int t, uint32_t (&k)[4]) {
-    const int p = t * SEL_TILE + 4 * tid;
-    float v[4] = {};
-    if (p + 4 <= n) {
-      load4(x + p, v);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (p + i < n) v[i] = x[p + i];
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) k[i] = score_key(v[i]);
-  };
-  if constexpr (NT > 0) {
-#pragma unroll
-    for (int t = 0; t < NT; ++t) fetch(t, held[t]);
-  }
-  // f(tile, keys) for every tile
-  auto each = [&](auto f) {
-    if constexpr (NT > 0) {
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-        if (t < tiles) f(t, held[t]);
-    } else {
-      for (int t = 0; t < tiles; ++t) {
-        uint32_t k[4];
-        fetch(t, k);
-        f(t, k);
-      }
-    }
-  };
-  uint32_t key = 0;
-  int need = need0;                                // of the keys that share the digits found so far
-  if (need0 < n) {
-#pragma unroll
-    for (int pass = 0; pass < 3; ++pass) {
-      const int low = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-      for (int i = tid; i < 2048 * 4; i += SEL_T) hist[i] = 0;
-      __syncthreads();
-      each([&](int t, const uint32_t (&k)[4]) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool in = t * SEL_TILE + 4 * tid + i < n && (pass == 0 || (k[i] >> (low + bits)) == key);
-          if (in) atomicAdd(&hist[((k[i] >> low) & ((1u << bits) - 1)) * 4 + (lane & 3)], 1u);
-        }
-      });
-      __syncthreads();
-      // thread j has bins 2047 - 2j and 2046 - 2j: sums from the largest key down
-      const uint4 hi = *(const uint4*)&hist[(2047 - 2 * tid) * 4], lo = *(const uint4*)&hist[(2046 - 2 * tid) * 4];
-      const int ch = (int)(hi.x + hi.y + hi.z + hi.w), cl = (int)(lo.x + lo.y + lo.z + lo.w);
-      int incl = wave_scan(ch + cl);
-      if (lane == 63) tot[0][wave] = incl;
-      __syncthreads();
-      for (int w = 0; w < wave; ++w) incl += tot[0][w];
-      const int before = incl - ch - cl;           // keys of larger digits
-      if (before < need && need <= incl) {
-        const bool first = need <= before + ch;
-        found[0] = first ? 2047 - 2 * tid : 2046 - 2 * tid;
-        found[1] = first ? before : before + ch;
-      }
-      __syncthreads();
-      key = (key << bits) | (uint32_t)found[0];
-      need -= found[1];
-    }
-  }
-  // positions above the key are all kept, of those at it the first `need`
-  int above = 0, at = 0;                           // of the tiles before
-  each([&](int t, const uint32_t (&k)[4]) {
-    int c = 0;
-    const int p = t * SEL_TILE + 4 * tid;
+// the keys of candidates t * 4096 + 4 tid .. + 3 of n
+__device__ inline void sel_fetch(const float* x, int n, int t, uint32_t (&k)[4]) {
+  const int p = t * SEL_TILE + 4 * threadIdx.x;
+  float v[4] = {};
+  if (p + 4 <= n) {
+    load4(x + p, v);
+  } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (p + i < n) c += k[i] > key ? 1 : k[i] == key ? 0x10000 : 0;
-    int incl = wave_scan(c);
-    if (lane == 63) tot[t & 1][wave] = incl;
+      if (p + i < n) v[i] = x[p + i];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) k[i] = score_key(v[i]);
+}
+
+constexpr int SEL_LOW[3] = {21, 10, 0}, SEL_BITS[3] = {11, 11, 10};
+struct SelShared {
+  // four copies of each bin, a lane's by its number: equal digits otherwise queue 64 deep
+  uint32_t hist[2048 * 4];
+  int tot[2][16];
+  int found[2];
+};
+
+// counts the pass's digits of a tile's keys whose earlier digits are `key`
+template <int PASS> __device__ inline void sel_count(SelShared& sh, int n, int t, const uint32_t (&k)[4], uint32_t key) {
+  constexpr int low = SEL_LOW[PASS], bits = SEL_BITS[PASS];
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool in = t * SEL_TILE + 4 * (int)threadIdx.x + i < n && (PASS == 0 || (k[i] >> (low + bits)) == key);
+    // positions that never got any weight are many, and alike: counted by the wave
+    const uint64_t zeros = __ballot(in && k[i] == ZERO_KEY);
+    if (zeros && lane == 0) atomicAdd(&sh.hist[((ZERO_KEY >> low) & ((1u << bits) - 1)) * 4], (uint32_t)__popcll(zeros));
+    if (in && k[i] != ZERO_KEY) atomicAdd(&sh.hist[((k[i] >> low) & ((1u << bits) - 1)) * 4 + (lane & 3)], 1u);
+  }
+}
+
+// The digit at which the keys counted from the largest down reach `need`, and how many lie above it: thread j brings the
+// counts of digits 2047 - 2j and 2046 - 2j
+__device__ inline void sel_find(SelShared& sh, int hi, int lo, int need) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int incl = wave_scan(hi + lo);
+  if (lane == 63) sh.tot[0][wave] = incl;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) incl += sh.tot[0][w];
+  const int before = incl - hi - lo;
+  if (before < need && need <= incl) {
+    const bool first = need <= before + hi;
+    sh.found[0] = first ? 2047 - 2 * tid : 2046 - 2 * tid;
+    sh.found[1] = first ? before : before + hi;
+  }
+  __syncthreads();
+}
+
+// Writes a tile's kept positions: those above the key, and of those at it the first `need`; above and at count the
+// tiles before
+__device__ inline void sel_write(SelShared& sh, const SelectArgs& a, int* out, int n, int t, int base, const uint32_t (&k)[4], uint32_t key,
+                                 int need, int& above, int& at) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, p = t * SEL_TILE + 4 * tid;
+  int c = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (p + i < n) c += k[i] > key ? 1 : k[i] == key ? 0x10000 : 0;
+  int incl = wave_scan(c);
+  if (lane == 63) sh.tot[t & 1][wave] = incl;
+  __syncthreads();
+  int all = 0, mine = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    if (w == wave) mine = all;
+    all += sh.tot[t & 1][w];
+  }
+  incl += mine - c;                                // before this thread, in this tile
+  int g = above + (incl & 0xffff), e = at + (incl >> 16);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (p + i >= n) continue;
+    if (k[i] > key) {
+      out[a.sinks + g + min(e, need)] = a.sinks + base + p + i;
+      ++g;
+    } else if (k[i] == key) {
+      if (e < need) out[a.sinks + g + e] = a.sinks + base + p + i;
+      ++e;
+    }
+  }
+  above += all & 0xffff;
+  at += all >> 16;
+}
+
+__device__ inline void sel_fixed(const SelectArgs& a, int* out) {
+  for (int i = threadIdx.x; i < a.sinks; i += SEL_T) out[i] = i;
+  for (int i = threadIdx.x; i < a.recent; i += SEL_T) out[a.keep - a.recent + i] = a.length - a.recent + i;
+}
+
+// all candidates or none
+__global__ __launch_bounds__(SEL_T) void select_all_kernel(const SelectArgs a) {
+  int* out = a.out + blockIdx.x * a.o_sb;
+  sel_fixed(a, out);
+  for (int i = a.sinks + threadIdx.x; i < a.keep - a.recent; i += SEL_T) out[i] = i;
+}
+
+// One workgroup a row, its NT tiles of 4096 candidates in registers
+template <int NT>
+__global__ __launch_bounds__(SEL_T) void select_kernel(const SelectArgs a) {
+  __shared__ SelShared sh;
+  const int tid = threadIdx.x;
+  const float* x = a.scores + blockIdx.x * a.s_sb + a.sinks;
+  int* out = a.out + blockIdx.x * a.o_sb;
+  const int n = a.length - a.sinks - a.recent, need0 = a.keep - a.sinks - a.recent, tiles = (n + SEL_TILE - 1) / SEL_TILE;
+  sel_fixed(a, out);
+  uint32_t held[NT][4];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) sel_fetch(x, n, t, held[t]);
+  uint32_t key = 0;
+  int need = need0;                                // of the keys that share the digits found so far
+  auto pass = [&](auto P) {
+    constexpr int p = decltype(P)::value;
+    for (int i = tid; i < 2048 * 4; i += SEL_T) sh.hist[i] = 0;
     __syncthreads();
-    int all = 0, mine = 0;
 #pragma unroll
-    for (int w = 0; w < 16; ++w) {
-      if (w == wave) mine = all;
-      all += tot[t & 1][w];
-    }
-    incl += mine - c;                              // before this thread, in this tile
-    int g = above + (incl & 0xffff), e = at + (incl >> 16);
+    for (int t = 0; t < NT; ++t)
+      if (t < tiles) sel_count<p>(sh, n, t, held[t], key);
+    __syncthreads();
+    const uint4 hi = *(const uint4*)&sh.hist[(2047 - 2 * tid) * 4], lo = *(const uint4*)&sh.hist[(2046 - 2 * tid) * 4];
+    sel_find(sh, (int)(hi.x + hi.y + hi.z + hi.w), (int)(lo.x + lo.y + lo.z + lo.w), need);
+    key = (key << SEL_BITS[p]) | (uint32_t)sh.found[0];
+    need -= sh.found[1];
+  };
+  pass(std::integral_constant<int, 0>());
+  pass(std::integral_constant<int, 1>());
+  pass(std::integral_constant<int, 2>());
+  int above = 0, at = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (p + i >= n) continue;
-      if (k[i] > key) {
-        out[a.sinks + g + min(e, need)] = a.sinks + p + i;
-        ++g;
-      } else if (k[i] == key) {
-        if (e < need) out[a.sinks + g + e] = a.sinks + p + i;
-        ++e;
-      }
+  for (int t = 0; t < NT; ++t)
+    if (t < tiles) sel_write(sh, a, out, n, t, 0, held[t], key, need, above, at);
+}
+
+// Long rows: a workgroup counts the digits of a piece (its own histogram in memory, no atomics between workgroups); the
+// next launch adds the pieces up, finds the digit and counts the next; the last finds its place from the histograms of
+// the pieces before it, and writes.  state[row][pass]: (key so far, keys still needed at it).
+template <int PASS>
+__device__ inline void sel_join(SelShared& sh, const SelectArgs& a, int need0, uint32_t& key, int& need) {
+  const int tid = threadIdx.x, row = blockIdx.y;
+  key = 0;
+  need = need0;
+  if constexpr (PASS > 1) { const int2 s = a.state[row * 3 + PASS - 2]; key = (uint32_t)s.x; need = s.y; }
+  const uint2* h = (const uint2*)(a.hist + ((int64_t)(PASS - 1) * a.B + row) * a.pieces * 2048) + (1023 - tid);
+  int hi = 0, lo = 0;
+#pragma unroll 8
+  for (int i = 0; i < a.pieces; ++i) {
+    const uint2 v = h[(int64_t)i * 1024];          // digits 2046 - 2 tid, 2047 - 2 tid
+    lo += (int)v.x;
+    hi += (int)v.y;
+  }
+  sel_find(sh, hi, lo, need);
+  key = (key << SEL_BITS[PASS - 1]) | (uint32_t)sh.found[0];
+  need -= sh.found[1];
+  if (blockIdx.x == 0 && tid == 0) a.state[row * 3 + PASS - 1] = make_int2((int)key, need);
+}
+
+// f(tile, keys) for the tiles of a piece, two asked for at a time under the work of the two before
+template <typename F> __device__ inline void sel_each(const float* x, int n, F f) {
+  const int tiles = (n + SEL_TILE - 1) / SEL_TILE;
+  uint32_t k[2][4], cur[2][4];
+  sel_fetch(x, n, 0, k[0]);
+  sel_fetch(x, n, 1, k[1]);
+  for (int t = 0; t < tiles; t += 2) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) cur[i][j] = k[i][j];
+      sel_fetch(x, n, t + 2 + i, k[i]);
     }
-    above += all & 0xffff;
-    at += all >> 16;
-  });
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (t + i < tiles) f(t + i, cur[i]);
+  }
+}
+
+template <int PASS>
+__global__ __launch_bounds__(SEL_T) void select_count_kernel(const SelectArgs a) {
+  __shared__ SelShared sh;
+  const int tid = threadIdx.x, row = blockIdx.y, n = a.length - a.sinks - a.recent, p0 = blockIdx.x * a.piece_len;
+  uint32_t key = 0;
+  int need;
+  if constexpr (PASS > 0) sel_join<PASS>(sh, a, a.keep - a.sinks - a.recent, key, need);
+  for (int i = tid; i < 2048 * 4; i += SEL_T) sh.hist[i] = 0;
+  __syncthreads();
+  const int m = min(a.piece_len, n - p0);
+  sel_each(a.scores + row * a.s_sb + a.sinks + p0, m, [&](int t, const uint32_t (&k)[4]) { sel_count<PASS>(sh, m, t, k, key); });
+  __syncthreads();
+  uint2* out = (uint2*)(a.hist + (((int64_t)PASS * a.B + row) * a.pieces + blockIdx.x) * 2048) + tid;
+  const uint4 lo = *(const uint4*)&sh.hist[tid * 8], hi = *(const uint4*)&sh.hist[tid * 8 + 4];
+  *out = make_uint2(lo.x + lo.y + lo.z + lo.w, hi.x + hi.y + hi.z + hi.w);
+}
+
+__global__ __launch_bounds__(SEL_T) void select_write_kernel(const SelectArgs a) {
+  __shared__ SelShared sh;
+  const int tid = threadIdx.x, row = blockIdx.y, n = a.length - a.sinks - a.recent, p0 = blockIdx.x * a.piece_len;
+  int* out = a.out + row * a.o_sb;
+  if (blockIdx.x == 0) sel_fixed(a, out);
+  uint32_t key;
+  int need;
+  sel_join<3>(sh, a, a.keep - a.sinks - a.recent, key, need);
+  // keys above the threshold, and at it, in the pieces before
+  int above = 0, at = 0;
+#pragma unroll
+  for (int pass = 0; pass < 3; ++pass) {
+    const int digit = (int)((key >> SEL_LOW[pass]) & ((1u << SEL_BITS[pass]) - 1));
+    const uint2* h = (const uint2*)(a.hist + ((int64_t)pass * a.B + row) * a.pieces * 2048) + tid;
+#pragma unroll 4
+    for (int i = 0; i < (int)blockIdx.x; ++i) {
+      const uint2 v = h[(int64_t)i * 1024];
+      above += (2 * tid > digit ? (int)v.x : 0) + (2 * tid + 1 > digit ? (int)v.y : 0);
+      if (pass == 2) at += (2 * tid == digit ? (int)v.x : 0) + (2 * tid + 1 == digit ? (int)v.y : 0);
+    }
+  }
+  __syncthreads();
+  sh.hist[tid] = (uint32_t)above;
+  sh.hist[SEL_T + tid] = (uint32_t)at;
+  __syncthreads();
+  for (int w = SEL_T / 2; w >= 1; w >>= 1) {
+    if (tid < w) {
+      sh.hist[tid] += sh.hist[tid + w];
+      sh.hist[SEL_T + tid] += sh.hist[SEL_T + tid + w];
+    }
+    __syncthreads();
+  }
+  above = (int)sh.hist[0];
+  at = (int)sh.hist[SEL_T];
+  const int m = min(a.piece_len, n - p0);
+  sel_each(a.scores + row * a.s_sb + a.sinks + p0, m,
+           [&](int t, const uint32_t (&k)[4]) { sel_write(sh, a, out, m, t, p0, k, key, need, above, at); });
 }
 
 // ---------------------------------------------------------------------------
 // Moving rows
 // ---------------------------------------------------------------------------
-constexpr int MOVE_U = 8;                          // pieces in flight per thread
+constexpr int MOVE_U = 8, MOVE_T = 1024;           // pieces in flight per thread, threads
 typedef uint32_t piece16 __attribute__((ext_vector_type(4)));
 typedef uint32_t piece8 __attribute__((ext_vector_type(2)));
 
@@ -305,32 +426,60 @@ __device__ inline void move_rows(const MoveArgs& a, const int* pos, uint8_t* bas
   typedef P Q __attribute__((aligned(1)));
   const int tid = threadIdx.x, np = (w + (int)sizeof(P) - 1) / (int)sizeof(P);
   const int sh = np <= 1 ? 0 : 32 - __builtin_clz(np - 1);          // lanes of a row: np rounded up to 2^sh
-  const int c = tid & ((1 << sh) - 1), r = tid >> sh, rp = 256 >> sh;
+  const int c = tid & ((1 << sh) - 1), r = tid >> sh, rp = MOVE_T >> sh;
   const int off = min(c * (int)sizeof(P), w - (int)sizeof(P));
-  for (int i0 = 0; i0 < a.keep; i0 += MOVE_U * rp) {
-    P v[MOVE_U];
-    bool ok[MOVE_U];
+  const int n = MOVE_U * rp;                       // rows of a chunk
+  P v[2][MOVE_U];
+  int pos_of[2][MOVE_U];                           // where row i comes from; i itself: it stays
+  auto places = [&](int i0, int (&p)[MOVE_U]) {
 #pragma unroll
     for (int u = 0; u < MOVE_U; ++u) {
       const int i = i0 + u * rp + r;
-      const int p = i < a.keep ? pos[i] : i;
-      const bool in = p >= i && p < a.length;
-      if (i < a.keep && !in && a.err != nullptr) *a.err = 1;
-      ok[u] = c < np && in && p != i && i < a.keep;
-      if (ok[u]) v[u] = *(const Q*)(base + (int64_t)p * pitch + off);
+      p[u] = i < a.keep ? pos[i] : i;
     }
-    loads_done();                                  // of the whole workgroup: the writes begin
-    __syncthreads();
+  };
+  auto load = [&](int i0, int (&p)[MOVE_U], P (&to)[MOVE_U]) {
 #pragma unroll
-    for (int u = 0; u < MOVE_U; ++u)
-      if (ok[u]) *(Q*)(base + (int64_t)(i0 + u * rp + r) * pitch + off) = v[u];
+    for (int u = 0; u < MOVE_U; ++u) {
+      const int i = i0 + u * rp + r;
+      if (i < a.keep && (p[u] < i || p[u] >= a.length)) {
+        if (a.err != nullptr) *a.err = 1;
+        p[u] = i;
+      }
+      if (c >= np) p[u] = i;
+      if (p[u] != i) to[u] = *(const Q*)(base + (int64_t)p[u] * pitch + off);
+    }
+  };
+  // a chunk's rows are asked for a chunk ahead, its positions two
+  places(0, pos_of[0]);
+  load(0, pos_of[0], v[0]);
+  places(n, pos_of[1]);
+  for (int i0 = 0; i0 < a.keep; i0 += 2 * n) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int at = i0 + s * n;
+      if (at >= a.keep) break;
+      loads_done();                                // of the whole workgroup: the chunk's writes begin
+      __syncthreads();
+      load(at + n, pos_of[s ^ 1], v[s ^ 1]);
+      bool moved[MOVE_U];
+#pragma unroll
+      for (int u = 0; u < MOVE_U; ++u) moved[u] = pos_of[s][u] != at + u * rp + r;
+      places(at + 2 * n, pos_of[s]);
+#pragma unroll
+      for (int u = 0; u < MOVE_U; ++u)
+        if (moved[u]) *(Q*)(base + (int64_t)(at + u * rp + r) * pitch + off) = v[s][u];
+    }
   }
 }
 
-__global__ __launch_bounds__(256) void move_kernel(const MoveArgs a) {
-  const int b = blockIdx.y;
+__global__ __launch_bounds__(MOVE_T) void move_kernel(const MoveArgs a) {
+  // a row's slices on one XCD: the lines that two of them share are read, and written back, once
+  int unit = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3), kind = 0;
+  const int b = unit / a.per_row;
+  if (b >= a.B) return;
+  unit %= a.per_row;
   const int* pos = a.pos + b * a.p_sb;
-  int unit = blockIdx.x, kind = 0;
   while (unit >= a.units[kind]) unit -= a.units[kind++];
   uint8_t* base;
   int64_t pitch;
@@ -340,22 +489,21 @@ __global__ __launch_bounds__(256) void move_kernel(const MoveArgs a) {
     move_rows<uint32_t>(a, pos, (uint8_t*)s, 4, 4);
     loads_done();
     __syncthreads();
-    for (int i = a.keep + threadIdx.x; i < a.length; i += 256) s[i] = 0.f;
+    for (int i = a.keep + threadIdx.x; i < a.length; i += MOVE_T) s[i] = 0.f;
     return;
   }
-  if (kind < MOVE_V) {
-    const int h = unit;
-    const bool second = kind == MOVE_K2 || kind == MOVE_KS2;
-    if (kind == MOVE_K1 || kind == MOVE_K2) {
-      base = (second ? a.k2 + b * a.k2_sb + a.off2[h] : a.k1 + b * a.k1_sb + a.off1[h]);
-      pitch = second ? a.pitch2[h] : a.pitch1[h];
-      nb = second ? a.nb2[h] : a.nb1[h];
-      if (nb == 0) return;
-    } else {
-      base = second ? a.ks2 + b * a.ks2_sb + h * a.ks2_sh : a.ks1 + b * a.ks1_sb + h * a.ks1_sh;
-      pitch = 2;
-      nb = 2;
-    }
+  if (kind == MOVE_K1 || kind == MOVE_K2) {
+    const int h = unit % a.Hk;
+    const bool second = kind == MOVE_K2;
+    base = second ? a.k2 + b * a.k2_sb + a.off2[h] : a.k1 + b * a.k1_sb + a.off1[h];
+    pitch = second ? a.pitch2[h] : a.pitch1[h];
+    nb = second ? a.nb2[h] : a.nb1[h];
+    slice = unit / a.Hk * MOVE_SLICE;
+    if (slice >= nb) return;
+  } else if (kind < MOVE_V) {
+    base = kind == MOVE_KS2 ? a.ks2 + b * a.ks2_sb + unit * a.ks2_sh : a.ks1 + b * a.ks1_sb + unit * a.ks1_sh;
+    pitch = 2;
+    nb = 2;
   } else {
     const MoveRows& v = a.v[kind - MOVE_V];
     base = v.base + b * v.sb;
@@ -393,21 +541,35 @@ int launch_scores(const ScoreArgs& a, int dtype, bool fused, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
-int launch_select(const SelectArgs& a, int B, hipStream_t st) {
-  const int tiles = (int)ceil_div(a.length - a.sinks - a.recent, SEL_TILE);
-  const dim3 grid((unsigned)B), block(SEL_T);
-  if (tiles <= 1) hipLaunchKernelGGL(select_kernel<1>, grid, block, 0, st, a);
-  else if (tiles <= 4) hipLaunchKernelGGL(select_kernel<4>, grid, block, 0, st, a);
-  else if (tiles <= 8) hipLaunchKernelGGL(select_kernel<8>, grid, block, 0, st, a);
-  else hipLaunchKernelGGL(select_kernel<0>, grid, block, 0, st, a);
+// Candidates per workgroup of a long row: at least 8192, at most 64 pieces; 0: one workgroup takes the row
+int select_piece(int n, int keep_of_them) {
+  if (n <= 8 * SEL_TILE || keep_of_them == 0 || keep_of_them == n) return 0;
+  return (int)round_up(std::max<int64_t>(8192, ceil_div(n, 64)), SEL_TILE);
+}
+
+int launch_select(const SelectArgs& a, hipStream_t st) {
+  const int n = a.length - a.sinks - a.recent, need = a.keep - a.sinks - a.recent, tiles = (int)ceil_div(n, SEL_TILE);
+  const dim3 grid((unsigned)a.B), block(SEL_T);
+  if (a.piece_len) {
+    const dim3 pieces((unsigned)a.pieces, (unsigned)a.B);
+    hipLaunchKernelGGL(select_count_kernel<0>, pieces, block, 0, st, a);
+    hipLaunchKernelGGL(select_count_kernel<1>, pieces, block, 0, st, a);
+    hipLaunchKernelGGL(select_count_kernel<2>, pieces, block, 0, st, a);
+    hipLaunchKernelGGL(select_write_kernel, pieces, block, 0, st, a);
+  } else if (need == 0 || need == n) {
+    hipLaunchKernelGGL(select_all_kernel, grid, block, 0, st, a);
+  } else if (tiles <= 1) {
+    hipLaunchKernelGGL(select_kernel<1>, grid, block, 0, st, a);
+  } else if (tiles <= 4) {
+    hipLaunchKernelGGL(select_kernel<4>, grid, block, 0, st, a);
+  } else {
+    hipLaunchKernelGGL(select_kernel<8>, grid, block, 0, st, a);
+  }
   return (int)hipGetLastError();
 }
 
-int launch_move(const MoveArgs& a, int B, hipStream_t st) {
-  int n = 0;
-  for (int k = 0; k < MOVE_KINDS; ++k) n += a.units[k];
-  if (n == 0) return 0;
-  hipLaunchKernelGGL(move_kernel, dim3((unsigned)n, (unsigned)B), dim3(256), 0, st, a);
+int launch_move(const MoveArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL(move_kernel, dim3((unsigned)round_up((int64_t)a.per_row * a.B, 8)), dim3(MOVE_T), 0, st, a);
   return (int)hipGetLastError();
 }
 

@@ -339,15 +339,20 @@ struct ScoreArgs {
 struct SelectArgs {
   const float* scores; int64_t s_sb;
   int* out; int64_t o_sb;
-  int length, keep, sinks, recent;
+  int length, keep, sinks, recent, B;
+  int piece_len, pieces;                           // long rows: candidates of a workgroup
+  uint32_t* hist; int2* state;                     // ... [3][B][pieces][2048], [B][3]
 };
-constexpr int MOVE_SLICE = 256;                    // bytes of a row per workgroup
+// Bytes of a row per workgroup: more workgroups against lines shared by two of them.  4 x 32768 positions to 8192, 32 heads
+// of 51 ranks 192 bytes apart, V 1640: 187 us by 128, 185 by 256; one such sequence 48 and 65; 8 int8 / int4 ones of 8449 to
+// 2048 31 and 36.
+constexpr int MOVE_SLICE = 128;
 // what a workgroup moves: K rows (both blocks) and their scales by head, V rows and their scales by slice, scores
 constexpr int MOVE_K1 = 0, MOVE_K2 = 1, MOVE_KS1 = 2, MOVE_KS2 = 3, MOVE_V = 4, MOVE_SCORES = 9, MOVE_KINDS = 10;
 struct MoveRows { uint8_t* base; int64_t sb, pitch; int nb; };           // bytes
 struct MoveArgs {
   const int* pos; int64_t p_sb;
-  int keep, length;
+  int keep, length, Hk;
   int* err;                                        // optional: set to 1 where a position is none
   uint8_t* k1; int64_t k1_sb;
   uint8_t* k2; int64_t k2_sb;
@@ -357,7 +362,7 @@ struct MoveArgs {
   int nb1[K_MAX_KV], nb2[K_MAX_KV];
   MoveRows v[MOVE_SCORES - MOVE_V];                // data, data2, scale, scale2, zero
   float* scores; int64_t scores_sb;
-  int units[MOVE_KINDS];                           // workgroups of each kind
+  int units[MOVE_KINDS], per_row, B;               // workgroups of each kind, of a sequence
 };
 
 // ---------------------------------------------------------------------------
@@ -567,8 +572,9 @@ int up_slice_width(int n_kv, int Rv, int cus);        // V-rank columns per up-p
 int up_chunk_sets(int n_kv, int n_sl, int n_c2, int cus);   // chunk sets per (slice, KV head)
 int score_pieces(int S);                              // pieces of a logit row: their statistics are 8 bytes each
 int launch_scores(const ScoreArgs& a, int dtype, bool fused, hipStream_t st);
-int launch_select(const SelectArgs& a, int B, hipStream_t st);
-int launch_move(const MoveArgs& a, int B, hipStream_t st);
+int select_piece(int n, int keep_of_them);
+int launch_select(const SelectArgs& a, hipStream_t st);
+int launch_move(const MoveArgs& a, hipStream_t st);
 int launch_prefix_pack(const PrefixPackArgs& a, int dtype, hipStream_t st);
 int launch_prefix_logits(const PrefixArgs& a, int dtype, hipStream_t st);
 int launch_own_logits(const PrefixArgs& a, int dtype, hipStream_t st);

@@ -285,7 +285,7 @@ EXPORTS = (
     "starkv_fp8_quantize", "starkv_fp8_gemm_workspace_bytes", "starkv_fp8_gemm",
     "starkv_token_logprobs_workspace_bytes", "starkv_token_logprobs",
     "starkv_attention_scores_workspace_bytes", "starkv_attention_scores", "starkv_decode_attention_scores",
-    "starkv_select_positions", "starkv_keep_positions",
+    "starkv_select_positions_workspace_bytes", "starkv_select_positions", "starkv_keep_positions",
     "starkv_prefix_bytes", "starkv_prefix_pack", "starkv_prefix_decode_workspace_bytes", "starkv_prefix_decode",
 )
 
@@ -355,10 +355,11 @@ def lib() -> ctypes.CDLL:
                                                  ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
     L.starkv_prefix_bytes.restype = ctypes.c_size_t
     L.starkv_prefix_bytes.argtypes = [ctypes.POINTER(PrefixPackDesc)]
-    for name, desc in (("select_positions", SelectDesc), ("keep_positions", KeepDesc), ("prefix_pack", PrefixPackDesc)):
+    for name, desc in (("keep_positions", KeepDesc), ("prefix_pack", PrefixPackDesc)):
         f = getattr(L, f"starkv_{name}")
         f.restype, f.argtypes = ctypes.c_int, [ctypes.POINTER(desc), ctypes.c_void_p]
     for name, desc in (("fp8_gemm", Fp8GemmDesc), ("token_logprobs", LogprobsDesc), ("attention_scores", ScoresDesc),
+                       ("select_positions", SelectDesc),
                        ("prefix_decode", PrefixDecodeDesc)):
         wsf, f = getattr(L, f"starkv_{name}_workspace_bytes"), getattr(L, f"starkv_{name}")
         wsf.restype, f.restype = ctypes.c_size_t, ctypes.c_int
@@ -374,9 +375,22 @@ def check(status: int, what: str) -> None:
         raise StarKVError(f"{what} failed with status {status}: {msg}")
 
 
+_ARRAYS: dict = {}                    # (element type, length) -> array type: making one costs more than filling it
+
+
+def _array(ctype, vals):
+    t = _ARRAYS.get((ctype, len(vals)))
+    if t is None:
+        t = _ARRAYS[ctype, len(vals)] = ctype * len(vals)
+    try:
+        return t(*vals)
+    except TypeError:                 # numbers of other types
+        return t(*map(int, vals))
+
+
 def i64_array(vals):
-    return (ctypes.c_int64 * len(vals))(*[int(v) for v in vals])
+    return _array(ctypes.c_int64, vals)
 
 
 def int_array(vals):
-    return (ctypes.c_int * len(vals))(*[int(v) for v in vals])
+    return _array(ctypes.c_int, vals)

@@ -134,19 +134,19 @@ class KLatentSpec:
                  pos_stride2: Optional[Sequence[int]] = None, stride2_b: int = 0,
                  scale2: Optional[torch.Tensor] = None, scale2_stride_b: int = 0, scale2_stride_h: int = 0):
         self.data, self.bk, self.scale = data, bk, scale
-        self.ranks = [int(r) for r in ranks]
-        self.head_offset = [int(v) for v in head_offset]
-        self.pos_stride = [int(v) for v in pos_stride]
+        self.ranks = list(map(int, ranks))
+        self.head_offset = list(map(int, head_offset))
+        self.pos_stride = list(map(int, pos_stride))
         self.stride_b = int(stride_b)
-        self.bk_head_offset = [int(v) for v in bk_head_offset]
+        self.bk_head_offset = list(map(int, bk_head_offset))
         self.bk_row_stride = int(bk_row_stride)
         self.fmt = fmt
         self.scale_stride_b, self.scale_stride_h = int(scale_stride_b), int(scale_stride_h)
         self.split, self.split_fmt = int(split), split_fmt
         self.data2, self.scale2 = data2, scale2
         n = len(self.ranks)
-        self.head_offset2 = [int(v) for v in (head_offset2 or [0] * n)]
-        self.pos_stride2 = [int(v) for v in (pos_stride2 or [0] * n)]
+        self.head_offset2 = list(map(int, head_offset2)) if head_offset2 else [0] * n
+        self.pos_stride2 = list(map(int, pos_stride2)) if pos_stride2 else [0] * n
         self.stride2_b = int(stride2_b)
         self.scale2_stride_b, self.scale2_stride_h = int(scale2_stride_b), int(scale2_stride_h)
 

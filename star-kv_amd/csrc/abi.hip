@@ -63,8 +63,11 @@ int device_cus() {
 int choose_splits(int64_t groups, int slots, int n_units, int max_n, double c0, double frac_per_split) {
   int best = 1;
   double best_t = 1e300;
+  int last = 0;
   for (int n = 1; n <= std::max(1, std::min(max_n, n_units)); ++n) {
-    const int len = (int)ceil_div(n_units, n);
+    const int len = (n_units + n - 1) / n;
+    if (len == last) continue;                     // the same plan again
+    last = len;
     const int ne = (int)ceil_div(n_units, len);
     const int64_t rounds = ceil_div(groups * ne, slots);
     const double t = (double)rounds * (len + c0) * (1.0 + frac_per_split * ne);
@@ -1871,19 +1874,23 @@ struct PrefixLayout {
   DecodeLayout own;
   PrefixSpace space;
   bool has_own, own_here;
-  int oc_len, gs, M, Mp, bm, tiles_m, tiles_n, n_split, sp_len, n_ch, ch_len, n_hg, sw, n_sl;
-  size_t off_p, off_stat, off_cmax, off_rmax, off_part, off_lsum, off_jpart, off_jsum, off_jmax, off_ypart, total;
+  int oc_len, gs, M, Mp, bm, tiles_m, tiles_n, n_split, sp_len, n_ch, ch_len, n_hg, sc, n_sl;
+  size_t off_p, off_stat, off_cmax, off_rmax, off_part, off_lsum, off_jsum, off_jmax, off_ypart, total;
 };
 
-// Strips per P V split: the least modelled time, rounds of one workgroup a CU, each its strips and a fixed time, times the
-// share of the splits' partials (a round of workgroups that is hardly begun costs as much as a full one: 65536 positions of
-// 512 rows in 19 splits of 14 tiles ran 198 us, in 36 161, in 18 SPLIT18).
+// Strips per P V split: the least modelled time in strips (about 1 us each), rounds of one workgroup a CU, each its strips
+// and a fixed time, and 0.12 for each split that the join adds up.  A round of workgroups that is hardly begun costs as
+// much as a full one (65536 positions of 512 rows in 19 splits of 14 tiles: 198 us, in 36 161, in 18 152); 16384 of 128 rows
+// in 128 splits of 2 tiles: 14 us and 22 for the join, in 64 14 and 17.
 int prefix_split_len(int tiles, int cus, int strips) {
   int best = 0;
   double least = 0;
-  for (int len = 1; len <= strips; ++len) {
+  // as many splits as whole rounds hold, and halves and quarters of a round
+  for (int quarters = 1; quarters <= 32; quarters = quarters < 4 ? 2 * quarters : quarters + 4) {
+    const int want = (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)quarters * cus / 4 / tiles, PX_MAX_SPLITS));
+    const int len = (int)ceil_div(strips, want);
     const int64_t n = ceil_div(strips, len);
-    const double t = (double)ceil_div(tiles * n, cus) * (len + 3.0) * (1.0 + 0.004 * std::min<int64_t>(n, 64));
+    const double t = (double)ceil_div(tiles * n, cus) * (len + 3.0) + 0.12 * (double)n;
     if (!best || t < least * 0.9999) { best = len; least = t; }
   }
   return best;
@@ -1937,8 +1944,10 @@ int prefix_layout(const starkv_prefix_decode_desc* d, PrefixLayout& L) {
   L.ch_len = (int)round_up(ceil_div(strips, want), 8);
   L.n_ch = (int)ceil_div(strips, L.ch_len);
   L.n_hg = head_groups(Hq);
-  L.sw = up_slice_width(d->n_kv_heads, d->v_rank, cus);
-  L.n_sl = (int)ceil_div(d->v_rank, L.sw);
+  // columns of an up-projection workgroup: wide ones read whole lines of the partials, narrow ones fill the CUs
+  const int64_t row_blocks = (int64_t)d->n_kv_heads * ceil_div((int64_t)B * L.gs, 32);
+  L.sc = row_blocks * ceil_div(d->v_rank, 128) >= cus ? 128 : row_blocks * ceil_div(d->v_rank, 64) >= cus ? 64 : 32;
+  L.n_sl = (int)ceil_div(d->v_rank, L.sc);
   const size_t BQ = (size_t)B * L.n_hg, Mp = L.Mp;
   size_t off = L.has_own ? L.own.total : 0;
   auto take = [&](size_t& at, size_t n) { at = off; off = a256(off + n); };
@@ -1949,10 +1958,9 @@ int prefix_layout(const starkv_prefix_decode_desc* d, PrefixLayout& L) {
   take(L.off_rmax, Mp * 4);
   take(L.off_part, (size_t)L.n_split * L.M * Rvp * 2);
   take(L.off_lsum, (size_t)L.n_split * Mp * 4);
-  take(L.off_jpart, BQ * 32 * Rvp * 4);
   take(L.off_jsum, BQ * 32 * 4);
   take(L.off_jmax, (size_t)L.M * 4);
-  take(L.off_ypart, (size_t)d->n_kv_heads * L.n_sl * ((size_t)B * L.gs) * HEAD_DIM * 4);
+  take(L.off_ypart, (size_t)L.n_sl * L.M * HEAD_DIM * 4);
   L.total = off;
   return STARKV_OK;
 }
@@ -2024,7 +2032,9 @@ int starkv_prefix_decode(const starkv_prefix_decode_desc* d, void* workspace, si
   a.cmax = (float*)(ws + L.off_cmax); a.n_ch = L.n_ch; a.ch_len = L.ch_len; a.rmax = (float*)(ws + L.off_rmax);
   a.bm = L.bm; a.tiles_m = L.tiles_m; a.tiles_n = L.tiles_n; a.n_split = L.n_split; a.sp_len = L.sp_len;
   a.part = (_Float16*)(ws + L.off_part); a.lsum = (float*)(ws + L.off_lsum);
-  a.n_hg = L.n_hg; a.jpart = (float*)(ws + L.off_jpart); a.jsum = (float*)(ws + L.off_jsum);
+  a.n_hg = L.n_hg; a.jsum = (float*)(ws + L.off_jsum);
+  a.uv = o.uv; a.uv_rs = o.uv_row_stride; a.Rv = d->v_rank; a.sc = L.sc; a.n_sl = L.n_sl; a.ypart = (float*)(ws + L.off_ypart);
+  a.out = o.out; a.o_sb = o.out_stride_b; a.o_sh = o.out_stride_h;
   a.jmax = score ? (float*)(ws + L.off_jmax) : nullptr;
   if (L.has_own) {
     a.own_max = (float*)(ws + L.own.off_cmax); a.own_sum = (const float*)(ws + L.own.off_psum);
@@ -2046,15 +2056,7 @@ int starkv_prefix_decode(const starkv_prefix_decode_desc* d, void* workspace, si
   if ((st = launch_prefix_logits(a, o.dtype, s))) return st;
   PVArgs pa;
   if (L.has_own && (st = decode_pv(&o, L.own, ws, s, pa))) return st;
-  if ((st = launch_prefix_pv(a, s)) || (st = launch_prefix_join(a, s))) return st;
-  UPArgs ua;
-  ua.part = a.jpart; ua.psum = a.jsum; ua.part16 = 0; ua.n_c2 = 1; ua.Rvp = a.Rvp; ua.n_hg = L.n_hg;
-  ua.uv = o.uv; ua.uv_rs = o.uv_row_stride;
-  ua.out = o.out; ua.o_sb = o.out_stride_b; ua.o_sh = o.out_stride_h;
-  ua.B = o.batch; ua.Hq = o.n_q_heads; ua.gs = L.gs; ua.Rv = d->v_rank;
-  ua.sw = L.sw; ua.n_sl = L.n_sl; ua.n_cs = 1; ua.ypart = (float*)(ws + L.off_ypart);
-  ua.out_f32 = o.out_dtype == STARKV_F32;
-  if ((st = launch_up_proj(ua, o.dtype, al(o.uv, 16) && al64(o.uv_row_stride * 2, 16), s))) return st;
+  if ((st = launch_prefix_pv(a, s)) || (st = launch_prefix_up(a, o.dtype, o.out_dtype == STARKV_F32, s))) return st;
   if (score) return decode_scores(&o, L.own, ws, a.jmax, 1, a.jsum, 1, d->scores, d->scores_stride_b, s);
   return STARKV_OK;
 }

@@ -371,6 +371,7 @@ struct MoveArgs {
 constexpr int PX_STRIP = 64;                       // positions of a strip
 constexpr int PX_GROUPS = 2;                       // groups of 32 query rows that a logits workgroup holds
 constexpr int PX_BN = 256;                         // columns of a P V workgroup
+constexpr int PX_MAX_SPLITS = 256;                 // of P V: their weights lie in LDS
 constexpr int PX_HEAD_BYTES = 256;                 // (K multiplier, V multiplier), largest magnitudes
 struct PrefixPackArgs {
   const void* k; const void* bk; const void* v;    // dense latents of one sequence, act dtype, strides in elements
@@ -405,7 +406,12 @@ struct PrefixArgs {
   const void* mask; int64_t m_sb, m_sh; int mask_dtype;
   const int* last_pos;
   float* ol; int64_t ol_sb, ol_st;                 // logits [b][32 positions][Hq][32]
-  float* jpart; float* jsum; float* jmax;          // joined [B*n_hg][32][Rvp], [B*n_hg][32], optional [B][Hq]
+  // joined: sums [B*n_hg][32] and maxima [B][Hq] where scores are wanted; products by column slice [n_sl][M][128]
+  float* jsum; float* jmax;
+  const void* uv; int64_t uv_rs;
+  int Rv, sc, n_sl;                                // columns of a slice, slices
+  float* ypart;
+  void* out; int64_t o_sb, o_sh;
 };
 
 // A decode step's cache writes and query rotation in one launch (quant.hip)
@@ -579,7 +585,7 @@ int launch_prefix_pack(const PrefixPackArgs& a, int dtype, hipStream_t st);
 int launch_prefix_logits(const PrefixArgs& a, int dtype, hipStream_t st);
 int launch_own_logits(const PrefixArgs& a, int dtype, hipStream_t st);
 int launch_prefix_pv(const PrefixArgs& a, hipStream_t st);
-int launch_prefix_join(const PrefixArgs& a, hipStream_t st);
+int launch_prefix_up(const PrefixArgs& a, int dtype, bool out_f32, hipStream_t st);
 int launch_fill_i32(int* p, int n, int v, hipStream_t st);
 int launch_k_append(const KAppendArgs& a, int dtype, hipStream_t st);
 int launch_v_append(const VAppendArgs& a, int dtype, hipStream_t st);

@@ -25,9 +25,10 @@
 //    row's largest weight still keep all bits of fp16.  Each split's sums leave
 //    divided by its weights' sum, in fp16 (half of them: a mean of values up to
 //    65504 that is rounded up stays finite).
-// 3. prefix_join_kernel adds the splits and, if the sequences have positions of
+// 3. prefix_up_kernel adds the splits and, if the sequences have positions of
 //    their own, the decode kernels' sums over those, in a fixed order, relative to
-//    the larger of the two maxima; the decode's up-projection ends the call.
+//    the larger of the two maxima, and multiplies them by U_v; prefix_finish_kernel
+//    adds the products of its column slices.
 //
 // Range: queries are scaled by a power of two to [1, 2) per row, K latents by one
 // that bounds every key by 2^15, bf16 value latents by one that brings the largest
@@ -117,6 +118,12 @@ __global__ __launch_bounds__(256) void px_amax_kernel(const PrefixPackArgs a) {
 
 // 2^e, |e| <= 126
 __device__ inline float pow2f(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
+// exponent that brings a row's largest magnitude (its bits) to [2^14, 2^15)
+__device__ inline int px_row_exp(uint32_t top) {
+  const int e = (int)(top >> 23) - 141;
+  return top == 0 || top >= 0x7f800000u ? 0 : max(e, -112);
+}
 
 // exponent by which K latents are scaled down: |K| <= bound = |X| |B_k| ranks sqrt 2 (the rotation) becomes at most 2^15
 __device__ inline int px_k_exp(const PrefixPackArgs& a) {
@@ -704,72 +711,195 @@ __global__ __launch_bounds__(512, 2) void prefix_pv_kernel(const PrefixArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Join: row (b, q)'s sums over the prefix's splits and over its own positions' chunks
+// Join and up-projection
 // ---------------------------------------------------------------------------
-// Workgroup = (row, 512 columns), a lane 8 columns, wave w splits and chunks w, w + 4, ...
-__global__ __launch_bounds__(256) void prefix_join_kernel(const PrefixArgs a) {
-  __shared__ float red[3][64][9];
-  const int row = blockIdx.x, nr = a.B * a.gs, h = row / nr, b = row % nr / a.gs, q = h * a.gs + row % a.gs;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t bq = (int64_t)b * a.n_hg + (q >> 5);
-  const float mp = a.rmax[row];
-  float ms = -INFINITY;                            // in units of log 2, as the prefix's
-  for (int c = 0; c < a.n_c1; ++c) ms = fmaxf(ms, a.own_max[((int64_t)b * a.Hq + q) * a.n_c1 + c] * LOG2E);
-  const float m = fmaxf(mp, ms);
-  const float wp = __builtin_amdgcn_exp2f((mp - m) - PX_LIFT);
-  const float wo = ms > -INFINITY ? __builtin_amdgcn_exp2f(ms - m) : 0.f;
-  const float vmul = 2.f * a.head[1];
-  const float* psum = a.own_sum + (bq * a.n_c2) * 32 + (q & 31);
-  const int n_own = wo > 0.f ? a.n_c2 : 0;         // own positions without weight are not looked at (their sums may be NaN)
-  if (threadIdx.x == 0 && blockIdx.y == 0) {
-    float l = 0.f, o = 0.f;
-#pragma unroll 8
-    for (int s = 0; s < a.n_split; ++s) l += a.lsum[(int64_t)s * a.Mp + row];
-#pragma unroll 8
-    for (int c = 0; c < n_own; ++c) o += psum[(int64_t)c * 32];
-    a.jsum[bq * 32 + (q & 31)] = n_own ? l * wp + o * wo : l * wp;
-    if (a.jmax) a.jmax[(int64_t)b * a.Hq + q] = m * (1.f / LOG2E);
-  }
-  const int c0 = blockIdx.y * 512 + 8 * lane;
-  float v[8] = {};
-  if (c0 < a.Rvp) {
-    const _Float16* p = a.part + (int64_t)row * a.Rvp + c0;
-#pragma unroll 8
-    for (int s = wave; s < a.n_split; s += 4) {
-      const half8 e = *(const half8*)(p + (int64_t)s * a.M * a.Rvp);
-      const float f = a.lsum[(int64_t)s * a.Mp + row];
+// 32 bits of fp32 in a type of 16: fp16 as a sum of two (of a row scaled to its
+// largest value: 22 bits), bf16 as a sum of three (24 bits)
+template <typename WT> struct PxTerms;
+template <> struct PxTerms<_Float16> { static constexpr int N = 2; };
+template <> struct PxTerms<__bf16> { static constexpr int N = 3; };
+
+// Workgroup = (SC columns of the V rank, KV head, 32 of its rows (sequence, head of
+// the group)).  It adds the rows' sums over the prefix's splits and over their own
+// positions' chunks, in a fixed order, relative to the larger of the two maxima and
+// divided by the weights' sum, and multiplies them by its columns of U_v: a term of
+// the output, [column slice][row][128], that prefix_finish_kernel adds up.
+template <typename WT, int SC>
+__global__ __launch_bounds__(256) void prefix_up_kernel(const PrefixArgs a) {
+  constexpr int NT = PxTerms<WT>::N, PIECES = 32 * SC / 8, PP = PIECES >= 256 ? PIECES / 256 : 1, GR = PIECES >= 256 ? 1 : 256 / PIECES;
+  __shared__ uint4 op[NT][SC / 8][32];             // the rows' terms, [8 columns][row]
+  __shared__ float wsplit[32][PX_MAX_SPLITS + 1], wown[32];
+  __shared__ uint32_t row_top[32];
+  __shared__ float red[GR > 1 ? (GR - 1) * PIECES : 1][8];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5, n = lane & 31;
+  const int j0 = blockIdx.x * SC, h = blockIdx.y, nr = a.B * a.gs, r0 = blockIdx.z * 32, rows = min(32, nr - r0);
+  // this wave's 32 dims of U_v: lane n one, 8 columns a piece
+  uint4 uf[SC / 16];
+  const WT* u = (const WT*)a.uv + (int64_t)(h * HEAD_DIM + 32 * wave + n) * a.uv_rs;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = fmaf((float)e[i], f, v[i]);
+  for (int k = 0; k < SC / 16; ++k) {
+    const int c = j0 + 16 * k + 8 * hh;
+    if (c + 8 <= a.Rv) {
+      __builtin_memcpy(&uf[k], u + c, 16);
+    } else {
+      WT e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = c + i < a.Rv ? u[c + i] : (WT)0.f;
+      __builtin_memcpy(&uf[k], e, 16);
     }
+  }
+  // the rows' weights, eight lanes a row
+  {
+    const int r = min(tid >> 3, rows - 1), i0 = tid & 7, row = h * nr + r0 + r, b = (r0 + r) / a.gs, q = h * a.gs + (r0 + r) % a.gs;
+    const int64_t bq = (int64_t)b * a.n_hg + (q >> 5);
+    const float mp = a.rmax[row];
+    float ms = -INFINITY;                          // in units of log 2, as the prefix's
+    for (int c = i0; c < a.n_c1; c += 8) ms = fmaxf(ms, a.own_max[((int64_t)b * a.Hq + q) * a.n_c1 + c] * LOG2E);
+    float lp = 0.f, lo = 0.f;
+    for (int s = i0; s < a.n_split; s += 8) {
+      const float l = a.lsum[(int64_t)s * a.Mp + row];
+      wsplit[tid >> 3][s] = l;
+      lp += l;
+    }
+    const float* psum = a.own_sum + bq * a.n_c2 * 32 + (q & 31);
+    for (int c = i0; c < a.n_c2; c += 8) lo += psum[(int64_t)c * 32];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= wp * vmul;
-#pragma unroll 2
-    for (int c = wave; c < n_own; c += 4) {
-      const int64_t at = ((bq * a.n_c2 + c) * 32 + (q & 31)) * a.own_Rvp + c0;
-      if (a.own_part16) {
-        const half8 e = *(const half8*)((const _Float16*)a.own_part + at);
-        const float f = wo * psum[(int64_t)c * 32];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = fmaf((float)e[i], f, v[i]);
-      } else {
-        const float4* e = (const float4*)((const float*)a.own_part + at);
-        const float4 x = e[0], y = e[1];
-        v[0] = fmaf(x.x, wo, v[0]); v[1] = fmaf(x.y, wo, v[1]); v[2] = fmaf(x.z, wo, v[2]); v[3] = fmaf(x.w, wo, v[3]);
-        v[4] = fmaf(y.x, wo, v[4]); v[5] = fmaf(y.y, wo, v[5]); v[6] = fmaf(y.z, wo, v[6]); v[7] = fmaf(y.w, wo, v[7]);
+    for (int o = 4; o >= 1; o >>= 1) {
+      ms = fmaxf(ms, __shfl_xor(ms, o, 8));
+      lp += __shfl_xor(lp, o, 8);
+      lo += __shfl_xor(lo, o, 8);
+    }
+    const float m = fmaxf(mp, ms);
+    const float wp = __builtin_amdgcn_exp2f((mp - m) - PX_LIFT);
+    // own positions without weight are not looked at (their sums may be NaN)
+    const float wo = ms > -INFINITY ? __builtin_amdgcn_exp2f(ms - m) : 0.f;
+    const float l = wo > 0.f ? lp * wp + lo * wo : lp * wp, inv = 1.f / l;
+    for (int s = i0; s < a.n_split; s += 8) wsplit[tid >> 3][s] *= 2.f * a.head[1] * wp * inv;
+    if (i0 == 0) {
+      wown[tid >> 3] = wo > 0.f ? wo * inv : 0.f;
+      row_top[tid >> 3] = 0;
+      if (a.jmax && blockIdx.x == 0 && (tid >> 3) < rows) {
+        a.jmax[(int64_t)b * a.Hq + q] = m * (1.f / LOG2E);
+        a.jsum[bq * 32 + (q & 31)] = l;
       }
     }
   }
-  if (wave) {
+  __syncthreads();
+  float v[PP][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) red[wave - 1][lane][i] = v[i];
+  for (int i = 0; i < PP; ++i) {
+    const int e = tid % PIECES + 256 * i, grp = tid / PIECES, r = e / (SC / 8), c = j0 + e % (SC / 8) * 8;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[i][k] = 0.f;
+    if (r >= rows || c >= a.Rvp) continue;
+    const int b = (r0 + r) / a.gs, q = h * a.gs + (r0 + r) % a.gs;
+    const _Float16* p = a.part + (int64_t)(h * nr + r0 + r) * a.Rvp + c;
+    const int64_t step = (int64_t)a.M * a.Rvp;
+#pragma unroll 8
+    for (int s = grp; s < a.n_split; s += GR) {
+      const half8 x = *(const half8*)(p + s * step);
+      const float f = wsplit[r][s];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[i][k] = fmaf((float)x[k], f, v[i][k]);
+    }
+    const float wo = wown[r];
+    if (wo == 0.f) continue;
+    const int64_t bq = (int64_t)b * a.n_hg + (q >> 5);
+    const float* psum = a.own_sum + bq * a.n_c2 * 32 + (q & 31);
+#pragma unroll 4
+    for (int s = grp; s < a.n_c2; s += GR) {
+      const int64_t at = ((bq * a.n_c2 + s) * 32 + (q & 31)) * a.own_Rvp + c;
+      if (a.own_part16) {
+        const half8 x = *(const half8*)((const _Float16*)a.own_part + at);
+        const float f = wo * psum[(int64_t)s * 32];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[i][k] = fmaf((float)x[k], f, v[i][k]);
+      } else {
+        const floatx4* x = (const floatx4*)((const float*)a.own_part + at);
+        const floatx4 lo = x[0], hi = x[1];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          v[i][k] = fmaf(lo[k], wo, v[i][k]);
+          v[i][4 + k] = fmaf(hi[k], wo, v[i][4 + k]);
+        }
+      }
+    }
+  }
+  if constexpr (GR > 1) {
+    const int e = tid % PIECES, grp = tid / PIECES;
+    if (grp) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) red[(grp - 1) * PIECES + e][k] = v[0][k];
+    }
+    __syncthreads();
+    if (!grp) {
+      for (int g = 0; g < GR - 1; ++g)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[0][k] += red[g * PIECES + e][k];
+    }
+  }
+  const bool holds = GR == 1 || tid < PIECES;
+  // columns past the rank hold what their tiles left (the packed zeros' sums, or none at all of own positions)
+#pragma unroll
+  for (int i = 0; i < PP; ++i) {
+    const int e = tid % PIECES + 256 * i, c = j0 + e % (SC / 8) * 8;
+    uint32_t top = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (c + k >= a.Rv) v[i][k] = 0.f;
+      top = max(top, __float_as_uint(v[i][k]) & 0x7fffffffu);
+    }
+    if (__is_same(WT, _Float16) && holds) atomicMax(&row_top[e / (SC / 8)], top);
   }
   __syncthreads();
-  if (wave || c0 >= a.Rvp) return;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] += (red[0][lane][i] + red[1][lane][i]) + red[2][lane][i];
-  float4* o = (float4*)(a.jpart + (bq * 32 + (q & 31)) * a.Rvp + c0);
-  o[0] = make_float4(v[0], v[1], v[2], v[3]);
-  o[1] = make_float4(v[4], v[5], v[6], v[7]);
+  for (int i = 0; i < PP; ++i) {
+    const int e = tid % PIECES + 256 * i, r = e / (SC / 8);
+    float f = 1.f;
+    if constexpr (__is_same(WT, _Float16)) f = pow2f(-px_row_exp(row_top[r]));
+    WT w[NT][8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      float x = v[i][k] * f;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        w[t][k] = (WT)x;
+        x -= (float)w[t][k];
+      }
+    }
+    if (holds) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) __builtin_memcpy(&op[t][e % (SC / 8)][r], w[t], 16);
+    }
+  }
+  __syncthreads();
+  floatx16 acc = {};
+#pragma unroll
+  for (int k = 0; k < SC / 16; ++k)
+#pragma unroll
+    for (int t = NT - 1; t >= 0; --t) acc = px_mfma<WT>(op[t][2 * k + hh][n], uf[k], acc);
+  float* out = a.ypart + (((int64_t)blockIdx.x * a.Hkv + h) * nr + r0) * HEAD_DIM + 32 * wave + n;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int row = 8 * (r >> 2) + 4 * hh + (r & 3);
+    float f = 1.f;
+    if constexpr (__is_same(WT, _Float16)) f = pow2f(px_row_exp(row_top[row]));
+    if (row < rows) out[row * HEAD_DIM] = acc[r] * f;
+  }
+}
+
+// the output: the terms of the column slices added in order
+template <typename OT>
+__global__ __launch_bounds__(256) void prefix_finish_kernel(const PrefixArgs a) {
+  const int row = blockIdx.x * 2 + (threadIdx.x >> 7), d = threadIdx.x & 127, nr = a.B * a.gs;
+  if (row >= a.M) return;
+  const float* p = a.ypart + (int64_t)row * HEAD_DIM + d;
+  const int64_t step = (int64_t)a.M * HEAD_DIM;
+  float s = 0.f;
+#pragma unroll 8
+  for (int i = 0; i < a.n_sl; ++i) s += p[i * step];
+  const int h = row / nr, b = row % nr / a.gs, q = h * a.gs + row % a.gs;
+  ((OT*)a.out)[b * a.o_sb + q * a.o_sh + d] = (OT)s;
 }
 
 }  // namespace
@@ -822,8 +952,19 @@ int launch_prefix_pv(const PrefixArgs& a, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
-int launch_prefix_join(const PrefixArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL(prefix_join_kernel, dim3((unsigned)a.M, (unsigned)ceil_div(a.Rvp, 512)), dim3(256), 0, st, a);
+template <typename WT> static void launch_up(const PrefixArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)a.n_sl, (unsigned)a.Hkv, (unsigned)ceil_div((int64_t)a.B * a.gs, 32));
+  if (a.sc == 128) hipLaunchKernelGGL((prefix_up_kernel<WT, 128>), grid, dim3(256), 0, st, a);
+  else if (a.sc == 64) hipLaunchKernelGGL((prefix_up_kernel<WT, 64>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((prefix_up_kernel<WT, 32>), grid, dim3(256), 0, st, a);
+}
+int launch_prefix_up(const PrefixArgs& a, int dtype, bool out_f32, hipStream_t st) {
+  if (dtype == STARKV_F16) launch_up<_Float16>(a, st);
+  else launch_up<__bf16>(a, st);
+  const dim3 grid((unsigned)ceil_div(a.M, 2));
+  if (out_f32) hipLaunchKernelGGL(prefix_finish_kernel<float>, grid, dim3(256), 0, st, a);
+  else if (dtype == STARKV_F16) hipLaunchKernelGGL(prefix_finish_kernel<_Float16>, grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL(prefix_finish_kernel<__bf16>, grid, dim3(256), 0, st, a);
   return (int)hipGetLastError();
 }
 

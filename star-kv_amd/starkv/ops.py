@@ -221,21 +221,16 @@ class KLatentSpec:
 
     def c_struct(self, keep: list) -> KLatent:
         arrs = (int_array(self.ranks), i64_array(self.head_offset), i64_array(self.pos_stride),
-                i64_array(self.bk_head_offset), i64_array(self.head_offset2), i64_array(self.pos_stride2))
-        keep.extend(arrs)
-        k = KLatent()
-        k.n_kv_heads = self.n_kv_heads
-        k.rank, k.head_offset, k.pos_stride, k.bk_head_offset = arrs[:4]
-        k.stride_b = self.stride_b
-        k.format = self.fmt
-        k.data = self.data.data_ptr()
-        k.scale = self.scale.data_ptr() if self.scale is not None else None
-        k.scale_stride_b, k.scale_stride_h = self.scale_stride_b, self.scale_stride_h
-        k.bk = self.bk.data_ptr()
-        k.bk_row_stride = self.bk_row_stride
-        k.split, k.split_format = self.split, self.split_fmt
-        k.head_offset2, k.pos_stride2 = arrs[4], arrs[5]
+                i64_array(self.bk_head_offset))
+        keep.append(arrs)
+        scale = self.scale
+        k = KLatent(len(self.ranks), *arrs[:3], self.stride_b, self.fmt, self.data.data_ptr(),
+                    scale.data_ptr() if scale is not None else None, self.scale_stride_b, self.scale_stride_h,
+                    self.bk.data_ptr(), arrs[3], self.bk_row_stride, self.split, self.split_fmt)
         if self.data2 is not None:
+            lower = (i64_array(self.head_offset2), i64_array(self.pos_stride2))
+            keep.append(lower)
+            k.head_offset2, k.pos_stride2 = lower
             k.data2, k.stride2_b = self.data2.data_ptr(), self.stride2_b
         if self.scale2 is not None:
             k.scale2, k.scale2_stride_b, k.scale2_stride_h = (self.scale2.data_ptr(), self.scale2_stride_b,

@@ -40,6 +40,7 @@ class SharedPrefix:
         if len(devices) > 1:
             raise StarKVError(f"K latents, B_k and V latents lie on different devices: {devices}")
         self.length, self.ranks, self.v_rank, self.rope = n, list(k.ranks), vs.rank, rope
+        self.span = -(-n // 64) * 64               # positions of the rotation table that the kernels read
         self.dtype, self.device = k.data.dtype, vs.data.device
         keep: list = []
         d = PrefixPackDesc()
@@ -77,40 +78,49 @@ def prefix_decode_attention(q: torch.Tensor, prefix: SharedPrefix, k: Optional[K
     which the weights of own positions are added, summed over the heads (the
     prefix's weights are in the softmax but not in the sums)."""
     q = _q3(q)
-    B, Hq, _ = q.shape
+    B = q.shape[0]
     if (k is None) != (xv is None):
         raise StarKVError("own latents are k and xv together")
-    n = 0 if k is None else int(_vspec(xv).data.shape[1] if seq_len is None else seq_len)
-    if k is None and (seq_len or mask is not None or last_pos is not None):
+    n, v = 0, None
+    if k is not None:
+        v = _vspec(xv)
+        n = int(v.data.shape[1] if seq_len is None else seq_len)
+    elif seq_len or mask is not None or last_pos is not None:
         raise StarKVError("seq_len, mask and last_pos describe own latents: k and xv")
     if n < 0:
         raise StarKVError(f"seq_len must not be negative, got {n}")
     _require_cuda(q, uv_weight, scores)
+    device = q.device
     if q.dtype != prefix.dtype or uv_weight.dtype != prefix.dtype:
         raise StarKVError(f"q and uv_weight must be {prefix.dtype} as the prefix is, got {q.dtype} and {uv_weight.dtype}")
-    if q.device != prefix.device or uv_weight.device != prefix.device:
-        raise StarKVError(f"the prefix lies on {prefix.device}, q on {q.device}, uv_weight on {uv_weight.device}")
-    span = max(-(-prefix.length // 64) * 64, n)
-    own_rank = prefix.v_rank if k is None else _vspec(xv).rank
-    if n and (k.ranks != prefix.ranks or own_rank != prefix.v_rank):
-        raise StarKVError(f"own latents have K ranks {k.ranks} and V rank {own_rank}, the prefix {prefix.ranks} and "
-                          f"{prefix.v_rank}")
-    if n and (_vspec(xv).data.shape[0] < B or _vspec(xv).data.shape[1] < n):
-        raise StarKVError(f"the V latent {tuple(_vspec(xv).data.shape)} does not hold {B} sequences of {n} positions")
+    if device != prefix.device or uv_weight.device != device:
+        raise StarKVError(f"the prefix lies on {prefix.device}, q on {device}, uv_weight on {uv_weight.device}")
+    if n:
+        if k.ranks != prefix.ranks or v.rank != prefix.v_rank:
+            raise StarKVError(f"own latents have K ranks {k.ranks} and V rank {v.rank}, the prefix {prefix.ranks} and "
+                              f"{prefix.v_rank}")
+        rows = v.data.shape
+        if rows[0] < B or rows[1] < n:
+            raise StarKVError(f"the V latent {tuple(rows)} does not hold {B} sequences of {n} positions")
+        if k.fmt == FMT_DENSE and k.data.dtype != prefix.dtype or v.fmt == FMT_DENSE and v.data.dtype != prefix.dtype:
+            raise StarKVError(f"dense own latents must be {prefix.dtype}, got {k.data.dtype} and {v.data.dtype}")
     if scores is not None:
-        _check_scores(scores, B, n, q.device)
-    with torch.cuda.device(q.device):
-        table, cap = rope_table(prefix.rope, span, q.device)
-        if n:
-            own, out, keep = _decode_desc(q, k, xv, uv_weight, prefix.rope, n, mask, scale, out, out_dtype, last_pos)
-        else:
-            own, out, keep = _prefix_only(q, prefix, uv_weight, scale, out, out_dtype)
-        own.rope_table, own.rope_max_positions = table.data_ptr(), cap
-        d = PrefixDecodeDesc(own, len(prefix.ranks), prefix.v_rank, prefix.length, prefix._rank, prefix.data.data_ptr(),
-                             prefix.data.numel(), prefix._cos, prefix._sin)
-        if scores is not None and n:
-            d.scores, d.scores_stride_b = scores.data_ptr(), scores.stride(0)
-        _launch("starkv_prefix_decode", d, q.device, workspace=True)
+        _check_scores(scores, B, n, device)
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return prefix_decode_attention(q, prefix, k, xv, uv_weight, seq_len, mask, scale, out, out_dtype, last_pos, scores)
+    if n:
+        own, out, keep = _decode_desc(q, k, v, uv_weight, prefix.rope, n, mask, scale, out, out_dtype, last_pos)
+    else:
+        own, out, keep = _prefix_only(q, prefix, uv_weight, scale, out, out_dtype)
+    if own.rope_max_positions < prefix.span:
+        table, own.rope_max_positions = rope_table(prefix.rope, prefix.span, device)
+        own.rope_table = table.data_ptr()
+    d = PrefixDecodeDesc(own, len(prefix.ranks), prefix.v_rank, prefix.length, prefix._rank, prefix.data.data_ptr(),
+                         prefix.data.numel(), prefix._cos, prefix._sin)
+    if scores is not None and n:
+        d.scores, d.scores_stride_b = scores.data_ptr(), scores.stride(0)
+    _launch("starkv_prefix_decode", d, device, workspace=True)
     return out
 
 

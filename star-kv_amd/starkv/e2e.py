@@ -29,10 +29,11 @@ from .cache import LatentCache
 from .fp8 import fp8_linear, fp8_quantize_weight
 from .logprobs import MAX_TOP, TokenLogprobs, token_logprobs
 from .ops import GEMM_ADD, GEMM_SILU_MUL, SKINNY_MAX_ROWS, decode_attention, prefill_attention, skinny_linear
+from .prefix import SharedPrefix, prefix_decode_attention
 from .rope import RopeConfig
 
 __all__ = ["LatentAttention", "DecodeGraphState", "build_model", "fuse_layers_", "generate", "generate_graphed",
-           "decode_graphed", "score"]
+           "decode_graphed", "score", "share_prompt", "drop_prompt", "generate_bounded"]
 
 HEAD_DIM = 128
 SCORE_LOGITS = 1 << 27                 # logits that score() holds at a time
@@ -102,6 +103,8 @@ class LatentAttention(nn.Module):
         self.reference = False
         self.events: Optional[list] = None     # (start, end) CUDA events of the decode kernels, when set
         self.graph: Optional[DecodeGraphState] = None   # set: single-token forwards in graph-replay form
+        self.prefix: Optional[SharedPrefix] = None      # set: every sequence follows it (share_prompt)
+        self.scores: Optional[torch.Tensor] = None      # set: fp32 [B, capacity], decode adds its weights by position
 
     def reset_parameters_(self, gen: Optional[torch.Generator] = None, std: float = 0.02):
         """Random weights of the scales a trained STAR-KV layer has: N(0, std)
@@ -200,11 +203,21 @@ class LatentAttention(nn.Module):
         o = self.core(hidden_states, position_embeddings)
         return self.o_proj(o), None
 
+    def _decode(self, q: torch.Tensor, kspec, vspec, S: int, last_pos: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """[B, Hq, 128]: one query position over the cache's first S positions, behind the shared prefix if there is one."""
+        if self.prefix is not None:
+            return prefix_decode_attention(q, self.prefix, kspec, vspec, self.v_u.weight, seq_len=S, scale=self.scaling,
+                                           last_pos=last_pos, scores=self.scores)
+        return decode_attention(q, kspec, vspec, self.v_u.weight, rope=self.rope, seq_len=S, scale=self.scaling,
+                                last_pos=last_pos, scores=self.scores)
+
     def core(self, hidden_states: torch.Tensor, position_embeddings=None,
              rms_eps: Optional[float] = None) -> torch.Tensor:
         """The attention of the layer input without the output projection: [B, T, Hq*128]
         (``rms_eps``: as in ``_project``)."""
         B, T, _ = hidden_states.shape
+        if self.prefix is not None and (T > 1 or self.reference):
+            raise StarKVError("behind a shared prompt sequences go on a token at a time, on the kernels")
         q, k_new, v_new = self._project(hidden_states, rms_eps)
         # k_new [B, T, sum(r)]: the writer takes the heads packed.  The cache
         # writes and the query rotation (positions continuing the cache) run as
@@ -215,8 +228,7 @@ class LatentAttention(nn.Module):
         elif self.graph is not None and T == 1:
             kspec, vspec = self.cache.append_at(k_new, v_new, self.bk, self.graph.pos, error_flag=self.graph.error,
                                                 q=q, rope=self.rope)
-            o = decode_attention(q[:, :, 0], kspec, vspec, self.v_u.weight, rope=self.rope,
-                                 seq_len=self.graph.capacity, scale=self.scaling, last_pos=self.graph.pos)
+            o = self._decode(q[:, :, 0], kspec, vspec, self.graph.capacity, self.graph.pos)
             return o.unsqueeze(1).reshape(B, T, self.n_heads * HEAD_DIM)
         if self.reference:
             kspec, vspec, S = self.cache.append(k_new, v_new, self.bk)
@@ -229,8 +241,7 @@ class LatentAttention(nn.Module):
             if self.events is not None:
                 e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
                 e0.record()
-            o = decode_attention(q[:, :, 0], kspec, vspec, self.v_u.weight, rope=self.rope, seq_len=S,
-                                 scale=self.scaling)
+            o = self._decode(q[:, :, 0], kspec, vspec, S)
             if self.events is not None:
                 e1.record()
                 self.events.append((e0, e1))
@@ -689,3 +700,82 @@ def decode_graphed(model, tok: torch.Tensor, steps: int, keep_logits: bool = Tru
     state.check()
     toks = torch.cat(toks, 1)
     return (toks, logits) if logprobs is None else (toks, logits, _stack_steps(probs))
+
+
+@torch.no_grad()
+def share_prompt(model, prompt: torch.Tensor) -> torch.Tensor:
+    """Read ``prompt`` [1, P] once for all sequences of the model's batch: its
+    latents become the layers' shared prefix, the sequences' own caches are
+    emptied, and the logits of its last position [1, V] are returned (to take
+    a first token for each sequence from).  Afterwards ``decode_graphed`` (or
+    single-token forwards) goes on with B sequences behind it; positions count
+    from the sequences' own first token.  ``drop_prompt`` ends it."""
+    if prompt.dim() != 2 or prompt.shape[0] != 1 or prompt.shape[1] < 1:
+        raise StarKVError(f"share_prompt: the prompt must be [1, P] with P at least 1, got {tuple(prompt.shape)}")
+    atts = attention_layers(model)
+    P, dev = prompt.shape[1], prompt.device
+    own = [(att.cache, att.scores) for att in atts]
+    model.model.norm.starkv_reference = False
+    try:
+        for att, (c, _) in zip(atts, own):
+            att.reference = False
+            att.prefix = att.scores = None
+            att.cache = LatentCache(1, c.ranks, c.Rv, P, c.dtype, c.device, c.fmt)
+        out = model(input_ids=prompt, position_ids=torch.arange(P, device=dev)[None], use_cache=False, logits_to_keep=1)
+        prefixes = [att.cache.share(att.bk, att.rope) for att in atts]
+    finally:
+        for att, (c, s) in zip(atts, own):
+            att.cache, att.scores = c, s
+    for att, prefix in zip(atts, prefixes):
+        att.prefix = prefix
+        att.cache.length = 0
+        if att.scores is not None:
+            att.scores.zero_()
+    return out.logits[:, -1]
+
+
+def drop_prompt(model) -> None:
+    """Forget the shared prompt and what follows it."""
+    for att in attention_layers(model):
+        att.prefix = None
+        att.cache.length = 0
+
+
+@torch.no_grad()
+def generate_bounded(model, prompt: torch.Tensor, steps: int, keep: int, sinks: int = 4, recent: int = 32,
+                     forced: Optional[torch.Tensor] = None):
+    """Greedy decoding with caches that never outgrow their capacity: where a
+    layer's cache is full, it keeps ``keep`` positions -- the first ``sinks``,
+    the last ``recent``, and those that the decode steps since have given the
+    most attention, by layer and sequence -- and goes on (``LatentCache.bound``).
+    ``forced`` [B, steps] as in ``generate``.  Returns (tokens [B, steps + 1],
+    logits of the last position per forward)."""
+    atts = attention_layers(model)
+    B, P = prompt.shape
+    if not 0 <= sinks + recent <= keep or min(sinks, recent) < 0:
+        raise StarKVError(f"generate_bounded: need 0 <= sinks + recent <= keep, got {sinks}, {recent}, {keep}")
+    if any(att.prefix is not None or att.cache.length + P > att.cache.cap or keep >= att.cache.cap for att in atts):
+        raise StarKVError("generate_bounded: the caches must hold the prompt and more than `keep` positions, behind no shared one")
+    before = [att.scores for att in atts]
+    for att in atts:
+        att.reference = False
+        att.scores = torch.zeros(att.cache.B, att.cache.cap, device=prompt.device)
+    model.model.norm.starkv_reference = False
+    try:
+        out = model(input_ids=prompt, position_ids=torch.arange(P, device=prompt.device)[None].expand(B, P),
+                    use_cache=False, logits_to_keep=1)
+        logits = [out.logits[:, -1].float()]
+        toks = [logits[-1].argmax(-1, keepdim=True)]
+        for t in range(steps):
+            for att in atts:
+                if att.cache.length == att.cache.cap:
+                    att.cache.bound(keep, att.scores, sinks, recent)
+            inp = forced[:, t:t + 1] if forced is not None else toks[-1]
+            pos = torch.full((B, 1), atts[0].cache.length, device=prompt.device, dtype=torch.long)
+            out = model(input_ids=inp, position_ids=pos, use_cache=False, logits_to_keep=1)
+            logits.append(out.logits[:, -1].float())
+            toks.append(logits[-1].argmax(-1, keepdim=True))
+    finally:
+        for att, s in zip(atts, before):
+            att.scores = s
+    return torch.cat(toks, 1), logits

@@ -396,7 +396,9 @@ __device__ __forceinline__ void px_prefix_logits(const PrefixArgs& a, uint8_t* l
       top[g] = fmaxf(top[g], m);
       float l = 0.f;
       uint8_t* o = (uint8_t*)(a.p + (int64_t)8 * s * a.Mp);
-      const uint32_t at = (uint32_t)(2 * hh * a.Mp + row) * 16, step = (uint32_t)a.Mp * 16;
+      uint32_t at = (uint32_t)(2 * hh * a.Mp + row) * 16;
+      const uint32_t step = (uint32_t)a.Mp * 16;
+      asm("" : "+v"(at));                          // formed here: kept across the loop its sums were spilled, and a reload waits for the fetch
 #pragma unroll
       for (int pt = 0; pt < 2; ++pt) {
         half8 v[2];
@@ -538,7 +540,9 @@ __device__ __forceinline__ void px_own_logits(const PrefixArgs& a, uint8_t* lds,
       }
       top[g] = fmaxf(top[g], max_halves(m));
       if (rl < a.gs) {
-        float4* o = (float4*)(a.ol + b * a.ol_sb + t * a.ol_st + (h * a.gs + rl) * 32 + 16 * hh);
+        uint32_t at = (uint32_t)((h * a.gs + rl) * 32 + 16 * hh) * 4;
+        asm("" : "+v"(at));                        // formed here, as above
+        float4* o = (float4*)((uint8_t*)(a.ol + b * a.ol_sb + t * a.ol_st) + at);
 #pragma unroll
         for (int r = 0; r < 4; ++r) o[r] = make_float4(acc[g][4 * r], acc[g][4 * r + 1], acc[g][4 * r + 2], acc[g][4 * r + 3]);
       }
@@ -549,7 +553,7 @@ __device__ __forceinline__ void px_own_logits(const PrefixArgs& a, uint8_t* lds,
 }
 
 template <typename XT, int NG>
-__global__ __launch_bounds__(512, NG == 1 ? 4 : 3) void own_logits_kernel(const PrefixArgs a) {
+__global__ __launch_bounds__(512, NG == 1 ? 4 : 2) void own_logits_kernel(const PrefixArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t px_lds[];
   const int bx = blockIdx.x, chunk = bx % a.n_c1, h = bx / a.n_c1 % a.Hkv, b = bx / a.n_c1 / a.Hkv, kp = (a.rank[h] + 31) / 32;
   if (kp == 1) px_own_logits<XT, NG, 1>(a, px_lds, chunk, h, b);

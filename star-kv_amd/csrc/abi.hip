@@ -1756,6 +1756,49 @@ int starkv_select_positions(const starkv_select_desc* d, void* workspace, size_t
   return launch_select(a, (hipStream_t)stream);
 }
 
+// Whether rows 0 .. L - 1 of `nb[h]` bytes of all heads and sequences lie apart (pitch[h] >= nb[h]): a move in place writes
+// each of them once.
+static bool rows_apart(int H, const int64_t* off, const int64_t* pitch, const int* nb, int B, int64_t sb, int L) {
+  auto end = [&](int h) { return off[h] + (L - 1) * pitch[h] + nb[h]; };
+  int64_t lo = INT64_MAX, hi = 0, row = 0;
+  bool even = true, stacked = true, inside = true;   // one pitch; heads one behind another; heads side by side in a row
+  int last = -1;
+  for (int h = 0; h < H; ++h) {
+    if (!nb[h]) continue;
+    if (last >= 0) {
+      even &= pitch[h] == pitch[last];
+      stacked &= off[h] >= end(last);
+      inside &= off[h] >= off[last] + nb[last];
+    }
+    last = h;
+    lo = std::min(lo, off[h]); hi = std::max(hi, end(h)); row = std::max(row, off[h] + nb[h]);
+  }
+  if (last < 0) return true;
+  row -= lo;
+  inside &= even && row <= pitch[last];
+  if (!stacked && !inside) {
+    for (int g = 0; g < H; ++g)
+      for (int h = 0; h < H; ++h) {                // off[g] <= off[h]; at equal pitch only the nearest rows can meet
+        if (g == h || !nb[g] || !nb[h] || off[g] > off[h] || (off[g] == off[h] && g > h)) continue;
+        const int64_t d = off[h] - off[g], p = pitch[g];
+        if (pitch[h] != p) {
+          if (off[h] < end(g)) return false;
+        } else if ((d / p < L && d % p < nb[g]) || (d / p + 1 < L && p - d % p < nb[h])) {
+          return false;
+        }
+      }
+  }
+  if (B == 1 || sb >= hi - lo || (inside && sb >= row && pitch[last] >= (B - 1) * sb + row)) return true;
+  // each head's sequences one behind another, and the heads' ranges apart
+  for (int g = 0; g < H; ++g) {
+    if (!nb[g]) continue;
+    if (sb < end(g) - off[g]) return false;
+    for (int h = 0; h < H; ++h)
+      if (g != h && nb[h] && off[g] <= off[h] && off[h] < end(g) + (B - 1) * sb) return false;
+  }
+  return true;
+}
+
 int starkv_keep_positions(const starkv_keep_desc* d, void* stream) {
   if (!d) return STARKV_ERR_NULL;
   if (d->batch < 1 || d->length < 0 || d->keep < 0 || d->keep > d->length) return STARKV_ERR_SHAPE;
@@ -1794,8 +1837,17 @@ int starkv_keep_positions(const starkv_keep_desc* d, void* stream) {
     a.ks2 = (uint8_t*)k.scale2; a.ks2_sb = 2 * k.scale2_stride_b; a.ks2_sh = 2 * k.scale2_stride_h;
     a.units[MOVE_KS2] = H;
   }
-  if (many && (!a.k1_sb || (lower && !a.k2_sb) || (!dense && !a.ks1_sb) || (lower && !a.ks2_sb))) return STARKV_ERR_SHAPE;
-  if (H > 1 && ((!dense && !a.ks1_sh) || (lower && !a.ks2_sh))) return STARKV_ERR_SHAPE;
+  const int B = d->batch, L = d->length;
+  if (!rows_apart(H, a.off1, a.pitch1, a.nb1, B, a.k1_sb, L) || !rows_apart(H, a.off2, a.pitch2, a.nb2, B, a.k2_sb, L))
+    return STARKV_ERR_SHAPE;
+  int64_t s_off[2][K_MAX_KV], s_pitch[K_MAX_KV];
+  int s_nb[2][K_MAX_KV];
+  for (int h = 0; h < H; ++h) {
+    s_off[0][h] = h * a.ks1_sh; s_off[1][h] = h * a.ks2_sh; s_pitch[h] = 2;
+    s_nb[0][h] = dense ? 0 : 2; s_nb[1][h] = lower ? 2 : 0;
+  }
+  if (!rows_apart(H, s_off[0], s_pitch, s_nb[0], B, a.ks1_sb, L) || !rows_apart(H, s_off[1], s_pitch, s_nb[1], B, a.ks2_sb, L))
+    return STARKV_ERR_SHAPE;
   // V rows, the lower block's, their scales and zero points
   const int vs = vq == VQ_DENSE ? 2 : 1, groups = vq == VQ_G64 ? (v.rank + 63) / 64 : 1;
   a.v[0] = {(uint8_t*)v.data, v.stride_b * vs, v.stride_s * vs, vq == VQ_DENSE ? 2 * v.rank : pv.xnb};
@@ -1809,11 +1861,13 @@ int starkv_keep_positions(const starkv_keep_desc* d, void* stream) {
   a.units[MOVE_K2] = lower ? H * (int)ceil_div(nk2, MOVE_SLICE) : 0;
   for (int i = 0; i < MOVE_SCORES - MOVE_V; ++i) a.units[MOVE_V + i] = (int)ceil_div(a.v[i].nb, MOVE_SLICE);
   for (int i = 0; i < MOVE_SCORES - MOVE_V; ++i) {
-    if (a.v[i].nb && (a.v[i].pitch < a.v[i].nb || (many && !a.v[i].sb))) return STARKV_ERR_SHAPE;
+    const int64_t at = 0, pitch = a.v[i].pitch;
+    if (a.v[i].nb && (pitch < a.v[i].nb || !rows_apart(1, &at, &pitch, &a.v[i].nb, B, a.v[i].sb, L))) return STARKV_ERR_SHAPE;
   }
   if (d->scores) { a.scores = d->scores; a.scores_sb = d->scores_stride_b; a.units[MOVE_SCORES] = 1; }
-  a.B = d->batch;
+  a.B = B;
   for (int k = 0; k < MOVE_KINDS; ++k) a.per_row += a.units[k];
+  if ((int64_t)a.per_row * B > MAX_THREADS_1D / 1024 - 8) return STARKV_ERR_LIMIT;       // workgroups of 1024 threads
   return launch_move(a, (hipStream_t)stream);
 }
 
@@ -2041,13 +2095,13 @@ int starkv_prefix_decode(const starkv_prefix_decode_desc* d, void* workspace, si
     a.own_part = ws + L.own.off_part;
     a.n_c1 = L.own.n_c1; a.n_c2 = L.own.pv.n_c2; a.own_Rvp = L.own.pv.Rvp; a.own_part16 = L.own.part16;
     a.S = o.seq_len;
+    a.mask = o.mask; a.m_sb = o.mask_stride_b; a.m_sh = o.mask_stride_h; a.mask_dtype = o.mask_dtype;
+    a.ol = (float*)(ws + L.own.off_logits); a.ol_sb = (int64_t)o.n_q_heads * L.own.S_pad; a.ol_st = (int64_t)o.n_q_heads * TILE;
     if (L.own_here) {
       a.oc_len = L.oc_len;
       a.ox = o.k.data; a.ox_sb = o.k.stride_b;
       for (int h = 0; h < d->n_kv_heads; ++h) { a.oxoff[h] = o.k.head_offset[h]; a.oxpitch[h] = o.k.pos_stride[h]; }
-      a.mask = o.mask; a.m_sb = o.mask_stride_b; a.m_sh = o.mask_stride_h; a.mask_dtype = o.mask_dtype;
       a.last_pos = o.last_pos_device;
-      a.ol = (float*)(ws + L.own.off_logits); a.ol_sb = (int64_t)o.n_q_heads * L.own.S_pad; a.ol_st = (int64_t)o.n_q_heads * TILE;
       if ((st = launch_own_logits(a, o.dtype, s))) return st;
     } else if ((st = decode_logits(&o, L.own, L.gs, ws, s))) {
       return st;

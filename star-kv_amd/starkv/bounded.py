@@ -70,8 +70,8 @@ def keep_positions(k: KLatentSpec, v, positions: torch.Tensor, length: int, scor
     ``k`` and ``v`` (any format; a VLatentSpec or a dense tensor) to rows 0 ..
     keep - 1, in place; rows from keep on stay as they are.  ``scores`` [B, >=
     length] move along, zeros behind.  A position that breaks the rule leaves
-    its row as it is and sets ``error_flag`` (int32 device tensor) to 1.  Keys
-    are cached before rotation: a moved row takes the angle of its new place,
+    its row as it is and sets ``error_flag`` (int32 device tensor) to 1.  Rows
+    that share memory (an expanded head or batch) are refused.  Keys are cached before rotation: a moved row takes the angle of its new place,
     and the next token's position is ``keep``."""
     vs = _vspec(v)
     _require_cuda(positions, scores, error_flag, *k.tensors, *vs.tensors)
@@ -83,7 +83,7 @@ def keep_positions(k: KLatentSpec, v, positions: torch.Tensor, length: int, scor
     if B < 1 or not 0 <= keep <= length:
         raise StarKVError(f"need at least one sequence and 0 <= keep <= length, got positions {tuple(positions.shape)}, "
                           f"length {length}")
-    if vs.data.shape[0] != B or vs.data.shape[1] < length or k.data.shape[0] != B:
+    if vs.data.shape[0] != B or vs.data.shape[1] < length or k.data.shape[0] != B or (length and not k.holds(B, length)):
         raise StarKVError(f"the caches must hold {B} sequences of at least {length} positions: K "
                           f"{tuple(k.data.shape)}, V {tuple(vs.data.shape)}")
     device = vs.data.device

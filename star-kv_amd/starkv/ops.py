@@ -158,6 +158,11 @@ class KLatentSpec:
     def n_kv_heads(self) -> int:
         return len(self.ranks)
 
+    def holds(self, batch: int, rows: int) -> bool:
+        """Whether ``data`` reaches to row rows - 1 of sequence batch - 1."""
+        last = max(o + (rows - 1) * p for o, p in zip(self.head_offset, self.pos_stride)) + (batch - 1) * self.stride_b
+        return last <= sum((n - 1) * s for n, s in zip(self.data.shape, self.data.stride()))
+
     @classmethod
     def from_reference(cls, x: torch.Tensor, b: torch.Tensor) -> "KLatentSpec":
         """The reference layouts: x = K latent cache [B, Hkv, S, r]

@@ -342,3 +342,55 @@ def test_refusals():
         with pytest.raises(StarKVError):
             f()
             pytest.fail(f"call {i} was not refused")
+
+
+def test_keep_offsets_past_32_bits():
+    """A V latent of 4.9 GB, in pieces that are checked one by one."""
+    n, w = 300000, 8192
+    v = torch.empty(1, n, w, dtype=torch.float16, device=DEV)
+    rows = torch.arange(n, device=DEV)
+    v.copy_((rows % 2039)[None, :, None])                                          # exact in fp16
+    v[0, :, -1] = (rows // 2039).half()
+    k = torch.stack((rows % 2039, rows // 2039), -1).half()[None, None].contiguous()
+    spec = KLatentSpec(k, [2], [0], [2], k.stride(0), k, [0], 128)
+    pos = torch.cat((torch.arange(3), torch.arange(n - 280001, n - 1)))[None].int().to(DEV)
+    keep_positions(spec, v, pos, n)
+    for i in range(0, pos.shape[1], 20000):
+        want = pos[0, i:i + 20000].long()
+        got = v[0, i:i + len(want)]
+        assert torch.equal(got[:, :-1], (want % 2039).half()[:, None].expand(-1, w - 1))
+        assert torch.equal(got[:, -1], (want // 2039).half())
+        assert torch.equal(k[0, 0, i:i + len(want)], torch.stack((want % 2039, want // 2039), -1).half())
+    assert torch.equal(v[0, pos.shape[1]:, 0], (rows[pos.shape[1]:] % 2039).half())
+
+
+@pytest.mark.parametrize("order", ["position, sequence, head", "head, sequence, position", "sequence, position, head"])
+def test_keep_of_other_orders(order):
+    """Latents whose sequences or heads lie inside a position's row, or behind another."""
+    B, H, n, r = 3, 2, 50, 24
+    dims = {"sequence": B, "position": n, "head": H}
+    names = order.split(", ")
+    g = torch.Generator().manual_seed(7)
+    x = torch.randn(*(dims[a] for a in names), r, generator=g).half().to(DEV)
+    x = x.permute(*(names.index(a) for a in ("sequence", "head", "position")), 3)  # [B, H, n, r]
+    spec = KLatentSpec(x, [r] * H, [h * x.stride(1) for h in range(H)], [x.stride(2)] * H, x.stride(0), x, [0] * H, 128)
+    v = torch.randn(n, B, 16, generator=g).half().to(DEV).transpose(0, 1)
+    pos = kept(B, n, 20).to(DEV)
+    at = pos.long()
+    want_k = x.gather(2, at[:, None, :, None].expand(B, H, 20, r))
+    want_v, rest = v.gather(1, at[..., None].expand(B, 20, 16)), v[:, 20:].clone()
+    keep_positions(spec, v, pos, n)
+    assert torch.equal(x[:, :, :20], want_k) and torch.equal(v[:, :20], want_v) and torch.equal(v[:, 20:], rest)
+
+
+def test_keep_refuses_shared_rows():
+    k0 = torch.zeros(2, 1, 8, 16, device=DEV).half()
+    v = torch.zeros(2, 8, 16, device=DEV).half()
+    p = torch.arange(3, dtype=torch.int32, device=DEV).expand(2, 3).contiguous()
+    for x in (k0.expand(2, 3, 8, 16), k0[:1].expand(2, 1, 8, 16)):
+        spec = KLatentSpec(x, [16] * x.shape[1], [h * x.stride(1) for h in range(x.shape[1])], [16] * x.shape[1], x.stride(0),
+                           k0, [0] * x.shape[1], 128)
+        with pytest.raises(StarKVError):
+            keep_positions(spec, v, p, 8)
+    with pytest.raises(StarKVError):
+        keep_positions(KLatentSpec(k0[:, :, :7], [16], [0], [16], k0.stride(0), k0, [0], 128), v, p, 8)

@@ -227,3 +227,25 @@ def test_host_tensors_are_refused():
               lambda: starkv.keep_positions(k, v, torch.zeros(1, 2, dtype=torch.int32), 8)):
         with pytest.raises(starkv.StarKVError):
             f()
+
+
+def spread(**kw):
+    """Two heads of rank 16 and 40 at offsets and pitches of one's own."""
+    off, pitch = L.i64_array(kw.pop("off")), L.i64_array(kw.pop("pitch"))
+    d = keep_desc(k_kw=dict(n_kv_heads=2, head_offset=off, pos_stride=pitch, stride_b=kw.pop("stride_b")), **kw)
+    d._more = (off, pitch)
+    return d
+
+
+@pytest.mark.parametrize("off,pitch,stride_b", [
+    ([0, 0], [40, 40], 8000), ([0, 8], [64, 64], 8000), ([0, 56], [64, 64], 8000), ([24, 0], [56, 56], 8000),
+    ([0, 1599], [16, 40], 8000), ([3999, 0], [16, 40], 8000), ([0, 16], [56, 56], 5599), ([0, 1600], [16, 40], 5599),
+    ([0, 16], [112, 112], 55), ([0, 16], [111, 111], 56), ([0, 640], [64, 64], 1), ([0, 3200], [16, 40], 1599)])
+def test_keep_refuses_rows_that_overlap(off, pitch, stride_b):
+    d = spread(off=off, pitch=pitch, stride_b=stride_b)
+    assert L.lib().starkv_keep_positions(ctypes.byref(d), None) == SHAPE
+
+
+def test_keep_refuses_more_workgroups_than_a_grid_holds():
+    d = keep_desc(batch=65535, v_kw=dict(rank=8192, stride_s=8192, stride_b=819200))
+    assert L.lib().starkv_keep_positions(ctypes.byref(d), None) == LIMIT

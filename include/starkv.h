@@ -642,8 +642,9 @@ int starkv_decode_attention_scores(const starkv_decode_desc* d, float* scores, i
  * a position that breaks it leaves row i as it is and sets *error_flag
  * (optional device int, never cleared by the library) to 1.  The keys are
  * stored before rotation, so a moved row takes the angle of its new place.
- * B_k's fields of k are not read.  dtype: of dense latents.  batch <= 65535;
- * rows of different positions, heads or sequences must not overlap.
+ * B_k's fields of k are not read.  dtype: of dense latents.  batch <= 65535.
+ * Rows of different positions, heads or sequences that overlap (or may: heads
+ * of different pitch whose ranges do) are STARKV_ERR_SHAPE.
  * ------------------------------------------------------------------- */
 typedef struct {
   int batch, length, keep, sinks, recent;
@@ -682,9 +683,11 @@ int starkv_keep_positions(const starkv_keep_desc* d, void* stream);
  *   own position s:    scale * q[b,q] . RoPE_s(x_k[b,s] B_k) (+ mask)
  * that is, own.q is rotated at its position behind the sequence's own first one
  * (as the cache writer does, whose positions are the cache's), and the prefix
- * lies before that one.  own: as for starkv_decode_attention; own.seq_len 0:
+ * lies before that one.  own: as for starkv_decode_attention, with the B_k that
+ * the prefix was packed with (dense latents meet the packed one); own.seq_len 0:
  * no own positions (k, v, mask and last_pos_device are not read).  A sequence
- * whose mask leaves none of its own positions attends to the prefix alone.
+ * whose mask leaves none of its own positions attends to the prefix alone; own
+ * logits that are NaN and not masked make its output NaN.
  * turn_cos / turn_sin: host arrays [64], the (unscaled) rotation of frequency i
  * by `length` positions.  The prefix's rank, v_rank, length and dtype are those
  * it was packed with; rope_max_positions >= round_up(length, 64).  scores

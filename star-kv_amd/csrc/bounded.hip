@@ -200,15 +200,19 @@ struct SelShared {
 // counts the pass's digits of a tile's keys whose earlier digits are `key`
 template <int PASS> __device__ inline void sel_count(SelShared& sh, int n, int t, const uint32_t (&k)[4], uint32_t key) {
   constexpr int low = SEL_LOW[PASS], bits = SEL_BITS[PASS];
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, p = t * SEL_TILE + 4 * (int)threadIdx.x;
+  // positions that never got any weight are many, and alike: counted by the wave
+  int zeros = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const bool in = t * SEL_TILE + 4 * (int)threadIdx.x + i < n && (PASS == 0 || (k[i] >> (low + bits)) == key);
-    // positions that never got any weight are many, and alike: counted by the wave
-    const uint64_t zeros = __ballot(in && k[i] == ZERO_KEY);
-    if (zeros && lane == 0) atomicAdd(&sh.hist[((ZERO_KEY >> low) & ((1u << bits) - 1)) * 4], (uint32_t)__popcll(zeros));
-    if (in && k[i] != ZERO_KEY) atomicAdd(&sh.hist[((k[i] >> low) & ((1u << bits) - 1)) * 4 + (lane & 3)], 1u);
+  for (int i = 0; i < 4; ++i) zeros += p + i < n && k[i] == ZERO_KEY;
+  if ((PASS == 0 || key == ZERO_KEY >> (low + bits) % 32) && __any(zeros)) {
+    const int all = wave_scan(zeros);
+    if (lane == 63) atomicAdd(&sh.hist[((ZERO_KEY >> low) & ((1u << bits) - 1)) * 4], (uint32_t)all);
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (p + i < n && k[i] != ZERO_KEY && (PASS == 0 || (k[i] >> (low + bits) % 32) == key))
+      atomicAdd(&sh.hist[((k[i] >> low) & ((1u << bits) - 1)) * 4 + (lane & 3)], 1u);
 }
 
 // The digit at which the keys counted from the largest down reach `need`, and how many lie above it: thread j brings the

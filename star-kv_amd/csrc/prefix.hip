@@ -723,6 +723,14 @@ template <typename WT> struct PxTerms;
 template <> struct PxTerms<_Float16> { static constexpr int N = 2; };
 template <> struct PxTerms<__bf16> { static constexpr int N = 3; };
 
+// whether element `at` of the mask leaves nothing of a position (as low as the lowest value of a type, or -inf)
+__device__ inline bool px_masked(const PrefixArgs& a, int64_t at) {
+  if (a.mask == nullptr) return false;
+  if (a.mask_dtype == STARKV_F32) return ((const float*)a.mask)[at] <= -65504.f;
+  const uint16_t v = ((const uint16_t*)a.mask)[at];
+  return (a.mask_dtype == STARKV_F16 ? (float)__builtin_bit_cast(_Float16, v) : bf16_bits_to_float(v)) <= -65504.f;
+}
+
 // Workgroup = (SC columns of the V rank, KV head, 32 of its rows (sequence, head of
 // the group)).  It adds the rows' sums over the prefix's splits and over their own
 // positions' chunks, in a fixed order, relative to the larger of the two maxima and
@@ -773,14 +781,23 @@ __global__ __launch_bounds__(256) void prefix_up_kernel(const PrefixArgs a) {
       lp += __shfl_xor(lp, o, 8);
       lo += __shfl_xor(lo, o, 8);
     }
+    // no own logit above -inf: all masked, or latents that are not numbers, which have to show
+    bool bad = false;
+    if (ms == -INFINITY)
+      for (int t = i0; t < a.S; t += 8) {
+        const float l = a.ol[b * a.ol_sb + (t >> 5) * a.ol_st + q * 32 + (t & 31)];
+        bad |= !(l == l) && !px_masked(a, (int64_t)b * a.m_sb + (int64_t)q * a.m_sh + t);
+      }
+#pragma unroll
+    for (int o = 4; o >= 1; o >>= 1) bad |= __shfl_xor((int)bad, o, 8) != 0;
     const float m = fmaxf(mp, ms);
     const float wp = __builtin_amdgcn_exp2f((mp - m) - PX_LIFT);
     // own positions without weight are not looked at (their sums may be NaN)
-    const float wo = ms > -INFINITY ? __builtin_amdgcn_exp2f(ms - m) : 0.f;
-    const float l = wo > 0.f ? lp * wp + lo * wo : lp * wp, inv = 1.f / l;
+    const float wo = bad ? NAN : ms > -INFINITY ? __builtin_amdgcn_exp2f(ms - m) : 0.f;
+    const float l = wo == 0.f ? lp * wp : lp * wp + lo * wo, inv = 1.f / l;
     for (int s = i0; s < a.n_split; s += 8) wsplit[tid >> 3][s] *= 2.f * a.head[1] * wp * inv;
     if (i0 == 0) {
-      wown[tid >> 3] = wo > 0.f ? wo * inv : 0.f;
+      wown[tid >> 3] = wo == 0.f ? 0.f : wo * inv;
       row_top[tid >> 3] = 0;
       if (a.jmax && blockIdx.x == 0 && (tid >> 3) < rows) {
         a.jmax[(int64_t)b * a.Hq + q] = m * (1.f / LOG2E);

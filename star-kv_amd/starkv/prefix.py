@@ -33,6 +33,8 @@ class SharedPrefix:
         n = int(vs.data.shape[1] if length is None else length)
         if not 1 <= n <= vs.data.shape[1] or not 0 <= row < vs.data.shape[0]:
             raise StarKVError(f"row {row} of the V latent {tuple(vs.data.shape)} does not hold {n} positions")
+        if not k.holds(row + 1, n):
+            raise StarKVError(f"row {row} of the K latent {tuple(k.data.shape)} does not hold {n} positions")
         if k.data.dtype != vs.data.dtype or k.bk.dtype != k.data.dtype:
             raise StarKVError(f"K latents, B_k and V latents must share a type, got {k.data.dtype}, {k.bk.dtype}, "
                               f"{vs.data.dtype}")
@@ -68,8 +70,8 @@ def prefix_decode_attention(q: torch.Tensor, prefix: SharedPrefix, k: Optional[K
     """``decode_attention`` of sequences that all follow ``prefix``: attention
     over its positions, computed once for the batch, and over each sequence's
     own latents (``k``, ``xv``, ``seq_len``, ``mask`` and ``last_pos`` as
-    there; ``k`` and ``xv`` None, or ``seq_len`` 0: none yet).  A sequence
-    whose mask leaves none of its own positions (-inf, or a value as low as a
+    there; ``k`` and ``xv`` None, or ``seq_len`` 0: none yet).  B_k is the
+    layer's, as the prefix was packed with it.  A sequence whose mask leaves none of its own positions (-inf, or a value as low as a
     type's lowest) attends to the prefix alone.
 
     Positions are those of the sequences' own caches: ``q`` [B, Hq, 128] is
@@ -102,8 +104,14 @@ def prefix_decode_attention(q: torch.Tensor, prefix: SharedPrefix, k: Optional[K
         rows = v.data.shape
         if rows[0] < B or rows[1] < n:
             raise StarKVError(f"the V latent {tuple(rows)} does not hold {B} sequences of {n} positions")
+        if not k.holds(B, n):
+            raise StarKVError(f"the K latent {tuple(k.data.shape)} does not hold {B} sequences of {n} positions")
+        if any(t is not None and t.device != device for t in (k.data, v.data, mask, last_pos)):
+            raise StarKVError(f"own latents, mask and last_pos must lie on {device} as q does")
         if k.fmt == FMT_DENSE and k.data.dtype != prefix.dtype or v.fmt == FMT_DENSE and v.data.dtype != prefix.dtype:
             raise StarKVError(f"dense own latents must be {prefix.dtype}, got {k.data.dtype} and {v.data.dtype}")
+    if out is not None and (out.shape != (B, q.shape[1], HEAD_DIM) or out.device != device):
+        raise StarKVError(f"out must be {(B, q.shape[1], HEAD_DIM)} on {device}, got {tuple(out.shape)} on {out.device}")
     if scores is not None:
         _check_scores(scores, B, n, device)
     if device.index != torch.cuda.current_device():

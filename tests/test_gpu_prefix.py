@@ -389,3 +389,66 @@ def test_refusals():
         with pytest.raises(StarKVError):
             f()
             pytest.fail(f"call {i} was not refused")
+
+
+@pytest.mark.parametrize("dense", [True, False])
+def test_own_latents_that_are_no_numbers_show(dense):
+    c = Case(3, 8, 4, 70, 5, 16, 32, 64, torch.float16, seed=51)
+    c.ranks = [16] * 4
+    bk = c.bk[:, :16].contiguous().to(DEV)
+    if dense:
+        k = c.k[..., :16].contiguous().to(DEV)
+        k[1] = math.nan
+        k = KLatentSpec.from_reference(k, bk)
+    else:
+        scale = torch.full((3, 4, 5, 1), 0.01, device=DEV).half()
+        scale[1] = math.nan
+        k = KLatentSpec.from_reference_quant(torch.ones(3, 4, 5, 16, dtype=torch.int8, device=DEV), scale, bk, 16)
+    args = c.q.to(DEV), c.prefix(), k, c.v.to(DEV), c.uv.to(DEV)
+    got = prefix_decode_attention(*args)
+    assert torch.isnan(got[1]).all() and torch.isfinite(got[::2]).all()
+    alone = prefix_decode_attention(args[0], args[1], None, None, args[4])
+    for low in (-math.inf, torch.finfo(torch.float32).min):
+        mask = torch.zeros(3, 1, 5)
+        mask[1] = low
+        got = prefix_decode_attention(*args, mask=mask.to(DEV))
+        # nothing that is masked is looked at: the prefix alone, whose sums another split count may round anew
+        # (fp32, 2^-16 as above) before the output's rounding
+        want = alone[1].float()
+        assert ((got[1].float() - want).abs() <= 2.0 ** -10 * want.abs() + 2.0 ** -14).all()
+
+
+def test_offsets_past_32_bits():
+    """Latents whose rows lie so far apart that byte offsets pass 2^32: the same bits as the same rows packed."""
+    g = torch.Generator().manual_seed(3)
+    P, S, wide = 700, 40, 1 << 22
+    bk = torch.randn(1, 16, 128, generator=g).half().to(DEV)
+    uv, q = torch.randn(128, 32, generator=g).half().to(DEV), torch.randn(2, 2, 128, generator=g).half().to(DEV)
+    base = torch.empty(P, wide, dtype=torch.float16, device=DEV)                   # 5.9 GB
+    pk, pv = base[:, :16], base[:, 64:96]
+    own_k, own_v = [base[:2 * S, a:b].unflatten(0, (S, 2)).transpose(0, 1) for a, b in ((128, 144), (192, 224))]
+    for t in (pk, pv, own_k, own_v):
+        t.copy_(torch.randn(t.shape, generator=g))
+    spec = lambda x: KLatentSpec(x, [16], [0], [x.stride(1)], x.stride(0), bk, [0], 128)
+    run = lambda f: prefix_decode_attention(q, SharedPrefix(spec(f(pk[None])), f(pv[None])), spec(f(own_k)), f(own_v), uv)
+    assert torch.equal(run(lambda t: t), run(lambda t: t.contiguous()))
+
+
+def test_refuses_latents_that_end_before():
+    c = Case(2, 8, 4, 64, 8, 16, 32, 64, torch.float16, seed=47)
+    p, v, uv, q = c.prefix(), c.dev(c.v), c.dev(c.uv), c.q.to(DEV)
+    short = c.spec(c.k[:, :, :7].contiguous().to(DEV), c.bk.to(DEV))
+    one = c.spec(c.k[:1].to(DEV), c.bk.to(DEV))
+    k = c.spec(c.k.to(DEV), c.bk.to(DEV))
+    bad = [
+        lambda: prefix_decode_attention(q, p, short, v, uv),
+        lambda: prefix_decode_attention(q, p, one, v, uv),
+        lambda: prefix_decode_attention(q, p, k, v, uv, out=torch.empty(1, 8, 128, device=DEV).half()),
+        lambda: prefix_decode_attention(q, p, None, None, uv, out=torch.empty(2, 8, 64, device=DEV).half()),
+        lambda: SharedPrefix(short, v, 8, row=1),
+        lambda: SharedPrefix(one, v, 8, row=1),
+    ]
+    for i, f in enumerate(bad):
+        with pytest.raises(StarKVError):
+            f()
+            pytest.fail(f"call {i} was not refused")

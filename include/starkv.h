@@ -631,7 +631,7 @@ int starkv_decode_attention_scores(const starkv_decode_desc* d, float* scores, i
  * `recent`, and of those between the keep - sinks - recent with the largest
  * scores (equal ones: the lowest positions; NaN counts as -infinity).
  * 0 <= sinks + recent <= keep <= length <= 2^24, batch <= 65535.  Workspace:
- * only for rows of more than 32768 positions between (0 otherwise).
+ * only for rows of more than 28672 positions between (0 otherwise).
  * scores (b, p) at scores + b*scores_stride_b + p; positions (b, i) at
  * positions + b*positions_stride_b + i.
  *

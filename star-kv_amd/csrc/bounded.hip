@@ -12,8 +12,8 @@
 //    and only the second kernel runs.  Statistics and sums are fp32.
 // 2. Selection.  select_kernel finds the key (the score's bits, ordered) of the
 //    last position kept by radix selection, 11 + 11 + 10 bits from the top, one
-//    workgroup a row, and writes the kept positions in ascending order with a
-//    running prefix sum: positions above the key, and the first few at it.
+//    workgroup a row (long rows: many), and writes the kept positions in ascending
+//    order by prefix sums: positions above the key, and the first few at it.
 // 3. Moving rows.  Row positions[i] >= i goes to row i.  A workgroup owns a slice
 //    of a row's bytes and takes the rows in order, a chunk at a time: every row
 //    that a chunk writes lies before every row that a later chunk reads, and the
@@ -153,6 +153,7 @@ __global__ __launch_bounds__(256) void score_kernel(const ScoreArgs a) {
 // Selection
 // ---------------------------------------------------------------------------
 constexpr int SEL_T = 1024, SEL_TILE = 4 * SEL_T;
+constexpr int SEL_TILES = 7;                       // whose keys fit LDS beside the histogram
 
 // a score's bits in ascending order of value: NaN counts as -infinity, -0 as 0
 __device__ inline uint32_t score_key(float x) {
@@ -163,18 +164,21 @@ __device__ inline uint32_t score_key(float x) {
 
 constexpr uint32_t ZERO_KEY = 0x80000000u;
 
-// inclusive sum over the wave's lanes
+// inclusive sum over the wave's lanes, in six adds that take another lane's value (by exchanges through LDS four scans cost
+// 2 us of a row's 13)
+template <int CTRL, int ROWS> __device__ inline int dpp_add(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
 __device__ inline int wave_scan(int v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int t = __shfl_up(v, o, 64);
-    if (lane >= o) v += t;
-  }
-  return v;
+  v = dpp_add<0x111, 0xf>(v);                      // 1, 2, 4 and 8 lanes on within rows of 16
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  v = dpp_add<0x118, 0xf>(v);
+  v = dpp_add<0x142, 0xa>(v);                      // a row's sum to the odd rows, that of 32 lanes to the upper 32
+  return dpp_add<0x143, 0xc>(v);
 }
 
-// the keys of candidates t * 4096 + 4 tid .. + 3 of n
+// the keys of candidates t * 4096 + 4 tid .. + 3 of n, 0 behind the last
 __device__ inline void sel_fetch(const float* x, int n, int t, uint32_t (&k)[4]) {
   const int p = t * SEL_TILE + 4 * threadIdx.x;
   float v[4] = {};
@@ -186,7 +190,7 @@ __device__ inline void sel_fetch(const float* x, int n, int t, uint32_t (&k)[4])
       if (p + i < n) v[i] = x[p + i];
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) k[i] = score_key(v[i]);
+  for (int i = 0; i < 4; ++i) k[i] = p + i < n ? score_key(v[i]) : 0;
 }
 
 constexpr int SEL_LOW[3] = {21, 10, 0}, SEL_BITS[3] = {11, 11, 10};
@@ -197,22 +201,29 @@ struct SelShared {
   int found[2];
 };
 
-// counts the pass's digits of a tile's keys whose earlier digits are `key`
-template <int PASS> __device__ inline void sel_count(SelShared& sh, int n, int t, const uint32_t (&k)[4], uint32_t key) {
-  constexpr int low = SEL_LOW[PASS], bits = SEL_BITS[PASS];
-  const int lane = threadIdx.x & 63, p = t * SEL_TILE + 4 * (int)threadIdx.x;
-  // positions that never got any weight are many, and alike: counted by the wave
-  int zeros = 0;
+// counts the digits [low, low + bits) of four keys a thread whose digits above are `key`.  (Keys of no candidate, behind the
+// last, are 0: below every score's, so the largest ones are found before they are reached.)
+__device__ inline void sel_count(SelShared& sh, int low, int bits, const uint32_t (&k)[4], uint32_t key) {
+  const int lane = threadIdx.x & 63, top = low + bits;
+  const uint32_t digits = (1u << bits) - 1;
+  uint32_t* mine = &sh.hist[lane & 3];
+  auto all = [&](auto one) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) zeros += p + i < n && k[i] == ZERO_KEY;
-  if ((PASS == 0 || key == ZERO_KEY >> (low + bits) % 32) && __any(zeros)) {
-    const int all = wave_scan(zeros);
-    if (lane == 63) atomicAdd(&sh.hist[((ZERO_KEY >> low) & ((1u << bits) - 1)) * 4], (uint32_t)all);
+    for (int i = 0; i < 4; ++i)
+      if ((top == 32 || (k[i] >> (top & 31)) == key) && one(k[i])) atomicAdd(mine + ((k[i] >> low) & digits) * 4, 1u);
+  };
+  const bool zero = k[0] == ZERO_KEY || k[1] == ZERO_KEY || k[2] == ZERO_KEY || k[3] == ZERO_KEY;
+  if ((top == 32 || key == ZERO_KEY >> (top & 31)) && __any(zero)) {
+    // positions that never got any weight are many, and alike: counted by the wave
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n += k[i] == ZERO_KEY;
+    n = wave_scan(n);
+    if (lane == 63) atomicAdd(&sh.hist[((ZERO_KEY >> low) & digits) * 4], (uint32_t)n);
+    all([](uint32_t v) { return v != ZERO_KEY; });
+  } else {
+    all([](uint32_t) { return true; });
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (p + i < n && k[i] != ZERO_KEY && (PASS == 0 || (k[i] >> (low + bits) % 32) == key))
-      atomicAdd(&sh.hist[((k[i] >> low) & ((1u << bits) - 1)) * 4 + (lane & 3)], 1u);
 }
 
 // The digit at which the keys counted from the largest down reach `need`, and how many lie above it: thread j brings the
@@ -222,7 +233,8 @@ __device__ inline void sel_find(SelShared& sh, int hi, int lo, int need) {
   int incl = wave_scan(hi + lo);
   if (lane == 63) sh.tot[0][wave] = incl;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) incl += sh.tot[0][w];
+#pragma unroll
+  for (int w = 0; w < 15; ++w) incl += w < wave ? sh.tot[0][w] : 0;
   const int before = incl - hi - lo;
   if (before < need && need <= incl) {
     const bool first = need <= before + hi;
@@ -232,39 +244,27 @@ __device__ inline void sel_find(SelShared& sh, int hi, int lo, int need) {
   __syncthreads();
 }
 
-// Writes a tile's kept positions: those above the key, and of those at it the first `need`; above and at count the
-// tiles before
-__device__ inline void sel_write(SelShared& sh, const SelectArgs& a, int* out, int n, int t, int base, const uint32_t (&k)[4], uint32_t key,
-                                 int need, int& above, int& at) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, p = t * SEL_TILE + 4 * tid;
+// how many of four keys a thread lie above `key` (low half), and at it
+__device__ inline int sel_compare(const uint32_t (&k)[4], uint32_t key) {
   int c = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (p + i < n) c += k[i] > key ? 1 : k[i] == key ? 0x10000 : 0;
-  int incl = wave_scan(c);
-  if (lane == 63) sh.tot[t & 1][wave] = incl;
-  __syncthreads();
-  int all = 0, mine = 0;
-#pragma unroll
-  for (int w = 0; w < 16; ++w) {
-    if (w == wave) mine = all;
-    all += sh.tot[t & 1][w];
-  }
-  incl += mine - c;                                // before this thread, in this tile
-  int g = above + (incl & 0xffff), e = at + (incl >> 16);
+  for (int i = 0; i < 4; ++i) c += k[i] > key ? 1 : k[i] == key ? 0x10000 : 0;
+  return c;
+}
+
+// Writes the kept ones of a thread's four candidates, number p of the row on: those above the key, and of those at
+// it the first `need`; g above and e at it lie before them
+__device__ inline void sel_put(const SelectArgs& a, int* out, int p, const uint32_t (&k)[4], uint32_t key, int need, int g, int e) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if (p + i >= n) continue;
     if (k[i] > key) {
-      out[a.sinks + g + min(e, need)] = a.sinks + base + p + i;
+      out[a.sinks + g + min(e, need)] = a.sinks + p + i;
       ++g;
     } else if (k[i] == key) {
-      if (e < need) out[a.sinks + g + e] = a.sinks + base + p + i;
+      if (e < need) out[a.sinks + g + e] = a.sinks + p + i;
       ++e;
     }
   }
-  above += all & 0xffff;
-  at += all >> 16;
 }
 
 __device__ inline void sel_fixed(const SelectArgs& a, int* out) {
@@ -279,40 +279,71 @@ __global__ __launch_bounds__(SEL_T) void select_all_kernel(const SelectArgs a) {
   for (int i = a.sinks + threadIdx.x; i < a.keep - a.recent; i += SEL_T) out[i] = i;
 }
 
-// One workgroup a row, its NT tiles of 4096 candidates in registers
-template <int NT>
+// One workgroup a row, its keys in LDS.  About 7 us of it are the sixteen barriers, three histograms and the first load
+// (100 positions: 9.5 us with the launch), then 1.5 us a tile of 4096 (8 rows of 8449: 11.6 us, of 16384 14.4): the tile's
+// instructions on its one CU.  A row in pieces takes four launches, 28 us at 100000 positions, so it starts where the keys
+// no longer fit LDS (28672: 19 us here, 27 in pieces).
 __global__ __launch_bounds__(SEL_T) void select_kernel(const SelectArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t sel_keys[];
   __shared__ SelShared sh;
-  const int tid = threadIdx.x;
+  __shared__ int place[SEL_TILES * 16];            // [tile][wave]: above (low half) and at the key, then those before
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float* x = a.scores + blockIdx.x * a.s_sb + a.sinks;
   int* out = a.out + blockIdx.x * a.o_sb;
-  const int n = a.length - a.sinks - a.recent, need0 = a.keep - a.sinks - a.recent, tiles = (n + SEL_TILE - 1) / SEL_TILE;
-  sel_fixed(a, out);
-  uint32_t held[NT][4];
+  const int n = a.length - a.sinks - a.recent, tiles = (n + SEL_TILE - 1) / SEL_TILE;
+#pragma unroll 1
+  for (int j0 = 0; j0 < 4 * tiles; j0 += 16) {
+    float v[16];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) sel_fetch(x, n, t, held[t]);
+    for (int j = 0; j < 16; ++j) v[j] = x[min((j0 + j) * SEL_T + tid, n - 1)];
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (j0 + j < 4 * tiles) sel_keys[(j0 + j) * SEL_T + tid] = (j0 + j) * SEL_T + tid < n ? score_key(v[j]) : 0;
+  }
+  auto four = [&](int t, uint32_t (&k)[4]) { __builtin_memcpy(k, __builtin_assume_aligned(&sel_keys[t * SEL_TILE + 4 * tid], 16), 16); };
   uint32_t key = 0;
-  int need = need0;                                // of the keys that share the digits found so far
-  auto pass = [&](auto P) {
-    constexpr int p = decltype(P)::value;
-    for (int i = tid; i < 2048 * 4; i += SEL_T) sh.hist[i] = 0;
+  int need = a.keep - a.sinks - a.recent;          // of the keys that share the digits found so far
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int low = pass == 0 ? SEL_LOW[0] : pass == 1 ? SEL_LOW[1] : SEL_LOW[2], bits = pass == 2 ? SEL_BITS[2] : SEL_BITS[0];
+    uint4* clear = (uint4*)sh.hist + tid;
+    clear[0] = clear[SEL_T] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-      if (t < tiles) sel_count<p>(sh, n, t, held[t], key);
+#pragma unroll 1
+    for (int t = 0; t < tiles; ++t) {
+      uint32_t k[4];
+      four(t, k);
+      sel_count(sh, low, bits, k, key);
+    }
     __syncthreads();
     const uint4 hi = *(const uint4*)&sh.hist[(2047 - 2 * tid) * 4], lo = *(const uint4*)&sh.hist[(2046 - 2 * tid) * 4];
     sel_find(sh, (int)(hi.x + hi.y + hi.z + hi.w), (int)(lo.x + lo.y + lo.z + lo.w), need);
-    key = (key << SEL_BITS[p]) | (uint32_t)sh.found[0];
+    key = (key << bits) | (uint32_t)sh.found[0];
     need -= sh.found[1];
-  };
-  pass(std::integral_constant<int, 0>());
-  pass(std::integral_constant<int, 1>());
-  pass(std::integral_constant<int, 2>());
-  int above = 0, at = 0;
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-    if (t < tiles) sel_write(sh, a, out, n, t, 0, held[t], key, need, above, at);
+  }
+#pragma unroll 1
+  for (int t = 0; t < tiles; ++t) {
+    uint32_t k[4];
+    four(t, k);
+    const int sum = wave_scan(sel_compare(k, key));
+    if (lane == 63) place[t * 16 + wave] = sum;
+  }
+  sel_fixed(a, out);
+  __syncthreads();
+  if (wave == 0) {                                 // (halves of 16 bits: fewer than 65536 candidates)
+    static_assert(SEL_TILES * 16 <= 128 && SEL_TILES * SEL_TILE < 65536, "two a lane");
+    const int i = 2 * lane, x0 = i < 16 * tiles ? place[i] : 0, x1 = i < 16 * tiles ? place[i + 1] : 0;
+    const int before = wave_scan(x0 + x1) - x0 - x1;
+    if (i < 16 * tiles) { place[i] = before; place[i + 1] = before + x0; }
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int t = 0; t < tiles; ++t) {
+    uint32_t k[4];
+    four(t, k);
+    const int c = sel_compare(k, key), at = place[t * 16 + wave] + wave_scan(c) - c;
+    sel_put(a, out, t * SEL_TILE + 4 * tid, k, key, need, at & 0xffff, at >> 16);
+  }
 }
 
 // Long rows: a workgroup counts the digits of a piece (its own histogram in memory, no atomics between workgroups); the
@@ -326,19 +357,24 @@ __device__ inline void sel_join(SelShared& sh, const SelectArgs& a, int need0, u
   if constexpr (PASS > 1) { const int2 s = a.state[row * 3 + PASS - 2]; key = (uint32_t)s.x; need = s.y; }
   const uint2* h = (const uint2*)(a.hist + ((int64_t)(PASS - 1) * a.B + row) * a.pieces * 2048) + (1023 - tid);
   int hi = 0, lo = 0;
-#pragma unroll 8
-  for (int i = 0; i < a.pieces; ++i) {
-    const uint2 v = h[(int64_t)i * 1024];          // digits 2046 - 2 tid, 2047 - 2 tid
-    lo += (int)v.x;
-    hi += (int)v.y;
+  for (int i0 = 0; i0 < a.pieces; i0 += 16) {
+    uint2 v[16];                                   // digits 2046 - 2 tid, 2047 - 2 tid
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = h[(int64_t)min(i0 + i, a.pieces - 1) * 1024];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      lo += i0 + i < a.pieces ? (int)v[i].x : 0;
+      hi += i0 + i < a.pieces ? (int)v[i].y : 0;
+    }
   }
+  if (PASS == 3 && tid < 512) hi = lo = 0;         // digits past 1023: none (the last word holds another count)
   sel_find(sh, hi, lo, need);
   key = (key << SEL_BITS[PASS - 1]) | (uint32_t)sh.found[0];
   need -= sh.found[1];
   if (blockIdx.x == 0 && tid == 0) a.state[row * 3 + PASS - 1] = make_int2((int)key, need);
 }
 
-// f(tile, keys) for the tiles of a piece, two asked for at a time under the work of the two before
+// f(tile, keys of it and the next) for the tiles of a piece, two at a time, asked for under the work of the two before
 template <typename F> __device__ inline void sel_each(const float* x, int n, F f) {
   const int tiles = (n + SEL_TILE - 1) / SEL_TILE;
   uint32_t k[2][4], cur[2][4];
@@ -351,9 +387,7 @@ template <typename F> __device__ inline void sel_each(const float* x, int n, F f
       for (int j = 0; j < 4; ++j) cur[i][j] = k[i][j];
       sel_fetch(x, n, t + 2 + i, k[i]);
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (t + i < tiles) f(t + i, cur[i]);
+    f(t, cur);
   }
 }
 
@@ -362,12 +396,23 @@ __global__ __launch_bounds__(SEL_T) void select_count_kernel(const SelectArgs a)
   __shared__ SelShared sh;
   const int tid = threadIdx.x, row = blockIdx.y, n = a.length - a.sinks - a.recent, p0 = blockIdx.x * a.piece_len;
   uint32_t key = 0;
-  int need;
+  int need, above = 0;
   if constexpr (PASS > 0) sel_join<PASS>(sh, a, a.keep - a.sinks - a.recent, key, need);
   for (int i = tid; i < 2048 * 4; i += SEL_T) sh.hist[i] = 0;
   __syncthreads();
   const int m = min(a.piece_len, n - p0);
-  sel_each(a.scores + row * a.s_sb + a.sinks + p0, m, [&](int t, const uint32_t (&k)[4]) { sel_count<PASS>(sh, m, t, k, key); });
+  sel_each(a.scores + row * a.s_sb + a.sinks + p0, m, [&](int, const uint32_t (&k)[2][4]) {
+    sel_count(sh, SEL_LOW[PASS], SEL_BITS[PASS], k[0], key);
+    sel_count(sh, SEL_LOW[PASS], SEL_BITS[PASS], k[1], key);
+    if constexpr (PASS == 2) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) above += k[i >> 2][i & 3] >> SEL_BITS[2] > key;
+    }
+  });
+  if constexpr (PASS == 2) {                       // bins that the last pass leaves free: what lies above the key's other digits
+    above = wave_scan(above);
+    if ((tid & 63) == 63) atomicAdd(&sh.hist[2047 * 4], (uint32_t)above);
+  }
   __syncthreads();
   uint2* out = (uint2*)(a.hist + (((int64_t)PASS * a.B + row) * a.pieces + blockIdx.x) * 2048) + tid;
   const uint4 lo = *(const uint4*)&sh.hist[tid * 8], hi = *(const uint4*)&sh.hist[tid * 8 + 4];
@@ -384,16 +429,21 @@ __global__ __launch_bounds__(SEL_T) void select_write_kernel(const SelectArgs a)
   sel_join<3>(sh, a, a.keep - a.sinks - a.recent, key, need);
   // keys above the threshold, and at it, in the pieces before
   int above = 0, at = 0;
+  {
+    const int before = blockIdx.x, digit = (int)(key & 1023);
+    const uint2* h = (const uint2*)(a.hist + ((int64_t)2 * a.B + row) * a.pieces * 2048) + tid;
+    if (tid < 512 || tid == 1023)
+      for (int i0 = 0; i0 < before; i0 += 16) {
+        uint2 v[16];
 #pragma unroll
-  for (int pass = 0; pass < 3; ++pass) {
-    const int digit = (int)((key >> SEL_LOW[pass]) & ((1u << SEL_BITS[pass]) - 1));
-    const uint2* h = (const uint2*)(a.hist + ((int64_t)pass * a.B + row) * a.pieces * 2048) + tid;
-#pragma unroll 4
-    for (int i = 0; i < (int)blockIdx.x; ++i) {
-      const uint2 v = h[(int64_t)i * 1024];
-      above += (2 * tid > digit ? (int)v.x : 0) + (2 * tid + 1 > digit ? (int)v.y : 0);
-      if (pass == 2) at += (2 * tid == digit ? (int)v.x : 0) + (2 * tid + 1 == digit ? (int)v.y : 0);
-    }
+        for (int i = 0; i < 16; ++i) v[i] = h[(int64_t)min(i0 + i, before - 1) * 1024];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if (i0 + i >= before) continue;
+          above += (2 * tid > digit && tid != 1023 ? (int)v[i].x : 0) + (2 * tid + 1 > digit ? (int)v[i].y : 0);
+          if (2 * tid <= digit) at += 2 * tid == digit ? (int)v[i].x : 2 * tid + 1 == digit ? (int)v[i].y : 0;
+        }
+      }
   }
   __syncthreads();
   sh.hist[tid] = (uint32_t)above;
@@ -410,7 +460,30 @@ __global__ __launch_bounds__(SEL_T) void select_write_kernel(const SelectArgs a)
   at = (int)sh.hist[SEL_T];
   const int m = min(a.piece_len, n - p0);
   sel_each(a.scores + row * a.s_sb + a.sinks + p0, m,
-           [&](int t, const uint32_t (&k)[4]) { sel_write(sh, a, out, m, t, p0, k, key, need, above, at); });
+           [&](int t, const uint32_t (&k)[2][4]) {
+    int c[2], sum[2];
+    __syncthreads();                               // the totals before have been read
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      c[i] = sel_compare(k[i], key);
+      sum[i] = wave_scan(c[i]);
+      if ((tid & 63) == 63) sh.tot[i][tid >> 6] = sum[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      int all = 0, mine = 0;
+#pragma unroll
+      for (int w = 0; w < 16; ++w) {
+        if (w == tid >> 6) mine = all;
+        all += sh.tot[i][w];
+      }
+      const int before = sum[i] + mine - c[i];     // of this thread, in this tile
+      sel_put(a, out, p0 + (t + i) * SEL_TILE + 4 * tid, k[i], key, need, above + (before & 0xffff), at + (before >> 16));
+      above += all & 0xffff;
+      at += all >> 16;
+    }
+  });
 }
 
 // ---------------------------------------------------------------------------
@@ -547,7 +620,7 @@ int launch_scores(const ScoreArgs& a, int dtype, bool fused, hipStream_t st) {
 
 // Candidates per workgroup of a long row: at least 8192, at most 64 pieces; 0: one workgroup takes the row
 int select_piece(int n, int keep_of_them) {
-  if (n <= 8 * SEL_TILE || keep_of_them == 0 || keep_of_them == n) return 0;
+  if (n <= SEL_TILES * SEL_TILE || keep_of_them == 0 || keep_of_them == n) return 0;
   return (int)round_up(std::max<int64_t>(8192, ceil_div(n, 64)), SEL_TILE);
 }
 
@@ -562,12 +635,13 @@ int launch_select(const SelectArgs& a, hipStream_t st) {
     hipLaunchKernelGGL(select_write_kernel, pieces, block, 0, st, a);
   } else if (need == 0 || need == n) {
     hipLaunchKernelGGL(select_all_kernel, grid, block, 0, st, a);
-  } else if (tiles <= 1) {
-    hipLaunchKernelGGL(select_kernel<1>, grid, block, 0, st, a);
-  } else if (tiles <= 4) {
-    hipLaunchKernelGGL(select_kernel<4>, grid, block, 0, st, a);
   } else {
-    hipLaunchKernelGGL(select_kernel<8>, grid, block, 0, st, a);
+    const size_t lds = (size_t)tiles * SEL_TILE * 4;
+    if (lds > 16384) {                             // past 64 KB with the histogram: allowed by attribute
+      const int e = (int)hipFuncSetAttribute((const void*)select_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, SEL_TILES * SEL_TILE * 4);
+      if (e) return e;
+    }
+    hipLaunchKernelGGL(select_kernel, grid, block, lds, st, a);
   }
   return (int)hipGetLastError();
 }

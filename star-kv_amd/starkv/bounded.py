@@ -59,7 +59,7 @@ def select_positions(scores: torch.Tensor, keep: int, length: Optional[int] = No
                           f"keep {keep}, length {n}")
     out = _out(B, keep, dtype=torch.int32, device=scores.device)
     d = SelectDesc(B, n, keep, sinks, recent, scores.data_ptr(), scores.stride(0), out.data_ptr(), keep)
-    _launch("starkv_select_positions", d, scores.device, workspace=n > 32768)
+    _launch("starkv_select_positions", d, scores.device, workspace=n > 28672)
     return out
 
 

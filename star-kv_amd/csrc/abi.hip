@@ -1100,7 +1100,7 @@ static int decode_scores(const starkv_decode_desc* d, const DecodeLayout& L, con
   a.B = d->batch; a.H = d->n_q_heads; a.S = d->seq_len; a.add = 1;
   a.rmax = rmax; a.n_max = n_max; a.rsum = rsum; a.n_sum = n_sum; a.n_hg = L.n_hg;
   a.out = scores; a.o_sb = stride;
-  return launch_scores(a, STARKV_F32, true, s);
+  return launch_decode_scores(a, s);
 }
 
 static int check_scores(const starkv_decode_desc* d, const float* scores, int64_t stride) {
@@ -1707,7 +1707,7 @@ int starkv_attention_scores(const starkv_scores_desc* d, void* workspace, size_t
   a.B = d->batch; a.H = d->n_heads; a.S = d->seq_len; a.add = d->add != 0;
   a.stat = (float2*)workspace; a.n_max = score_pieces(d->seq_len);
   a.out = d->scores; a.o_sb = d->scores_stride_b;
-  return launch_scores(a, d->dtype, false, (hipStream_t)stream);
+  return launch_scores(a, d->dtype, (hipStream_t)stream);
 }
 
 int starkv_decode_attention_scores(const starkv_decode_desc* d, float* scores, int64_t scores_stride_b, void* workspace,

@@ -577,7 +577,8 @@ int launch_up_proj(const UPArgs& a, int dtype, bool fast, hipStream_t st);
 int up_slice_width(int n_kv, int Rv, int cus);        // V-rank columns per up-projection workgroup
 int up_chunk_sets(int n_kv, int n_sl, int n_c2, int cus);   // chunk sets per (slice, KV head)
 int score_pieces(int S);                              // pieces of a logit row: their statistics are 8 bytes each
-int launch_scores(const ScoreArgs& a, int dtype, bool fused, hipStream_t st);
+int launch_scores(const ScoreArgs& a, int dtype, hipStream_t st);
+int launch_decode_scores(const ScoreArgs& a, hipStream_t st);  // behind a decode call, whose statistics and fp32 logits they are
 int select_piece(int n, int keep_of_them);
 int launch_select(const SelectArgs& a, hipStream_t st);
 int launch_move(const MoveArgs& a, hipStream_t st);

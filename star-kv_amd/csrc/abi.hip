@@ -2102,12 +2102,11 @@ int starkv_prefix_decode(const starkv_prefix_decode_desc* d, void* workspace, si
       a.ox = o.k.data; a.ox_sb = o.k.stride_b;
       for (int h = 0; h < d->n_kv_heads; ++h) { a.oxoff[h] = o.k.head_offset[h]; a.oxpitch[h] = o.k.pos_stride[h]; }
       a.last_pos = o.last_pos_device;
-      if ((st = launch_own_logits(a, o.dtype, s))) return st;
     } else if ((st = decode_logits(&o, L.own, L.gs, ws, s))) {
       return st;
     }
   }
-  if ((st = launch_prefix_logits(a, o.dtype, s))) return st;
+  if ((st = launch_prefix_logits(a, o.dtype, L.own_here, s))) return st;
   PVArgs pa;
   if (L.has_own && (st = decode_pv(&o, L.own, ws, s, pa))) return st;
   if ((st = launch_prefix_pv(a, s)) || (st = launch_prefix_up(a, o.dtype, o.out_dtype == STARKV_F32, s))) return st;

@@ -583,8 +583,7 @@ int select_piece(int n, int keep_of_them);
 int launch_select(const SelectArgs& a, hipStream_t st);
 int launch_move(const MoveArgs& a, hipStream_t st);
 int launch_prefix_pack(const PrefixPackArgs& a, int dtype, hipStream_t st);
-int launch_prefix_logits(const PrefixArgs& a, int dtype, hipStream_t st);
-int launch_own_logits(const PrefixArgs& a, int dtype, hipStream_t st);
+int launch_prefix_logits(const PrefixArgs& a, int dtype, bool own, hipStream_t st);
 int launch_prefix_pv(const PrefixArgs& a, hipStream_t st);
 int launch_prefix_up(const PrefixArgs& a, int dtype, bool out_f32, hipStream_t st);
 int launch_fill_i32(int* p, int n, int v, hipStream_t st);

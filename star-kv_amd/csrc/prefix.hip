@@ -34,6 +34,7 @@
 // that bounds every key by 2^15, bf16 value latents by one that brings the largest
 // to [2^14, 2^15); each is undone in fp32.
 #include <algorithm>
+#include <type_traits>
 
 #include "fp8.hpp"
 
@@ -212,16 +213,21 @@ __global__ __launch_bounds__(256) void px_pack_kernel(const PrefixPackArgs a) {
 // and at once multiplied with the queries' same dims, so few registers are held and
 // four waves a SIMD cover each other's waits.  KP: pairs of 16 ranks, so that the
 // operand reads and products of a tile are one block of code (a test of the rank
-// before each product left every one waiting for its own read); the dims are a
-// rolled loop (unrolled, a wave that runs through it once or twice waited for
-// instructions: 33 us for 4 x 1024 positions of 8 heads, now 8).
+// before each product left every one waiting for its own read).
+//
+// What bounds it is the vector unit: 32 heads x 32768 positions of 16 rows are
+// 26 GFLOP of products and 134 M rotated pairs (16 us of the 49), which take 16
+// conversions, 64 multiply-adds and 32 exponentials a lane and strip; reads taken
+// out as a trial it still took 44.  Two waves a SIMD with two tiles each took 61,
+// the next keys formed under this rotation at three waves a SIMD 64.
 //
 // NG: groups of 32 query rows.  acc[g][r] += the logits of query row n of group g
 // and positions px_pos, in register order, of the tile whose latents are in xf.
-// PIPE: the next 32 dims' keys are formed under this one's rotation, in code of
-// their own (registers for both; three waves a SIMD).  `between` runs when xf has
-// been used for the last time.
-template <typename XT, int NG, int KP, bool PIPE, typename F>
+// STRAIGHT: the four tiles of dims as straight code (strips that follow one another,
+// 54 us rolled); rolled otherwise: a wave that runs through the code once or twice
+// waited for its instructions (4 x 1024 own positions of 8 heads: 33 us straight, 13
+// rolled).  `between` runs when xf has been used for the last time.
+template <typename XT, int NG, int KP, bool STRAIGHT, typename F>
 __device__ __forceinline__ void px_tile(const uint4* bl, const uint4* ql, const uint4* rope, const uint4 (&xf)[2 * KP], float down,
                                         floatx16 (&acc)[NG], F between) {
   const int lane = threadIdx.x & 63;
@@ -243,7 +249,7 @@ __device__ __forceinline__ void px_tile(const uint4* bl, const uint4* ql, const 
         for (int i = 0; i < 2; ++i) {
           float k0 = kx[4 * g + j + i], k1 = kx[8 + 4 * g + j + i];
           const float c = (float)t[2 * (j + i)], sp = (float)t[2 * (j + i) + 1];
-          if constexpr (!PIPE && __is_same(XT, __bf16)) { k0 *= down; k1 *= down; }
+          if constexpr (!STRAIGHT && __is_same(XT, __bf16)) { k0 *= down; k1 *= down; }
           // (k sin + 0 takes the table's fp16 as it is; a plain product would convert it first)
           l[i] = fmaf(c, k0, -fmaf(sp, k1, 0.f));
           u[i] = fmaf(c, k1, fmaf(sp, k0, 0.f));
@@ -258,7 +264,7 @@ __device__ __forceinline__ void px_tile(const uint4* bl, const uint4* ql, const 
       acc[g] = px_mfma<_Float16>(make_uint4(hi[0], hi[1], hi[2], hi[3]), ql[(g * 8 + 2 * w + 1) * 64 + lane], acc[g]);
     }
   };
-  if constexpr (PIPE) {
+  if constexpr (STRAIGHT) {
     uint4 rt[2][2] = {{rope[0], rope[64]}, {}};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
@@ -421,17 +427,10 @@ __device__ __forceinline__ void px_prefix_logits(const PrefixArgs& a, uint8_t* l
   if (tid < NG * 32 && r0 + tid < nr) a.cmax[(int64_t)chunk * a.Mp + (int64_t)h * nr + r0 + tid] = wm[tid];
 }
 
-template <typename XT, int NG>
-__global__ __launch_bounds__(512, NG == 1 ? 4 : 2) void prefix_logits_kernel(const PrefixArgs a) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t px_lds[];
-  // workgroups of one chunk of strips on one XCD: its L2 serves the rotation table to all heads
-  const int bx = blockIdx.x, chunk = (bx & 7) + 8 * ((bx >> 3) / a.Hkv), h = (bx >> 3) % a.Hkv, kp = (a.rank[h] + 31) / 32;
-  if (chunk >= a.n_ch) return;
-  if (kp == 1) px_prefix_logits<XT, NG, 1>(a, px_lds, chunk, h);
-  else if (kp == 2) px_prefix_logits<XT, NG, 2>(a, px_lds, chunk, h);
-  else if (kp == 3) px_prefix_logits<XT, NG, 3>(a, px_lds, chunk, h);
-  else px_prefix_logits<XT, NG, 4>(a, px_lds, chunk, h);
-}
+// a logit under its mask; one of no number in a place that the mask takes out (at or below a type's lowest value) is not
+// looked at
+constexpr float PX_MASKED = -65504.f;
+__device__ inline float px_mask(float l, float m) { return !(l == l) && m <= PX_MASKED ? -INFINITY : l + m; }
 
 // A sequence's own positions: dense latents where they lie (rows at any alignment),
 // the queries of one KV head and sequence, and the logits go out in fp32 as the
@@ -521,23 +520,26 @@ __device__ __forceinline__ void px_own_logits(const PrefixArgs& a, uint8_t* lds,
         const int64_t at = b * a.m_sb + (h * a.gs + rl) * a.m_sh;
         if (a.mask_dtype == STARKV_F32) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) acc[g][r] += ((const float*)a.mask)[at + min(p0 + r, a.S - 1)];
+          for (int r = 0; r < 16; ++r) acc[g][r] = px_mask(acc[g][r], ((const float*)a.mask)[at + min(p0 + r, a.S - 1)]);
         } else {
           const uint16_t* mk = (const uint16_t*)a.mask + at;
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const uint16_t v = mk[min(p0 + r, a.S - 1)];
-            acc[g][r] += a.mask_dtype == STARKV_F16 ? (float)__builtin_bit_cast(_Float16, v) : bf16_bits_to_float(v);
+            acc[g][r] = px_mask(acc[g][r], a.mask_dtype == STARKV_F16 ? (float)__builtin_bit_cast(_Float16, v) : bf16_bits_to_float(v));
           }
         }
       }
       float m = -INFINITY;
+      bool bad = false;                            // not a number: a maximum of +inf, by which the join makes the row NaN
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         if (p0 + r > last_pos) acc[g][r] = -1e30f;
         if (p0 + r >= a.S) acc[g][r] = -INFINITY;
         m = fmaxf(m, acc[g][r]);
+        bad |= !(acc[g][r] == acc[g][r]);
       }
+      if (bad) m = INFINITY;
       top[g] = fmaxf(top[g], max_halves(m));
       if (rl < a.gs) {
         uint32_t at = (uint32_t)((h * a.gs + rl) * 32 + 16 * hh) * 4;
@@ -552,14 +554,30 @@ __device__ __forceinline__ void px_own_logits(const PrefixArgs& a, uint8_t* lds,
   if (tid < a.gs) a.own_max[((int64_t)b * a.Hq + h * a.gs + tid) * a.n_c1 + chunk] = wm[tid];
 }
 
-template <typename XT, int NG>
-__global__ __launch_bounds__(512, NG == 1 ? 4 : 2) void own_logits_kernel(const PrefixArgs a) {
+// f(a constant of the pairs of 16 ranks)
+template <typename F> __device__ __forceinline__ void px_pairs(int rank, F f) {
+  const int kp = (rank + 31) / 32;
+  if (kp == 1) f(std::integral_constant<int, 1>());
+  else if (kp == 2) f(std::integral_constant<int, 2>());
+  else if (kp == 3) f(std::integral_constant<int, 3>());
+  else f(std::integral_constant<int, 4>());
+}
+
+// The prefix's workgroups, then the sequences' own (NG and NO groups of rows), in one launch: neither fills the chip where
+// prompts are short (8 behind 4099 positions: 11.8 + 11 us one after the other, 13; 4 behind 16384: 27, 20).  One group takes
+// 128 registers, four waves a SIMD; two groups in one workgroup, which form the keys once for 64 rows, two.
+template <typename XT, int NG, int NO>
+__global__ __launch_bounds__(512, NG == 1 ? 4 : 2) void prefix_logits_kernel(const PrefixArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t px_lds[];
-  const int bx = blockIdx.x, chunk = bx % a.n_c1, h = bx / a.n_c1 % a.Hkv, b = bx / a.n_c1 / a.Hkv, kp = (a.rank[h] + 31) / 32;
-  if (kp == 1) px_own_logits<XT, NG, 1>(a, px_lds, chunk, h, b);
-  else if (kp == 2) px_own_logits<XT, NG, 2>(a, px_lds, chunk, h, b);
-  else if (kp == 3) px_own_logits<XT, NG, 3>(a, px_lds, chunk, h, b);
-  else px_own_logits<XT, NG, 4>(a, px_lds, chunk, h, b);
+  const int bx = blockIdx.x, n_prefix = (a.n_ch + 7) / 8 * 8 * a.Hkv;
+  if (bx < n_prefix) {
+    // workgroups of one chunk of strips on one XCD: its L2 serves the rotation table to all heads
+    const int chunk = (bx & 7) + 8 * ((bx >> 3) / a.Hkv), h = (bx >> 3) % a.Hkv;
+    if (chunk < a.n_ch) px_pairs(a.rank[h], [&](auto kp) { px_prefix_logits<XT, NG, decltype(kp)::value>(a, px_lds, chunk, h); });
+  } else if (blockIdx.y == 0) {
+    const int at = bx - n_prefix, chunk = at % a.n_c1, h = at / a.n_c1 % a.Hkv, b = at / a.n_c1 / a.Hkv;
+    px_pairs(a.rank[h], [&](auto kp) { px_own_logits<XT, NO, decltype(kp)::value>(a, px_lds, chunk, h, b); });
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -726,9 +744,9 @@ template <> struct PxTerms<__bf16> { static constexpr int N = 3; };
 // whether element `at` of the mask leaves nothing of a position (as low as the lowest value of a type, or -inf)
 __device__ inline bool px_masked(const PrefixArgs& a, int64_t at) {
   if (a.mask == nullptr) return false;
-  if (a.mask_dtype == STARKV_F32) return ((const float*)a.mask)[at] <= -65504.f;
+  if (a.mask_dtype == STARKV_F32) return ((const float*)a.mask)[at] <= PX_MASKED;
   const uint16_t v = ((const uint16_t*)a.mask)[at];
-  return (a.mask_dtype == STARKV_F16 ? (float)__builtin_bit_cast(_Float16, v) : bf16_bits_to_float(v)) <= -65504.f;
+  return (a.mask_dtype == STARKV_F16 ? (float)__builtin_bit_cast(_Float16, v) : bf16_bits_to_float(v)) <= PX_MASKED;
 }
 
 // Workgroup = (SC columns of the V rank, KV head, 32 of its rows (sequence, head of
@@ -781,13 +799,15 @@ __global__ __launch_bounds__(256) void prefix_up_kernel(const PrefixArgs a) {
       lp += __shfl_xor(lp, o, 8);
       lo += __shfl_xor(lo, o, 8);
     }
-    // no own logit above -inf: all masked, or latents that are not numbers, which have to show
+    // no own logit above -inf: all masked, or (of quantised latents) none that is a number, which has to show
     bool bad = false;
-    if (ms == -INFINITY)
+    if (a.oc_len == 0 && ms == -INFINITY) {
+#pragma unroll 8
       for (int t = i0; t < a.S; t += 8) {
         const float l = a.ol[b * a.ol_sb + (t >> 5) * a.ol_st + q * 32 + (t & 31)];
         bad |= !(l == l) && !px_masked(a, (int64_t)b * a.m_sb + (int64_t)q * a.m_sh + t);
       }
+    }
 #pragma unroll
     for (int o = 4; o >= 1; o >>= 1) bad |= __shfl_xor((int)bad, o, 8) != 0;
     const float m = fmaxf(mp, ms);
@@ -942,26 +962,17 @@ int launch_prefix_pack(const PrefixPackArgs& a, int dtype, hipStream_t st) {
 
 static size_t px_logits_lds(const PrefixArgs& a, int ng) { return (size_t)round_up(a.ks_max, 2) * 4096 + ng * (8192 + 32 * 4 * 9); }
 
-template <typename XT> static void launch_logits(const PrefixArgs& a, hipStream_t st) {
+template <typename XT> static void launch_logits(const PrefixArgs& a, bool own, hipStream_t st) {
   const int groups = (int)ceil_div((int64_t)a.B * a.gs, 32);
-  const dim3 grid((unsigned)(round_up(a.n_ch, 8) * a.Hkv), (unsigned)ceil_div(groups, groups == 1 ? 1 : PX_GROUPS));
-  if (groups == 1) hipLaunchKernelGGL((prefix_logits_kernel<XT, 1>), grid, dim3(512), px_logits_lds(a, 1), st, a);
-  else hipLaunchKernelGGL((prefix_logits_kernel<XT, PX_GROUPS>), grid, dim3(512), px_logits_lds(a, PX_GROUPS), st, a);
+  const dim3 grid((unsigned)(round_up(a.n_ch, 8) * a.Hkv + (own ? a.B * a.Hkv * a.n_c1 : 0)), (unsigned)ceil_div(groups, groups == 1 ? 1 : PX_GROUPS));
+  const size_t lds = px_logits_lds(a, groups == 1 ? 1 : PX_GROUPS);
+  if (groups == 1) hipLaunchKernelGGL((prefix_logits_kernel<XT, 1, 1>), grid, dim3(512), lds, st, a);
+  else if (a.gs <= 32) hipLaunchKernelGGL((prefix_logits_kernel<XT, PX_GROUPS, 1>), grid, dim3(512), lds, st, a);
+  else hipLaunchKernelGGL((prefix_logits_kernel<XT, PX_GROUPS, 2>), grid, dim3(512), lds, st, a);
 }
-int launch_prefix_logits(const PrefixArgs& a, int dtype, hipStream_t st) {
-  if (dtype == STARKV_F16) launch_logits<_Float16>(a, st);
-  else launch_logits<__bf16>(a, st);
-  return (int)hipGetLastError();
-}
-
-template <typename XT> static void launch_own(const PrefixArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)(a.B * a.Hkv * a.n_c1));
-  if (a.gs <= 32) hipLaunchKernelGGL((own_logits_kernel<XT, 1>), grid, dim3(512), px_logits_lds(a, 1), st, a);
-  else hipLaunchKernelGGL((own_logits_kernel<XT, 2>), grid, dim3(512), px_logits_lds(a, 2), st, a);
-}
-int launch_own_logits(const PrefixArgs& a, int dtype, hipStream_t st) {
-  if (dtype == STARKV_F16) launch_own<_Float16>(a, st);
-  else launch_own<__bf16>(a, st);
+int launch_prefix_logits(const PrefixArgs& a, int dtype, bool own, hipStream_t st) {
+  if (dtype == STARKV_F16) launch_logits<_Float16>(a, own, st);
+  else launch_logits<__bf16>(a, own, st);
   return (int)hipGetLastError();
 }
 

@@ -452,3 +452,19 @@ def test_refuses_latents_that_end_before():
         with pytest.raises(StarKVError):
             f()
             pytest.fail(f"call {i} was not refused")
+
+
+@pytest.mark.parametrize("mdtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_padding_that_is_no_number_is_not_looked_at(mdtype):
+    """Own dense K latents of NaN in masked places of rows that keep others: as if they held zeros."""
+    c = Case(3, 8, 4, 130, 40, 16, 32, 64, torch.bfloat16, seed=53)
+    keep = torch.tensor([40, 17, 0])
+    mask = torch.zeros(3, 1, 40).masked_fill_(torch.arange(40) >= keep[:, None, None], torch.finfo(mdtype).min).to(mdtype)
+    pad = (mask[:, 0] < 0)[:, None, :, None]
+    c.k = c.k.masked_fill(pad, 0.0)
+    want = c.run(mask)
+    c.k = c.k.masked_fill(pad, math.nan)
+    assert torch.equal(c.run(mask), want)
+    c.k[1, :, 3] = math.nan
+    got = c.run(mask)
+    assert torch.isnan(got[1]).all() and torch.equal(got[::2], want[::2])

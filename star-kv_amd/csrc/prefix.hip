@@ -216,9 +216,9 @@ __global__ __launch_bounds__(256) void px_pack_kernel(const PrefixPackArgs a) {
 // before each product left every one waiting for its own read).
 //
 // What bounds it is the vector unit: 32 heads x 32768 positions of 16 rows are
-// 26 GFLOP of products and 134 M rotated pairs (16 us of the 49), which take 16
-// conversions, 64 multiply-adds and 32 exponentials a lane and strip; reads taken
-// out as a trial it still took 44.  Two waves a SIMD with two tiles each took 61,
+// 26 GFLOP of products, and 256 multiply-adds of the rotation (16 us of the 49), 64
+// conversions and 32 exponentials a lane and strip; reads taken out as a trial it
+// still took 44.  Two waves a SIMD with two tiles each took 61,
 // the next keys formed under this rotation at three waves a SIMD 64.
 //
 // NG: groups of 32 query rows.  acc[g][r] += the logits of query row n of group g
@@ -596,8 +596,8 @@ template <int N> __device__ inline void px_stage_ready() {
 
 // Workgroup of 8 waves = (split of the strips, BM rows, 256 columns), wave (wm, wn)
 // of WM x WN: RM x RN MFMA tiles, two waves a SIMD.  Steps of 32 positions go
-// through a ring of four LDS stages, three of them in flight; the strips' factors
-// are formed 56 strips at a time.
+// through a ring of four LDS stages, two of them in flight behind the one that is
+// read ahead; the strips' factors are formed 56 strips at a time.
 template <int RM, int RN, int WM, int WN>
 __global__ __launch_bounds__(512, 2) void prefix_pv_kernel(const PrefixArgs a) {
   constexpr int BM = 32 * RM * WM, BN = 32 * RN * WN, RING = 4;
@@ -670,45 +670,58 @@ __global__ __launch_bounds__(512, 2) void prefix_pv_kernel(const PrefixArgs a) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // only copies are counted from here on
 #pragma unroll
   for (int i = 0; i < RING - 1; ++i) issue(i);
+  // operands of 16 positions, read under the products of the 16 before them
+  uint4 fa[2][RM], fb[2][RN];
+  auto read = [&](int slot, int kk) {
+    const uint4* sa = ring + slot * STAGE + (2 * kk + hh) * BM + (wm * RM) * 32 + n;
+    const uint4* sb = ring + slot * STAGE + 4 * BM + (2 * kk + hh) * BN + (wn * RN) * 32 + n;
+#pragma unroll
+    for (int i = 0; i < RM; ++i) fa[kk][i] = sa[32 * i];
+#pragma unroll
+    for (int j = 0; j < RN; ++j) fb[kk][j] = sb[32 * j];
+    __builtin_amdgcn_sched_barrier(0);
+  };
   kh2 fc[RM];
+  auto strip_factors = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < RM; ++i) {
+      const _Float16 f = fac[(t / 2 % FS) * BM + (wm * RM + i) * 32 + n];
+      fc[i] = kh2{f, f};
+    }
+  };
+  auto products = [&](int kk) {
+#pragma unroll
+    for (int i = 0; i < RM; ++i) {
+      uint4 v = fa[kk][i];
+      v.x = __builtin_bit_cast(uint32_t, __builtin_bit_cast(kh2, v.x) * fc[i]);
+      v.y = __builtin_bit_cast(uint32_t, __builtin_bit_cast(kh2, v.y) * fc[i]);
+      v.z = __builtin_bit_cast(uint32_t, __builtin_bit_cast(kh2, v.z) * fc[i]);
+      v.w = __builtin_bit_cast(uint32_t, __builtin_bit_cast(kh2, v.w) * fc[i]);
+#pragma unroll
+      for (int j = 0; j < RN; ++j) acc[i][j] = px_mfma<_Float16>(v, fb[kk][j], acc[i][j]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  px_stage_ready<(RING - 2) * NI>();
+  read(0, 0);
+  strip_factors(0);
   for (int t0 = 0; t0 < steps; t0 += RING) {
     if (t0 && t0 % (2 * FS) == 0) {
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");        // the last ones have been used
       factors(t0 / 2);
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      strip_factors(t0);
     }
 #pragma unroll
     for (int u = 0; u < RING; ++u) {
       if (t0 + u >= steps) break;
-      px_stage_ready<(RING - 2) * NI>();
+      px_stage_ready<(RING - 3) * NI>();           // the next step's copies; all reads of the one before have ended
       issue((u + RING - 1) % RING);
-      if (u % 2 == 0) {
-#pragma unroll
-        for (int i = 0; i < RM; ++i) {
-          const _Float16 f = fac[((t0 + u) / 2 % FS) * BM + (wm * RM + i) * 32 + n];
-          fc[i] = kh2{f, f};
-        }
-      }
-      const uint4* sa = ring + u * STAGE + (wm * RM) * 32 + n;
-      const uint4* sb = ring + u * STAGE + 4 * BM + (wn * RN) * 32 + n;
-#pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        uint4 fa[RM], fb[RN];
-#pragma unroll
-        for (int j = 0; j < RN; ++j) fb[j] = sb[(2 * kk + hh) * BN + 32 * j];
-#pragma unroll
-        for (int i = 0; i < RM; ++i) {
-          const uint4 v = sa[(2 * kk + hh) * BM + 32 * i];
-          fa[i].x = __builtin_bit_cast(uint32_t, __builtin_bit_cast(kh2, v.x) * fc[i]);
-          fa[i].y = __builtin_bit_cast(uint32_t, __builtin_bit_cast(kh2, v.y) * fc[i]);
-          fa[i].z = __builtin_bit_cast(uint32_t, __builtin_bit_cast(kh2, v.z) * fc[i]);
-          fa[i].w = __builtin_bit_cast(uint32_t, __builtin_bit_cast(kh2, v.w) * fc[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < RM; ++i)
-#pragma unroll
-          for (int j = 0; j < RN; ++j) acc[i][j] = px_mfma<_Float16>(fa[i], fb[j], acc[i][j]);
-      }
+      read(u, 1);
+      products(0);
+      read((u + 1) % RING, 0);
+      products(1);
+      if (u % 2) strip_factors(t0 + u + 1);        // (stale where they are formed anew, and read again there)
     }
   }
   if (tid < BM) {

@@ -754,6 +754,10 @@ template <typename WT> struct PxTerms;
 template <> struct PxTerms<_Float16> { static constexpr int N = 2; };
 template <> struct PxTerms<__bf16> { static constexpr int N = 3; };
 
+// threads: with few workgroups more of them to ask for the partials (4 behind 16384 positions: 13.4 us, 256 threads 16.8),
+// with many fewer (batch 16 behind 32768: 24 of 256, 29 of 512)
+template <int SC> constexpr int PX_UP_T = SC == 128 ? 256 : 512;
+
 // whether element `at` of the mask leaves nothing of a position (as low as the lowest value of a type, or -inf)
 __device__ inline bool px_masked(const PrefixArgs& a, int64_t at) {
   if (a.mask == nullptr) return false;
@@ -768,17 +772,18 @@ __device__ inline bool px_masked(const PrefixArgs& a, int64_t at) {
 // divided by the weights' sum, and multiplies them by its columns of U_v: a term of
 // the output, [column slice][row][128], that prefix_finish_kernel adds up.
 template <typename WT, int SC>
-__global__ __launch_bounds__(256) void prefix_up_kernel(const PrefixArgs a) {
-  constexpr int NT = PxTerms<WT>::N, PIECES = 32 * SC / 8, PP = PIECES >= 256 ? PIECES / 256 : 1, GR = PIECES >= 256 ? 1 : 256 / PIECES;
+__global__ __launch_bounds__(PX_UP_T<SC>) void prefix_up_kernel(const PrefixArgs a) {
+  constexpr int NT = PxTerms<WT>::N, PIECES = 32 * SC / 8, T = PX_UP_T<SC>, RL = T / 32;
+  constexpr int PP = PIECES > T ? PIECES / T : 1, GR = PIECES > T ? 1 : T / PIECES;
   __shared__ uint4 op[NT][SC / 8][32];             // the rows' terms, [8 columns][row]
   __shared__ float wsplit[32][PX_MAX_SPLITS + 1], wown[32];
   __shared__ uint32_t row_top[32];
   __shared__ float red[GR > 1 ? (GR - 1) * PIECES : 1][8];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hh = lane >> 5, n = lane & 31;
   const int j0 = blockIdx.x * SC, h = blockIdx.y, nr = a.B * a.gs, r0 = blockIdx.z * 32, rows = min(32, nr - r0);
-  // this wave's 32 dims of U_v: lane n one, 8 columns a piece
+  // 32 dims of U_v of each of the first four waves: lane n one, 8 columns a piece
   uint4 uf[SC / 16];
-  const WT* u = (const WT*)a.uv + (int64_t)(h * HEAD_DIM + 32 * wave + n) * a.uv_rs;
+  const WT* u = (const WT*)a.uv + (int64_t)(h * HEAD_DIM + 32 * (wave & 3) + n) * a.uv_rs;
 #pragma unroll
   for (int k = 0; k < SC / 16; ++k) {
     const int c = j0 + 16 * k + 8 * hh;
@@ -791,77 +796,83 @@ __global__ __launch_bounds__(256) void prefix_up_kernel(const PrefixArgs a) {
       __builtin_memcpy(&uf[k], e, 16);
     }
   }
-  // the rows' weights, eight lanes a row
+  // the rows' weights, RL lanes a row
   {
-    const int r = min(tid >> 3, rows - 1), i0 = tid & 7, row = h * nr + r0 + r, b = (r0 + r) / a.gs, q = h * a.gs + (r0 + r) % a.gs;
+    const int r = min(tid / RL, rows - 1), i0 = tid % RL, row = h * nr + r0 + r, b = (r0 + r) / a.gs, q = h * a.gs + (r0 + r) % a.gs;
     const int64_t bq = (int64_t)b * a.n_hg + (q >> 5);
     const float mp = a.rmax[row];
     float ms = -INFINITY;                          // in units of log 2, as the prefix's
-    for (int c = i0; c < a.n_c1; c += 8) ms = fmaxf(ms, a.own_max[((int64_t)b * a.Hq + q) * a.n_c1 + c] * LOG2E);
+    for (int c = i0; c < a.n_c1; c += RL) ms = fmaxf(ms, a.own_max[((int64_t)b * a.Hq + q) * a.n_c1 + c] * LOG2E);
     float lp = 0.f, lo = 0.f;
-    for (int s = i0; s < a.n_split; s += 8) {
+    for (int s = i0; s < a.n_split; s += RL) {
       const float l = a.lsum[(int64_t)s * a.Mp + row];
-      wsplit[tid >> 3][s] = l;
+      wsplit[tid / RL][s] = l;
       lp += l;
     }
     const float* psum = a.own_sum + bq * a.n_c2 * 32 + (q & 31);
-    for (int c = i0; c < a.n_c2; c += 8) lo += psum[(int64_t)c * 32];
+    for (int c = i0; c < a.n_c2; c += RL) lo += psum[(int64_t)c * 32];
 #pragma unroll
-    for (int o = 4; o >= 1; o >>= 1) {
-      ms = fmaxf(ms, __shfl_xor(ms, o, 8));
-      lp += __shfl_xor(lp, o, 8);
-      lo += __shfl_xor(lo, o, 8);
+    for (int o = RL / 2; o >= 1; o >>= 1) {
+      ms = fmaxf(ms, __shfl_xor(ms, o, RL));
+      lp += __shfl_xor(lp, o, RL);
+      lo += __shfl_xor(lo, o, RL);
     }
     // no own logit above -inf: all masked, or (of quantised latents) none that is a number, which has to show
     bool bad = false;
     if (a.oc_len == 0 && ms == -INFINITY) {
 #pragma unroll 8
-      for (int t = i0; t < a.S; t += 8) {
+      for (int t = i0; t < a.S; t += RL) {
         const float l = a.ol[b * a.ol_sb + (t >> 5) * a.ol_st + q * 32 + (t & 31)];
         bad |= !(l == l) && !px_masked(a, (int64_t)b * a.m_sb + (int64_t)q * a.m_sh + t);
       }
     }
 #pragma unroll
-    for (int o = 4; o >= 1; o >>= 1) bad |= __shfl_xor((int)bad, o, 8) != 0;
+    for (int o = RL / 2; o >= 1; o >>= 1) bad |= __shfl_xor((int)bad, o, RL) != 0;
     const float m = fmaxf(mp, ms);
     const float wp = __builtin_amdgcn_exp2f((mp - m) - PX_LIFT);
     // own positions without weight are not looked at (their sums may be NaN)
     const float wo = bad ? NAN : ms > -INFINITY ? __builtin_amdgcn_exp2f(ms - m) : 0.f;
     const float l = wo == 0.f ? lp * wp : lp * wp + lo * wo, inv = 1.f / l;
-    for (int s = i0; s < a.n_split; s += 8) wsplit[tid >> 3][s] *= 2.f * a.head[1] * wp * inv;
+    for (int s = i0; s < a.n_split; s += RL) wsplit[tid / RL][s] *= 2.f * a.head[1] * wp * inv;
     if (i0 == 0) {
-      wown[tid >> 3] = wo == 0.f ? 0.f : wo * inv;
-      row_top[tid >> 3] = 0;
-      if (a.jmax && blockIdx.x == 0 && (tid >> 3) < rows) {
+      wown[tid / RL] = wo == 0.f ? 0.f : wo * inv;
+      row_top[tid / RL] = 0;
+      if (a.jmax && blockIdx.x == 0 && (tid / RL) < rows) {
         a.jmax[(int64_t)b * a.Hq + q] = m * (1.f / LOG2E);
         a.jsum[bq * 32 + (q & 31)] = l;
       }
     }
   }
   __syncthreads();
-  float v[PP][8];
+  // piece i of this thread: 8 columns (from 8 ec) of row er + i * T / (SC / 8), the splits grp, grp + GR, ...
+  float v[PP][8] = {};
+  const int e = tid % PIECES, grp = GR == 1 ? 0 : tid / PIECES, er = e / (SC / 8), ec = e % (SC / 8);
+  constexpr int RS = T / (SC / 8);
 #pragma unroll
   for (int i = 0; i < PP; ++i) {
-    const int e = tid % PIECES + 256 * i, grp = tid / PIECES, r = e / (SC / 8), c = j0 + e % (SC / 8) * 8;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[i][k] = 0.f;
+    const int r = er + i * RS, c = j0 + 8 * ec;
     if (r >= rows || c >= a.Rvp) continue;
     const int b = (r0 + r) / a.gs, q = h * a.gs + (r0 + r) % a.gs;
     const _Float16* p = a.part + (int64_t)(h * nr + r0 + r) * a.Rvp + c;
     const int64_t step = (int64_t)a.M * a.Rvp;
-#pragma unroll 8
-    for (int s = grp; s < a.n_split; s += GR) {
-      const half8 x = *(const half8*)(p + s * step);
-      const float f = wsplit[r][s];
+    for (int s0 = grp; s0 < a.n_split; s0 += 8 * GR) {
+      half8 x[8] = {};
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[i][k] = fmaf((float)x[k], f, v[i][k]);
+      for (int g = 0; g < 8; ++g)
+        if (s0 + GR * g < a.n_split) x[g] = *(const half8*)(p + (s0 + GR * g) * step);
+#pragma unroll
+      for (int g = 0; g < 8; ++g) {
+        if (s0 + GR * g >= a.n_split) break;
+        const float f = wsplit[r][s0 + GR * g];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[i][k] = fmaf((float)x[g][k], f, v[i][k]);
+      }
     }
     const float wo = wown[r];
-    if (wo == 0.f) continue;
     const int64_t bq = (int64_t)b * a.n_hg + (q >> 5);
     const float* psum = a.own_sum + bq * a.n_c2 * 32 + (q & 31);
 #pragma unroll 4
-    for (int s = grp; s < a.n_c2; s += GR) {
+    for (int s = grp; s < (wo == 0.f ? 0 : a.n_c2); s += GR) {
       const int64_t at = ((bq * a.n_c2 + s) * 32 + (q & 31)) * a.own_Rvp + c;
       if (a.own_part16) {
         const half8 x = *(const half8*)((const _Float16*)a.own_part + at);
@@ -880,7 +891,6 @@ __global__ __launch_bounds__(256) void prefix_up_kernel(const PrefixArgs a) {
     }
   }
   if constexpr (GR > 1) {
-    const int e = tid % PIECES, grp = tid / PIECES;
     if (grp) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) red[(grp - 1) * PIECES + e][k] = v[0][k];
@@ -892,23 +902,22 @@ __global__ __launch_bounds__(256) void prefix_up_kernel(const PrefixArgs a) {
         for (int k = 0; k < 8; ++k) v[0][k] += red[g * PIECES + e][k];
     }
   }
-  const bool holds = GR == 1 || tid < PIECES;
   // columns past the rank hold what their tiles left (the packed zeros' sums, or none at all of own positions)
 #pragma unroll
   for (int i = 0; i < PP; ++i) {
-    const int e = tid % PIECES + 256 * i, c = j0 + e % (SC / 8) * 8;
-    uint32_t top = 0;
+    uint32_t most = 0;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      if (c + k >= a.Rv) v[i][k] = 0.f;
-      top = max(top, __float_as_uint(v[i][k]) & 0x7fffffffu);
+      if (j0 + 8 * ec + k >= a.Rv) v[i][k] = 0.f;
+      most = max(most, __float_as_uint(v[i][k]) & 0x7fffffffu);
     }
-    if (__is_same(WT, _Float16) && holds) atomicMax(&row_top[e / (SC / 8)], top);
+    if (__is_same(WT, _Float16) && grp == 0) atomicMax(&row_top[er + i * RS], most);
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < PP; ++i) {
-    const int e = tid % PIECES + 256 * i, r = e / (SC / 8);
+    if (grp) continue;
+    const int r = er + i * RS;
     float f = 1.f;
     if constexpr (__is_same(WT, _Float16)) f = pow2f(-px_row_exp(row_top[r]));
     WT w[NT][8];
@@ -921,12 +930,11 @@ __global__ __launch_bounds__(256) void prefix_up_kernel(const PrefixArgs a) {
         x -= (float)w[t][k];
       }
     }
-    if (holds) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t) __builtin_memcpy(&op[t][e % (SC / 8)][r], w[t], 16);
-    }
+    for (int t = 0; t < NT; ++t) __builtin_memcpy(&op[t][ec][r], w[t], 16);
   }
   __syncthreads();
+  if (wave >= 4) return;
   floatx16 acc = {};
 #pragma unroll
   for (int k = 0; k < SC / 16; ++k)
@@ -999,9 +1007,9 @@ int launch_prefix_pv(const PrefixArgs& a, hipStream_t st) {
 
 template <typename WT> static void launch_up(const PrefixArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)a.n_sl, (unsigned)a.Hkv, (unsigned)ceil_div((int64_t)a.B * a.gs, 32));
-  if (a.sc == 128) hipLaunchKernelGGL((prefix_up_kernel<WT, 128>), grid, dim3(256), 0, st, a);
-  else if (a.sc == 64) hipLaunchKernelGGL((prefix_up_kernel<WT, 64>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((prefix_up_kernel<WT, 32>), grid, dim3(256), 0, st, a);
+  if (a.sc == 128) hipLaunchKernelGGL((prefix_up_kernel<WT, 128>), grid, dim3(PX_UP_T<128>), 0, st, a);
+  else if (a.sc == 64) hipLaunchKernelGGL((prefix_up_kernel<WT, 64>), grid, dim3(PX_UP_T<64>), 0, st, a);
+  else hipLaunchKernelGGL((prefix_up_kernel<WT, 32>), grid, dim3(PX_UP_T<32>), 0, st, a);
 }
 int launch_prefix_up(const PrefixArgs& a, int dtype, bool out_f32, hipStream_t st) {
   if (dtype == STARKV_F16) launch_up<_Float16>(a, st);

@@ -33,6 +33,12 @@
 // Range: queries are scaled by a power of two to [1, 2) per row, K latents by one
 // that bounds every key by 2^15, bf16 value latents by one that brings the largest
 // to [2^14, 2^15); each is undone in fp32.
+//
+// Roundings to fp16, as the decode kernels have them: the query after its turn, the
+// key after its rotation, the rotation's table (2^-11 each, of the vectors' lengths: a
+// logit's error, of which a matrix operand of 16 bits takes the first two in any case);
+// weights, strip factors and split means (2^-11 of a term).  Statistics and sums are
+// fp32, and the up-projection takes its operand in terms that keep 22 bits or more.
 #include <algorithm>
 #include <type_traits>
 
@@ -223,8 +229,8 @@ __global__ __launch_bounds__(256) void px_pack_kernel(const PrefixPackArgs a) {
 //
 // NG: groups of 32 query rows.  acc[g][r] += the logits of query row n of group g
 // and positions px_pos, in register order, of the tile whose latents are in xf.
-// STRAIGHT: the four tiles of dims as straight code (strips that follow one another,
-// 54 us rolled); rolled otherwise: a wave that runs through the code once or twice
+// STRAIGHT: the four tiles of dims as straight code (strips that follow one another;
+// with own positions 64 us, rolled 70); rolled otherwise: a wave that runs through the code once or twice
 // waited for its instructions (4 x 1024 own positions of 8 heads: 33 us straight, 13
 // rolled).  `between` runs when xf has been used for the last time.
 template <typename XT, int NG, int KP, bool STRAIGHT, typename F>
@@ -597,7 +603,11 @@ template <int N> __device__ inline void px_stage_ready() {
 // Workgroup of 8 waves = (split of the strips, BM rows, 256 columns), wave (wm, wn)
 // of WM x WN: RM x RN MFMA tiles, two waves a SIMD.  Steps of 32 positions go
 // through a ring of four LDS stages, two of them in flight behind the one that is
-// read ahead; the strips' factors are formed 56 strips at a time.
+// read ahead; the strips' factors are formed 56 strips at a time.  Weights and
+// factors are fp16 (2^-11 of each position's term, of either sign), sums fp32.
+// 512 rows x 32768 positions x 1640 columns: 69 us, 871 TFLOP/s of the tiles' products
+// (1792 columns), 66 with every load from the caches: matrix unit and LDS reads,
+// nearly level (operands read when they are needed, not a step ahead: 74).
 template <int RM, int RN, int WM, int WN>
 __global__ __launch_bounds__(512, 2) void prefix_pv_kernel(const PrefixArgs a) {
   constexpr int BM = 32 * RM * WM, BN = 32 * RN * WN, RING = 4;
@@ -770,7 +780,9 @@ __device__ inline bool px_masked(const PrefixArgs& a, int64_t at) {
 // the group)).  It adds the rows' sums over the prefix's splits and over their own
 // positions' chunks, in a fixed order, relative to the larger of the two maxima and
 // divided by the weights' sum, and multiplies them by its columns of U_v: a term of
-// the output, [column slice][row][128], that prefix_finish_kernel adds up.
+// the output, [column slice][row][128], that prefix_finish_kernel adds up.  Batch 16
+// behind 32768: 18 splits of 512 rows, 30 MB, in 24 us; where workgroups are few (13 to
+// 15 us) two to four batches of loads, one after another.
 template <typename WT, int SC>
 __global__ __launch_bounds__(PX_UP_T<SC>) void prefix_up_kernel(const PrefixArgs a) {
   constexpr int NT = PxTerms<WT>::N, PIECES = 32 * SC / 8, T = PX_UP_T<SC>, RL = T / 32;

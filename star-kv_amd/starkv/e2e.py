@@ -714,18 +714,18 @@ def share_prompt(model, prompt: torch.Tensor) -> torch.Tensor:
         raise StarKVError(f"share_prompt: the prompt must be [1, P] with P at least 1, got {tuple(prompt.shape)}")
     atts = attention_layers(model)
     P, dev = prompt.shape[1], prompt.device
-    own = [(att.cache, att.scores) for att in atts]
+    own = [(att.cache, att.scores, att.prefix) for att in atts]
     model.model.norm.starkv_reference = False
     try:
-        for att, (c, _) in zip(atts, own):
+        for att, (c, _, _) in zip(atts, own):
             att.reference = False
             att.prefix = att.scores = None
             att.cache = LatentCache(1, c.ranks, c.Rv, P, c.dtype, c.device, c.fmt)
         out = model(input_ids=prompt, position_ids=torch.arange(P, device=dev)[None], use_cache=False, logits_to_keep=1)
         prefixes = [att.cache.share(att.bk, att.rope) for att in atts]
     finally:
-        for att, (c, s) in zip(atts, own):
-            att.cache, att.scores = c, s
+        for att, (c, s, before) in zip(atts, own):
+            att.cache, att.scores, att.prefix = c, s, before
     for att, prefix in zip(atts, prefixes):
         att.prefix = prefix
         att.cache.length = 0

@@ -44,6 +44,7 @@ class SharedPrefix:
         self.length, self.ranks, self.v_rank, self.rope = n, list(k.ranks), vs.rank, rope
         self.span = -(-n // 64) * 64               # positions of the rotation table that the kernels read
         self.dtype, self.device = k.data.dtype, vs.data.device
+        rope_table(rope, self.span, self.device)   # here, not in a decode call that may be captured
         keep: list = []
         d = PrefixPackDesc()
         d.length, d.dtype = n, _dt(k.data)

@@ -468,3 +468,23 @@ def test_padding_that_is_no_number_is_not_looked_at(mdtype):
     c.k[1, :, 3] = math.nan
     got = c.run(mask)
     assert torch.isnan(got[1]).all() and torch.equal(got[::2], want[::2])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shape", [
+    # more than 32 query heads a KV head; the widest V; column slices of 128 and 64; KV heads up to 64, one query head each
+    (2, 64, 1, 100, 40, 100, 128, 65), (3, 40, 1, 70, 33, 17, 33, 40), (2, 64, 1, 64, 1, 1, 7, 33), (3, 16, 4, 500, 77, 64, 128, 8192),
+    (16, 32, 32, 200, 9, 8, 96, 1000), (2, 32, 32, 130, 70, 8, 96, 600), (1, 64, 64, 90, 300, 1, 128, 200)], ids=str)
+def test_matches_definition_at_the_ends(shape, dtype):
+    c = Case(*shape, dtype, seed=sum(shape), pad=shape[3] % 3)
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_long_splits(dtype):
+    """So many tiles of P V that a split holds all 121 strips: the strips' factors are formed anew on the way."""
+    c = Case(64, 32, 1, 7700, 0, 128, 128, 8192, dtype, seed=61)
+    got = c.run()
+    pick = [0, 17, 63]
+    c.q, c.B = c.q[pick], len(pick)                       # the definition of some sequences
+    c.check(got[pick])

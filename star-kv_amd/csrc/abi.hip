@@ -553,14 +553,17 @@ int check_mask(const void* mask, int mask_dtype) {
 // ---- P.V geometry: workgroup = 4 waves x NTW column tiles of one position chunk
 struct PVGeom {
   int Rvp, n_cb, n_c2, c2_len, n_grp;   // n_grp > 1: two-level split reduction
+  int ntw;                              // column tiles per wave
 };
 
 // row_bytes: the largest row pitch (bytes) of the V latent's streams; the
 // kernel addresses a chunk with 32-bit offsets, so a chunk stays below 2 GB
-PVGeom pv_geometry(int B, int S, int Rv, bool fused, int vq, int64_t row_bytes) {
+// ntw: column tiles per wave (0: as the storage kind asks)
+PVGeom pv_geometry(int B, int S, int Rv, bool fused, int vq, int64_t row_bytes, int ntw = 0) {
   PVGeom g;
   g.Rvp = (int)round_up(Rv, 32);
-  const int ntw = pv_tiles_per_wave(g.Rvp, fused, vq);
+  if (!ntw) ntw = pv_tiles_per_wave(g.Rvp, fused, vq);
+  g.ntw = ntw;
   // one 8-wave workgroup for all columns (its 24-bit row offsets need
   // every pitch below 16 MB)
   const bool wide = pv_wide_tiles(g.Rvp, fused, vq) > 0 && row_bytes < V_MAX_PITCH;
@@ -607,7 +610,7 @@ struct DecodeLayout {
 // V keeps them in fp16 there too, halving the partials' share of its traffic
 // (55 of 613 MB at B16 S32768), dense V in fp32.
 DecodeLayout decode_layout(int B, int Hq, int Hkv, int S, int Rv, int n_wg, int k1pc, int vq, int64_t v_row_bytes,
-                           bool f16) {
+                           bool f16, int pv_ntw = 0) {
   DecodeLayout L;
   L.S_pad = (int)round_up(S, 64);
   const int n_tiles = (int)ceil_div(S, TILE);
@@ -616,7 +619,7 @@ DecodeLayout decode_layout(int B, int Hq, int Hkv, int S, int Rv, int n_wg, int 
   L.tiles_per_chunk = (int)ceil_div(n_tiles, L.n_c1);
   L.n_c1 = (int)ceil_div(n_tiles, L.tiles_per_chunk);
   L.n_hg = head_groups(Hq);
-  L.pv = pv_geometry(B * L.n_hg, S, Rv, true, vq, v_row_bytes);
+  L.pv = pv_geometry(B * L.n_hg, S, Rv, true, vq, v_row_bytes, pv_ntw);
   L.sw = up_slice_width(Hkv, Rv, cus);
   L.n_sl = (int)ceil_div(Rv, L.sw);
   L.n_cs = up_chunk_sets(Hkv, L.n_sl, L.pv.n_c2, cus);
@@ -1088,7 +1091,7 @@ static int decode_pv(const starkv_decode_desc* d, const DecodeLayout& L, char* w
   pa.chunkmax = (const float*)(ws + L.off_cmax); pa.n_chunk1 = L.n_c1;
   pa.part = (float*)(ws + L.off_part); pa.psum = (float*)(ws + L.off_psum); pa.part16 = L.part16;
   pa.S = d->seq_len; pa.H = Hq; pa.n_hg = L.n_hg; pa.Rv = d->v.rank; pa.Rvp = L.pv.Rvp;
-  pa.n_cb = L.pv.n_cb; pa.n_c2 = L.pv.n_c2; pa.c2_len = L.pv.c2_len;
+  pa.n_cb = L.pv.n_cb; pa.n_c2 = L.pv.n_c2; pa.c2_len = L.pv.c2_len; pa.ntw = L.pv.ntw;
   return launch_pv(pa, d->dtype, vq, true, v_fast(d->v, pa), B, s);
 }
 
@@ -1876,6 +1879,10 @@ int starkv_keep_positions(const starkv_keep_desc* d, void* stream) {
 // ---------------------------------------------------------------------------
 namespace {
 
+// Up to so many own positions P V takes four column tiles a wave: more column blocks and fewer splits, whose partials are
+// most of what short ones move (with the join, 8 x 333 of bf16, Rv 1228: 27 us, as decode has it 33; 16 x 512 of fp16, Rv
+// 1640: 34, 41; 16 x 2048: 49, 53; 16 x 8192: 118, 112)
+constexpr int PX_OWN_SHORT = 4096;
 constexpr int64_t PX_MAX_ROWS = 1 << 20;           // (sequence, query head) rows of a call
 
 // offsets of a packed prefix
@@ -1964,7 +1971,7 @@ int prefix_layout(const starkv_prefix_decode_desc* d, PrefixLayout& L) {
     for (int h = 0; h < d->n_kv_heads; ++h)
       if (o.k.rank[h] != d->rank[h]) return STARKV_ERR_SHAPE;
     L.own = decode_layout(o.batch, o.n_q_heads, d->n_kv_heads, o.seq_len, o.v.rank, n_wg, k1pc, vq, v_row_bytes(o.v),
-                          o.dtype == STARKV_F16);
+                          o.dtype == STARKV_F16, vq == VQ_DENSE && o.seq_len <= PX_OWN_SHORT ? 4 : 0);
     L.own_here = own_logits_here(o);
     if (L.own_here) {
       // chunks of at least one tile a wave, two workgroups a CU
@@ -2069,7 +2076,7 @@ int starkv_prefix_decode(const starkv_prefix_decode_desc* d, void* workspace, si
   if (!al(workspace, 256)) return STARKV_ERR_ALIGN;
   char* ws = (char*)workspace;
   hipStream_t s = (hipStream_t)stream;
-  PrefixArgs a = {};
+  PrefixLogitsArgs a = {};
   const char* p = (const char*)d->prefix;
   a.head = (const float*)p; a.xk = (const uint8_t*)p + L.space.off_xk; a.xb = (const uint8_t*)p + L.space.off_xb;
   a.xv = (const uint4*)(p + L.space.off_xv);

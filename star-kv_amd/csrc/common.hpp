@@ -128,6 +128,7 @@ struct PVArgs {
   float* part2; int n_grp;                         // drop-in two-level reduction: [B*n_hg][n_grp][32][Rvp]
   void* out; int64_t o_sb, o_sh;                   // drop-in: act-dtype [B][H][Rv]
   int S, H, n_hg, Rv, Rvp, n_cb, n_c2, c2_len;
+  int ntw;                                         // fused: column tiles per wave (0: as the storage kind asks)
 };
 
 // ---------------------------------------------------------------------------
@@ -384,9 +385,6 @@ struct PrefixPackArgs {
 };
 struct PrefixArgs {
   const float* head; const uint8_t* xk; const uint8_t* xb; const uint4* xv;
-  int64_t xkoff[K_MAX_KV], xboff[K_MAX_KV];
-  int rank[K_MAX_KV];
-  float cos_p[64], sin_p[64];                      // the rotation by P positions
   const uint4* rope;
   const void* q; int64_t q_sb, q_sh;
   float scale;
@@ -400,9 +398,9 @@ struct PrefixArgs {
   // own positions (n_c1 = 0: none): the decode kernels' maxima, sums and partials
   float* own_max; const float* own_sum; const void* own_part;
   int n_c1, n_c2, n_hg, own_Rvp, own_part16;
-  // ... for own_logits_kernel (dense latents)
+  // ... whose logits are formed with the prefix's (dense latents; oc_len 0: they are there)
   int S, oc_len;                                   // positions; tiles of 32 in one of their n_c1 chunks
-  const void* ox; int64_t ox_sb, oxoff[K_MAX_KV], oxpitch[K_MAX_KV];       // elements
+  const void* ox; int64_t ox_sb;                   // elements
   const void* mask; int64_t m_sb, m_sh; int mask_dtype;
   const int* last_pos;
   float* ol; int64_t ol_sb, ol_st;                 // logits [b][32 positions][Hq][32]
@@ -412,6 +410,12 @@ struct PrefixArgs {
   int Rv, sc, n_sl;                                // columns of a slice, slices
   float* ypart;
   void* out; int64_t o_sb, o_sh;
+};
+// what the logits alone read of each head (as arguments of every launch they cost the host 0.6 to 1.6 us a call)
+struct PrefixLogitsArgs : PrefixArgs {
+  int64_t xkoff[K_MAX_KV], xboff[K_MAX_KV], oxoff[K_MAX_KV], oxpitch[K_MAX_KV];
+  int rank[K_MAX_KV];
+  float cos_p[64], sin_p[64];                      // the rotation by P positions
 };
 
 // A decode step's cache writes and query rotation in one launch (quant.hip)
@@ -425,7 +429,7 @@ struct StepAppendArgs {
 
 // these are passed by value as kernel arguments (at most 4 KiB)
 static_assert(sizeof(KArgs) <= 4096 && sizeof(PFArgs) <= 4096 && sizeof(StepAppendArgs) <= 4096 && sizeof(MoveArgs) <= 4096 &&
-                  sizeof(PrefixPackArgs) <= 4096 && sizeof(PrefixArgs) <= 4096,
+                  sizeof(PrefixPackArgs) <= 4096 && sizeof(PrefixLogitsArgs) <= 4096,
               "kernel argument size");
 
 // ---------------------------------------------------------------------------
@@ -583,7 +587,7 @@ int select_piece(int n, int keep_of_them);
 int launch_select(const SelectArgs& a, hipStream_t st);
 int launch_move(const MoveArgs& a, hipStream_t st);
 int launch_prefix_pack(const PrefixPackArgs& a, int dtype, hipStream_t st);
-int launch_prefix_logits(const PrefixArgs& a, int dtype, bool own, hipStream_t st);
+int launch_prefix_logits(const PrefixLogitsArgs& a, int dtype, bool own, hipStream_t st);
 int launch_prefix_pv(const PrefixArgs& a, hipStream_t st);
 int launch_prefix_up(const PrefixArgs& a, int dtype, bool out_f32, hipStream_t st);
 int launch_fill_i32(int* p, int n, int v, hipStream_t st);

@@ -300,7 +300,7 @@ __device__ __forceinline__ void px_tile(const uint4* bl, const uint4* ql, const 
 // B_k's operands of one head and the query rows r0 .. of it into LDS: the rows of (sequence, head of the group) from
 // sequence b0 on, turned by (cos, sin), scaled to [1, 2) by a power of two each, in the operand's order
 template <typename XT, int NG, int KP, int NW>
-__device__ __forceinline__ void px_stage(const PrefixArgs& a, int h, int b0, int r0, int nr, float cs, float sn, float kmul, uint4* bl,
+__device__ __forceinline__ void px_stage(const PrefixLogitsArgs& a, int h, int b0, int r0, int nr, float cs, float sn, float kmul, uint4* bl,
                                          uint4* ql, float* mul) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, ks_n = ((a.rank[h] + 7) / 8 + 1) / 2;
   const uint4* src = (const uint4*)(a.xb + a.xboff[h]);
@@ -347,7 +347,7 @@ template <int NG, int NW> __device__ __forceinline__ void px_row_max(const float
 
 // Workgroup of eight waves = (chunk of strips, KV head, NG groups of rows), a wave a strip at a time.
 template <typename XT, int NG, int KP>
-__device__ __forceinline__ void px_prefix_logits(const PrefixArgs& a, uint8_t* lds, int chunk, int h) {
+__device__ __forceinline__ void px_prefix_logits(const PrefixLogitsArgs& a, uint8_t* lds, int chunk, int h) {
   constexpr int KS = 2 * KP;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5, n = lane & 31;
   const int nr = a.B * a.gs, r0 = blockIdx.y * NG * 32, nc = (a.rank[h] + 7) / 8;
@@ -443,7 +443,7 @@ __device__ inline float px_mask(float l, float m) { return !(l == l) && m <= PX_
 // decode's P.V kernels read them.  Workgroup = (sequence, KV head, chunk of tiles
 // of 32 positions), a wave a tile at a time.
 template <typename XT, int NG, int KP>
-__device__ __forceinline__ void px_own_logits(const PrefixArgs& a, uint8_t* lds, int chunk, int h, int b) {
+__device__ __forceinline__ void px_own_logits(const PrefixLogitsArgs& a, uint8_t* lds, int chunk, int h, int b) {
   constexpr int KS = 2 * KP;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5, n = lane & 31;
   const int rank = a.rank[h], nc = (rank + 7) / 8, tail = rank & 7, pn = px_pos(n);
@@ -573,7 +573,7 @@ template <typename F> __device__ __forceinline__ void px_pairs(int rank, F f) {
 // prompts are short (8 behind 4099 positions: 11.8 + 11 us one after the other, 13; 4 behind 16384: 27, 20).  One group takes
 // 128 registers, four waves a SIMD; two groups in one workgroup, which form the keys once for 64 rows, two.
 template <typename XT, int NG, int NO>
-__global__ __launch_bounds__(512, NG == 1 ? 4 : 2) void prefix_logits_kernel(const PrefixArgs a) {
+__global__ __launch_bounds__(512, NG == 1 ? 4 : 2) void prefix_logits_kernel(const PrefixLogitsArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t px_lds[];
   const int bx = blockIdx.x, n_prefix = (a.n_ch + 7) / 8 * 8 * a.Hkv;
   if (bx < n_prefix) {
@@ -993,9 +993,9 @@ int launch_prefix_pack(const PrefixPackArgs& a, int dtype, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
-static size_t px_logits_lds(const PrefixArgs& a, int ng) { return (size_t)round_up(a.ks_max, 2) * 4096 + ng * (8192 + 32 * 4 * 9); }
+static size_t px_logits_lds(const PrefixLogitsArgs& a, int ng) { return (size_t)round_up(a.ks_max, 2) * 4096 + ng * (8192 + 32 * 4 * 9); }
 
-template <typename XT> static void launch_logits(const PrefixArgs& a, bool own, hipStream_t st) {
+template <typename XT> static void launch_logits(const PrefixLogitsArgs& a, bool own, hipStream_t st) {
   const int groups = (int)ceil_div((int64_t)a.B * a.gs, 32);
   const dim3 grid((unsigned)(round_up(a.n_ch, 8) * a.Hkv + (own ? a.B * a.Hkv * a.n_c1 : 0)), (unsigned)ceil_div(groups, groups == 1 ? 1 : PX_GROUPS));
   const size_t lds = px_logits_lds(a, groups == 1 ? 1 : PX_GROUPS);
@@ -1003,7 +1003,7 @@ template <typename XT> static void launch_logits(const PrefixArgs& a, bool own, 
   else if (a.gs <= 32) hipLaunchKernelGGL((prefix_logits_kernel<XT, PX_GROUPS, 1>), grid, dim3(512), lds, st, a);
   else hipLaunchKernelGGL((prefix_logits_kernel<XT, PX_GROUPS, 2>), grid, dim3(512), lds, st, a);
 }
-int launch_prefix_logits(const PrefixArgs& a, int dtype, bool own, hipStream_t st) {
+int launch_prefix_logits(const PrefixLogitsArgs& a, int dtype, bool own, hipStream_t st) {
   if (dtype == STARKV_F16) launch_logits<_Float16>(a, own, st);
   else launch_logits<__bf16>(a, own, st);
   return (int)hipGetLastError();

@@ -1645,7 +1645,7 @@ static void launch_pv_wide_n(const PVArgs& a, int vq, bool fast, int B, hipStrea
 
 template <typename VT, bool FUSED>
 static int launch_pv_t(const PVArgs& a, int vq, bool fast, int B, hipStream_t st) {
-  const int ntw = pv_tiles_per_wave(a.Rvp, FUSED, vq);
+  const int ntw = a.ntw ? a.ntw : pv_tiles_per_wave(a.Rvp, FUSED, vq);
   const int BQ = B * a.n_hg;
   if constexpr (FUSED) {
     // the host's geometry chose the all-columns kernel (one column block)

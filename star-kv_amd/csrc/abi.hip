@@ -558,10 +558,12 @@ struct PVGeom {
 
 // row_bytes: the largest row pitch (bytes) of the V latent's streams; the
 // kernel addresses a chunk with 32-bit offsets, so a chunk stays below 2 GB
-// ntw: column tiles per wave (0: as the storage kind asks)
+// ntw: column tiles per wave (0: as the storage kind asks; given behind a shared prefix, where a partial costs four times
+// as much: the join reads it again with few workgroups, 8 x 333 of bf16 27 us -> 24, 4 x 1024 22 -> 20, twelve times 24 and 22)
 PVGeom pv_geometry(int B, int S, int Rv, bool fused, int vq, int64_t row_bytes, int ntw = 0) {
   PVGeom g;
   g.Rvp = (int)round_up(Rv, 32);
+  const double part_cost = ntw ? 4.0 : 1.0;
   if (!ntw) ntw = pv_tiles_per_wave(g.Rvp, fused, vq);
   g.ntw = ntw;
   // one 8-wave workgroup for all columns (its 24-bit row offsets need
@@ -579,7 +581,7 @@ PVGeom pv_geometry(int B, int S, int Rv, bool fused, int vq, int64_t row_bytes, 
   const double vbytes = vq == VQ_DENSE ? 2.0 * Rv : Rv / 2.0 + 4.0 * ceil_div(Rv, 64);
   // (below ~8K positions the launch is latency-bound and partials are cheap)
   const double frac = 32.0 * g.Rvp * 8.0 / g.n_cb / ((double)std::max(S, 8192) * (vbytes / g.n_cb + 128.0));
-  int n = choose_splits((int64_t)B * g.n_cb, device_cus() * wg_per_cu, n_ks, 512, 4.0, frac);
+  int n = choose_splits((int64_t)B * g.n_cb, device_cus() * wg_per_cu, n_ks, 512, 4.0, part_cost * frac);
   const int64_t max_ks = std::max<int64_t>(1, ((int64_t)1 << 31) / std::max<int64_t>(row_bytes, 1) / KSTEP);
   n = std::max<int64_t>(n, ceil_div(n_ks, max_ks));
   g.c2_len = (int)ceil_div(n_ks, n) * KSTEP;

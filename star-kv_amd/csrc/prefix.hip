@@ -768,14 +768,6 @@ template <> struct PxTerms<__bf16> { static constexpr int N = 3; };
 // with many fewer (batch 16 behind 32768: 24 of 256, 29 of 512)
 template <int SC> constexpr int PX_UP_T = SC == 128 ? 256 : 512;
 
-// whether element `at` of the mask leaves nothing of a position (as low as the lowest value of a type, or -inf)
-__device__ inline bool px_masked(const PrefixArgs& a, int64_t at) {
-  if (a.mask == nullptr) return false;
-  if (a.mask_dtype == STARKV_F32) return ((const float*)a.mask)[at] <= PX_MASKED;
-  const uint16_t v = ((const uint16_t*)a.mask)[at];
-  return (a.mask_dtype == STARKV_F16 ? (float)__builtin_bit_cast(_Float16, v) : bf16_bits_to_float(v)) <= PX_MASKED;
-}
-
 // Workgroup = (SC columns of the V rank, KV head, 32 of its rows (sequence, head of
 // the group)).  It adds the rows' sums over the prefix's splits and over their own
 // positions' chunks, in a fixed order, relative to the larger of the two maxima and
@@ -829,21 +821,10 @@ __global__ __launch_bounds__(PX_UP_T<SC>) void prefix_up_kernel(const PrefixArgs
       lp += __shfl_xor(lp, o, RL);
       lo += __shfl_xor(lo, o, RL);
     }
-    // no own logit above -inf: all masked, or (of quantised latents) none that is a number, which has to show
-    bool bad = false;
-    if (a.oc_len == 0 && ms == -INFINITY) {
-#pragma unroll 8
-      for (int t = i0; t < a.S; t += RL) {
-        const float l = a.ol[b * a.ol_sb + (t >> 5) * a.ol_st + q * 32 + (t & 31)];
-        bad |= !(l == l) && !px_masked(a, (int64_t)b * a.m_sb + (int64_t)q * a.m_sh + t);
-      }
-    }
-#pragma unroll
-    for (int o = RL / 2; o >= 1; o >>= 1) bad |= __shfl_xor((int)bad, o, RL) != 0;
     const float m = fmaxf(mp, ms);
     const float wp = __builtin_amdgcn_exp2f((mp - m) - PX_LIFT);
     // own positions without weight are not looked at (their sums may be NaN)
-    const float wo = bad ? NAN : ms > -INFINITY ? __builtin_amdgcn_exp2f(ms - m) : 0.f;
+    const float wo = ms > -INFINITY ? __builtin_amdgcn_exp2f(ms - m) : 0.f;
     const float l = wo == 0.f ? lp * wp : lp * wp + lo * wo, inv = 1.f / l;
     for (int s = i0; s < a.n_split; s += RL) wsplit[tid / RL][s] *= 2.f * a.head[1] * wp * inv;
     if (i0 == 0) {
@@ -962,18 +943,43 @@ __global__ __launch_bounds__(PX_UP_T<SC>) void prefix_up_kernel(const PrefixArgs
   }
 }
 
-// the output: the terms of the column slices added in order
+// whether element `at` of the mask leaves nothing of a position (as low as the lowest value of a type, or -inf)
+__device__ inline bool px_masked(const PrefixArgs& a, int64_t at) {
+  if (a.mask == nullptr) return false;
+  if (a.mask_dtype == STARKV_F32) return ((const float*)a.mask)[at] <= PX_MASKED;
+  const uint16_t v = ((const uint16_t*)a.mask)[at];
+  return (a.mask_dtype == STARKV_F16 ? (float)__builtin_bit_cast(_Float16, v) : bf16_bits_to_float(v)) <= PX_MASKED;
+}
+
+// The output: the terms of the column slices added in order.  Of quantised own latents the logits' maxima pass over what is
+// no number: a row that has none above -inf is looked through here, and NaN unless its mask takes them all out.
 template <typename OT>
 __global__ __launch_bounds__(256) void prefix_finish_kernel(const PrefixArgs a) {
-  const int row = blockIdx.x * 2 + (threadIdx.x >> 7), d = threadIdx.x & 127, nr = a.B * a.gs;
-  if (row >= a.M) return;
+  __shared__ int live[2], bad[2];
+  const int half = threadIdx.x >> 7, row = min(blockIdx.x * 2 + half, a.M - 1), d = threadIdx.x & 127, nr = a.B * a.gs;
+  const int h = row / nr, b = row % nr / a.gs, q = h * a.gs + row % a.gs;
   const float* p = a.ypart + (int64_t)row * HEAD_DIM + d;
   const int64_t step = (int64_t)a.M * HEAD_DIM;
   float s = 0.f;
 #pragma unroll 8
   for (int i = 0; i < a.n_sl; ++i) s += p[i * step];
-  const int h = row / nr, b = row % nr / a.gs, q = h * a.gs + row % a.gs;
-  ((OT*)a.out)[b * a.o_sb + q * a.o_sh + d] = (OT)s;
+  if (a.n_c1 && a.oc_len == 0) {
+    if (d == 0) live[half] = bad[half] = 0;
+    __syncthreads();
+    for (int c = d; c < a.n_c1; c += 128)
+      if (a.own_max[((int64_t)b * a.Hq + q) * a.n_c1 + c] > -INFINITY) live[half] = 1;
+    __syncthreads();
+    if (!live[half]) {
+#pragma unroll 8
+      for (int t = d; t < a.S; t += 128) {
+        const float l = a.ol[b * a.ol_sb + (t >> 5) * a.ol_st + q * 32 + (t & 31)];
+        if (!(l == l) && !px_masked(a, (int64_t)b * a.m_sb + (int64_t)q * a.m_sh + t)) bad[half] = 1;
+      }
+    }
+    __syncthreads();
+    if (bad[half]) s = NAN;
+  }
+  if ((int)(blockIdx.x * 2 + half) < a.M) ((OT*)a.out)[b * a.o_sb + q * a.o_sh + d] = (OT)s;
 }
 
 }  // namespace

@@ -773,8 +773,8 @@ template <int SC> constexpr int PX_UP_T = SC == 128 ? 256 : 512;
 // positions' chunks, in a fixed order, relative to the larger of the two maxima and
 // divided by the weights' sum, and multiplies them by its columns of U_v: a term of
 // the output, [column slice][row][128], that prefix_finish_kernel adds up.  Batch 16
-// behind 32768: 18 splits of 512 rows, 30 MB, in 24 us; where workgroups are few (13 to
-// 15 us) two to four batches of loads, one after another.
+// behind 32768: 18 splits of 512 rows, 30 MB, and own partials in 19 us; where workgroups
+// are few (11 to 13 us) two to four batches of loads, one after another.
 template <typename WT, int SC>
 __global__ __launch_bounds__(PX_UP_T<SC>) void prefix_up_kernel(const PrefixArgs a) {
   constexpr int NT = PxTerms<WT>::N, PIECES = 32 * SC / 8, T = PX_UP_T<SC>, RL = T / 32;

@@ -394,3 +394,16 @@ def test_keep_refuses_shared_rows():
             keep_positions(spec, v, p, 8)
     with pytest.raises(StarKVError):
         keep_positions(KLatentSpec(k0[:, :, :7], [16], [0], [16], k0.stride(0), k0, [0], 128), v, p, 8)
+
+
+@pytest.mark.parametrize("between", [28672, 28673, 57345])
+@pytest.mark.parametrize("kind", ["spread", "one value", "all -inf"])
+def test_select_where_rows_begin_to_be_split(between, kind):
+    """The longest row of one workgroup, the shortest in pieces, and a last piece of one position."""
+    g = torch.Generator().manual_seed(between)
+    x = torch.exp(2 * torch.randn(2, between + 9, generator=g))
+    if kind != "spread":
+        x.fill_(1.5 if kind == "one value" else -math.inf)
+    for keep in (10, between // 3, between + 8):
+        got = select_positions(x.to(DEV), keep, sinks=4, recent=5)
+        assert torch.equal(got.cpu(), select_oracle(x, keep, between + 9, 4, 5))

@@ -687,7 +687,8 @@ int starkv_keep_positions(const starkv_keep_desc* d, void* stream);
  * the prefix was packed with (dense latents meet the packed one); own.seq_len 0:
  * no own positions (k, v, mask and last_pos_device are not read).  A sequence
  * whose mask leaves none of its own positions attends to the prefix alone; own
- * logits that are NaN and not masked make its output NaN.
+ * logits that are NaN and not masked (at or below -65504, or behind
+ * last_pos_device) make its output NaN, and with it its weights in scores.
  * turn_cos / turn_sin: host arrays [64], the (unscaled) rotation of frequency i
  * by `length` positions.  The prefix's rank, v_rank, length and dtype are those
  * it was packed with; rope_max_positions >= round_up(length, 64).  scores

@@ -952,7 +952,8 @@ __device__ inline bool px_masked(const PrefixArgs& a, int64_t at) {
 }
 
 // The output: the terms of the column slices added in order.  Of quantised own latents the logits' maxima pass over what is
-// no number: a row that has none above -inf is looked through here, and NaN unless its mask takes them all out.
+// no number, and the join over the sums of own positions without weight: such a row (all its maxima -inf, or as far below the
+// prefix as a finite mask or last_pos_device puts them) is looked through here, and NaN unless its mask takes them all out.
 template <typename OT>
 __global__ __launch_bounds__(256) void prefix_finish_kernel(const PrefixArgs a) {
   __shared__ int live[2], bad[2];
@@ -966,8 +967,11 @@ __global__ __launch_bounds__(256) void prefix_finish_kernel(const PrefixArgs a) 
   if (a.n_c1 && a.oc_len == 0) {
     if (d == 0) live[half] = bad[half] = 0;
     __syncthreads();
-    for (int c = d; c < a.n_c1; c += 128)
-      if (a.own_max[((int64_t)b * a.Hq + q) * a.n_c1 + c] > -INFINITY) live[half] = 1;
+    const float mp = a.rmax[row];
+    for (int c = d; c < a.n_c1; c += 128) {        // (a weight that the join takes for 0 is 0 here)
+      const float ms = a.own_max[((int64_t)b * a.Hq + q) * a.n_c1 + c] * LOG2E;
+      if (ms > -INFINITY && __builtin_amdgcn_exp2f(ms - fmaxf(mp, ms)) != 0.f) live[half] = 1;
+    }
     __syncthreads();
     if (!live[half]) {
 #pragma unroll 8
@@ -977,7 +981,10 @@ __global__ __launch_bounds__(256) void prefix_finish_kernel(const PrefixArgs a) 
       }
     }
     __syncthreads();
-    if (bad[half]) s = NAN;
+    if (bad[half]) {
+      s = NAN;
+      if (a.jmax && d == 0) a.jsum[((int64_t)b * a.n_hg + (q >> 5)) * 32 + (q & 31)] = NAN;   // and every weight of the row
+    }
   }
   if ((int)(blockIdx.x * 2 + half) < a.M) ((OT*)a.out)[b * a.o_sb + q * a.o_sh + d] = (OT)s;
 }

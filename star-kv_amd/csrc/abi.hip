@@ -2019,7 +2019,7 @@ int prefix_layout(const starkv_prefix_decode_desc* d, PrefixLayout& L) {
   take(L.off_stat, (size_t)strips * Mp * 8);
   take(L.off_cmax, (size_t)L.n_ch * Mp * 4);
   take(L.off_rmax, Mp * 4);
-  take(L.off_part, (size_t)L.n_split * L.M * Rvp * 2);
+  take(L.off_part, (size_t)L.n_split * L.M * Rvp * 4);
   take(L.off_lsum, (size_t)L.n_split * Mp * 4);
   take(L.off_jsum, BQ * 32 * 4);
   take(L.off_jmax, (size_t)L.M * 4);
@@ -2094,7 +2094,7 @@ int starkv_prefix_decode(const starkv_prefix_decode_desc* d, void* workspace, si
   a.p = (uint4*)(ws + L.off_p); a.stat = (float2*)(ws + L.off_stat);
   a.cmax = (float*)(ws + L.off_cmax); a.n_ch = L.n_ch; a.ch_len = L.ch_len; a.rmax = (float*)(ws + L.off_rmax);
   a.bm = L.bm; a.tiles_m = L.tiles_m; a.tiles_n = L.tiles_n; a.n_split = L.n_split; a.sp_len = L.sp_len;
-  a.part = (_Float16*)(ws + L.off_part); a.lsum = (float*)(ws + L.off_lsum);
+  a.part = (float*)(ws + L.off_part); a.lsum = (float*)(ws + L.off_lsum);
   a.n_hg = L.n_hg; a.jsum = (float*)(ws + L.off_jsum);
   a.uv = o.uv; a.uv_rs = o.uv_row_stride; a.Rv = d->v_rank; a.sc = L.sc; a.n_sl = L.n_sl; a.ypart = (float*)(ws + L.off_ypart);
   a.out = o.out; a.o_sb = o.out_stride_b; a.o_sh = o.out_stride_h;

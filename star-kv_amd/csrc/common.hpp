@@ -394,7 +394,7 @@ struct PrefixArgs {
   float* cmax; int n_ch, ch_len;                   // maxima [chunk][row], strips of a logits chunk
   float* rmax;                                     // [row]
   int bm, tiles_m, tiles_n, n_split, sp_len;       // P V: tile rows, tiles, splits and their strips
-  _Float16* part; float* lsum;                     // [split][M][Rvp] means / 2, [split][Mp] sums
+  float* part; float* lsum;                        // [split][M][Rvp] means, [split][Mp] sums
   // own positions (n_c1 = 0: none): the decode kernels' maxima, sums and partials
   float* own_max; const float* own_sum; const void* own_part;
   int n_c1, n_c2, n_hg, own_Rvp, own_part16;

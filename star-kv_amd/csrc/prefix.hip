@@ -23,8 +23,8 @@
 //    brought to the row's maximum over the whole prefix by a factor
 //    2^15 exp(strip maximum - row maximum) on the operand: strips 2^-29 below the
 //    row's largest weight still keep all bits of fp16.  Each split's sums leave
-//    divided by its weights' sum, in fp16 (half of them: a mean of values up to
-//    65504 that is rounded up stays finite).
+//    divided by its weights' sum, in fp32: fp16 means of values that cancel, or that
+//    are small beside the latent's largest, would be subnormal.
 // 3. prefix_up_kernel adds the splits and, if the sequences have positions of
 //    their own, the decode kernels' sums over those, in a fixed order, relative to
 //    the larger of the two maxima, and multiplies them by U_v; prefix_finish_kernel
@@ -37,8 +37,9 @@
 // Roundings to fp16, as the decode kernels have them: the query after its turn, the
 // key after its rotation, the rotation's table (2^-11 each, of the vectors' lengths: a
 // logit's error, of which a matrix operand of 16 bits takes the first two in any case);
-// weights, strip factors and split means (2^-11 of a term).  Statistics and sums are
-// fp32, and the up-projection takes its operand in terms that keep 22 bits or more.
+// weights and strip factors (2^-11 of a term).  Statistics, sums and split means are
+// fp32, and the up-projection takes its operand in terms that keep 22 bits or more (fp16:
+// of what is above 2^-18 of a row's largest value, 2^-39 of it below).
 #include <algorithm>
 #include <type_traits>
 
@@ -618,7 +619,7 @@ __global__ __launch_bounds__(512, 2) void prefix_pv_kernel(const PrefixArgs a) {
   static_assert(WM * WN == 8 && BN == PX_BN, "eight waves");
   __shared__ uint4 ring[RING * STAGE];
   __shared__ _Float16 fac[FS * BM];                // [strip][row]
-  __shared__ float row_f[BM];                      // 1 / (2 sum)
+  __shared__ float row_f[BM];                      // 1 / sum
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hh = lane >> 5, n = lane & 31;
   const int wm = wave / WN, wn = wave % WN;
   // consecutive (split, tile) pairs on one XCD: a split's tiles share its weights and latents in that L2
@@ -735,11 +736,11 @@ __global__ __launch_bounds__(512, 2) void prefix_pv_kernel(const PrefixArgs a) {
     }
   }
   if (tid < BM) {
-    row_f[tid] = lsum == 0.f ? 0.f : 0.5f / lsum;
+    row_f[tid] = lsum == 0.f ? 0.f : 1.f / lsum;
     if (n0 == 0) a.lsum[(int64_t)split * a.Mp + m0 + tid] = lsum;
   }
   px_stage_ready<0>();                             // the sums, and the last copies before the LDS is another's
-  _Float16* out = a.part + ((int64_t)split * a.M + m0) * a.Rvp + n0;
+  float* out = a.part + ((int64_t)split * a.M + m0) * a.Rvp + n0;
 #pragma unroll
   for (int i = 0; i < RM; ++i)
 #pragma unroll
@@ -750,7 +751,7 @@ __global__ __launch_bounds__(512, 2) void prefix_pv_kernel(const PrefixArgs a) {
 #pragma unroll
       for (int j = 0; j < RN; ++j) {
         const int col = (wn * RN + j) * 32 + n;
-        if (n0 + col < a.Rvp) out[(int64_t)row * a.Rvp + col] = (_Float16)(acc[i][j][r] * inv);
+        if (n0 + col < a.Rvp) out[(int64_t)row * a.Rvp + col] = acc[i][j][r] * inv;
       }
     }
 }
@@ -826,7 +827,7 @@ __global__ __launch_bounds__(PX_UP_T<SC>) void prefix_up_kernel(const PrefixArgs
     // own positions without weight are not looked at (their sums may be NaN)
     const float wo = ms > -INFINITY ? __builtin_amdgcn_exp2f(ms - m) : 0.f;
     const float l = wo == 0.f ? lp * wp : lp * wp + lo * wo, inv = 1.f / l;
-    for (int s = i0; s < a.n_split; s += RL) wsplit[tid / RL][s] *= 2.f * a.head[1] * wp * inv;
+    for (int s = i0; s < a.n_split; s += RL) wsplit[tid / RL][s] *= a.head[1] * wp * inv;
     if (i0 == 0) {
       wown[tid / RL] = wo == 0.f ? 0.f : wo * inv;
       row_top[tid / RL] = 0;
@@ -846,19 +847,23 @@ __global__ __launch_bounds__(PX_UP_T<SC>) void prefix_up_kernel(const PrefixArgs
     const int r = er + i * RS, c = j0 + 8 * ec;
     if (r >= rows || c >= a.Rvp) continue;
     const int b = (r0 + r) / a.gs, q = h * a.gs + (r0 + r) % a.gs;
-    const _Float16* p = a.part + (int64_t)(h * nr + r0 + r) * a.Rvp + c;
+    const float* p = a.part + (int64_t)(h * nr + r0 + r) * a.Rvp + c;
     const int64_t step = (int64_t)a.M * a.Rvp;
     for (int s0 = grp; s0 < a.n_split; s0 += 8 * GR) {
-      half8 x[8] = {};
+      floatx4 x[8][2] = {};
 #pragma unroll
       for (int g = 0; g < 8; ++g)
-        if (s0 + GR * g < a.n_split) x[g] = *(const half8*)(p + (s0 + GR * g) * step);
+        if (s0 + GR * g < a.n_split) {
+          const floatx4* from = (const floatx4*)(p + (s0 + GR * g) * step);
+          x[g][0] = from[0];
+          x[g][1] = from[1];
+        }
 #pragma unroll
       for (int g = 0; g < 8; ++g) {
         if (s0 + GR * g >= a.n_split) break;
         const float f = wsplit[r][s0 + GR * g];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[i][k] = fmaf((float)x[g][k], f, v[i][k]);
+        for (int k = 0; k < 8; ++k) v[i][k] = fmaf(x[g][k >> 2][k & 3], f, v[i][k]);
       }
     }
     const float wo = wown[r];

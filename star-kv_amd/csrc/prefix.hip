@@ -31,8 +31,9 @@
 //    adds the products of its column slices.
 //
 // Range: queries are scaled by a power of two to [1, 2) per row, K latents by one
-// that bounds every key by 2^15, bf16 value latents by one that brings the largest
-// to [2^14, 2^15); each is undone in fp32.
+// that bounds every key by 2^15 (the prefix's by one for all, dense own ones by one
+// for each position), bf16 value latents by one that brings the largest to [2^14,
+// 2^15); each is undone in fp32.
 //
 // Roundings to fp16, as the decode kernels have them: the query after its turn, the
 // key after its rotation, the rotation's table (2^-11 each, of the vectors' lengths: a
@@ -235,7 +236,7 @@ __global__ __launch_bounds__(256) void px_pack_kernel(const PrefixPackArgs a) {
 // waited for its instructions (4 x 1024 own positions of 8 heads: 33 us straight, 13
 // rolled).  `between` runs when xf has been used for the last time.
 template <typename XT, int NG, int KP, bool STRAIGHT, typename F>
-__device__ __forceinline__ void px_tile(const uint4* bl, const uint4* ql, const uint4* rope, const uint4 (&xf)[2 * KP], float down,
+__device__ __forceinline__ void px_tile(const uint4* bl, const uint4* ql, const uint4* rope, const uint4 (&xf)[2 * KP],
                                         floatx16 (&acc)[NG], F between) {
   const int lane = threadIdx.x & 63;
   auto keys = [&](int w) {
@@ -254,9 +255,8 @@ __device__ __forceinline__ void px_tile(const uint4* bl, const uint4* ql, const 
         float l[2], u[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float k0 = kx[4 * g + j + i], k1 = kx[8 + 4 * g + j + i];
+          const float k0 = kx[4 * g + j + i], k1 = kx[8 + 4 * g + j + i];
           const float c = (float)t[2 * (j + i)], sp = (float)t[2 * (j + i) + 1];
-          if constexpr (!STRAIGHT && __is_same(XT, __bf16)) { k0 *= down; k1 *= down; }
           // (k sin + 0 takes the table's fp16 as it is; a plain product would convert it first)
           l[i] = fmaf(c, k0, -fmaf(sp, k1, 0.f));
           u[i] = fmaf(c, k1, fmaf(sp, k0, 0.f));
@@ -382,7 +382,7 @@ __device__ __forceinline__ void px_prefix_logits(const PrefixLogitsArgs& a, uint
 #pragma unroll
     for (int pt = 0; pt < 2; ++pt) {
       clear();
-      px_tile<XT, NG, KP, true>(bl, ql, a.rope + (int64_t)(2 * s + pt) * 512 + at_lane, xf, 1.f, acc[pt],
+      px_tile<XT, NG, KP, true>(bl, ql, a.rope + (int64_t)(2 * s + pt) * 512 + at_lane, xf, acc[pt],
                                 [&]() { fetch(pt == 0 ? 2 * s + 1 : 2 * min(s + 8, s_end - 1)); });
     }
 #pragma unroll
@@ -438,6 +438,52 @@ __device__ __forceinline__ void px_prefix_logits(const PrefixLogitsArgs& a, uint
 // looked at
 constexpr float PX_MASKED = -65504.f;
 __device__ inline float px_mask(float l, float m) { return !(l == l) && m <= PX_MASKED ? -INFINITY : l + m; }
+
+// The exponent by which a position's key may pass 2^15 (0: it does not): |key| <= |latent| per_latent, the latent's chunks in
+// the lanes of both halves.  By the 2-norm in fp16 (one instruction for two ranks; the largest magnitude takes two), by
+// the largest magnitude in bf16, whose squares pass fp32's range.  None for infinities and NaN.
+template <typename XT, int KS> __device__ __forceinline__ int px_own_exp(const uint4 (&xf)[KS], float per_latent) {
+  float size;
+  if constexpr (__is_same(XT, _Float16)) {
+    float s[2] = {};
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const kh2 x = __builtin_bit_cast(kh2, j == 0 ? xf[k].x : j == 1 ? xf[k].y : j == 2 ? xf[k].z : xf[k].w);
+        s[j & 1] = __builtin_amdgcn_fdot2(x, x, s[j & 1], false);
+      }
+    size = __builtin_amdgcn_sqrtf(add_halves(s[0] + s[1]));
+  } else {
+    uint32_t big = 0;
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+      big = max2_u16(max2_u16(max2_u16(big, xf[k].x & 0x7fff7fffu), xf[k].y & 0x7fff7fffu),
+                     max2_u16(xf[k].z & 0x7fff7fffu, xf[k].w & 0x7fff7fffu));
+    size = max_halves(fmaxf(__uint_as_float(big << 16), __uint_as_float(big & 0xffff0000u)));
+  }
+  const float bound = size * per_latent;
+  return bound > 32768.f && bound < INFINITY ? min((int)(__float_as_uint(bound) >> 23) - 141, 100) : 0;
+}
+// The latents times 2^-e: exact in bf16.  fp16 ones may round at 2^-25, which beside the scaled latent (2^-12 or more: B_k
+// below 2^16, 128 ranks) is less than the key's own rounding; twice half the way, as 2^-e itself may be too small a number.
+template <typename XT, int KS> __device__ __forceinline__ void px_scale_down(uint4 (&xf)[KS], int e) {
+  const float f = pow2f(-e), f1 = pow2f(-(e >> 1)), f2 = pow2f(-(e - (e >> 1)));
+#pragma unroll
+  for (int k = 0; k < KS; ++k) {
+    uint32_t w[4] = {xf[k].x, xf[k].y, xf[k].z, xf[k].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (__is_same(XT, _Float16)) {
+        const kh2 d1 = {(_Float16)f1, (_Float16)f1}, d2 = {(_Float16)f2, (_Float16)f2};
+        w[j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(kh2, w[j]) * d1 * d2);
+      } else {                                     // (every product is a bf16 number: its low bits are zeros)
+        w[j] = __float_as_uint(__uint_as_float(w[j] << 16) * f) >> 16 | (__float_as_uint(__uint_as_float(w[j] & 0xffff0000u) * f) & 0xffff0000u);
+      }
+    }
+    xf[k] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
 
 // A sequence's own positions: dense latents where they lie (rows at any alignment),
 // the queries of one KV head and sequence, and the logits go out in fp32 as the
@@ -498,28 +544,26 @@ __device__ __forceinline__ void px_own_logits(const PrefixLogitsArgs& a, uint8_t
       if (2 * k + hh >= nc) lo = hi = 0;
       xf[k] = make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
     }
-    // bf16 keys can pass fp16's range: scaled by what bounds them (the prefix's were when it was packed)
-    float up = 1.f, down = 1.f;
-    if constexpr (__is_same(XT, __bf16)) {
-      uint32_t big = 0;
-#pragma unroll
-      for (int k = 0; k < KS; ++k)
-        big = max2_u16(max2_u16(max2_u16(big, xf[k].x & 0x7fff7fffu), xf[k].y & 0x7fff7fffu),
-                       max2_u16(xf[k].z & 0x7fff7fffu, xf[k].w & 0x7fff7fffu));
-      const float bound = px_wave_max(fmaxf(__uint_as_float(big << 16), __uint_as_float(big & 0xffff0000u))) * a.head[5];
-      if (bound > 32768.f && bound < INFINITY) {
-        const int e = min((int)(__float_as_uint(bound) >> 23) - 141, 100);
-        up = pow2f(e);
-        down = pow2f(-e);
-      }
-    }
+    // keys can pass fp16's range: each position's latent is scaled by what bounds its key (the prefix's were when it was
+    // packed; by position, not by tile: what lies in masked places has no say in the others' bits)
+    int e = px_own_exp<XT, KS>(xf, a.head[5]);
+    const bool scaled = __any(e != 0);
+    if (scaled) px_scale_down<XT, KS>(xf, e);
     floatx16 acc[NG] = {};
-    px_tile<XT, NG, KP, false>(bl, ql, a.rope + (int64_t)t * 512 + 32 * hh + pn, xf, down, acc,
+    px_tile<XT, NG, KP, false>(bl, ql, a.rope + (int64_t)t * 512 + 32 * hh + pn, xf, acc,
                                [&]() { if (t + 8 < t_end) fetch(t + 8); });
     const int p0 = 32 * t + 16 * hh;
+    if (scaled) {                                  // undone: position 16 hh + r of the tile lies in lane (r / 4) * 8 + 4 hh + r % 4
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float up = pow2f(__shfl(e, (r >> 2) * 8 + 4 * hh + (r & 3), 64));
+#pragma unroll
+        for (int g = 0; g < NG; ++g) acc[g][r] *= up;
+      }
+    }
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      const float f = mul[g * 32 + n] * up;
+      const float f = mul[g * 32 + n];
       const int rl = g * 32 + n;
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[g][r] *= f;

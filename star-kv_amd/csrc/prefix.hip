@@ -434,10 +434,10 @@ __device__ __forceinline__ void px_prefix_logits(const PrefixLogitsArgs& a, uint
   if (tid < NG * 32 && r0 + tid < nr) a.cmax[(int64_t)chunk * a.Mp + (int64_t)h * nr + r0 + tid] = wm[tid];
 }
 
-// a logit under its mask; one of no number in a place that the mask takes out (at or below a type's lowest value) is not
-// looked at
+// a logit under its mask; one of no finite number in a place that the mask takes out (at or below a type's lowest value) is
+// not looked at
 constexpr float PX_MASKED = -65504.f;
-__device__ inline float px_mask(float l, float m) { return !(l == l) && m <= PX_MASKED ? -INFINITY : l + m; }
+__device__ inline float px_mask(float l, float m) { return !(fabsf(l) < INFINITY) && m <= PX_MASKED ? -INFINITY : l + m; }
 
 // The exponent by which a position's key may pass 2^15 (0: it does not): |key| <= |latent| per_latent, the latent's chunks in
 // the lanes of both halves.  By the 2-norm in fp16 (one instruction for two ranks; the largest magnitude takes two), by

@@ -41,6 +41,39 @@ def test_rows_of_one_tile_keep_their_own_scale(dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("mdtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_padding_of_infinities_is_not_looked_at(mdtype, bad, dtype):
+    """Own dense K latents that are no finite numbers in masked places, beside keys past 65504: as if they held zeros."""
+    for low in (torch.finfo(mdtype).min, -math.inf):
+        c = Case(3, 8, 4, 130, 40, 16, 32, 64, dtype, seed=53, kx=15000.0, qx=1e-5)
+        for t in (c.k, c.pk):                                    # as above
+            t.clamp_(-torch.finfo(dtype).max, torch.finfo(dtype).max)
+        c.bk = (c.bk.float() * 8).to(dtype)
+        keep = torch.tensor([40, 17, 0])
+        mask = torch.zeros(3, 1, 40).masked_fill_(torch.arange(40) >= keep[:, None, None], low).to(mdtype)
+        pad = (mask[:, 0] < 0)[:, None, :, None]
+        c.k = c.k.masked_fill(pad, 0.0)
+        want = c.run(mask)
+        c.check(want, mask)
+        c.k = c.k.masked_fill(pad, bad)
+        assert torch.equal(c.run(mask), want)
+        c.k[1, :, 3] = bad
+        got = c.run(mask)
+        assert torch.isnan(got[1]).all() and torch.equal(got[::2], want[::2])
+
+
+def test_one_infinite_rank_in_a_masked_place():
+    """A single infinite element gives infinite keys, which a finite mask does not take out."""
+    c = Case(3, 8, 4, 130, 40, 16, 32, 64, torch.float16, seed=53)
+    mask = torch.zeros(3, 1, 40)
+    mask[:, :, 20:] = torch.finfo(torch.float32).min
+    want = c.run(mask)
+    c.k[:, :, 25, 2] = math.inf
+    assert torch.equal(c.run(mask), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_finite_value_padding_has_no_weight(dtype):
     """Own V rows in masked places may hold any finite number (their weight is 0, not their place in the product)."""
     c = Case(3, 8, 4, 130, 40, 16, 32, 64, dtype, seed=53)

@@ -82,3 +82,15 @@ def test_finite_value_padding_has_no_weight(dtype):
     want = c.run(mask)
     c.v = c.v.masked_fill((mask[:, 0] < 0)[:, :, None], torch.finfo(dtype).max)
     assert torch.equal(c.run(mask), want)
+
+
+def test_value_padding_that_is_no_number_shows_where_others_are_kept():
+    """V rows have to be finite: a NaN one in a masked place makes its row NaN if the row keeps other own positions, as
+    decode_attention has it, and is not read if it keeps none."""
+    c = Case(3, 8, 4, 130, 40, 16, 32, 64, torch.float16, seed=53)
+    keep = torch.tensor([40, 17, 0])
+    mask = torch.zeros(3, 1, 40).masked_fill_(torch.arange(40) >= keep[:, None, None], -math.inf)
+    want = c.run(mask)
+    c.v = c.v.masked_fill((mask[:, 0] < 0)[:, :, None], math.nan)
+    got = c.run(mask)
+    assert torch.isnan(got[1]).all() and torch.equal(got[::2], want[::2])

@@ -56,7 +56,7 @@ class SharedPrefix:
         self.data = _out(max(nb, 1), dtype=torch.uint8, device=self.device)
         d.prefix, d.prefix_bytes = self.data.data_ptr(), nb
         _launch("starkv_prefix_pack", d, self.device)
-        angle = (rope.inv_freq() * torch.tensor(n, dtype=torch.float32)).double()
+        angle = rope.inv_freq().double() * n       # (an fp32 product is off by up to 2^-9 rad at 65000 positions)
         self._cos = (ctypes.c_float * 64)(*angle.cos().tolist())
         self._sin = (ctypes.c_float * 64)(*angle.sin().tolist())
         self._rank = int_array(self.ranks)

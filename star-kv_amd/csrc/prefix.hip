@@ -18,11 +18,12 @@
 //    (d, d + 64) in one lane, so it is rotated in registers and is, as fp16, the
 //    A operand of K q^T as it stands.  There each lane holds 32 logits of one
 //    query row: maximum and sum take one exchange of the wave's halves.  It
-//    writes p = exp(l - strip maximum) in fp16, and the strip's (maximum, sum).
+//    writes p = 2^(l - m) in fp16, l in units of log 2 and m the strip's maximum
+//    rounded up to a whole number, and the strip's (m, sum).
 // 2. prefix_pv_kernel: the product P V, split over strips.  A strip's rows are
 //    brought to the row's maximum over the whole prefix by a factor
-//    2^15 exp(strip maximum - row maximum) on the operand: strips 2^-29 below the
-//    row's largest weight still keep all bits of fp16.  Each split's sums leave
+//    2^15 2^(m - the row's m) on the operand, a power of two, so exact: strips 2^-28
+//    below the row's largest weight still keep all bits of fp16.  Each split's sums leave
 //    divided by its weights' sum, in fp32: fp16 means of values that cancel, or that
 //    are small beside the latent's largest, would be subnormal.
 // 3. prefix_up_kernel adds the splits and, if the sequences have positions of
@@ -38,7 +39,7 @@
 // Roundings to fp16, as the decode kernels have them: the query after its turn, the
 // key after its rotation, the rotation's table (2^-11 each, of the vectors' lengths: a
 // logit's error, of which a matrix operand of 16 bits takes the first two in any case);
-// weights and strip factors (2^-11 of a term).  Statistics, sums and split means are
+// weights (2^-11 of a term, once).  Statistics, sums and split means are
 // fp32, and the up-projection takes its operand in terms that keep 22 bits or more (fp16:
 // of what is above 2^-18 of a row's largest value, 2^-39 of it below).
 #include <algorithm>
@@ -405,7 +406,9 @@ __device__ __forceinline__ void px_prefix_logits(const PrefixLogitsArgs& a, uint
       for (int pt = 0; pt < 2; ++pt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[pt][g][r]);
-      m = fmaxf(max_halves(m), -3.0e38f);          // a strip of -inf alone: weights 0
+      // a whole power of two at or above the largest, so that a weight is rounded once: its strip's factor and their product
+      // are exact.  A strip of -inf alone: weights 0
+      m = __builtin_ceilf(fmaxf(max_halves(m), -3.0e38f));
       top[g] = fmaxf(top[g], m);
       float l = 0.f;
       uint8_t* o = (uint8_t*)(a.p + (int64_t)8 * s * a.Mp);
@@ -648,8 +651,8 @@ template <int N> __device__ inline void px_stage_ready() {
 // Workgroup of 8 waves = (split of the strips, BM rows, 256 columns), wave (wm, wn)
 // of WM x WN: RM x RN MFMA tiles, two waves a SIMD.  Steps of 32 positions go
 // through a ring of four LDS stages, two of them in flight behind the one that is
-// read ahead; the strips' factors are formed 56 strips at a time.  Weights and
-// factors are fp16 (2^-11 of each position's term, of either sign), sums fp32.
+// read ahead; the strips' factors are formed 56 strips at a time.  Weights are
+// fp16 (2^-11 of each position's term, of either sign), factors powers of two, sums fp32.
 // 512 rows x 32768 positions x 1640 columns: 69 us, 871 TFLOP/s of the tiles' products
 // (1792 columns), 66 with every load from the caches: matrix unit and LDS reads,
 // nearly level (operands read when they are needed, not a step ahead: 74).

@@ -35,3 +35,24 @@ def test_turn_past_a_long_prefix(theta):
     got = prefix_decode_attention(c.q.to(DEV), c.prefix(), None, None, c.uv.to(DEV), out_dtype=torch.float32)
     rel = ((got.double().cpu() - want).abs() / want.abs()).max()
     assert rel < 3 * 2.0 ** -11, rel
+
+
+@pytest.mark.parametrize("a,b,c3", [(-0.765625, -1.654296875, -0.70263671875), (2.966796875, 2.025390625, 2.990234375),
+                                    (2.453125, 1.556640625, 2.48828125), (-0.9765625, -1.876953125, -0.96435546875)])
+def test_weights_are_rounded_once(a, b, c3):
+    """63 positions of one weight in a strip whose maximum is another's, below the next strip's: where values are all 1,
+    the output is off by their rounding alone, 2^-11 at most (and fp32 sums).  (At these logits the roundings of the
+    weight, the strip's factor and their product would fall the same way, 1.7 times 2^-11.)"""
+    c = Case(1, 1, 1, 128, 0, 1, 1, 1, torch.float16, seed=1, theta=1e9)
+    for t in (c.pk, c.bk, c.q):
+        t.zero_()
+    c.q[..., 63] = 8                                             # the slowest frequency: no turn to speak of
+    c.bk[0, 0, 63] = 1
+    c.pk[0, :64, 0] = b
+    c.pk[0, 0, 0] = a
+    c.pk[0, 64:, 0] = -80.0
+    c.pk[0, 64, 0] = c3
+    c.pv.fill_(1.0)
+    c.uv = torch.ones(128, 1).half()
+    got = prefix_decode_attention(c.q.to(DEV), c.prefix(), None, None, c.uv.to(DEV), out_dtype=torch.float32)
+    assert (got.double() - 1).abs().max() <= 2.0 ** -11 + 2.0 ** -16

@@ -83,12 +83,13 @@ def keep_positions(k: KLatentSpec, v, positions: torch.Tensor, length: int, scor
     if B < 1 or not 0 <= keep <= length:
         raise StarKVError(f"need at least one sequence and 0 <= keep <= length, got positions {tuple(positions.shape)}, "
                           f"length {length}")
-    if vs.data.shape[0] != B or vs.data.shape[1] < length or k.data.shape[0] != B or (length and not k.holds(B, length)):
-        raise StarKVError(f"the caches must hold {B} sequences of at least {length} positions: K "
+    if vs.data.shape[0] != B or k.data.shape[0] != B or (length and not (k.holds(B, length) and vs.holds(B, length))):
+        raise StarKVError(f"the caches must hold {B} sequences of at least {length} positions, and their scales too: K "
                           f"{tuple(k.data.shape)}, V {tuple(vs.data.shape)}")
     device = vs.data.device
-    if any(t.device != device for t in (positions, k.data)):
-        raise StarKVError(f"positions and the K latent must lie on {device} as the V latent does")
+    moved = [positions, k.data, k.scale, k.data2, k.scale2, error_flag, *vs.tensors]
+    if any(t is not None and t.device != device for t in moved):
+        raise StarKVError(f"positions, the error flag, latents and scales must lie on {device} as the V latent does")
     if scores is not None:
         _check_scores(scores, B, length, device)
     dense = k.data.dtype in (torch.float16, torch.bfloat16)

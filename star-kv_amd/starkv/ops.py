@@ -120,6 +120,11 @@ def _launch(name: str, desc, device, workspace: Optional[bool] = None) -> None:
         check(st, name)
 
 
+def _extent(t: torch.Tensor) -> int:
+    """Elements from a tensor's first to its last."""
+    return 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else 0
+
+
 class KLatentSpec:
     """Where the key latent of every KV head lives (see include/starkv.h,
     starkv_klatent).  Element (b, h, s, j) is at
@@ -159,9 +164,36 @@ class KLatentSpec:
         return len(self.ranks)
 
     def holds(self, batch: int, rows: int) -> bool:
-        """Whether ``data`` reaches to row rows - 1 of sequence batch - 1."""
-        last = max(o + (rows - 1) * p for o, p in zip(self.head_offset, self.pos_stride)) + (batch - 1) * self.stride_b
-        return last <= sum((n - 1) * s for n, s in zip(self.data.shape, self.data.stride()))
+        """Whether the latents and their scales reach to the end of row rows - 1 of sequence batch - 1 (B_k apart)."""
+        r, b, n = self.ranks, batch - 1, rows - 1
+        two = self.fmt == FMT_INT4_REF and self.split > 0
+        if self.fmt == FMT_DENSE:
+            width = r
+        elif (self.split_fmt if two else self.fmt) == FMT_INT8_SYM:
+            width = [min(x, self.split) for x in r] if two else r
+        else:
+            width = [(min(x, self.split) + 1) // 2 if two else (x + 1) // 2 for x in r]
+        ends = [o + n * p + w for o, p, w in zip(self.head_offset, self.pos_stride, width)]
+        if max(ends) + b * self.stride_b > _extent(self.data):
+            return False
+        if self.fmt == FMT_DENSE:
+            return True
+        heads = len(r) - 1
+        if self.scale is None or b * self.scale_stride_b + heads * self.scale_stride_h + rows > _extent(self.scale):
+            return False
+        lower = [(h, x - self.split) for h, x in enumerate(r) if x > self.split] if two else []
+        if not lower:
+            return True
+        if self.data2 is None or self.scale2 is None:
+            return False
+        end = max(self.head_offset2[h] + n * self.pos_stride2[h] + (x + 1) // 2 for h, x in lower)
+        return end + b * self.stride2_b <= _extent(self.data2) and \
+            b * self.scale2_stride_b + heads * self.scale2_stride_h + rows <= _extent(self.scale2)
+
+    def holds_bk(self) -> bool:
+        """Whether B_k reaches to the end of every head's last row, its rows contiguous."""
+        last = max(o + (r - 1) * self.bk_row_stride for o, r in zip(self.bk_head_offset, self.ranks))
+        return self.bk.stride(-1) == 1 and last + HEAD_DIM <= _extent(self.bk)
 
     @classmethod
     def from_reference(cls, x: torch.Tensor, b: torch.Tensor) -> "KLatentSpec":
@@ -368,6 +400,23 @@ class VLatentSpec:
         if scale.stride() != zero.stride():
             raise StarKVError("scale and zero must share strides")
         return cls(rank, FMT_INT4_G64, packed, scale, zero=zero)
+
+    def holds(self, batch: int, rows: int) -> bool:
+        """Whether the latents, their scales and zero points hold ``rows`` positions of ``batch`` sequences."""
+        def has(t, width):
+            return t is not None and t.shape[0] >= batch and t.shape[1] >= rows and (t.shape[2] if t.dim() > 2 else 1) >= width
+
+        r = self.rank
+        if self.fmt == FMT_DENSE:
+            return has(self.data, r)
+        if self.fmt == FMT_INT4_G64:
+            groups = (r + 63) // 64
+            return has(self.data, (r + 1) // 2) and has(self.scale, groups) and has(self.zero, groups)
+        two = self.fmt == FMT_INT4_REF and self.data2 is not None and 0 < self.split < r
+        up = self.split if two else r
+        wide = (self.split_fmt if two else self.fmt) == FMT_INT8_SYM
+        return has(self.data, up if wide else (up + 1) // 2) and has(self.scale, 1) and \
+            (not two or has(self.data2, (r - up + 1) // 2) and has(self.scale2, 1))
 
     def c_struct(self) -> VLatent:
         v = VLatent()

@@ -35,6 +35,8 @@ class SharedPrefix:
             raise StarKVError(f"row {row} of the V latent {tuple(vs.data.shape)} does not hold {n} positions")
         if not k.holds(row + 1, n):
             raise StarKVError(f"row {row} of the K latent {tuple(k.data.shape)} does not hold {n} positions")
+        if not k.holds_bk():
+            raise StarKVError(f"B_k {tuple(k.bk.shape)} does not hold {k.ranks} rows of {HEAD_DIM} contiguous elements")
         if k.data.dtype != vs.data.dtype or k.bk.dtype != k.data.dtype:
             raise StarKVError(f"K latents, B_k and V latents must share a type, got {k.data.dtype}, {k.bk.dtype}, "
                               f"{vs.data.dtype}")
@@ -105,12 +107,11 @@ def prefix_decode_attention(q: torch.Tensor, prefix: SharedPrefix, k: Optional[K
         if k.ranks != prefix.ranks or v.rank != prefix.v_rank:
             raise StarKVError(f"own latents have K ranks {k.ranks} and V rank {v.rank}, the prefix {prefix.ranks} and "
                               f"{prefix.v_rank}")
-        rows = v.data.shape
-        if rows[0] < B or rows[1] < n:
-            raise StarKVError(f"the V latent {tuple(rows)} does not hold {B} sequences of {n} positions")
+        if not v.holds(B, n):
+            raise StarKVError(f"the V latent {tuple(v.data.shape)} does not hold {B} sequences of {n} positions")
         if not k.holds(B, n):
             raise StarKVError(f"the K latent {tuple(k.data.shape)} does not hold {B} sequences of {n} positions")
-        if any(t is not None and t.device != device for t in (k.data, v.data, mask, last_pos)):
+        if any(t is not None and t.device != device for t in (mask, last_pos, *k.tensors, *v.tensors)):
             raise StarKVError(f"own latents, mask and last_pos must lie on {device} as q does")
         if k.fmt == FMT_DENSE and k.data.dtype != prefix.dtype or v.fmt == FMT_DENSE and v.data.dtype != prefix.dtype:
             raise StarKVError(f"dense own latents must be {prefix.dtype}, got {k.data.dtype} and {v.data.dtype}")

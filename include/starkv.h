@@ -644,7 +644,8 @@ int starkv_decode_attention_scores(const starkv_decode_desc* d, float* scores, i
  * stored before rotation, so a moved row takes the angle of its new place.
  * B_k's fields of k are not read.  dtype: of dense latents.  batch <= 65535.
  * Rows of different positions, heads or sequences that overlap (or may: heads
- * of different pitch whose ranges do) are STARKV_ERR_SHAPE.
+ * of different pitch whose ranges do) are STARKV_ERR_SHAPE; sequences, heads
+ * and positions may lie in any order.
  * ------------------------------------------------------------------- */
 typedef struct {
   int batch, length, keep, sinks, recent;

@@ -1794,6 +1794,20 @@ static bool rows_apart(int H, const int64_t* off, const int64_t* pitch, const in
       }
   }
   if (B == 1 || sb >= hi - lo || (inside && sb >= row && pitch[last] >= (B - 1) * sb + row)) return true;
+  // sequences side by side within a head's row: heads beside one another in a position's row, or one behind another
+  bool rows = true, beside = even, behind = true;
+  int prev = -1;
+  for (int h = 0; h < H; ++h) {
+    if (!nb[h]) continue;
+    rows &= sb >= nb[h] && pitch[h] >= (B - 1) * sb + nb[h];
+    if (prev >= 0) {
+      beside &= off[h] >= off[prev] + (B - 1) * sb + nb[prev];
+      behind &= off[h] >= end(prev) + (B - 1) * sb;
+    }
+    beside &= off[h] + (B - 1) * sb + nb[h] - lo <= pitch[h];
+    prev = h;
+  }
+  if (rows && (beside || behind)) return true;
   // each head's sequences one behind another, and the heads' ranges apart
   for (int g = 0; g < H; ++g) {
     if (!nb[g]) continue;

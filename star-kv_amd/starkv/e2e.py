@@ -739,6 +739,8 @@ def drop_prompt(model) -> None:
     for att in attention_layers(model):
         att.prefix = None
         att.cache.length = 0
+        if att.scores is not None:
+            att.scores.zero_()
 
 
 @torch.no_grad()

@@ -20,7 +20,6 @@
 //    chunk's own rows are in registers before its first write.  So the move is in
 //    place without a copy of the cache, and slices run side by side.
 #include <algorithm>
-#include <type_traits>
 
 #include "common.hpp"
 
@@ -55,11 +54,6 @@ __device__ inline void row4(const ScoreArgs& a, const T* row, int s, float (&v)[
   }
 }
 
-__device__ inline float wave_max(float v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-  return v;
-}
 __device__ inline float wave_sum(float v) {
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);

@@ -473,6 +473,11 @@ __device__ inline float wave_max32(float v) {   // max over the 32 lanes of a ha
   for (int o = 16; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
   return v;
 }
+__device__ inline float wave_max(float v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
 
 typedef _Float16 kh2 __attribute__((ext_vector_type(2)));
 

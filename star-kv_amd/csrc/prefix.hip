@@ -66,12 +66,6 @@ __device__ inline float max_halves(float v) {
   return fmaxf(__int_as_float(x[0]), __int_as_float(x[1]));
 }
 
-__device__ inline float px_wave_max(float v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-  return v;
-}
-
 // two fp32 values as fp16, nearest even (an instruction for both; left to itself the compiler joins each conversion to
 // the sum before it, in a form that takes twice as long)
 __device__ inline uint32_t px_pack(float a, float b) {
@@ -322,7 +316,7 @@ __device__ __forceinline__ void px_stage(const PrefixLogitsArgs& a, int h, int b
   for (int i = 0; i < RW; ++i) {
     const int r = wave + NW * i;
     const float x0 = to_f32(q0[i]), x1 = to_f32(q1[i]), y0 = x0 * cs - x1 * sn, y1 = x1 * cs + x0 * sn;
-    const float m = px_wave_max(fmaxf(fabsf(y0), fabsf(y1)));
+    const float m = wave_max(fmaxf(fabsf(y0), fabsf(y1)));
     const int e = m < INFINITY && m > 0.f ? min(max((int)(__float_as_uint(m) >> 23), 1), 253) - 127 : 0;
     const float f = pow2f(-e);
     _Float16* dst = (_Float16*)(ql + ((r >> 5) * 8 + 2 * (lane >> 4)) * 64 + ((lane >> 2) & 1) * 32 + (r & 31)) +

@@ -9,8 +9,8 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._lib import FMT_DENSE, DecodeDesc, PrefixDecodeDesc, PrefixPackDesc, StarKVError, check, int_array
-from .ops import (HEAD_DIM, KLatentSpec, VLatentSpec, _check_scores, _decode_desc, _dt, _launch, _out, _q3,
+from ._lib import FMT_DENSE, DecodeDesc, PrefixDecodeDesc, PrefixPackDesc, StarKVError, int_array
+from .ops import (HEAD_DIM, KLatentSpec, _check_scores, _decode_desc, _dt, _launch, _out, _q3,
                   _require_cuda, _vspec)
 from .rope import RopeConfig, rope_table
 

@@ -122,6 +122,8 @@ def _launch(name: str, desc, device, workspace: Optional[bool] = None) -> None:
 
 def _extent(t: torch.Tensor) -> int:
     """Elements from a tensor's first to its last."""
+    if t.is_contiguous():
+        return t.numel()
     return 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else 0
 
 
@@ -167,26 +169,22 @@ class KLatentSpec:
         """Whether the latents and their scales reach to the end of row rows - 1 of sequence batch - 1 (B_k apart)."""
         r, b, n = self.ranks, batch - 1, rows - 1
         two = self.fmt == FMT_INT4_REF and self.split > 0
-        if self.fmt == FMT_DENSE:
-            width = r
-        elif (self.split_fmt if two else self.fmt) == FMT_INT8_SYM:
-            width = [min(x, self.split) for x in r] if two else r
-        else:
-            width = [(min(x, self.split) + 1) // 2 if two else (x + 1) // 2 for x in r]
-        ends = [o + n * p + w for o, p, w in zip(self.head_offset, self.pos_stride, width)]
-        if max(ends) + b * self.stride_b > _extent(self.data):
+        split = self.split if two else 128
+        width = r if self.fmt == FMT_DENSE or not two else [x if x < split else split for x in r]
+        if self.fmt != FMT_DENSE and (self.split_fmt if two else self.fmt) != FMT_INT8_SYM:
+            width = [(x + 1) // 2 for x in width]
+        if max([o + n * p + w for o, p, w in zip(self.head_offset, self.pos_stride, width)]) + b * self.stride_b > _extent(self.data):
             return False
         if self.fmt == FMT_DENSE:
             return True
         heads = len(r) - 1
         if self.scale is None or b * self.scale_stride_b + heads * self.scale_stride_h + rows > _extent(self.scale):
             return False
-        lower = [(h, x - self.split) for h, x in enumerate(r) if x > self.split] if two else []
-        if not lower:
+        if not two or max(r) <= split:
             return True
         if self.data2 is None or self.scale2 is None:
             return False
-        end = max(self.head_offset2[h] + n * self.pos_stride2[h] + (x + 1) // 2 for h, x in lower)
+        end = max([o + n * p + (x - split + 1) // 2 for o, p, x in zip(self.head_offset2, self.pos_stride2, r) if x > split])
         return end + b * self.stride2_b <= _extent(self.data2) and \
             b * self.scale2_stride_b + heads * self.scale2_stride_h + rows <= _extent(self.scale2)
 
@@ -404,7 +402,10 @@ class VLatentSpec:
     def holds(self, batch: int, rows: int) -> bool:
         """Whether the latents, their scales and zero points hold ``rows`` positions of ``batch`` sequences."""
         def has(t, width):
-            return t is not None and t.shape[0] >= batch and t.shape[1] >= rows and (t.shape[2] if t.dim() > 2 else 1) >= width
+            if t is None:
+                return False
+            shape = t.shape
+            return shape[0] >= batch and shape[1] >= rows and (shape[2] if len(shape) > 2 else 1) >= width
 
         r = self.rank
         if self.fmt == FMT_DENSE:

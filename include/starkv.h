@@ -669,9 +669,9 @@ int starkv_keep_positions(const starkv_keep_desc* d, void* stream);
 
 /* ---------------------------------------------------------------------
  * Decode of a batch whose sequences share a prefix (a system prompt, the
- * prompt of several samples): attention over the prefix is computed once for
- * all.  No counterpart in the reference, which holds a copy of the prefix for
- * each sequence.
+ * prompt of several samples): the prefix is held once for all, and attention
+ * over it computed for all together.  No counterpart in the reference, which
+ * holds a copy of the prefix for each sequence.
  *
  * starkv_prefix_pack lays out one sequence's dense latents (positions [0,
  * length) of k and v, whose stride_b is not read) and B_k for
@@ -699,7 +699,7 @@ int starkv_keep_positions(const starkv_keep_desc* d, void* stream);
  * (optional): the weights of own positions, summed over the query heads, are
  * added onto scores[b * scores_stride_b + s].
  * Keys over the prefix are fp16 between the reconstruction and the logits,
- * weights fp16 relative to a strip of 64 positions, sums fp32.
+ * weights fp16 relative to a strip of 64 positions, sums and means fp32.
  * Results do not depend on the order of atomics.
  * ------------------------------------------------------------------- */
 typedef struct {

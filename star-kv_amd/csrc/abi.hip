@@ -1958,7 +1958,7 @@ struct PrefixLayout {
 // Strips per P V split: the least modelled time in strips (about 1 us each), rounds of one workgroup a CU, each its strips
 // and a fixed time, and 0.12 for each split that the join adds up.  A round of workgroups that is hardly begun costs as
 // much as a full one (65536 positions of 512 rows in 19 splits of 14 tiles: 198 us, in 36 161, in 18 152); 16384 of 128 rows
-// in 128 splits of 2 tiles: 14 us and 22 for the join, in 64 14 and 17.
+// in 128 splits of 2 tiles: 13.8 us and 15 for the join, in 64 14.6 and 11.3.
 int prefix_split_len(int tiles, int cus, int strips) {
   int best = 0;
   double least = 0;

@@ -647,9 +647,10 @@ template <int N> __device__ inline void px_stage_ready() {
 // through a ring of four LDS stages, two of them in flight behind the one that is
 // read ahead; the strips' factors are formed 56 strips at a time.  Weights are
 // fp16 (2^-11 of each position's term, of either sign), factors powers of two, sums fp32.
-// 512 rows x 32768 positions x 1640 columns: 69 us, 871 TFLOP/s of the tiles' products
-// (1792 columns), 66 with every load from the caches: matrix unit and LDS reads,
-// nearly level (operands read when they are needed, not a step ahead: 74).
+// 512 rows x 32768 positions x 1640 columns: 71 us, 846 TFLOP/s of the tiles' products
+// (1792 columns; 69 with means of 16 bits, 66 of those with every load from the caches):
+// matrix unit and LDS reads, nearly level (operands read when they are needed, not a step
+// ahead: 5 us more).
 template <int RM, int RN, int WM, int WN>
 __global__ __launch_bounds__(512, 2) void prefix_pv_kernel(const PrefixArgs a) {
   constexpr int BM = 32 * RM * WM, BN = 32 * RN * WN, RING = 4;
@@ -806,8 +807,8 @@ template <typename WT> struct PxTerms;
 template <> struct PxTerms<_Float16> { static constexpr int N = 2; };
 template <> struct PxTerms<__bf16> { static constexpr int N = 3; };
 
-// threads: with few workgroups more of them to ask for the partials (4 behind 16384 positions: 13.4 us, 256 threads 16.8),
-// with many fewer (batch 16 behind 32768: 24 of 256, 29 of 512)
+// threads: with few workgroups more of them to ask for the partials (4 behind 16384 positions: 11.3 us, 256 threads 15.0),
+// with many fewer (batch 16 behind 32768: 25 of 256, 36 of 512)
 template <int SC> constexpr int PX_UP_T = SC == 128 ? 256 : 512;
 
 // Workgroup = (SC columns of the V rank, KV head, 32 of its rows (sequence, head of
@@ -815,7 +816,7 @@ template <int SC> constexpr int PX_UP_T = SC == 128 ? 256 : 512;
 // positions' chunks, in a fixed order, relative to the larger of the two maxima and
 // divided by the weights' sum, and multiplies them by its columns of U_v: a term of
 // the output, [column slice][row][128], that prefix_finish_kernel adds up.  Batch 16
-// behind 32768: 18 splits of 512 rows, 30 MB, and own partials in 19 us; where workgroups
+// behind 32768: 18 splits of 512 rows, 61 MB, and own partials in 24 us; where workgroups
 // are few (11 to 13 us) two to four batches of loads, one after another.
 template <typename WT, int SC>
 __global__ __launch_bounds__(PX_UP_T<SC>) void prefix_up_kernel(const PrefixArgs a) {

@@ -71,8 +71,9 @@ def keep_positions(k: KLatentSpec, v, positions: torch.Tensor, length: int, scor
     keep - 1, in place; rows from keep on stay as they are.  ``scores`` [B, >=
     length] move along, zeros behind.  A position that breaks the rule leaves
     its row as it is and sets ``error_flag`` (int32 device tensor) to 1.  Rows
-    that share memory (an expanded head or batch) are refused.  Keys are cached before rotation: a moved row takes the angle of its new place,
-    and the next token's position is ``keep``."""
+    that share memory (an expanded head or batch) and tensors that end before
+    the rows are refused.  Keys are cached before rotation: a moved row takes
+    the angle of its new place, and the next token's position is ``keep``."""
     vs = _vspec(v)
     _require_cuda(positions, scores, error_flag, *k.tensors, *vs.tensors)
     if positions.dim() != 2 or positions.dtype != torch.int32 or (positions.shape[1] > 1 and positions.stride(1) != 1):

@@ -750,6 +750,8 @@ def generate_bounded(model, prompt: torch.Tensor, steps: int, keep: int, sinks: 
     layer's cache is full, it keeps ``keep`` positions -- the first ``sinks``,
     the last ``recent``, and those that the decode steps since have given the
     most attention, by layer and sequence -- and goes on (``LatentCache.bound``).
+    The prompt's own attention is not counted: a cache that the prompt fills
+    keeps the lowest positions between, so leave some capacity behind it.
     ``forced`` [B, steps] as in ``generate``.  Returns (tokens [B, steps + 1],
     logits of the last position per forward)."""
     atts = attention_layers(model)

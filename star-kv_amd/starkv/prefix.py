@@ -71,7 +71,7 @@ def prefix_decode_attention(q: torch.Tensor, prefix: SharedPrefix, k: Optional[K
                             last_pos: Optional[torch.Tensor] = None,
                             scores: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``decode_attention`` of sequences that all follow ``prefix``: attention
-    over its positions, computed once for the batch, and over each sequence's
+    over its positions, computed for the batch together, and over each sequence's
     own latents (``k``, ``xv``, ``seq_len``, ``mask`` and ``last_pos`` as
     there; ``k`` and ``xv`` None, or ``seq_len`` 0: none yet).  B_k is the
     layer's, as the prefix was packed with it.  A sequence whose mask leaves

@@ -96,10 +96,11 @@ def rope_table(cfg: RopeConfig, positions: int, device: torch.device):
         table = torch.empty(nbytes // 4, dtype=torch.float32, device=device)
         inv = cfg.inv_freq().contiguous()
         inv_arr = (ctypes.c_float * 64)(*inv.tolist())
-        stream = torch.cuda.current_stream(device).cuda_stream
-        _lib.check(L.starkv_rope_build(inv_arr, ctypes.c_float(cfg.attention_scaling), cap,
-                                       ctypes.c_void_p(table.data_ptr()), nbytes, ctypes.c_void_p(stream)),
-                   "starkv_rope_build")
+        with torch.cuda.device(device):                # the launch takes the current device's code
+            stream = torch.cuda.current_stream(device).cuda_stream
+            _lib.check(L.starkv_rope_build(inv_arr, ctypes.c_float(cfg.attention_scaling), cap,
+                                           ctypes.c_void_p(table.data_ptr()), nbytes, ctypes.c_void_p(stream)),
+                       "starkv_rope_build")
         ent = (table, cap)
         _TABLES[key] = ent
         return ent

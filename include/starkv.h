@@ -690,8 +690,9 @@ int starkv_keep_positions(const starkv_keep_desc* d, void* stream);
  * whose mask leaves none of its own positions attends to the prefix alone; own
  * logits that are NaN and not masked (at or below -65504, or behind
  * last_pos_device) make its output NaN, and with it its weights in scores.
- * Masked dense K latents may hold anything; own V latents, and the scales of
- * quantised ones, have to be finite wherever s < own.seq_len, as for
+ * Masked dense K latents may hold NaN and infinities (finite logits have the
+ * mask added, whatever it is); own V latents, and the scales of quantised
+ * ones, have to be finite wherever s < own.seq_len, as for
  * starkv_decode_attention (a weight of 0 times NaN is NaN).
  * turn_cos / turn_sin: host arrays [64], the (unscaled) rotation of frequency i
  * by `length` positions.  The prefix's rank, v_rank, length and dtype are those

@@ -77,8 +77,9 @@ def prefix_decode_attention(q: torch.Tensor, prefix: SharedPrefix, k: Optional[K
     layer's, as the prefix was packed with it.  A sequence whose mask leaves
     none of its own positions (-inf, or a value as low as a type's lowest)
     attends to the prefix alone.  Masked positions of dense K latents may hold
-    anything; V latents, and the scales of quantised ones, have to be finite in
-    all ``seq_len`` positions (their weight there is 0, and 0 times NaN is NaN).
+    NaN and infinities (to finite logits a finite mask is added as it is); V
+    latents, and the scales of quantised ones, have to be finite in all
+    ``seq_len`` positions (their weight there is 0, and 0 times NaN is NaN).
 
     Positions are those of the sequences' own caches: ``q`` [B, Hq, 128] is
     rotated at its position behind the sequence's own first one, own key s at
